@@ -7,6 +7,8 @@ The public names mirror the reference package (KIROKOWA/ASRN, asrn/__init__.py:4
   - the model: ModeloASRN / ASRNModel, BloqueLocal / LocalBlock, ConfigASRN / ASRNConfig, TALLAS,
     crear_modelo / create_model, crear_desde_config / create_from_config;
   - training: crear_optimizador, tasa_aprendizaje, PasoGrafado, entrenar / train, evaluar / evaluate;
+  - fine-tuning losses: log_probabilidades / token_log_probs, perdida_preferencia / preference_loss,
+    perdida_politica / policy_loss;
   - files: guardar / save, cargar / load (the reference's format, v83 on);
   - generation: escribir / generate (the loop on the device), EscritorModelo / ModelWriter (the model's O(1) step),
     EscritorCapa / LayerWriter (one layer's);
@@ -16,6 +18,8 @@ cargar_biblioteca() opens the HIP library (the product has no CPU fallback).
 from . import ops, synth
 from ._lib import ASRNHipError, LIB_PATH
 from ._lib import load as cargar_biblioteca
+from .ajuste import (log_probabilidades, perdida_politica, perdida_preferencia, policy_loss, preference_loss,
+                     token_log_probs)
 from .archivo import cargar, guardar
 from .capa import (ASRNCoreLayer, ASRNLayer, CapaASRN, CapaASRNEstable, Protecciones, Protections, convertir,
                    firmas_de_piezas, ngramas)
@@ -39,4 +43,5 @@ __all__ = ['ASRNLayer', 'CapaASRNEstable', 'ASRNCoreLayer', 'CapaASRN', 'Protecc
            'TALLAS', 'crear_modelo', 'create_model', 'crear_desde_config', 'create_from_config', 'crear_optimizador',
            'tasa_aprendizaje', 'PasoGrafado', 'entrenar', 'train', 'evaluar', 'evaluate', 'guardar', 'save',
            'cargar', 'load', 'escribir', 'generate', 'EscritorModelo', 'ModelWriter', 'EscritorCapa', 'LayerWriter',
-           'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']
+           'log_probabilidades', 'token_log_probs', 'perdida_preferencia', 'preference_loss', 'perdida_politica',
+           'policy_loss', 'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']

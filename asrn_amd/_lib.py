@@ -15,6 +15,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/asrn_hip.h
 SIGNATURES = {
@@ -116,6 +117,15 @@ SIGNATURES = {
     'asrn_decode_produce': (ctypes.c_int, [_P] * 4 + [_I64, _I32] + [_P] * 9 + [_I32] * 4 + [_P, _P, _F32, _P, _P, _F32,
                                                                                               _F32, _P, _P, _I32]
                             + [_P] * 6 + [_I64, _I64, _P, _P, _P, _I64, _P]),
+    'asrn_token_logp_fwd': (ctypes.c_int, [_P, _I32] + [_I64] * 5 + [_P, _I64, _F32, _P, _P, _P, _P]),
+    'asrn_token_logp_bwd': (ctypes.c_int, [_P, _I32] + [_I64] * 5 + [_P, _I64, _F32] + [_P] * 6),
+    'asrn_preference_workspace': (_I64, [_I64, _I64]),
+    'asrn_preference_fwd': (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I32, _F64, _F64, _F64, _I32, _P, _P,
+                                           _P, _P, _I64, _P]),
+    'asrn_preference_bwd': (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P]),
+    'asrn_policy_workspace': (_I64, [_I64, _I64]),
+    'asrn_policy_fwd': (ctypes.c_int, [_P] * 7 + [_I64, _I64] + [_F64] * 5 + [_I32] + [_P] * 5 + [_I64, _P]),
+    'asrn_policy_bwd': (ctypes.c_int, [_P] * 5 + [_I64, _I64, _F64, _P, _P, _P]),
 }
 
 _lib = None

@@ -1,0 +1,184 @@
+// The preference loss over pairs of texts, from the log-probabilities of their tokens. Rows 0 .. P - 1 of lp (2P, L) are
+// the chosen texts, P .. 2P - 1 the rejected ones, m the tokens of the answers:
+//   R_i = sum_t m_it (lp_it - ref_it)  [/ sum_t m_it],   h_i = beta (R_i - R_{P+i}) - margin,
+//   sigmoid  -(1 - e) log sigma(h) - e log sigma(-h),   ipo  (h / beta - 1 / (2 beta))^2,   hinge  max(0, 1 - h),
+// averaged over the pairs. d loss / d lp_it = m_it c_i with one coefficient a row, formed in the forward.
+//
+//   k_pref_rows  a row in pieces of 4,096 tokens, one workgroup each: the masked sum and the count of a piece. Long rows
+//                and few rows alike spread over the chip; the sums are in double (a long text's log-probability is a
+//                small difference of large sums), each piece's in a fixed order.
+//   k_pref_loss  one workgroup, a pair a thread: the pieces added in order, the loss, the rewards and the coefficients.
+//   k_pref_bwd   d lp = m g c, written once.
+// HBM-bound for long batches (9 to 13 bytes a token each way), launches for short ones.
+#include <math.h>
+
+#include "common.h"
+#include "strided.h"
+
+namespace asrn {
+
+constexpr int kPfThreads = 256;
+constexpr int kPfUnroll = 4;
+constexpr int kPfPiece = 4096;              // tokens a workgroup sums
+
+struct PfPart { double sum; double n; };
+
+struct PfArgs {
+  Strided lp, ref, mask;                    // ref.p null: none; ref_rows: one sum a row (ref.st unused)
+  int64_t P, L;
+  int32_t ref_rows, kind, mean;
+  double beta, smooth, margin;
+  PfPart* part; uint32_t pieces;
+  float* loss; float* reward; float* coef;
+  const float* g; float* dlp;
+};
+
+__global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
+  __shared__ PfPart red[kPfThreads / kWave];
+  const int64_t row = blockIdx.x / a.pieces, t0 = (int64_t)(blockIdx.x % a.pieces) * kPfPiece;
+  const int64_t t1 = t0 + kPfPiece < a.L ? t0 + kPfPiece : a.L;
+  double s = 0.0;
+  int n = 0;
+  for (int64_t tb = t0 + threadIdx.x; tb < t1; tb += kPfUnroll * kPfThreads) {
+    float x[kPfUnroll], r[kPfUnroll];
+    bool m[kPfUnroll];
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) {
+      const int64_t t = tb + u * kPfThreads, tc = t < t1 ? t : tb;
+      m[u] = a.mask.on(row, tc) && t < t1;
+      x[u] = a.lp.at(row, tc);
+      r[u] = a.ref.p && !a.ref_rows ? a.ref.at(row, tc) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) {     // selected, not multiplied: what a mask hides may be infinite or NaN
+      s += m[u] ? (double)x[u] - (double)r[u] : 0.0;
+      n += m[u];
+    }
+  }
+  s = wave_sum_d(s);
+  double c = wave_sum_d((double)n);
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = PfPart{s, c};
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPfThreads / kWave; ++w) {
+      s += red[w].sum;
+      c += red[w].n;
+    }
+    a.part[blockIdx.x] = PfPart{s, c};
+  }
+}
+
+// log(1 + exp(-|h|)) + max(-h, 0) = -log sigma(h)
+__device__ __forceinline__ double neg_log_sigma(double h) { return log1p(exp(-fabs(h))) + (h < 0.0 ? -h : h != h ? h : 0.0); }
+
+__global__ __launch_bounds__(kPfThreads) void k_pref_loss(PfArgs a) {
+  __shared__ double red[kPfThreads / kWave];
+  double total = 0.0;
+  for (int64_t i = threadIdx.x; i < a.P; i += kPfThreads) {
+    double R[2], div[2];
+    for (int k = 0; k < 2; ++k) {
+      const int64_t row = i + k * a.P;
+      double s = 0.0, n = 0.0;
+      for (uint32_t p = 0; p < a.pieces; ++p) {
+        const PfPart q = a.part[row * a.pieces + p];
+        s += q.sum;
+        n += q.n;
+      }
+      if (a.ref.p && a.ref_rows) s -= (double)a.ref.at(row, 0);
+      div[k] = a.mean && n > 1.0 ? n : 1.0;     // an empty answer: a sum of nothing, divided by 1
+      R[k] = s / div[k];
+      a.reward[row] = (float)(a.beta * R[k]);
+    }
+    const double h = a.beta * (R[0] - R[1]) - a.margin;
+    double v, dh;
+    if (a.kind == 0) {
+      v = (1.0 - a.smooth) * neg_log_sigma(h) + (a.smooth != 0.0 ? a.smooth * neg_log_sigma(-h) : 0.0);
+      dh = a.smooth - 1.0 / (1.0 + exp(h));
+    } else if (a.kind == 1) {
+      const double q = (h - 0.5) / a.beta;
+      v = q * q;
+      dh = 2.0 * q / a.beta;
+    } else {
+      v = h < 1.0 ? 1.0 - h : h != h ? h : 0.0;
+      dh = h < 1.0 ? -1.0 : h != h ? h : 0.0;
+    }
+    total += v;
+    const double c = dh * a.beta / (double)a.P;
+    a.coef[i] = (float)(c / div[0]);
+    a.coef[i + a.P] = (float)(-c / div[1]);
+  }
+  total = wave_sum_d(total);
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPfThreads / kWave; ++w) total += red[w];
+    *a.loss = (float)(total / (double)a.P);
+  }
+}
+
+__global__ __launch_bounds__(kPfThreads) void k_pref_bwd(PfArgs a) {
+  const int64_t row = blockIdx.x / a.pieces, t0 = (int64_t)(blockIdx.x % a.pieces) * kPfPiece;
+  const float c = a.coef[row] * *a.g;
+  const int64_t t1 = t0 + kPfPiece < a.L ? t0 + kPfPiece : a.L;
+  for (int64_t t = t0 + threadIdx.x; t < t1; t += kPfThreads) a.dlp[row * a.L + t] = a.mask.on(row, t) ? c : 0.f;
+}
+
+}  // namespace asrn
+
+using namespace asrn;
+
+static int64_t pf_pieces(int64_t L) { return L > 0 ? (L + kPfPiece - 1) / kPfPiece : 1; }
+static bool pf_sizes(int64_t P, int64_t L) {
+  return P >= 1 && P < (int64_t(1) << 30) && L >= 0 && L < (int64_t(1) << 31) && 2 * P * pf_pieces(L) < (int64_t(1) << 31);
+}
+static int pf_check(int64_t P, int64_t L, const char* what) {
+  ASRN_REQUIRE(pf_sizes(P, L), "%s: bad sizes P=%lld L=%lld", what, (long long)P, (long long)L);
+  return 0;
+}
+
+extern "C" int64_t asrn_preference_workspace(int64_t P, int64_t L) {
+  if (!pf_sizes(P, L)) return -1;
+  return 2 * P * pf_pieces(L) * (int64_t)sizeof(PfPart);
+}
+
+extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const float* ref,
+                                   const int64_t* ref_strides, int32_t ref_rows, const uint8_t* mask,
+                                   const int64_t* mask_strides, int64_t P, int64_t L, int32_t kind, double beta,
+                                   double smoothing, double margin, int32_t mean, float* loss, float* rewards,
+                                   float* coef, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (pf_check(P, L, "asrn_preference_fwd")) return 1;
+  ASRN_REQUIRE(kind >= 0 && kind <= 2, "asrn_preference_fwd: kind=%d (0 sigmoid, 1 ipo, 2 hinge)", kind);
+  ASRN_REQUIRE(beta > 0.0 && beta < INFINITY && smoothing >= 0.0 && smoothing <= 1.0 && margin == margin,
+               "asrn_preference_fwd: beta=%g (positive) smoothing=%g (0 to 1) margin=%g", beta, smoothing, margin);
+  ASRN_REQUIRE((lp || L == 0) && lp_strides && loss && rewards && coef && (!ref || ref_strides) && (!mask || mask_strides),
+               "asrn_preference_fwd: null pointer");
+  const int64_t need = asrn_preference_workspace(P, L);
+  ASRN_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+               "asrn_preference_fwd: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  PfArgs a{};
+  a.lp = Strided{lp, lp_strides[0], lp_strides[1]};
+  if (ref) a.ref = Strided{ref, ref_strides[0], ref_rows ? 0 : ref_strides[1]};
+  if (mask) a.mask = Strided{mask, mask_strides[0], mask_strides[1]};
+  a.P = P; a.L = L; a.ref_rows = ref_rows; a.kind = kind; a.mean = mean;
+  a.beta = beta; a.smooth = smoothing; a.margin = margin;
+  a.part = (PfPart*)workspace; a.pieces = (uint32_t)pf_pieces(L);
+  a.loss = loss; a.reward = rewards; a.coef = coef;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(k_pref_rows, dim3((unsigned)(a.pieces * 2 * P)), dim3(kPfThreads), 0, st, a);
+  if (check_launch("asrn_preference_fwd")) return 1;
+  hipLaunchKernelGGL(k_pref_loss, dim3(1), dim3(kPfThreads), 0, st, a);
+  return check_launch("asrn_preference_fwd");
+}
+
+extern "C" int asrn_preference_bwd(const float* coef, const float* g, const uint8_t* mask, const int64_t* mask_strides,
+                                   int64_t P, int64_t L, float* dlp, void* stream) {
+  if (pf_check(P, L, "asrn_preference_bwd")) return 1;
+  if (L == 0) return 0;
+  ASRN_REQUIRE(coef && g && dlp && (!mask || mask_strides), "asrn_preference_bwd: null pointer");
+  PfArgs a{};
+  if (mask) a.mask = Strided{mask, mask_strides[0], mask_strides[1]};
+  a.P = P; a.L = L; a.coef = const_cast<float*>(coef); a.g = g; a.dlp = dlp;
+  a.pieces = (uint32_t)pf_pieces(L);
+  hipLaunchKernelGGL(k_pref_bwd, dim3((unsigned)(a.pieces * 2 * P)), dim3(kPfThreads), 0, (hipStream_t)stream, a);
+  return check_launch("asrn_preference_bwd");
+}

@@ -641,6 +641,58 @@ int asrn_gelu_norm_bwd(const float* x, const void* c, int32_t c_bf16, const floa
                        int64_t rows, int32_t d, const void* dy, int32_t dy_bf16, const float* dres, float* dx, void* dc,
                        float* dparams, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- fine-tuning: log-probabilities of given tokens -------------------------------------------------------------
+ * No counterpart in the reference (beside its loss, asrn/nucleo.py:1108). logits in fp32, bf16 or fp16 (type 0, 1, 2),
+ * row r of `rows` (< 2^31, a multiple of L) starting at element (r / L) stride_b + (r % L) stride_t, its V values
+ * adjacent; no alignment beyond the elements'. target (rows) int64. With z = (x - max x) inv_temperature:
+ * fwd: logp (rows) = z[target] - log sum exp z, entropy (rows, or null) = -sum p log p, both 0 where target ==
+ * ignore_index (the row is not read), logp NaN for a target outside [0, V); stats (rows, 2) for the backward.
+ * bwd: dlogits (rows, V) dense, in the logits' type = [g_logp (onehot - p) - g_entropy p (log p + H)]
+ * inv_temperature, 0 for ignored rows (rounded once); g_logp or g_entropy may be null, entropy is fwd's. */
+int asrn_token_logp_fwd(const void* logits, int32_t type, int64_t rows, int64_t L, int64_t V, int64_t stride_b,
+                        int64_t stride_t, const int64_t* target, int64_t ignore_index, float inv_temperature,
+                        float* logp, float* entropy, float* stats, void* stream);
+int asrn_token_logp_bwd(const void* logits, int32_t type, int64_t rows, int64_t L, int64_t V, int64_t stride_b,
+                        int64_t stride_t, const int64_t* target, int64_t ignore_index, float inv_temperature,
+                        const float* stats, const float* entropy, const float* g_logp, const float* g_entropy,
+                        void* dlogits, void* stream);
+
+/* ---- fine-tuning: the preference loss ------------------------------------------------------------------------------
+ * No counterpart in the reference. lp (2P, L): rows 0 .. P-1 the chosen texts, P .. 2P-1 the rejected ones; mask
+ * (2P, L) bytes or null; ref null, (2P, L), or (2P) sums with ref_rows. lp_strides, ref_strides, mask_strides: host
+ * arrays of the row and token strides in elements. R_i = the masked sum of lp - ref (mean: over the masked count, at
+ * least 1), h_i = beta (R_i - R_{P+i}) - margin; kind 0: -(1 - smoothing) log sigma(h) - smoothing log sigma(-h),
+ * 1: ((h - 1/2) / beta)^2, 2: max(0, 1 - h). *loss = the mean over the pairs, rewards (2P) = beta R, coef (2P) =
+ * d loss / d lp of a row's masked tokens. Sums in double, in a fixed order. bwd: dlp (2P, L) dense = *g coef, 0 where
+ * masked. workspace: asrn_preference_workspace(P, L) bytes, 16-byte aligned (-1: sizes refused). */
+int64_t asrn_preference_workspace(int64_t P, int64_t L);
+int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const float* ref, const int64_t* ref_strides,
+                        int32_t ref_rows, const uint8_t* mask, const int64_t* mask_strides, int64_t P, int64_t L,
+                        int32_t kind, double beta, double smoothing, double margin, int32_t mean, float* loss,
+                        float* rewards, float* coef, void* workspace, int64_t workspace_bytes, void* stream);
+int asrn_preference_bwd(const float* coef, const float* g, const uint8_t* mask, const int64_t* mask_strides, int64_t P,
+                        int64_t L, float* dlp, void* stream);
+
+/* ---- fine-tuning: the clipped policy loss --------------------------------------------------------------------------
+ * No counterpart in the reference. lp, advantage, old_lp, ref_lp, entropy (B, L) fp32 and mask (B, L) bytes, each
+ * read through two strides, strides (host) = theirs in that order, 12 values; old_lp (then r = 1), ref_lp, entropy and
+ * mask may be null. Per token, d = lp - old_lp, r = exp d, q = ref_lp - lp: -min(r A, clip(r, 1 - clip_low,
+ * 1 + clip_high) A), -cap A where A < 0 and r > cap (cap 0: none), + beta (exp q - 1 - q) - entropy_weight H.
+ * *loss = the mean over the masked tokens, or over the texts' means (by_text); stats (4) = means over the tokens of
+ * [clipped, r - 1 - d, exp q - 1 - q, H]; raw (B, L, or null) = each token's gradient with respect to lp, weight (B) =
+ * what a text's tokens are divided by. bwd: dlp (B, L) = *g raw / weight, dentropy (B, L) = -*g entropy_weight /
+ * weight (either null), 0 where masked. In double, fixed order. workspace: asrn_policy_workspace(B, L) bytes, 16-byte
+ * aligned (-1: sizes refused). */
+int64_t asrn_policy_workspace(int64_t B, int64_t L);
+int asrn_policy_fwd(const float* lp, const float* advantage, const float* old_lp, const float* ref_lp,
+                    const float* entropy, const uint8_t* mask, const int64_t* strides, int64_t B, int64_t L,
+                    double clip_low, double clip_high, double cap, double beta, double entropy_weight,
+                    int32_t by_text, float* raw, float* loss, float* stats, float* weight, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+int asrn_policy_bwd(const float* raw, const float* weight, const float* g, const uint8_t* mask,
+                    const int64_t* mask_strides, int64_t B, int64_t L, double entropy_weight, float* dlp,
+                    float* dentropy, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,72 @@
+"""The fine-tuning entry points' argument checks, which fail before any device work, and the public names."""
+import pytest
+import torch
+
+import asrn_amd
+from asrn_amd import _lib
+
+N = None
+
+
+@pytest.fixture(scope='module')
+def lib():
+    import os
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip('libasrn_hip.so not built (run `python -m asrn_amd.build`)')
+    return _lib.load()
+
+
+def _mal(lib, rc, texto):
+    assert rc != 0 and texto in lib.asrn_hip_last_error().decode(), lib.asrn_hip_last_error().decode()
+
+
+def test_token_logp_checks(lib):
+    f = lambda *a: lib.asrn_token_logp_fwd(N, *a, N, -100, 1.0, N, N, N, N)
+    _mal(lib, f(3, 4, 2, 10, 20, 10), 'type=3')
+    _mal(lib, f(0, 5, 2, 10, 20, 10), 'bad sizes')          # rows that are no multiple of L
+    _mal(lib, f(0, 4, 2, 0, 20, 10), 'bad sizes')
+    _mal(lib, f(0, 4, 2, 10, -20, 10), 'bad sizes')
+    _mal(lib, f(0, 1 << 31, 1, 10, 20, 10), 'bad sizes')
+    _mal(lib, f(0, 4, 2, 10, 20, 10), 'null pointer')
+    assert f(0, 0, 2, 10, 20, 10) == 0                      # no rows: no launch
+    _mal(lib, lib.asrn_token_logp_fwd(N, 0, 4, 2, 10, 20, 10, N, -100, 0.0, N, N, N, N), 'temperature')
+    _mal(lib, lib.asrn_token_logp_bwd(N, 1, 4, 2, 10, 20, 10, N, -100, 1.0, N, N, N, 16, N, N), 'entropy')
+    _mal(lib, lib.asrn_token_logp_bwd(N, 1, 4, 2, 10, 20, 10, N, -100, 1.0, N, N, 16, N, N, N), 'null pointer')
+
+
+def test_preference_checks(lib):
+    f = lambda P, L, kind, beta, e, margin, ws=0: lib.asrn_preference_fwd(16, 16, N, N, 0, N, N, P, L, kind, beta, e, margin, 0,
+                                                                          16, 16, 16, 16, ws, N)
+    _mal(lib, f(0, 5, 0, 0.1, 0.0, 0.0), 'bad sizes')
+    _mal(lib, f(1 << 30, 5, 0, 0.1, 0.0, 0.0), 'bad sizes')
+    _mal(lib, f(1, 5, 3, 0.1, 0.0, 0.0), 'kind=3')
+    _mal(lib, f(1, 5, 0, 0.0, 0.0, 0.0), 'beta')
+    _mal(lib, f(1, 5, 0, 0.1, 1.5, 0.0), 'smoothing')
+    _mal(lib, f(1, 5, 0, 0.1, 0.0, float('nan')), 'margin')
+    _mal(lib, f(2, 5000, 0, 0.1, 0.0, 0.0, 4 * 2 * 16 - 1), 'workspace')
+    assert lib.asrn_preference_workspace(2, 5000) == 4 * 2 * 16 and lib.asrn_preference_workspace(0, 5) == -1
+    _mal(lib, lib.asrn_preference_bwd(N, N, N, N, 1, 5, N, N), 'null pointer')
+    assert lib.asrn_preference_bwd(N, N, N, N, 1, 0, N, N) == 0
+
+
+def test_policy_checks(lib):
+    f = lambda B, L, lo, hi, cap, beta, w, ws=0: lib.asrn_policy_fwd(16, 16, N, N, N, N, 16, B, L, lo, hi, cap, beta, w, 0, 16, 16,
+                                                                     16, 16, 16, ws, N)
+    _mal(lib, f(0, 5, 0.2, 0.2, 0.0, 0.0, 0.0), 'bad sizes')
+    _mal(lib, f(1, 5, 1.2, 0.2, 0.0, 0.0, 0.0), 'clip_low')
+    _mal(lib, f(1, 5, 0.2, -0.2, 0.0, 0.0, 0.0), 'clip_high')
+    _mal(lib, f(1, 5, 0.2, 0.2, 0.5, 0.0, 0.0), 'cap')
+    _mal(lib, f(1, 5, 0.2, 0.2, 0.0, -1.0, 0.0), 'beta')
+    _mal(lib, f(1, 5, 0.2, 0.2, 0.0, 0.0, float('inf')), 'entropy_weight')
+    _mal(lib, f(3, 2049, 0.2, 0.2, 0.0, 0.0, 0.0, 3 * 2 * 48 - 1), 'workspace')
+    assert lib.asrn_policy_workspace(3, 2049) == 3 * 2 * 48 and lib.asrn_policy_workspace(1, -1) == -1
+    _mal(lib, lib.asrn_policy_bwd(N, N, N, N, N, 1, 5, 0.0, 16, N, N), 'null pointer')
+    assert lib.asrn_policy_bwd(N, N, N, N, N, 1, 5, 0.0, N, N, N) == 0
+
+
+def test_public_names_refuse_cpu_tensors():
+    lp = torch.zeros(2, 3)
+    for f in (lambda: asrn_amd.token_log_probs(torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.long)),
+              lambda: asrn_amd.preference_loss(lp), lambda: asrn_amd.policy_loss(lp, lp)):
+        with pytest.raises(RuntimeError, match='GPU only'):
+            f()
