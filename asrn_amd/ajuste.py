@@ -14,20 +14,29 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import call, ptr, query, stream_of
-from .ops import _c, _dev
+from ._lib import call, ptr, query
+from .ops import _dev
 
 TIPOS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # the kernels' logits
 FORMAS = ('sigmoide', 'ipo', 'bisagra')
 REDUCCIONES = ('fichas', 'textos')
 
 
+_corriente = torch._C._cuda_getCurrentRawStream       # the stream's handle without the Python object around it
+
+
 def _llamar(dev, nombre, *args):
     """call() on dev's current stream, with dev as the current device (a kernel launches on the current one)."""
-    if torch.cuda.current_device() == dev.index:
-        return call(nombre, *args, stream_of(dev))
-    with torch.cuda.device(dev):
-        return call(nombre, *args, stream_of(dev))
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        return call(nombre, *args, _corriente(i))
+    with torch.cuda.device(i):
+        return call(nombre, *args, _corriente(i))
+
+
+def _denso(g):
+    """An upstream gradient as contiguous fp32."""
+    return (g if g.dtype == torch.float32 else g.float()).contiguous()
 
 
 def _mismo_gpu(quien, dev, **tensores):
@@ -92,7 +101,8 @@ class LogProbabilidades(torch.autograd.Function):
         dev, V = logits.device, logits.shape[-1]
         filas, L, sb, st, x = _filas(logits)
         t = y.reshape(-1)
-        lp, stats = (torch.empty(s, dtype=torch.float32, device=dev) for s in (y.shape, (filas, 2)))
+        lp = torch.empty(y.shape, dtype=torch.float32, device=dev)
+        stats = torch.empty((filas, 2), dtype=torch.float32, device=dev)
         H = torch.empty(y.shape, dtype=torch.float32, device=dev) if entropia else None
         if filas:
             _llamar(dev, 'asrn_token_logp_fwd', ptr(x), TIPOS[x.dtype], filas, L, V, sb, st, ptr(t), ignorar, inv_t, ptr(lp),
@@ -109,7 +119,8 @@ class LogProbabilidades(torch.autograd.Function):
         filas, L, sb, st, ignorar, inv_t, forma = ctx.meta
         if g is None and gh is None:
             return None, None, None, None, None
-        g, gh = (None if v is None else _c(v, torch.float32) for v in (g, gh))
+        g = None if g is None else _denso(g)
+        gh = None if gh is None else _denso(gh)
         dx = torch.empty(forma, dtype=x.dtype, device=x.device)
         if filas:
             _llamar(x.device, 'asrn_token_logp_bwd', ptr(x), TIPOS[x.dtype], filas, L, forma[-1], sb, st, ptr(t), ignorar, inv_t,
@@ -150,16 +161,18 @@ class Preferencia(torch.autograd.Function):
     def forward(ctx, lp, m, ref, forma, beta, suavizado, margen, por_longitud):
         dev = lp.device
         P, L = lp.shape[0] // 2, lp.shape[1]
-        perdida, rec, coef = (torch.empty(s, dtype=torch.float32, device=dev) for s in ((), (2 * P,), (2 * P,)))
+        perdida = torch.empty((), dtype=torch.float32, device=dev)
+        rec = torch.empty((2 * P,), dtype=torch.float32, device=dev)
         wsb = query('asrn_preference_workspace', P, L)
-        ws = torch.empty((max(wsb, 1),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((max(wsb, 0) + 8 * P,), dtype=torch.uint8, device=dev)
+        coef = ws.data_ptr() + max(wsb, 0)           # the rows' coefficients, kept for the backward, behind the workspace
         por_fila = ref is not None and ref.dim() == 1
         ref_pasos = None if ref is None else (ctypes.c_int64 * 2)(ref.stride(0), 0) if por_fila else _pasos(ref)
         _llamar(dev, 'asrn_preference_fwd', ptr(lp), _pasos(lp), ptr(ref), ref_pasos, int(por_fila), ptr(m),
                 None if m is None else _pasos(m), P, L, FORMAS.index(forma), beta, suavizado, margen, int(por_longitud),
-                ptr(perdida), ptr(rec), ptr(coef), ptr(ws), wsb)
-        ctx.save_for_backward(coef, m)
-        ctx.meta = (P, L)
+                ptr(perdida), ptr(rec), coef, ptr(ws), wsb)
+        ctx.save_for_backward(ws, m)
+        ctx.meta = (P, L, max(wsb, 0))
         ctx.mark_non_differentiable(rec)
         ctx.set_materialize_grads(False)
         return perdida, rec
@@ -167,13 +180,14 @@ class Preferencia(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
-        coef, m = ctx.saved_tensors
-        P, L = ctx.meta
+        ws, m = ctx.saved_tensors
+        P, L, wsb = ctx.meta
         if g is None:
             return (None,) * 8
-        dlp = torch.empty((2 * P, L), dtype=torch.float32, device=coef.device)
-        gc = _c(g, torch.float32)
-        _llamar(coef.device, 'asrn_preference_bwd', ptr(coef), ptr(gc), ptr(m), None if m is None else _pasos(m), P, L, ptr(dlp))
+        dlp = torch.empty((2 * P, L), dtype=torch.float32, device=ws.device)
+        gc = _denso(g)
+        _llamar(ws.device, 'asrn_preference_bwd', ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), P, L,
+                ptr(dlp))
         return (dlp,) + (None,) * 7
 
 
@@ -222,14 +236,16 @@ class Politica(torch.autograd.Function):
     def forward(ctx, lp, H, A, vieja, ref, m, lo, hi, tope, beta, peso, por_texto):
         dev = lp.device
         B, L = lp.shape
-        perdida, datos, div = (torch.empty(s, dtype=torch.float32, device=dev) for s in ((), (4,), (B,)))
+        perdida = torch.empty((), dtype=torch.float32, device=dev)
+        datos = torch.empty((4,), dtype=torch.float32, device=dev)
         crudo = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
         wsb = query('asrn_policy_workspace', B, L)
-        ws = torch.empty((max(wsb, 1),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((max(wsb, 0) + 4 * B,), dtype=torch.uint8, device=dev)
+        div = ws.data_ptr() + max(wsb, 0)            # the texts' divisors, kept for the backward, behind the workspace
         _llamar(dev, 'asrn_policy_fwd', ptr(lp), ptr(A), ptr(vieja), ptr(ref), ptr(H), ptr(m), _pasos(lp, A, vieja, ref, H, m),
-                B, L, lo, hi, tope, beta, peso, int(por_texto), ptr(crudo), ptr(perdida), ptr(datos), ptr(div), ptr(ws), wsb)
-        ctx.save_for_backward(crudo, div, m)
-        ctx.meta = (B, L, peso)
+                B, L, lo, hi, tope, beta, peso, int(por_texto), ptr(crudo), ptr(perdida), ptr(datos), div, ptr(ws), wsb)
+        ctx.save_for_backward(crudo, ws, m)
+        ctx.meta = (B, L, peso, max(wsb, 0))
         ctx.mark_non_differentiable(datos)
         ctx.set_materialize_grads(False)
         return perdida, datos
@@ -237,15 +253,16 @@ class Politica(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
-        crudo, div, m = ctx.saved_tensors
-        B, L, peso = ctx.meta
+        crudo, ws, m = ctx.saved_tensors
+        B, L, peso, wsb = ctx.meta
         if g is None:
             return (None,) * 12
-        nueva = lambda i: (torch.empty((B, L), dtype=torch.float32, device=div.device) if ctx.needs_input_grad[i] else None)
-        dlp, dH = nueva(0), nueva(1)
-        gc = _c(g, torch.float32)
-        _llamar(div.device, 'asrn_policy_bwd', ptr(crudo), ptr(div), ptr(gc), ptr(m), None if m is None else _pasos(m), B, L, peso,
-                ptr(dlp), ptr(dH))
+        dev = ws.device
+        dlp = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        dH = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
+        gc = _denso(g)
+        _llamar(dev, 'asrn_policy_bwd', ptr(crudo), ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), B, L,
+                peso, ptr(dlp), ptr(dH))
         return (dlp, dH) + (None,) * 10
 
 

@@ -5,8 +5,8 @@
 //   d l / d lp = -r A where no clip holds, else 0, + beta (1 - exp q);   d l / d H = -w,
 // averaged over the masked tokens, or over the texts' own means (texts without tokens left out).
 // A token is clipped when d passes the border's logarithm: d in double is exact, so a value next to the border falls
-// where the definition puts it. exp q - 1 - q cancels for small q, where fp32 would keep no digit of it. All of it is
-// therefore formed in double, which costs nothing here: the kernels read 13 to 25 bytes a token and are bound by HBM.
+// where the definition puts it. exp q - 1 - q cancels for small q and is taken from its series there. The exponentials
+// are fp32's (in double they alone took 55 of 75 us at 3.2 M tokens), products and sums double.
 //
 //   k_pol_tokens  pieces of 2,048 tokens of a text, one workgroup each: the per-token gradient (not yet divided), and
 //                 the piece's count, loss, clipped tokens, KL to old (r - 1 - d) and to the reference, and entropy.
@@ -33,10 +33,35 @@ struct PoArgs {
   double lo, hi, log_lo, log_hi, cap, log_cap, beta, w_ent;     // cap 0: no second clip
   int32_t by_text;
   float* raw;                     // (B, L) gradient of each token's loss
-  PoPart* part; uint32_t pieces;
+  PoPart* part; uint32_t pieces; int lanes;
   float* loss; float* stats; float* weight;                     // weight (B): what a text's tokens are divided by
   const float* g; float* dlp; float* dent;
 };
+
+// exp d within two steps of fp32: expf of d rounded, and the rounding's own factor; past fp32's range in double
+__device__ __forceinline__ double po_exp(double d) {
+  const float f = (float)d;
+  if (f > 80.f) return exp(d);
+  const double e = expf(f), rest = d - (double)f;
+  return fabs(rest) < 1.0 ? e * (1.0 + rest) : e;        // -infinity and below fp32's range: expf's 0; NaN: NaN
+}
+// exp d - 1 - d to a few steps of fp32 at every d: its series up to |d| = 1/2, where the difference would cancel (the
+// first term left out, d^10 / 10!, is 2^-29 of the sum there), the difference past it
+__device__ __forceinline__ double po_kl(double d) {
+  const float f = (float)d;
+  if (fabsf(f) <= 0.5f) {
+    float p = 1.f / 362880.f;
+    p = fmaf(p, f, 1.f / 40320.f);
+    p = fmaf(p, f, 1.f / 5040.f);
+    p = fmaf(p, f, 1.f / 720.f);
+    p = fmaf(p, f, 1.f / 120.f);
+    p = fmaf(p, f, 1.f / 24.f);
+    p = fmaf(p, f, 1.f / 6.f);
+    p = fmaf(p, f, 0.5f);
+    return d * d * (double)p;
+  }
+  return (double)expm1f(f) - d;
+}
 
 __global__ __launch_bounds__(kPoThreads) void k_pol_tokens(PoArgs a) {
   __shared__ double red[kPoThreads / kWave][kPoSums];
@@ -62,18 +87,20 @@ __global__ __launch_bounds__(kPoThreads) void k_pol_tokens(PoArgs a) {
       if (t >= t1) break;
       double dl = 0.0;
       if (m[u]) {                             // what a mask hides may be infinite or NaN: nothing of it is used
-        const double A = adv[u], d = (double)lp[u] - (double)old[u], r = exp(d);
+        const double A = adv[u], d = (double)lp[u] - (double)old[u], r = po_exp(d);
         const bool cap = a.cap > 0.0 && A < 0.0 && d > a.log_cap;
         const bool out = (A > 0.0 && d > a.log_hi) || (A < 0.0 && d < a.log_lo);
         double l = cap ? -a.cap * A : out ? -(A > 0.0 ? a.hi : a.lo) * A : -r * A;
         dl = cap || out ? 0.0 : -r * A;
         s[0] += 1.0;
         s[2] += cap || out;
-        s[3] += expm1(d) - d;
+        s[3] += po_kl(d);
         if (a.ref.p) {
-          const double q = (double)ref[u] - (double)lp[u], e = expm1(q), kl = e - q;
-          l += a.beta * kl;
-          dl -= a.beta * e;
+          const double q = (double)ref[u] - (double)lp[u], kl = po_kl(q);
+          if (a.beta != 0.0) {
+            l += a.beta * kl;
+            dl -= a.beta * (double)expm1f((float)q);
+          }
           s[4] += kl;
         }
         if (a.ent.p) {
@@ -103,27 +130,25 @@ __global__ __launch_bounds__(kPoLossThreads) void k_pol_loss(PoArgs a) {
   __shared__ double total, texts;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   double s[kPoSums + 2] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};     // ..., the texts' means, texts with tokens
-  // a text of one piece takes a thread, of more a wave
-  const bool wide = a.pieces > 1;
-  for (int64_t b = wide ? wave : threadIdx.x; b < a.B; b += wide ? kPoLossThreads / kWave : kPoLossThreads) {
+  const int g = a.lanes, part = threadIdx.x & (g - 1);
+  // whole waves stay in the loop: a lane past the texts sums the last one again and keeps nothing
+  for (int64_t b0 = threadIdx.x / g; b0 - (threadIdx.x / g) < a.B; b0 += kPoLossThreads / g) {
+    const int64_t b = b0 < a.B ? b0 : a.B - 1;
     double r[kPoSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-    for (uint32_t p = wide ? lane : 0; p < a.pieces; p += kWave) {
+    for (uint32_t p = part; p < a.pieces; p += g) {
       const double* q = reinterpret_cast<const double*>(a.part + b * a.pieces + p);
 #pragma unroll
       for (int k = 0; k < kPoSums; ++k) r[k] += q[k];
     }
-    if (wide) {
 #pragma unroll
-      for (int k = 0; k < kPoSums; ++k) r[k] = wave_sum_d(r[k]);
-    }
-    if (!wide || lane == 0) {
-      const double n = r[0];
-      a.weight[b] = (float)(n > 0.0 ? n : 1.0);
+    for (int k = 0; k < kPoSums; ++k) r[k] = group_sum_d(r[k], g);
+    if (part != 0 || b0 >= a.B) continue;
+    const double n = r[0];
+    a.weight[b] = (float)(n > 0.0 ? n : 1.0);
 #pragma unroll
-      for (int k = 0; k < kPoSums; ++k) s[k] += r[k];
-      s[kPoSums] += n > 0.0 ? r[1] / n : 0.0;
-      s[kPoSums + 1] += n > 0.0 ? 1.0 : 0.0;
-    }
+    for (int k = 0; k < kPoSums; ++k) s[k] += r[k];
+    s[kPoSums] += n > 0.0 ? r[1] / n : 0.0;
+    s[kPoSums + 1] += n > 0.0 ? 1.0 : 0.0;
   }
 #pragma unroll
   for (int k = 0; k < kPoSums + 2; ++k) {
@@ -206,7 +231,7 @@ extern "C" int asrn_policy_fwd(const float* lp, const float* advantage, const fl
   a.log_lo = log1p(-clip_low); a.log_hi = log1p(clip_high);
   a.cap = cap; a.log_cap = cap > 0.0 ? log(cap) : 0.0;
   a.beta = beta; a.w_ent = entropy_weight; a.by_text = by_text;
-  a.raw = raw; a.part = (PoPart*)workspace; a.pieces = (uint32_t)po_pieces(L);
+  a.raw = raw; a.part = (PoPart*)workspace; a.pieces = (uint32_t)po_pieces(L); a.lanes = lanes_for(a.pieces);
   a.loss = loss; a.stats = stats; a.weight = weight;
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(k_pol_tokens, dim3((unsigned)(a.pieces * B)), dim3(kPoThreads), 0, st, a);

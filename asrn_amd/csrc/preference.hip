@@ -4,7 +4,7 @@
 //   sigmoid  -(1 - e) log sigma(h) - e log sigma(-h),   ipo  (h / beta - 1 / (2 beta))^2,   hinge  max(0, 1 - h),
 // averaged over the pairs. d loss / d lp_it = m_it c_i with one coefficient a row, formed in the forward.
 //
-//   k_pref_rows  a row in pieces of 4,096 tokens, one workgroup each: the masked sum and the count of a piece. Long rows
+//   k_pref_rows  a row in pieces of 2,048 tokens, one workgroup each: the masked sum and the count of a piece. Long rows
 //                and few rows alike spread over the chip; the sums are in double (a long text's log-probability is a
 //                small difference of large sums), each piece's in a fixed order.
 //   k_pref_loss  one workgroup, a pair a thread: the pieces added in order, the loss, the rewards and the coefficients.
@@ -18,8 +18,9 @@
 namespace asrn {
 
 constexpr int kPfThreads = 256;
-constexpr int kPfUnroll = 4;
-constexpr int kPfPiece = 4096;              // tokens a workgroup sums
+constexpr int kPfUnroll = 8;
+constexpr int kPfPiece = kPfUnroll * kPfThreads;       // tokens a workgroup sums, all loads in flight at once
+constexpr int kPfLossThreads = 1024;
 
 struct PfPart { double sum; double n; };
 
@@ -28,7 +29,7 @@ struct PfArgs {
   int64_t P, L;
   int32_t ref_rows, kind, mean;
   double beta, smooth, margin;
-  PfPart* part; uint32_t pieces;
+  PfPart* part; uint32_t pieces; int lanes;
   float* loss; float* reward; float* coef;
   const float* g; float* dlp;
 };
@@ -71,24 +72,31 @@ __global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
 // log(1 + exp(-|h|)) + max(-h, 0) = -log sigma(h)
 __device__ __forceinline__ double neg_log_sigma(double h) { return log1p(exp(-fabs(h))) + (h < 0.0 ? -h : h != h ? h : 0.0); }
 
-__global__ __launch_bounds__(kPfThreads) void k_pref_loss(PfArgs a) {
-  __shared__ double red[kPfThreads / kWave];
+__global__ __launch_bounds__(kPfLossThreads) void k_pref_loss(PfArgs a) {
+  __shared__ double red[kPfLossThreads / kWave];
   double total = 0.0;
-  for (int64_t i = threadIdx.x; i < a.P; i += kPfThreads) {
+  const int g = a.lanes, lane = threadIdx.x & (g - 1);
+  // whole waves stay in the loop: a lane past the pairs sums the last pair again and writes nothing
+  for (int64_t i0 = threadIdx.x / g; i0 - (threadIdx.x / g) < a.P; i0 += kPfLossThreads / g) {
+    const int64_t i = i0 < a.P ? i0 : a.P - 1;
     double R[2], div[2];
     for (int k = 0; k < 2; ++k) {
       const int64_t row = i + k * a.P;
       double s = 0.0, n = 0.0;
-      for (uint32_t p = 0; p < a.pieces; ++p) {
+      for (uint32_t p = lane; p < a.pieces; p += g) {
         const PfPart q = a.part[row * a.pieces + p];
         s += q.sum;
         n += q.n;
       }
+      s = group_sum_d(s, g);
+      n = group_sum_d(n, g);
       if (a.ref.p && a.ref_rows) s -= (double)a.ref.at(row, 0);
       div[k] = a.mean && n > 1.0 ? n : 1.0;     // an empty answer: a sum of nothing, divided by 1
       R[k] = s / div[k];
-      a.reward[row] = (float)(a.beta * R[k]);
     }
+    if (lane != 0 || i0 >= a.P) continue;
+    a.reward[i] = (float)(a.beta * R[0]);
+    a.reward[i + a.P] = (float)(a.beta * R[1]);
     const double h = a.beta * (R[0] - R[1]) - a.margin;
     double v, dh;
     if (a.kind == 0) {
@@ -111,7 +119,7 @@ __global__ __launch_bounds__(kPfThreads) void k_pref_loss(PfArgs a) {
   if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = total;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kPfThreads / kWave; ++w) total += red[w];
+    for (int w = 1; w < kPfLossThreads / kWave; ++w) total += red[w];
     *a.loss = (float)(total / (double)a.P);
   }
 }
@@ -161,12 +169,12 @@ extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, c
   if (mask) a.mask = Strided{mask, mask_strides[0], mask_strides[1]};
   a.P = P; a.L = L; a.ref_rows = ref_rows; a.kind = kind; a.mean = mean;
   a.beta = beta; a.smooth = smoothing; a.margin = margin;
-  a.part = (PfPart*)workspace; a.pieces = (uint32_t)pf_pieces(L);
+  a.part = (PfPart*)workspace; a.pieces = (uint32_t)pf_pieces(L); a.lanes = lanes_for(a.pieces);
   a.loss = loss; a.reward = rewards; a.coef = coef;
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(k_pref_rows, dim3((unsigned)(a.pieces * 2 * P)), dim3(kPfThreads), 0, st, a);
   if (check_launch("asrn_preference_fwd")) return 1;
-  hipLaunchKernelGGL(k_pref_loss, dim3(1), dim3(kPfThreads), 0, st, a);
+  hipLaunchKernelGGL(k_pref_loss, dim3(1), dim3(kPfLossThreads), 0, st, a);
   return check_launch("asrn_preference_fwd");
 }
 

@@ -15,9 +15,37 @@ struct Strided {
   }
 };
 
+// sums of doubles over the wave, in a fixed order: DPP rotations within each row of 16 lanes (no LDS), the rows by lane
+// reads
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t u = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double readlane_d(double v, int lane) {
+  const uint64_t u = __double_as_longlong(v);
+  return __longlong_as_double((long long)((uint64_t)(uint32_t)readlane_i((int)(uint32_t)(u >> 32), lane) << 32 |
+                                          (uint32_t)readlane_i((int)(uint32_t)u, lane)));
+}
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  v += dpp_d<0x128>(v);
+  v += dpp_d<0x124>(v);
+  v += dpp_d<0x122>(v);
+  v += dpp_d<0x121>(v);
+  return ((readlane_d(v, 0) + readlane_d(v, 16)) + readlane_d(v, 32)) + readlane_d(v, 48);
+}
+
+// lanes (a power of two up to a wave) that share a text's pieces in the reductions over them
+inline int lanes_for(int64_t pieces) {
+  int g = 1;
+  while (g < kWave && g < pieces) g *= 2;
+  return g;
+}
+// the sum over each aligned group of g lanes, in every lane of it
+__device__ __forceinline__ double group_sum_d(double v, int g) {
+  for (int m = g >> 1; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
   return v;
 }
 

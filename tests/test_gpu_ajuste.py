@@ -294,7 +294,18 @@ def politica_exacta(lp, A, vieja, m, lo, hi, tope, ref, beta, H, peso, reduccion
     media = lambda t: ((t * on).sum() / n.sum()).detach()
     est = torch.stack([media(fuera.double()), media(torch.expm1(d) - d), media(kl),
                        media(torch.zeros_like(vm) if h is None else torch.where(on > 0, h, 0.0))])
-    return loss.detach(), est, *torch.autograd.grad(loss, [v] + ([] if h is None else [h]))
+    peso_de = on / (n[:, None].clamp(min=1) * (n > 0).sum() if reduccion == 'textos' else n.sum())
+    q = torch.zeros_like(vm) if ref is None else torch.where(on > 0, ref.double(), 0.0) - vm
+    tam = [(t * peso_de).detach() for t in ((r * A).abs(), beta * torch.expm1(q).abs(), beta * kl)]
+    return (loss.detach(), est, *torch.autograd.grad(loss, [v] + ([] if h is None else [h]))), tam
+
+
+# The policy kernel's exponentials are fp32's, all else double. exp: expf within one step (2 U) and the factor of its
+# argument's rounding, 3 U; expm1: one step, and its argument rounded (U (1 + |q|) of the result for |q| < 4): 7 U; exp q -
+# 1 - q: its series' few roundings (4 U) up to |q| = 1/2, past it expm1's 2 U times expm1 / kl <= 4.4, 9 U, and the
+# argument's. So a token's loss is within 3 U r |A| + 12 U beta kl and its gradient within 3 U r |A| + 7 U beta |expm1 q|
+# (here with the divisor: tam), the statistics within 12 U of themselves, before the last roundings.
+EXP, EXPM1, KL = 3 * U, 7 * U, 12 * U
 
 
 @pytest.mark.parametrize('B,L', [(1, 1), (2, 50), (3, 2048), (3, 2049), (2, 7001), (700, 9)])
@@ -321,12 +332,13 @@ def test_policy(B, L, ventaja, tope, kl, entropia, vieja, reduccion):
                                              reduccion=reduccion, **args)
     hojas = [lp] + ([H] if entropia else [])
     ds = torch.autograd.grad(perdida, hojas, torch.tensor(-0.6, device=DEV))
-    e, ee, *ed = politica_exacta(lp, A, old if vieja else None, m, 0.2, 0.3, tope, ref, args['beta'], H, 0.02, reduccion)
+    (e, ee, *ed), tam = politica_exacta(lp, A, old if vieja else None, m, 0.2, 0.3, tope, ref, args['beta'], H, 0.02, reduccion)
     s = 2.0 ** -40
-    assert abs(perdida.double() - e) <= U * e.abs() + s and ((est.double() - ee).abs() <= U * ee.abs() + s).all()
+    assert abs(perdida.double() - e) <= U * e.abs() + EXP * tam[0].sum() + KL * tam[2].sum() + s
+    assert ((est.double() - ee).abs() <= (U + KL) * ee.abs() + s).all()
     # a token's gradient: rounded once, divided by its divisor (rounded twice more), times the loss's gradient
-    for a, b in zip(ds, ed):
-        assert ((a.double() + 0.6 * b).abs() <= 6 * U * b.abs() + s / L).all()
+    for a, b, t in zip(ds, ed, (EXP * tam[0] + EXPM1 * tam[1], 0.0)):
+        assert ((a.double() + 0.6 * b).abs() <= 6 * U * b.abs() + t + s / L).all()
 
 
 def test_policy_borders():
@@ -340,6 +352,13 @@ def test_policy_borders():
     d, = torch.autograd.grad(perdida, lp)
     fuera = lp.detach().double() > alto
     assert ((d == 0) == fuera).all() and abs(est[0].item() - fuera.double().mean().item()) <= 1e-7
+    # far apart: r past fp32's range under an advantage of 0, ratios at the ends of the type, a wide KL
+    lp = torch.tensor([[95.0, -3e38, -30.0, 1.0]], device=DEV, requires_grad=True)
+    old = torch.tensor([[0.0, 3e38, 30.0, 1.0]], device=DEV)
+    perdida, est = asrn_amd.perdida_politica(lp, torch.tensor([[0.0, 1.0, 1.0, 2.0]], device=DEV), old,
+                                             lp_ref=torch.zeros(1, 4, device=DEV))
+    d, = torch.autograd.grad(perdida, lp)
+    assert abs(perdida.item() + 0.5) <= 1e-7 and torch.allclose(d, torch.tensor([[0.0, 0.0, 0.0, -0.5]], device=DEV), atol=1e-20)
     lp = torch.tensor([[0.0, -math.inf, 200.0, -3.0]], device=DEV, requires_grad=True)
     A = torch.tensor([[0.0, 1.0, 1.0, -1.0]], device=DEV)
     perdida, _ = asrn_amd.perdida_politica(lp, A, torch.zeros(1, 4, device=DEV))
@@ -357,9 +376,10 @@ def test_policy_strides_and_masks():
     for m in (None, (torch.rand(B, L, generator=g, device=DEV) < 0.4).half(), torch.ones(B, 1, device=DEV).expand(B, L)):
         perdida, est = asrn_amd.perdida_politica(lp, A, old, m)
         d, = torch.autograd.grad(perdida, lp)
-        e, ee, ed = politica_exacta(lp, A.float(), old, m, 0.2, 0.2, None, None, 0.0, None, 0.0, 'fichas')
-        assert abs(perdida.double() - e) <= U * e.abs() + 2.0 ** -40 and ((est.double() - ee).abs() <= U * ee.abs() + 2.0 ** -40).all()
-        assert ((d.double() - ed).abs() <= 6 * U * ed.abs()).all()
+        (e, ee, ed), tam = politica_exacta(lp, A.float(), old, m, 0.2, 0.2, None, None, 0.0, None, 0.0, 'fichas')
+        assert abs(perdida.double() - e) <= U * e.abs() + EXP * tam[0].sum() + 2.0 ** -40
+        assert ((est.double() - ee).abs() <= (U + KL) * ee.abs() + 2.0 ** -40).all()
+        assert ((d.double() - ed).abs() <= 6 * U * ed.abs() + EXP * tam[0]).all()
 
 
 def test_policy_without_tokens_and_one_gradient():
@@ -445,12 +465,15 @@ def test_graph_replays():
 def test_side_stream():
     x = torch.randn(3, 17, 500, device=DEV).requires_grad_()
     y = torch.randint(0, 500, (3, 17), device=DEV)
-    lp = asrn_amd.log_probabilidades(x, y)
-    base, = torch.autograd.grad(lp.sum(), x)
+
+    def paso():
+        lp = asrn_amd.log_probabilidades(x, y)
+        return lp.detach(), torch.autograd.grad(lp.sum(), x)[0]
+
+    base = paso()
     lado = torch.cuda.Stream()
     lado.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(lado):
-        lp2 = asrn_amd.log_probabilidades(x, y)
-        otra, = torch.autograd.grad(lp2.sum(), x)
+        otra = paso()
     torch.cuda.current_stream().wait_stream(lado)
-    assert torch.equal(lp, lp2) and torch.equal(base, otra)
+    assert all(torch.equal(a, b) for a, b in zip(base, otra))
