@@ -126,6 +126,14 @@ SIGNATURES = {
     'asrn_policy_workspace': (_I64, [_I64, _I64]),
     'asrn_policy_fwd': (ctypes.c_int, [_P] * 7 + [_I64, _I64] + [_F64] * 5 + [_I32] + [_P] * 5 + [_I64, _P]),
     'asrn_policy_bwd': (ctypes.c_int, [_P] * 5 + [_I64, _I64, _F64, _P, _P, _P]),
+    'asrn_pack8': (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _P, _P]),
+    'asrn_unpack8': (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _I32, _P, _P]),
+    'asrn_gelu8_fwd': (ctypes.c_int, [_P, _I32, _P, _I64, _I64, _P, _P, _P, _P]),
+    'asrn_gelu8_bwd': (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I64, _I32, _P, _P]),
+    'asrn_norm8_fwd': (ctypes.c_int, [_P, _P, _P, _I64, _I32, _F32, _I32, _P, _P, _P, _P, _P]),
+    'asrn_norm8_bwd_workspace': (_I64, [_I64, _I32]),
+    'asrn_norm8_bwd': (ctypes.c_int, [_P] * 4 + [_I64, _I32, _P, _I32, _P, _P, _P, _P, _I64, _P]),
+    'asrn_norm8_read': (ctypes.c_int, [_P] * 5 + [_I64, _I64, _I32, _I32, _I32, _P, _P]),
 }
 
 _lib = None

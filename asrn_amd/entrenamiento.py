@@ -110,8 +110,8 @@ class PasoGrafado:
 
     The first `calentar` calls are ordinary steps, run on a side stream (they build AdamW's state and the layers'
     workspaces); the next call captures one step and every later call replays it. A step with a non-finite loss or
-    gradient norm changes nothing (the fused AdamW's found_inf), salto = 1. bf16 or fp32; no checkpointing, no
-    torch.compile, no accumulation. grabar=False runs every step eagerly (the same arithmetic; also on the CPU)."""
+    gradient norm changes nothing (the fused AdamW's found_inf), salto = 1. bf16 or fp32; no recomputation (checkpoint
+    'no' or 'ocho'), no torch.compile, no accumulation. grabar=False runs every step eagerly (the same arithmetic; also on the CPU)."""
 
     def __init__(self, modelo, optimizador, lote, largo, precision='bf16', recorte=1.0, calentar=3, grabar=None):
         base = _base(modelo)
@@ -121,8 +121,8 @@ class PasoGrafado:
             raise ValueError('PasoGrafado: a graph needs the model on the GPU (or grabar=False)')
         if precision == 'fp16':
             raise ValueError("PasoGrafado: fp16 needs a gradient scaler; use 'bf16' or 'fp32'")
-        if modelo is not base or getattr(base, 'checkpoint', 'no') != 'no':
-            raise ValueError('PasoGrafado: no checkpointing and no torch.compile')
+        if modelo is not base or getattr(base, 'checkpoint', 'no') not in ('no', 'ocho'):
+            raise ValueError('PasoGrafado: no checkpointing that recomputes and no torch.compile')
         if grabar and not all(g.get('capturable') and g.get('fused') for g in optimizador.param_groups):
             raise ValueError('PasoGrafado: the optimizer must be crear_optimizador(..., capturable=True) on the GPU')
         self.modelo, self.opt, self.precision, self.disp, self.grabar = base, optimizador, precision, disp, grabar

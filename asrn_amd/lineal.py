@@ -173,21 +173,47 @@ def column_sums(g2):
     return g2.sum(0, dtype=_acc_dtype(g2))
 
 
+def _producto(xc, wc, bc, propio):
+    """F.linear(xc, wc, bc), on asrn_gemm where that is faster."""
+    # rows flattened (which may copy) only for products that asrn_gemm takes by their size
+    x2 = None
+    if propio and xc.is_cuda and xc.dtype == torch.float32 and xc.numel() * wc.shape[0] >= MIN_PRODUCTO:
+        x2 = _rows(xc)
+    if x2 is not None and gemm_ok(x2, wc, True, bc):
+        return gemm(x2, False, wc, True, sesgo=bc).view(*xc.shape[:-1], wc.shape[0])
+    with torch.autocast(device_type=xc.device.type, enabled=False):
+        return F.linear(xc, wc, bc)
+
+
+def _gradientes(g, wc, leer, tipos, quiere):
+    """The gradients of a product's x, w and b (None where `quiere` is false) from its output's; leer() gives x's rows."""
+    xdt, wdt, bdt = tipos
+    gx = gw = gb = None
+    with torch.autocast(device_type=g.device.type, enabled=False):
+        g = g.to(wc.dtype)
+        g2 = _rows(g)
+        if quiere[0]:
+            if gemm_ok(g2, wc, False):
+                gx = gemm(g2, False, wc, False).view(*g.shape[:-1], wc.shape[1]).to(xdt)
+            else:
+                gx = g.matmul(wc).to(xdt)
+        con_sesgo = bdt is not None and quiere[2]
+        if quiere[1]:
+            gw = weight_grad(g2, leer(), con_sesgo)
+            if con_sesgo:
+                gw, gb = gw[0], gw[1].to(bdt)
+            gw = gw.to(wdt)
+        elif con_sesgo:
+            gb = column_sums(g2).to(bdt)
+    return gx, gw, gb
+
+
 class _Lineal(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, dt, propio):
         xc, wc = x.to(dt), w.to(dt)
-        bc = b.to(dt) if b is not None else None
-        # rows flattened (which may copy) only for products that asrn_gemm takes by their size
-        x2 = None
-        if propio and xc.is_cuda and xc.dtype == torch.float32 and xc.numel() * wc.shape[0] >= MIN_PRODUCTO:
-            x2 = _rows(xc)
-        if x2 is not None and gemm_ok(x2, wc, True, bc):
-            y = gemm(x2, False, wc, True, sesgo=bc).view(*x.shape[:-1], wc.shape[0])
-        else:
-            with torch.autocast(device_type=x.device.type, enabled=False):
-                y = F.linear(xc, wc, bc)
+        y = _producto(xc, wc, b.to(dt) if b is not None else None, propio)
         ctx.save_for_backward(xc, wc)
         ctx.meta = (x.dtype, w.dtype, None if b is None else b.dtype)
         return y
@@ -195,25 +221,25 @@ class _Lineal(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         xc, wc = ctx.saved_tensors
-        xdt, wdt, bdt = ctx.meta
-        gx = gw = gb = None
-        with torch.autocast(device_type=g.device.type, enabled=False):
-            g = g.to(wc.dtype)
-            g2 = _rows(g)
-            if ctx.needs_input_grad[0]:
-                if gemm_ok(g2, wc, False):
-                    gx = gemm(g2, False, wc, False).view(*g.shape[:-1], wc.shape[1]).to(xdt)
-                else:
-                    gx = g.matmul(wc).to(xdt)
-            con_sesgo = bdt is not None and ctx.needs_input_grad[2]
-            if ctx.needs_input_grad[1]:
-                gw = weight_grad(g2, _rows(xc), con_sesgo)
-                if con_sesgo:
-                    gw, gb = gw[0], gw[1].to(bdt)
-                gw = gw.to(wdt)
-            elif con_sesgo:
-                gb = column_sums(g2).to(bdt)
-        return gx, gw, gb, None, None
+        return (*_gradientes(g, wc, lambda: _rows(xc), ctx.meta, ctx.needs_input_grad), None, None)
+
+
+class _Lineal8(torch.autograd.Function):
+    """_Lineal whose weight gradient reads x back from the 8 bits that the op before it keeps (ops.Guardado8)."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, dt, leer, *guardados):
+        wc = w.to(dt)
+        y = _producto(x.to(dt), wc, b.to(dt) if b is not None else None, True)
+        ctx.save_for_backward(wc, *guardados)
+        ctx.meta = ((x.dtype, w.dtype, None if b is None else b.dtype), leer, dt, len(guardados))
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        wc, *guardados = ctx.saved_tensors
+        tipos, leer, dt, n = ctx.meta
+        return (*_gradientes(g, wc, lambda: leer(guardados, dt), tipos, ctx.needs_input_grad), *(None,) * (2 + n))
 
 
 def lineal(x, w, b=None, propio=True):
@@ -222,3 +248,13 @@ def lineal(x, w, b=None, propio=True):
     dev = x.device.type
     dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else x.dtype
     return _Lineal.apply(x, w, b, dt, propio)
+
+
+def lineal8(x, w, b, guardado):
+    """lineal(x, w, b) that does not keep x: the weight gradient reads it back through `guardado`, what ops.norma8,
+    ops.ventana8 or ops.gelu8 returned with x (None: lineal itself). The product and x's gradient are lineal's."""
+    if guardado is None or not torch.is_grad_enabled():
+        return lineal(x, w, b)
+    dev = x.device.type
+    dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else x.dtype
+    return _Lineal8.apply(x, w, b, dt, guardado.leer, *guardado.tensores)

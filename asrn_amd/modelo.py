@@ -16,14 +16,14 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .capa import CapaASRNEstable, ngramas
-from . import ops
+from . import ajuste, ops
 from .ops import escaneo
-from .lineal import lineal
+from .lineal import lineal, lineal8
 
 MEZCLAS = ('conv', 'memoria')
 OPCIONES_CAPA = ('n_tablas', 'n_bits', 'afin_oculto', 'chunk', 'tablas_contexto', 'confirmar', 'sufijo', 'vistos',
                  'nodos_racha', 'racha_max')
-MODOS_CHECKPOINT = ('no', 'asrn', 'todo')
+MODOS_CHECKPOINT = ('no', 'asrn', 'todo', 'ocho')
 # Embedding values (B L d) up to which a model's training step keeps its ASRN layers on one stream. A captured step
 # without branches replays with its launches back to back, one with a branch pays for them one by one, and below this
 # the launches cost more than the layers' two branches gain by running side by side (us a step, two streams / one: 512
@@ -33,10 +33,10 @@ MODOS_CHECKPOINT = ('no', 'asrn', 'todo')
 UNA_CORRIENTE = 1 << 20
 
 
-def _entiende_una(capa):
-    """Whether a call of the layer reaches CapaASRNEstable.forward itself: a wrapper or a replaced forward in its place
-    takes forward's other arguments, not the models' own una_corriente."""
-    return type(capa).forward is CapaASRNEstable.forward and 'forward' not in vars(capa)
+def _propio(m, clase):
+    """Whether a call of the module reaches clase.forward itself: a wrapper or a replaced forward in its place takes
+    forward's other arguments, not the models' own (una_corriente, ocho)."""
+    return type(m).forward is clase.forward and 'forward' not in vars(m)
 
 
 def _base(modelo):
@@ -45,11 +45,12 @@ def _base(modelo):
 
 
 def modo_checkpoint(valor):
-    """Recomputation mode of ModeloASRN (asrn/nucleo.py:1017-1022): False and None mean 'no', True means 'asrn'."""
+    """Memory mode of ModeloASRN's backward (asrn/nucleo.py:1017-1022): False and None mean 'no', True means 'asrn'; 'ocho'
+    is this package's own."""
     if not isinstance(valor, str):
         valor = 'asrn' if valor is True else 'no' if valor in (False, None) else valor
     if valor not in MODOS_CHECKPOINT:
-        raise ValueError(f"checkpoint: one of 'no', 'asrn', 'todo' (got {valor!r})")
+        raise ValueError(f"checkpoint: one of 'no', 'asrn', 'todo', 'ocho' (got {valor!r})")
     return valor
 
 
@@ -123,7 +124,11 @@ class BloqueLocal(nn.Module):
         m = escaneo(f.transpose(1, 2).contiguous(), ((1 - f) * u).transpose(1, 2).contiguous())
         return self.mem_o(m.transpose(1, 2).to(z.dtype))
 
-    def forward(self, h):
+    def forward(self, h, ocho=False):
+        """ocho: what the backward needs is kept in 8 bits (_en_ocho) where the block's products run in fp32 or bf16 on
+        the GPU; the output is the same."""
+        if ocho and h.is_cuda and h.dtype == torch.float32 and _dtype_producto(h) in (torch.float32, torch.bfloat16):
+            return self._en_ocho(h)
         # the LayerNorms run fused (ops.norma_residual): ln2's output comes out in the feed-forward's dtype, and the
         # residual path's gradient joins each LayerNorm's backward
         z, h = ops.norma_residual(self.ln1, h, torch.float32)
@@ -140,6 +145,34 @@ class BloqueLocal(nn.Module):
         h = h + self.drop(c)
         y, h = ops.norma_residual(self.ln2, h, _dtype_producto(h))
         return h + self.drop(self._ff(y))
+
+    def _en_ocho(self, h):
+        """forward with the inputs of the LayerNorms and the GELUs kept in 8 bits (ops.norma8, ops.gelu8) and the products'
+        inputs formed again from them (lineal8): a 'conv' block in bf16 keeps 5 d bytes a token and their scales in place
+        of 28 d. A 'memoria' block's mix keeps what it keeps otherwise, save the LayerNorm's and the GELU's inputs."""
+        dt = _dtype_producto(h)
+        z, h, g1 = ops.norma8(self.ln1, h, torch.float32)
+        if self.mezcla == 'conv' and 1 <= self.k <= 16:
+            cols, gc = ops.ventana8(z, self.k, dt, g1)
+            c = lineal8(cols, self.conv.weight.reshape(self.conv.weight.shape[0], -1), self.conv.bias, gc)
+        else:
+            c = (conv_causal if self.mezcla == 'conv' else conv_canal_causal)(z, self.conv.weight, self.conv.bias)
+        if self.mezcla == 'conv' and self._sin_drop():
+            h = ops.suma_gelu8(h, c)
+        else:
+            c = ops.gelu8(c)[0]
+            if self.mezcla == 'memoria':
+                c = c + self._memoria(z)
+            h = h + self.drop(c)
+        y, h, g2 = ops.norma8(self.ln2, h, dt)
+        f0, act, f2 = self.ff
+        u = lineal8(y, f0.weight, f0.bias, g2)
+        # an activation put in the GELU's place, or a GELU with hooks or the tanh form, runs as it is
+        if type(act) is nn.GELU and act.approximate == 'none' and ops.sin_ganchos(act):
+            y, gu = ops.gelu8(u)
+        else:
+            y, gu = act(u), None
+        return h + self.drop(lineal8(y, f2.weight, f2.bias, gu))
 
     def _sin_drop(self):
         """Whether self.drop leaves everything as it is and its calls may be left out: a plain nn.Dropout (a module put
@@ -176,7 +209,9 @@ def revisar_precision(modelo):
 class ModeloASRN(nn.Module):
     """Token ids -> n_capas local blocks, with an ASRN layer after block i when i % largo_cada == 0 and i is not the
     last block -> logits through the head, which is the embedding matrix (asrn/nucleo.py:1047-1125). No position table.
-    checkpoint: 'asrn' recomputes the ASRN layers in the backward, 'todo' the local blocks too. protecciones: the ASRN
+    checkpoint: 'asrn' recomputes the ASRN layers in the backward, 'todo' the local blocks too; 'ocho' recomputes nothing
+    and keeps the local blocks' activations in 8 bits (the same outputs; the gradients are those at the 8-bit values).
+    protecciones: the ASRN
     layers' Protecciones (group A by default); the remaining keywords are CapaASRNEstable's."""
 
     def __init__(self, V, d=64, n_capas=2, largo_cada=2, ff=None, k=4, init_profundo=None, checkpoint=False,
@@ -230,17 +265,19 @@ class ModeloASRN(nn.Module):
         E = ops.incrustar(self.emb, x)
         recalcular = self.training and torch.is_grad_enabled()
         ck_bloque = recalcular and self.checkpoint == 'todo'
-        ck_capa = recalcular and self.checkpoint != 'no'
+        ck_capa = recalcular and self.checkpoint in ('asrn', 'todo')
+        ocho = recalcular and self.checkpoint == 'ocho'
         # the n-gram sort depends on the token ids only: one for every ASRN layer
         ng = ngramas(x, self.largos[0]) if len(self.largos) and x.is_cuda else None
         una = recalcular and self._una_corriente(E, x)
         capas = iter(self.largos)
         h = E
         for i, bloque in enumerate(self.bloques):
-            h = torch.utils.checkpoint.checkpoint(bloque, h, use_reentrant=False) if ck_bloque else bloque(h)
+            en_ocho = {'ocho': True} if ocho and _propio(bloque, BloqueLocal) else {}
+            h = torch.utils.checkpoint.checkpoint(bloque, h, use_reentrant=False) if ck_bloque else bloque(h, **en_ocho)
             if i in self.pos_largo:
                 capa = next(capas)
-                extra = {'una_corriente': True} if una and _entiende_una(capa) else {}
+                extra = {'una_corriente': True} if una and _propio(capa, CapaASRNEstable) else {}
                 if ck_capa:
                     h = torch.utils.checkpoint.checkpoint(capa, E, h, x, use_reentrant=False, ngramas=ng, **extra)
                 else:
@@ -256,6 +293,11 @@ class ModeloASRN(nn.Module):
         """Mean fp32 cross-entropy of predicting y from x, both (B, L) (asrn/nucleo.py:1122-1125)."""
         logits = self(x)
         return ops.cross_entropy(logits, y, ignore_index=ignorar)
+
+    def log_probabilidades(self, x, y, ignorar=-100, temperatura=1.0, entropia=False):
+        """The log-probabilities of y under the model's logits for x, both (B, L), for the preference and policy losses
+        (ajuste.log_probabilidades)."""
+        return ajuste.log_probabilidades(self(x), y, ignorar, temperatura, entropia)
 
     def num_parametros(self):
         return sum(p.numel() for p in self.parameters())

@@ -10,10 +10,11 @@ import math
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr, query, stream_of
-from .lineal import column_sums, gemm, weight_grad
+from .lineal import column_sums, gemm, lineal8, weight_grad
 
 I32 = torch.int32
 
@@ -1585,3 +1586,211 @@ def norma_residual(ln, x, dtype):
         return NormaResidual.apply(x, ln.weight, ln.bias, ln.eps, dtype)
     y = ln(x)
     return (y if y.dtype == dtype else y.to(dtype)), x
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# activations in 8 bits for the backward pass
+# ---------------------------------------------------------------------------------------------------------------------
+
+GRUPO8 = 32                   # neighbouring channels that share a scale
+
+
+class Guardado8:
+    """What norma8, ventana8 or gelu8 keep of their input, for lineal8: leer(tensores, dtype) gives the rows of their
+    output (N, d), formed again from the 8 bits."""
+
+    def __init__(self, leer, tensores):
+        self.leer, self.tensores = leer, tuple(tensores)
+
+
+def _sitio8(x2):
+    """The codes (N, d) int8 and the groups' scale bytes for rows x2 (N, d)."""
+    N, d = x2.shape
+    return (torch.empty((N, d), dtype=torch.int8, device=x2.device),
+            torch.empty((N, -(-d // GRUPO8)), dtype=torch.uint8, device=x2.device))
+
+
+def guardar8(x):
+    """x (..., d) fp32 or bf16 in 8 bits: (codes int8 (N, d), scale bytes uint8 (N, ceil(d / 32))). Per 32 neighbouring
+    channels the smallest 2^e with max |x| <= 127 2^e (-126 <= e <= 121; the byte is e + 127) and the integers nearest to
+    x 2^-e; byte 255 for a group that holds an infinity, a NaN or a value past 127 2^121: it reads back as NaN (leer8)."""
+    dev = _dev(x)
+    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f'guardar8: {tuple(x.shape)} of {x.dtype}: (..., d) fp32 or bf16 is needed')
+    x2 = x.detach().contiguous().view(-1, x.shape[-1]) if x.numel() else x.detach().reshape(0, x.shape[-1])
+    q, e = _sitio8(x2)
+    call('asrn_pack8', ptr(x2), int(x2.dtype == torch.bfloat16), *x2.shape, ptr(q), ptr(e), stream_of(dev))
+    return q, e
+
+
+def leer8(q, e, dtype=torch.float32, gelu=False):
+    """The values that guardar8's codes and scales stand for (gelu: their GELU), (N, d) fp32 or bf16. The values fit bf16
+    exactly."""
+    dev = _dev(q, e)
+    if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() != 2 or e.device != dev or \
+            tuple(e.shape) != (q.shape[0], -(-q.shape[1] // GRUPO8)) or dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f'leer8: codes {tuple(q.shape)} of {q.dtype} with scales {tuple(e.shape)} of {e.dtype} to {dtype}')
+    q, e = q.contiguous(), e.contiguous()
+    out = torch.empty(q.shape, dtype=dtype, device=dev)
+    call('asrn_unpack8', ptr(q), ptr(e), *q.shape, int(gelu), int(dtype == torch.bfloat16), ptr(out), stream_of(dev))
+    return out
+
+
+class Gelu8(torch.autograd.Function):
+    """asrn_gelu8_fwd/bwd: gelu(u), or h + gelu(u) (h fp32; gelu rounds to u's dtype first, as the separate ops do), with
+    u kept in 8 bits for the backward; returns also the codes and scales."""
+
+    @staticmethod
+    def forward(ctx, u, h):
+        dev, d = u.device, u.shape[-1]
+        u2 = u.contiguous().view(-1, d)
+        q, e = _sitio8(u2)
+        bf16 = u.dtype == torch.bfloat16
+        h2 = None if h is None else h.contiguous()
+        out = torch.empty(u.shape, dtype=u.dtype if h is None else torch.float32, device=dev)
+        call('asrn_gelu8_fwd', ptr(u2), int(bf16), ptr(h2), *u2.shape, ptr(out), ptr(q), ptr(e), stream_of(dev))
+        ctx.save_for_backward(q, e)
+        ctx.meta = (bf16, u.shape)
+        ctx.mark_non_differentiable(q, e)
+        ctx.set_materialize_grads(False)
+        return out, q, e
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _, __):
+        q, e = ctx.saved_tensors
+        bf16, forma = ctx.meta
+        if g is None:
+            return None, None
+        gu = None
+        if ctx.needs_input_grad[0]:
+            gc = _c(g, g.dtype if g.dtype == torch.bfloat16 else torch.float32)
+            gu = torch.empty(forma, dtype=torch.bfloat16 if bf16 else torch.float32, device=q.device)
+            call('asrn_gelu8_bwd', ptr(q), ptr(e), ptr(gc), int(gc.dtype == torch.bfloat16), *q.shape, int(bf16), ptr(gu),
+                 stream_of(q.device))
+        return gu, g if ctx.needs_input_grad[1] else None
+
+
+def _gelu8_ok(u):
+    return u.is_cuda and u.dtype in (torch.float32, torch.bfloat16) and u.dim() >= 1 and u.numel() > 0 and torch.is_grad_enabled()
+
+
+def _leer_gelu8(ts, dtype):
+    return leer8(*ts, dtype, gelu=True)
+
+
+def gelu8(u):
+    """(F.gelu(u), what lineal8 reads it back from): u fp32 or bf16 is kept in 8 bits (guardar8's format) instead of as it
+    is, so its gradient is gelu' of the 8-bit values times the output's. Without gradients, off the GPU or in another
+    dtype: (F.gelu(u), None)."""
+    if not _gelu8_ok(u):
+        return F.gelu(u), None
+    y, q, e = Gelu8.apply(u, None)
+    return y, Guardado8(_leer_gelu8, (q, e))
+
+
+def suma_gelu8(h, u):
+    """h + F.gelu(u) with u kept in 8 bits: h fp32 of u's shape; else the separate ops, gelu8 among them."""
+    if _gelu8_ok(u) and h.dtype == torch.float32 and h.shape == u.shape and h.device == u.device:
+        return Gelu8.apply(u, h)[0]
+    return h + gelu8(u)[0]
+
+
+class Norma8(torch.autograd.Function):
+    """NormaResidual that keeps x in 8 bits (and (mean, rstd) per row, of x itself): asrn_norm8_fwd/bwd where d is a
+    multiple of 4 up to 1024, else the same with torch's LayerNorm and asrn_pack8. Returns also what was kept."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, dtype):
+        dev = _dev(x)
+        d, lead = x.shape[-1], x.shape[:-1]
+        x2 = x.contiguous().view(-1, d)
+        g, b = _c(gamma, torch.float32), _c(beta, torch.float32)
+        q, e = _sitio8(x2)
+        propio = _norma8_propia(d) and x2.data_ptr() % 16 == 0
+        if propio:
+            y = torch.empty((x2.shape[0], d), dtype=dtype, device=dev)
+            stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=dev)
+            call('asrn_norm8_fwd', ptr(x2), ptr(g), ptr(b), *x2.shape, float(eps), int(dtype == torch.bfloat16), ptr(y),
+                 ptr(stats), ptr(q), ptr(e), stream_of(dev))
+        else:
+            y, mu, rstd = torch.native_layer_norm(x2, (d,), g, b, eps)
+            y, stats = y.to(dtype), torch.cat([mu, rstd], 1)
+            call('asrn_pack8', ptr(x2), 0, *x2.shape, ptr(q), ptr(e), stream_of(dev))
+        ctx.save_for_backward(q, e, stats, g)
+        ctx.meta = (lead, gamma.shape, beta.shape)
+        ctx.mark_non_differentiable(q, e, stats)
+        return y.view(*lead, d), x2.view(*lead, d), q, e, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dres, *_):
+        q, e, stats, g = ctx.saved_tensors
+        lead, gshape, bshape = ctx.meta
+        N, d = q.shape
+        dev = q.device
+        bf16 = dy.dtype == torch.bfloat16
+        dyc = _a16(_c(dy) if bf16 else _c(dy, torch.float32)).view(N, d)
+        dr = None if dres is None else _a16(_c(dres, torch.float32)).view(N, d)
+        if _norma8_propia(d):
+            dx = torch.empty((N, d), dtype=torch.float32, device=dev)
+            dp = torch.empty((2 * d,), dtype=torch.float32, device=dev)
+            wsb = query('asrn_norm8_bwd_workspace', N, d)
+            ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+            call('asrn_norm8_bwd', ptr(q), ptr(e), ptr(g), ptr(stats), N, d, ptr(dyc), int(bf16), ptr(dr), ptr(dx), ptr(dp),
+                 ptr(ws), wsb, stream_of(dev))
+            return dx.view(*lead, d), dp[:d].view(gshape), dp[d:].view(bshape), None, None
+        xh = (leer8(q, e) - stats[:, :1]) * stats[:, 1:]
+        f = dyc.float()
+        p = f * g
+        dx = stats[:, 1:] * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True))
+        dx = dx if dr is None else dx + dr
+        return dx.view(*lead, d), (f * xh).sum(0).view(gshape), f.sum(0).view(bshape), None, None
+
+
+def _norma8_propia(d):
+    return d % 4 == 0 and d <= 1024
+
+
+def _a16(t):
+    """t, copied if its rows lie off the 16-byte boundary that the kernels read from."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _norma8_leer(ts, dtype, k=1, L=None):
+    """norma8's output again, (N, d k): the columns of a causal window of k tokens over texts of L (k = 1: as it was)."""
+    q, e, stats, g, b = ts
+    N, d = q.shape
+    g, b = _c(g.detach(), torch.float32), _c(b.detach(), torch.float32)
+    L = N if L is None else L
+    if _norma8_propia(d) and not (g.data_ptr() | b.data_ptr()) % 16:
+        out = torch.empty((N, d * k), dtype=dtype, device=q.device)
+        call('asrn_norm8_read', ptr(q), ptr(e), ptr(g), ptr(b), ptr(stats), N // L if L else 0, L, d, k,
+             int(dtype == torch.bfloat16), ptr(out), stream_of(q.device))
+        return out
+    y = (leer8(q, e) - stats[:, :1]) * stats[:, 1:] * g + b
+    if k == 1:
+        return y.to(dtype)
+    zp = F.pad(y.view(-1, L, d), (0, 0, k - 1, 0)).unfold(1, k, 1)
+    return zp.reshape(N, d * k).to(dtype)
+
+
+def norma8(ln, x, dtype):
+    """(LayerNorm ln of x in `dtype`, x for the residual path, what lineal8 and ventana8 read the first from):
+    norma_residual whose backward reads x back from 8 bits (guardar8's format) instead of keeping it, with the mean and
+    the deviation of x itself. The output is norma_residual's; the gradients of x and the parameters are those at the
+    8-bit values. x fp32, dtype fp32 or bf16. Without gradients, off the GPU or for another ln: norma_residual and None."""
+    d = x.shape[-1]
+    if not (x.is_cuda and x.dtype == torch.float32 and x.numel() > 0 and dtype in (torch.float32, torch.bfloat16)
+            and torch.is_grad_enabled() and ln.elementwise_affine and ln.bias is not None
+            and tuple(ln.normalized_shape) == (d,)):
+        return *norma_residual(ln, x, dtype), None
+    y, x, q, e, stats = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
+    return y, x, Guardado8(_norma8_leer, (q, e, stats, ln.weight, ln.bias))
+
+
+def ventana8(z, k, dtype, guardado):
+    """(ventana_causal(z, k, dtype), what lineal8 reads those columns from) for the output z (B, L, d) fp32 of norma8 and
+    what norma8 kept."""
+    L = z.shape[1]
+    return ventana_causal(z, k, dtype), guardado and Guardado8(lambda ts, dt: _norma8_leer(ts, dt, k, L), guardado.tensores)

@@ -693,6 +693,35 @@ int asrn_policy_bwd(const float* raw, const float* weight, const float* g, const
                     const int64_t* mask_strides, int64_t B, int64_t L, double entropy_weight, float* dlp,
                     float* dentropy, void* stream);
 
+/* ---- activations in 8 bits for the backward pass -------------------------------------------------------------------
+ * No counterpart in the reference (beside its recomputation modes, asrn/nucleo.py:1017-1022). The format, for rows of d
+ * channels: per 32 neighbouring channels a byte e + 127, 2^e the smallest power of two with max |x| <= 127 2^e
+ * (-126 <= e <= 121), e (rows, ceil(d / 32)); and x 2^-e rounded to the nearest integer, q (rows, d) int8. Byte 255: the
+ * group holds an infinity, a NaN or a value past 127 2^121 and reads back as NaN. All tensors dense.
+ * pack8: x fp32 or bf16 -> q, e. unpack8: q 2^e, or its GELU, in fp32 or bf16.
+ * gelu8_fwd: u fp32 or bf16 -> gelu(u) in u's type, or h + gelu(u) in fp32 (gelu rounded to u's type first) with h not
+ * null, and u's q, e. gelu8_bwd: du = gelu'(q 2^e) dy (dy, du fp32 or bf16).
+ * norm8_fwd: asrn_layer_norm_fwd with x's q, e. norm8_bwd: asrn_layer_norm_bwd with x read from q, e: xhat =
+ * (q 2^e - mean) rstd. norm8_read: y formed again from q, e and stats as the columns of a causal window of k tokens,
+ * out (B, L, d k), out[b, t, c k + j] = y[b, t + j - (k - 1), c], 0 before a row's start, 1 <= k <= 16. norm8: d a
+ * multiple of 4, <= 1024, rows 16-byte aligned (8 for bf16); workspace: asrn_norm8_bwd_workspace bytes, 256-byte
+ * aligned. */
+int asrn_pack8(const void* x, int32_t x_bf16, int64_t rows, int64_t d, int8_t* q, uint8_t* e, void* stream);
+int asrn_unpack8(const int8_t* q, const uint8_t* e, int64_t rows, int64_t d, int32_t gelu, int32_t out_bf16, void* out,
+                 void* stream);
+int asrn_gelu8_fwd(const void* u, int32_t u_bf16, const float* h, int64_t rows, int64_t d, void* out, int8_t* q, uint8_t* e,
+                   void* stream);
+int asrn_gelu8_bwd(const int8_t* q, const uint8_t* e, const void* dy, int32_t dy_bf16, int64_t rows, int64_t d,
+                   int32_t du_bf16, void* du, void* stream);
+int asrn_norm8_fwd(const float* x, const float* gamma, const float* beta, int64_t rows, int32_t d, float eps,
+                   int32_t out_bf16, void* y, float* stats, int8_t* q, uint8_t* e, void* stream);
+int64_t asrn_norm8_bwd_workspace(int64_t rows, int32_t d);
+int asrn_norm8_bwd(const int8_t* q, const uint8_t* e, const float* gamma, const float* stats, int64_t rows, int32_t d,
+                   const void* dy, int32_t dy_bf16, const float* dres, float* dx, float* dparams, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int asrn_norm8_read(const int8_t* q, const uint8_t* e, const float* gamma, const float* beta, const float* stats, int64_t B,
+                    int64_t L, int32_t d, int32_t k, int32_t out_bf16, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -43,8 +43,8 @@ def test_preference_checks(lib):
     _mal(lib, f(1, 5, 0, 0.0, 0.0, 0.0), 'beta')
     _mal(lib, f(1, 5, 0, 0.1, 1.5, 0.0), 'smoothing')
     _mal(lib, f(1, 5, 0, 0.1, 0.0, float('nan')), 'margin')
-    _mal(lib, f(2, 5000, 0, 0.1, 0.0, 0.0, 4 * 2 * 16 - 1), 'workspace')
-    assert lib.asrn_preference_workspace(2, 5000) == 4 * 2 * 16 and lib.asrn_preference_workspace(0, 5) == -1
+    _mal(lib, f(2, 5000, 0, 0.1, 0.0, 0.0, 4 * 3 * 16 - 1), 'workspace')
+    assert lib.asrn_preference_workspace(2, 5000) == 4 * 3 * 16 and lib.asrn_preference_workspace(0, 5) == -1
     _mal(lib, lib.asrn_preference_bwd(N, N, N, N, 1, 5, N, N), 'null pointer')
     assert lib.asrn_preference_bwd(N, N, N, N, 1, 0, N, N) == 0
 
@@ -62,6 +62,28 @@ def test_policy_checks(lib):
     assert lib.asrn_policy_workspace(3, 2049) == 3 * 2 * 48 and lib.asrn_policy_workspace(1, -1) == -1
     _mal(lib, lib.asrn_policy_bwd(N, N, N, N, N, 1, 5, 0.0, 16, N, N), 'null pointer')
     assert lib.asrn_policy_bwd(N, N, N, N, N, 1, 5, 0.0, N, N, N) == 0
+
+
+def test_eight_bit_checks(lib):
+    _mal(lib, lib.asrn_pack8(16, 0, 4, 0, 16, 16, N), 'bad sizes')
+    _mal(lib, lib.asrn_pack8(16, 0, 1 << 30, 1 << 20, 16, 16, N), 'bad sizes')
+    _mal(lib, lib.asrn_pack8(16, 0, 4, 32, N, 16, N), 'null pointer')
+    _mal(lib, lib.asrn_unpack8(16, 16, -1, 32, 0, 0, 16, N), 'bad sizes')
+    _mal(lib, lib.asrn_gelu8_fwd(16, 1, N, 4, 32, N, 16, 16, N), 'null pointer')
+    _mal(lib, lib.asrn_gelu8_bwd(16, 16, N, 1, 4, 32, 1, 16, N), 'null pointer')
+    _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 30, 1e-5, 0, 16, 16, 16, 16, N), 'multiple of 4')
+    _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 1028, 1e-5, 0, 16, 16, 16, 16, N), 'multiple of 4')
+    _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 32, 0.0, 0, 16, 16, 16, 16, N), 'eps')
+    _mal(lib, lib.asrn_norm8_fwd(24, 16, 16, 4, 32, 1e-5, 0, 16, 16, 16, 16, N), 'aligned')
+    need = lib.asrn_norm8_bwd_workspace(100, 64)
+    assert need >= 4 * 2 * 64 * 4 and lib.asrn_norm8_bwd_workspace(-1, 64) == -1 and lib.asrn_norm8_bwd_workspace(1, 4096) == -1
+    _mal(lib, lib.asrn_norm8_bwd(16, 16, 16, 16, 100, 64, 16, 0, N, 16, 16, 256, need - 1, N), 'workspace')
+    _mal(lib, lib.asrn_norm8_read(16, 16, 16, 16, 16, 2, 5, 64, 17, 0, 16, N), 'k=17')
+    _mal(lib, lib.asrn_norm8_read(16, 16, 16, 16, 16, 2, 5, 62, 4, 0, 16, N), 'multiple of 4')
+    for rc in (lib.asrn_pack8(N, 0, 0, 32, N, N, N), lib.asrn_unpack8(N, N, 0, 32, 0, 0, N, N), lib.asrn_gelu8_fwd(N, 0, N, 0, 32, N, N, N, N),
+               lib.asrn_gelu8_bwd(N, N, N, 0, 0, 32, 0, N, N), lib.asrn_norm8_fwd(N, N, N, 0, 32, 1e-5, 0, N, N, N, N, N),
+               lib.asrn_norm8_read(N, N, N, N, N, 0, 5, 64, 4, 0, N, N)):
+        assert rc == 0                                      # no rows: no launch
 
 
 def test_public_names_refuse_cpu_tensors():
