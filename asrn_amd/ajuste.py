@@ -14,24 +14,12 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import call, ptr, query
-from .ops import _dev
+from ._lib import ptr, query
+from .ops import _dev, _en
 
 TIPOS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # the kernels' logits
 FORMAS = ('sigmoide', 'ipo', 'bisagra')
 REDUCCIONES = ('fichas', 'textos')
-
-
-_corriente = torch._C._cuda_getCurrentRawStream       # the stream's handle without the Python object around it
-
-
-def _llamar(dev, nombre, *args):
-    """call() on dev's current stream, with dev as the current device (a kernel launches on the current one)."""
-    i = dev.index
-    if torch.cuda.current_device() == i:
-        return call(nombre, *args, _corriente(i))
-    with torch.cuda.device(i):
-        return call(nombre, *args, _corriente(i))
 
 
 def _denso(g):
@@ -63,6 +51,11 @@ def _mascara(quien, m, forma, dev):
 
 def _f32(t):
     return t if t is None or t.dtype == torch.float32 else t.float()
+
+
+def _fijo(t):
+    """A constant input: fp32, outside autograd."""
+    return t if t is None or (t.dtype == torch.float32 and not t.requires_grad) else t.detach().float()
 
 
 def _numero(quien, nombre, v, minimo, maximo=math.inf, abierto=False):
@@ -105,7 +98,7 @@ class LogProbabilidades(torch.autograd.Function):
         stats = torch.empty((filas, 2), dtype=torch.float32, device=dev)
         H = torch.empty(y.shape, dtype=torch.float32, device=dev) if entropia else None
         if filas:
-            _llamar(dev, 'asrn_token_logp_fwd', ptr(x), TIPOS[x.dtype], filas, L, V, sb, st, ptr(t), ignorar, inv_t, ptr(lp),
+            _en(dev, 'asrn_token_logp_fwd', ptr(x), TIPOS[x.dtype], filas, L, V, sb, st, ptr(t), ignorar, inv_t, ptr(lp),
                     ptr(H), ptr(stats))
         ctx.save_for_backward(x, t, stats, H)
         ctx.meta = (filas, L, sb, st, ignorar, inv_t, logits.shape)
@@ -123,7 +116,7 @@ class LogProbabilidades(torch.autograd.Function):
         gh = None if gh is None else _denso(gh)
         dx = torch.empty(forma, dtype=x.dtype, device=x.device)
         if filas:
-            _llamar(x.device, 'asrn_token_logp_bwd', ptr(x), TIPOS[x.dtype], filas, L, forma[-1], sb, st, ptr(t), ignorar, inv_t,
+            _en(x.device, 'asrn_token_logp_bwd', ptr(x), TIPOS[x.dtype], filas, L, forma[-1], sb, st, ptr(t), ignorar, inv_t,
                     ptr(stats), ptr(H), ptr(g), ptr(gh), ptr(dx))
         return dx, None, None, None, None
 
@@ -158,7 +151,8 @@ class Preferencia(torch.autograd.Function):
     forward."""
 
     @staticmethod
-    def forward(ctx, lp, m, ref, forma, beta, suavizado, margen, por_longitud):
+    def forward(ctx, lp, fijos):
+        m, ref, forma, beta, suavizado, margen, por_longitud = fijos      # constants: no autograd around them
         dev = lp.device
         P, L = lp.shape[0] // 2, lp.shape[1]
         perdida = torch.empty((), dtype=torch.float32, device=dev)
@@ -168,7 +162,7 @@ class Preferencia(torch.autograd.Function):
         coef = ws.data_ptr() + max(wsb, 0)           # the rows' coefficients, kept for the backward, behind the workspace
         por_fila = ref is not None and ref.dim() == 1
         ref_pasos = None if ref is None else (ctypes.c_int64 * 2)(ref.stride(0), 0) if por_fila else _pasos(ref)
-        _llamar(dev, 'asrn_preference_fwd', ptr(lp), _pasos(lp), ptr(ref), ref_pasos, int(por_fila), ptr(m),
+        _en(dev, 'asrn_preference_fwd', ptr(lp), _pasos(lp), ptr(ref), ref_pasos, int(por_fila), ptr(m),
                 None if m is None else _pasos(m), P, L, FORMAS.index(forma), beta, suavizado, margen, int(por_longitud),
                 ptr(perdida), ptr(rec), coef, ptr(ws), wsb)
         ctx.save_for_backward(ws, m)
@@ -183,12 +177,12 @@ class Preferencia(torch.autograd.Function):
         ws, m = ctx.saved_tensors
         P, L, wsb = ctx.meta
         if g is None:
-            return (None,) * 8
+            return None, None
         dlp = torch.empty((2 * P, L), dtype=torch.float32, device=ws.device)
         gc = _denso(g)
-        _llamar(ws.device, 'asrn_preference_bwd', ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), P, L,
+        _en(ws.device, 'asrn_preference_bwd', ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), P, L,
                 ptr(dlp))
-        return (dlp,) + (None,) * 7
+        return dlp, None
 
 
 def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', suavizado=0.0, margen=0.0,
@@ -213,7 +207,7 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
         if tuple(ref.shape) not in (tuple(lp.shape), (lp.shape[0],)) or not ref.is_floating_point():
             raise ValueError(f'{quien}: ref {tuple(ref.shape)} of {ref.dtype} against lp {tuple(lp.shape)}')
         _mismo_gpu(quien, dev, ref=ref)
-        ref = _f32(ref.detach())
+        ref = _fijo(ref)
     if tipo not in FORMAS:
         raise ValueError(f'{quien}: tipo={tipo!r}: one of {FORMAS}')
     beta = _numero(quien, 'beta', beta, 0.0, abierto=True)
@@ -221,7 +215,7 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
     if suavizado and tipo != 'sigmoide':
         raise ValueError(f"{quien}: suavizado belongs to tipo='sigmoide'")
     margen = _numero(quien, 'margen', margen, -math.inf)
-    return Preferencia.apply(_f32(lp), m, ref, tipo, beta, suavizado, margen, bool(por_longitud))
+    return Preferencia.apply(_f32(lp), (m, ref, tipo, beta, suavizado, margen, bool(por_longitud)))
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -233,19 +227,22 @@ class Politica(torch.autograd.Function):
     reduction are kept from the forward, in fp32."""
 
     @staticmethod
-    def forward(ctx, lp, H, A, vieja, ref, m, lo, hi, tope, beta, peso, por_texto):
+    def forward(ctx, lp, H, fijos):
+        A, vieja, ref, m, lo, hi, tope, beta, peso, por_texto = fijos     # constants: no autograd around them
         dev = lp.device
         B, L = lp.shape
         perdida = torch.empty((), dtype=torch.float32, device=dev)
         datos = torch.empty((4,), dtype=torch.float32, device=dev)
-        crudo = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        # one buffer: the workspace, then what the backward needs: the texts' divisors and the tokens' gradients
         wsb = query('asrn_policy_workspace', B, L)
-        ws = torch.empty((max(wsb, 0) + 4 * B,), dtype=torch.uint8, device=dev)
-        div = ws.data_ptr() + max(wsb, 0)            # the texts' divisors, kept for the backward, behind the workspace
-        _llamar(dev, 'asrn_policy_fwd', ptr(lp), ptr(A), ptr(vieja), ptr(ref), ptr(H), ptr(m), _pasos(lp, A, vieja, ref, H, m),
-                B, L, lo, hi, tope, beta, peso, int(por_texto), ptr(crudo), ptr(perdida), ptr(datos), div, ptr(ws), wsb)
-        ctx.save_for_backward(crudo, ws, m)
-        ctx.meta = (B, L, peso, max(wsb, 0))
+        fin = max(wsb, 0)
+        ws = torch.empty((fin + 4 * B + (4 * B * L if ctx.needs_input_grad[0] else 0),), dtype=torch.uint8, device=dev)
+        div = ws.data_ptr() + fin
+        crudo = div + 4 * B if ctx.needs_input_grad[0] else None
+        _en(dev, 'asrn_policy_fwd', ptr(lp), ptr(A), ptr(vieja), ptr(ref), ptr(H), ptr(m), _pasos(lp, A, vieja, ref, H, m),
+                B, L, lo, hi, tope, beta, peso, int(por_texto), crudo, ptr(perdida), ptr(datos), div, ptr(ws), wsb)
+        ctx.save_for_backward(ws, m)
+        ctx.meta = (B, L, peso, fin)
         ctx.mark_non_differentiable(datos)
         ctx.set_materialize_grads(False)
         return perdida, datos
@@ -253,17 +250,18 @@ class Politica(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
-        crudo, ws, m = ctx.saved_tensors
-        B, L, peso, wsb = ctx.meta
+        ws, m = ctx.saved_tensors
+        B, L, peso, fin = ctx.meta
         if g is None:
-            return (None,) * 12
+            return None, None, None
         dev = ws.device
         dlp = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
         dH = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
         gc = _denso(g)
-        _llamar(dev, 'asrn_policy_bwd', ptr(crudo), ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), B, L,
-                peso, ptr(dlp), ptr(dH))
-        return (dlp, dH) + (None,) * 10
+        div = ws.data_ptr() + fin
+        _en(dev, 'asrn_policy_bwd', div + 4 * B, div, ptr(gc), ptr(m), None if m is None else _pasos(m), B, L, peso, ptr(dlp),
+            ptr(dH))
+        return dlp, dH, None
 
 
 def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope=None, lp_ref=None, beta=0.0,
@@ -304,9 +302,8 @@ def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope
         raise ValueError(f'{quien}: peso_entropia={peso} needs entropia')
     if reduccion not in REDUCCIONES:
         raise ValueError(f'{quien}: reduccion={reduccion!r}: one of {REDUCCIONES}')
-    d = lambda t: None if t is None else _f32(t.detach())
-    return Politica.apply(_f32(lp), _f32(entropia), d(ventaja), d(lp_vieja), d(lp_ref), m, lo, hi, tope, beta, peso,
-                          reduccion == 'textos')
+    return Politica.apply(_f32(lp), _f32(entropia), (_fijo(ventaja), _fijo(lp_vieja), _fijo(lp_ref), m, lo, hi, tope, beta,
+                                                     peso, reduccion == 'textos'))
 
 
 token_log_probs, preference_loss, policy_loss = log_probabilidades, perdida_preferencia, perdida_politica

@@ -63,21 +63,27 @@ __device__ __forceinline__ uint32_t max_of8(uint32_t v) { return dpp_max<0x141>(
 // ---- GELU ----------------------------------------------------------------------------------------------------------
 // exact GELU, as torch forms it in fp32
 __device__ __forceinline__ float e8_gelu(float x) { return x * 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
-// Phi(x) and its density's exponential e = exp(-x^2 / 2), from Abramowitz and Stegun's 7.1.26 (erfc within 1.5e-7, and
-// in the lower tail, where it is taken without the subtraction, within 1e-5 of itself): one exponential and one
-// reciprocal serve the value and the derivative
-__device__ __forceinline__ float e8_phi(float x, float* e) {
-  const float a = fabsf(x) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
-  *e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float low = 0.5f * p * *e;
-  return x < 0.f ? low : x == x ? 1.f - low : x;
+// For the values read back: Phi(-|x|) = e p with e = exp(-x^2 / 2), from Abramowitz and Stegun's 7.1.26 (erfc within
+// 1.5e-7, and its tail, which is taken without a subtraction, within 1e-5 of itself). One exponential and one reciprocal
+// serve the value and the derivative: with m = Phi(-|x|) - |x| phi(x), gelu = max(x, 0) - |x| Phi(-|x|) and gelu' = m
+// below 0, 1 - m above (erff's two branches cost about twice the instructions, and these kernels run out of them first)
+__device__ __forceinline__ float e8_tail(float x, float* e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
+  const float z = x * 0.84932180028801904f;                        // sqrt(log2(e) / 2)
+  *e = __builtin_amdgcn_exp2f(-z * z);
+  return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                          0.5f * -0.284496736f), 0.5f * 0.254829592f);
+}
+__device__ __forceinline__ float e8_gelu_read(float x) {
+  float e;
+  const float p = e8_tail(x, &e);
+  return fmaf(-fabsf(x), p * e, fmaxf(x, 0.f));                    // p is NaN where x is
 }
 __device__ __forceinline__ float e8_dgelu(float x) {
   float e;
-  const float phi = e8_phi(x, &e);
-  return fmaf(x * 0.39894228040143268f, e, phi);
+  const float p = e8_tail(x, &e);
+  const float m = e * fmaf(-0.39894228040143268f, fabsf(x), p);
+  return x < 0.f ? m : 1.f - m;
 }
 
 // ---- elementwise kernels: 8 channels a lane, 4 lanes a group ---------------------------------------------------------
@@ -220,10 +226,7 @@ __global__ __launch_bounds__(kE8Threads) void k_gelu8_bwd(E8Args a) {
   }
   if constexpr (OP == kE8ReadGelu) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float e;
-      x[k] *= e8_phi(x[k], &e);
-    }
+    for (int k = 0; k < 8; ++k) x[k] = e8_gelu_read(x[k]);
   }
   e8_store<O16>(a.out, p.at, p.n, x);
 }
@@ -395,7 +398,52 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_bwd(N8Args a) {
 }
 
 // y again from x8 and the statistics, as columns of a causal window: out[b, t, c k + j] = y[b, t + j - (k - 1), c], 0
-// before a text's start. A thread takes 4 channels of a token.
+// before a text's start. For k = 1 and 4 a thread takes 4 channels of kN8Run tokens in a row and reads each token once,
+// all in flight (16384 x 768 bf16 with a token a thread: 17 and 37 us); any other k a token at a time.
+constexpr int kN8Run = 8;
+template <bool O16, int K>
+__global__ __launch_bounds__(kE8Threads) void k_norm8_run(N8Args a) {
+  const int d4 = a.d >> 2;
+  const int64_t runs = (a.L + kN8Run - 1) / kN8Run, texts = a.rows / a.L;
+  const int64_t i = (int64_t)blockIdx.x * kE8Threads + threadIdx.x;
+  if (i >= texts * runs * d4) return;
+  const int64_t run = texts * runs * d4 < (int64_t(1) << 32) ? (int64_t)((uint32_t)i / (uint32_t)d4) : i / d4;
+  const int c = (int)(i - run * d4);
+  const int64_t b = (uint32_t)run / (uint32_t)runs, t0 = (run - b * runs) * kN8Run, r0 = b * a.L;
+  const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], z = reinterpret_cast<const float4*>(a.beta)[c];
+  uint32_t q[kN8Run + K - 1], e[kN8Run + K - 1];
+  float2 st[kN8Run + K - 1];
+  float4 v[kN8Run + K - 1];
+#pragma unroll
+  for (int j = 0; j < kN8Run + K - 1; ++j) {            // tokens outside the text read its nearest, not used
+    int64_t t = t0 + j - (K - 1);
+    t = t < 0 ? 0 : t < a.L ? t : a.L - 1;
+    q[j] = a.q[(r0 + t) * d4 + c];
+    e[j] = a.e[(r0 + t) * a.groups + (c >> 3)];
+    st[j] = a.stats[r0 + t];
+  }
+#pragma unroll
+  for (int j = 0; j < kN8Run + K - 1; ++j) {
+    const float4 x = e8_open(q[j], e8_scale(e[j]));
+    v[j] = make_float4((x.x - st[j].x) * st[j].y * w.x + z.x, (x.y - st[j].x) * st[j].y * w.y + z.y,
+                       (x.z - st[j].x) * st[j].y * w.z + z.z, (x.w - st[j].x) * st[j].y * w.w + z.w);
+    if (t0 + j < K - 1) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int u = 0; u < kN8Run; ++u) {
+    if (t0 + u >= a.L) break;
+    const int64_t at = (r0 + t0 + u) * d4 + c;          // in groups of 4 channels
+    if constexpr (K == 1) {
+      n8_store<O16>(a.y, at, v[u]);
+    } else {
+      n8_store<O16>(a.y, 4 * at, make_float4(v[u].x, v[u + 1].x, v[u + 2].x, v[u + 3].x));
+      n8_store<O16>(a.y, 4 * at + 1, make_float4(v[u].y, v[u + 1].y, v[u + 2].y, v[u + 3].y));
+      n8_store<O16>(a.y, 4 * at + 2, make_float4(v[u].z, v[u + 1].z, v[u + 2].z, v[u + 3].z));
+      n8_store<O16>(a.y, 4 * at + 3, make_float4(v[u].w, v[u + 1].w, v[u + 2].w, v[u + 3].w));
+    }
+  }
+}
+
 template <bool O16>
 __global__ __launch_bounds__(kE8Threads) void k_norm8_read(N8Args a) {
   const int d4 = a.d >> 2;
@@ -405,35 +453,20 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_read(N8Args a) {
   const int c = (int)(i - r * d4);
   const int64_t t = (uint32_t)r % (uint32_t)a.L;       // rows, L < 2^31
   const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], b = reinterpret_cast<const float4*>(a.beta)[c];
-  for (int j0 = 0; j0 < a.k; j0 += 4) {       // 4 taps at a time
-    float v[4][4];
-    const int n = a.k - j0 < 4 ? a.k - j0 : 4;
+  for (int j = 0; j < a.k; ++j) {
+    const int64_t back = a.k - 1 - j;
+    const bool in = back <= t;
+    const int64_t s = r - (in ? back : 0);
+    const float2 st = a.stats[s];
+    const float4 x = e8_open(a.q[s * d4 + c], e8_scale(a.e[s * a.groups + (c >> 3)]));
+    const float v[4] = {(x.x - st.x) * st.y * w.x + b.x, (x.y - st.x) * st.y * w.y + b.y, (x.z - st.x) * st.y * w.z + b.z,
+                        (x.w - st.x) * st.y * w.w + b.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t back = a.k - 1 - (j0 + j);
-      const bool in = j < n && back <= t;
-      const int64_t s = r - (in ? back : 0);
-      const float2 st = a.stats[s];
-      const float4 x = e8_open(a.q[s * d4 + c], e8_scale(a.e[s * a.groups + (c >> 3)]));
-      v[0][j] = in ? (x.x - st.x) * st.y * w.x + b.x : 0.f;
-      v[1][j] = in ? (x.y - st.x) * st.y * w.y + b.y : 0.f;
-      v[2][j] = in ? (x.z - st.x) * st.y * w.z + b.z : 0.f;
-      v[3][j] = in ? (x.w - st.x) * st.y * w.w + b.w : 0.f;
-    }
-    const int64_t at = (r * a.d + 4 * c) * a.k + j0;
-    if (a.k == 1) {
-      n8_store<O16>(a.y, i, make_float4(v[0][0], v[1][0], v[2][0], v[3][0]));
-    } else if ((a.k & 3) == 0) {
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-        n8_store<O16>(a.y, (at + h * a.k) >> 2, make_float4(v[h][0], v[h][1], v[h][2], v[h][3]));
-    } else {
-      for (int h = 0; h < 4; ++h)
-        for (int j = 0; j < n; ++j) {
-          const float o = v[h][j];
-          if constexpr (O16) reinterpret_cast<uint16_t*>(a.y)[at + h * a.k + j] = (uint16_t)e8_pack_bf16(o, 0.f);
-          else reinterpret_cast<float*>(a.y)[at + h * a.k + j] = o;
-        }
+    for (int h = 0; h < 4; ++h) {
+      const int64_t at = (r * a.d + 4 * c + h) * a.k + j;
+      const float o = in ? v[h] : 0.f;
+      if constexpr (O16) reinterpret_cast<uint16_t*>(a.y)[at] = (uint16_t)e8_pack_bf16(o, 0.f);
+      else reinterpret_cast<float*>(a.y)[at] = o;
     }
   }
 }
@@ -615,9 +648,19 @@ extern "C" int asrn_norm8_read(const int8_t* q, const uint8_t* e, const float* g
   ASRN_REQUIRE(e8_aligned(gamma, 16) && e8_aligned(beta, 16) && e8_aligned(out, out_bf16 ? 8 : 16) && e8_aligned(q, 4) &&
                    e8_aligned(stats, 8),
                "asrn_norm8_read: rows and parameters must be 16-byte aligned (8 for bf16)");
-  const int64_t blocks = (a.rows * (d / 4) + kE8Threads - 1) / kE8Threads;
+  const bool run = k == 1 || k == 4;
+  const int64_t lanes = (run ? B * ((L + kN8Run - 1) / kN8Run) : a.rows) * (d / 4);
+  const int64_t blocks = (lanes + kE8Threads - 1) / kE8Threads;
   ASRN_REQUIRE(blocks < (int64_t(1) << 31), "asrn_norm8_read: too many values");
   hipStream_t st = (hipStream_t)stream;
+  if (run) {
+    const dim3 grid((unsigned)blocks), block(kE8Threads);
+    if (k == 1 && out_bf16) hipLaunchKernelGGL((k_norm8_run<true, 1>), grid, block, 0, st, a);
+    else if (k == 1) hipLaunchKernelGGL((k_norm8_run<false, 1>), grid, block, 0, st, a);
+    else if (out_bf16) hipLaunchKernelGGL((k_norm8_run<true, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_norm8_run<false, 4>), grid, block, 0, st, a);
+    return check_launch("asrn_norm8_read");
+  }
   if (out_bf16) hipLaunchKernelGGL(k_norm8_read<true>, dim3((unsigned)blocks), dim3(kE8Threads), 0, st, a);
   else hipLaunchKernelGGL(k_norm8_read<false>, dim3((unsigned)blocks), dim3(kE8Threads), 0, st, a);
   return check_launch("asrn_norm8_read");

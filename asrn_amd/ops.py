@@ -1603,11 +1603,29 @@ class Guardado8:
         self.leer, self.tensores = leer, tuple(tensores)
 
 
-def _sitio8(x2):
-    """The codes (N, d) int8 and the groups' scale bytes for rows x2 (N, d)."""
-    N, d = x2.shape
-    return (torch.empty((N, d), dtype=torch.int8, device=x2.device),
-            torch.empty((N, -(-d // GRUPO8)), dtype=torch.uint8, device=x2.device))
+_corriente = torch._C._cuda_getCurrentRawStream       # a stream's handle without the Python object around it
+
+
+def _en(dev, nombre, *args):
+    """call() on dev's current stream, with dev as the current device (a kernel launches on the current one)."""
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        return call(nombre, *args, _corriente(i))
+    with torch.cuda.device(i):
+        return call(nombre, *args, _corriente(i))
+
+
+def _partes8(N, d, datos=0):
+    """Where the parts of a buffer for rows (N, d) in 8 bits begin and end: the codes at 0, `datos` fp32 values a row, the
+    groups' scale bytes, its end; the values 16-byte aligned."""
+    m = -(-N * d // 16) * 16
+    s = m + -(-4 * datos * N // 16) * 16
+    return m, s, s + N * -(-d // GRUPO8)
+
+
+def _sitio8(N, d, dev, datos=0):
+    m, s, fin = _partes8(N, d, datos)
+    return torch.empty((fin,), dtype=torch.uint8, device=dev), m, s
 
 
 def guardar8(x):
@@ -1618,8 +1636,10 @@ def guardar8(x):
     if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'guardar8: {tuple(x.shape)} of {x.dtype}: (..., d) fp32 or bf16 is needed')
     x2 = x.detach().contiguous().view(-1, x.shape[-1]) if x.numel() else x.detach().reshape(0, x.shape[-1])
-    q, e = _sitio8(x2)
-    call('asrn_pack8', ptr(x2), int(x2.dtype == torch.bfloat16), *x2.shape, ptr(q), ptr(e), stream_of(dev))
+    N, d = x2.shape
+    q = torch.empty((N, d), dtype=torch.int8, device=dev)
+    e = torch.empty((N, -(-d // GRUPO8)), dtype=torch.uint8, device=dev)
+    _en(dev, 'asrn_pack8', ptr(x2), int(x2.dtype == torch.bfloat16), N, d, ptr(q), ptr(e))
     return q, e
 
 
@@ -1631,43 +1651,53 @@ def leer8(q, e, dtype=torch.float32, gelu=False):
             tuple(e.shape) != (q.shape[0], -(-q.shape[1] // GRUPO8)) or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f'leer8: codes {tuple(q.shape)} of {q.dtype} with scales {tuple(e.shape)} of {e.dtype} to {dtype}')
     q, e = q.contiguous(), e.contiguous()
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
-    call('asrn_unpack8', ptr(q), ptr(e), *q.shape, int(gelu), int(dtype == torch.bfloat16), ptr(out), stream_of(dev))
+    return _leer8(q.data_ptr(), e.data_ptr(), *q.shape, dev, dtype, gelu)
+
+
+def _leer8(q, e, N, d, dev, dtype, gelu=False):
+    out = torch.empty((N, d), dtype=dtype, device=dev)
+    _en(dev, 'asrn_unpack8', q, e, N, d, int(gelu), int(dtype == torch.bfloat16), ptr(out))
     return out
 
 
 class Gelu8(torch.autograd.Function):
     """asrn_gelu8_fwd/bwd: gelu(u), or h + gelu(u) (h fp32; gelu rounds to u's dtype first, as the separate ops do), with
-    u kept in 8 bits for the backward; returns also the codes and scales."""
+    u kept in 8 bits for the backward; returns also what is kept."""
 
     @staticmethod
     def forward(ctx, u, h):
-        dev, d = u.device, u.shape[-1]
-        u2 = u.contiguous().view(-1, d)
-        q, e = _sitio8(u2)
-        bf16 = u.dtype == torch.bfloat16
-        h2 = None if h is None else h.contiguous()
-        out = torch.empty(u.shape, dtype=u.dtype if h is None else torch.float32, device=dev)
-        call('asrn_gelu8_fwd', ptr(u2), int(bf16), ptr(h2), *u2.shape, ptr(out), ptr(q), ptr(e), stream_of(dev))
-        ctx.save_for_backward(q, e)
-        ctx.meta = (bf16, u.shape)
-        ctx.mark_non_differentiable(q, e)
+        dev, forma, bf16 = u.device, u.shape, u.dtype == torch.bfloat16
+        d = forma[-1]
+        u, N = u.contiguous(), u.numel() // d
+        sitio, _, s = _sitio8(N, d, dev)
+        if h is None:
+            out = torch.empty(forma, dtype=u.dtype, device=dev)
+        else:
+            h = h.contiguous()
+            out = torch.empty(forma, dtype=torch.float32, device=dev)
+        q = sitio.data_ptr()
+        _en(dev, 'asrn_gelu8_fwd', ptr(u), int(bf16), ptr(h), N, d, ptr(out), q, q + s)
+        ctx.save_for_backward(sitio)
+        ctx.meta = (bf16, forma, N, d, s)
+        ctx.mark_non_differentiable(sitio)
         ctx.set_materialize_grads(False)
-        return out, q, e
+        return out, sitio
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g, _, __):
-        q, e = ctx.saved_tensors
-        bf16, forma = ctx.meta
+    def backward(ctx, g, _):
+        sitio, = ctx.saved_tensors
+        bf16, forma, N, d, s = ctx.meta
         if g is None:
             return None, None
         gu = None
         if ctx.needs_input_grad[0]:
-            gc = _c(g, g.dtype if g.dtype == torch.bfloat16 else torch.float32)
-            gu = torch.empty(forma, dtype=torch.bfloat16 if bf16 else torch.float32, device=q.device)
-            call('asrn_gelu8_bwd', ptr(q), ptr(e), ptr(gc), int(gc.dtype == torch.bfloat16), *q.shape, int(bf16), ptr(gu),
-                 stream_of(q.device))
+            gc = g.contiguous()
+            if gc.dtype not in (torch.float32, torch.bfloat16):
+                gc = gc.float()
+            gu = torch.empty(forma, dtype=torch.bfloat16 if bf16 else torch.float32, device=sitio.device)
+            q = sitio.data_ptr()
+            _en(sitio.device, 'asrn_gelu8_bwd', q, q + s, ptr(gc), int(gc.dtype == torch.bfloat16), N, d, int(bf16), ptr(gu))
         return gu, g if ctx.needs_input_grad[1] else None
 
 
@@ -1675,8 +1705,11 @@ def _gelu8_ok(u):
     return u.is_cuda and u.dtype in (torch.float32, torch.bfloat16) and u.dim() >= 1 and u.numel() > 0 and torch.is_grad_enabled()
 
 
-def _leer_gelu8(ts, dtype):
-    return leer8(*ts, dtype, gelu=True)
+def _leer_gelu8(N, d):
+    def leer(ts, dtype):
+        q = ts[0].data_ptr()
+        return _leer8(q, q + _partes8(N, d)[1], N, d, ts[0].device, dtype, gelu=True)
+    return leer
 
 
 def gelu8(u):
@@ -1685,8 +1718,9 @@ def gelu8(u):
     dtype: (F.gelu(u), None)."""
     if not _gelu8_ok(u):
         return F.gelu(u), None
-    y, q, e = Gelu8.apply(u, None)
-    return y, Guardado8(_leer_gelu8, (q, e))
+    y, sitio = Gelu8.apply(u, None)
+    d = u.shape[-1]
+    return y, Guardado8(_leer_gelu8(u.numel() // d, d), (sitio,))
 
 
 def suma_gelu8(h, u):
@@ -1698,54 +1732,52 @@ def suma_gelu8(h, u):
 
 class Norma8(torch.autograd.Function):
     """NormaResidual that keeps x in 8 bits (and (mean, rstd) per row, of x itself): asrn_norm8_fwd/bwd where d is a
-    multiple of 4 up to 1024, else the same with torch's LayerNorm and asrn_pack8. Returns also what was kept."""
+    multiple of 4 up to 1024, else the same with torch's LayerNorm and asrn_pack8. Returns also what is kept."""
 
     @staticmethod
     def forward(ctx, x, gamma, beta, eps, dtype):
-        dev = _dev(x)
-        d, lead = x.shape[-1], x.shape[:-1]
-        x2 = x.contiguous().view(-1, d)
+        dev, forma = x.device, x.shape
+        d = forma[-1]
+        x2, N = x.contiguous(), x.numel() // d
         g, b = _c(gamma, torch.float32), _c(beta, torch.float32)
-        q, e = _sitio8(x2)
-        propio = _norma8_propia(d) and x2.data_ptr() % 16 == 0
-        if propio:
-            y = torch.empty((x2.shape[0], d), dtype=dtype, device=dev)
-            stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=dev)
-            call('asrn_norm8_fwd', ptr(x2), ptr(g), ptr(b), *x2.shape, float(eps), int(dtype == torch.bfloat16), ptr(y),
-                 ptr(stats), ptr(q), ptr(e), stream_of(dev))
+        sitio, m, s = _sitio8(N, d, dev, datos=2)
+        q = sitio.data_ptr()
+        if _norma8_propia(d) and not (x2.data_ptr() | g.data_ptr() | b.data_ptr()) % 16:
+            y = torch.empty(forma, dtype=dtype, device=dev)
+            _en(dev, 'asrn_norm8_fwd', ptr(x2), ptr(g), ptr(b), N, d, eps, int(dtype == torch.bfloat16), ptr(y), q + m, q, q + s)
         else:
             y, mu, rstd = torch.native_layer_norm(x2, (d,), g, b, eps)
-            y, stats = y.to(dtype), torch.cat([mu, rstd], 1)
-            call('asrn_pack8', ptr(x2), 0, *x2.shape, ptr(q), ptr(e), stream_of(dev))
-        ctx.save_for_backward(q, e, stats, g)
-        ctx.meta = (lead, gamma.shape, beta.shape)
-        ctx.mark_non_differentiable(q, e, stats)
-        return y.view(*lead, d), x2.view(*lead, d), q, e, stats
+            y = y.to(dtype)
+            sitio[m:m + 8 * N].view(torch.float32).view(N, 2).copy_(torch.cat([mu.view(N, 1), rstd.view(N, 1)], 1))
+            _en(dev, 'asrn_pack8', ptr(x2), 0, N, d, q, q + s)
+        ctx.save_for_backward(sitio, g)
+        ctx.meta = (forma, N, d, m, s)
+        ctx.mark_non_differentiable(sitio)
+        return y, x2.view(forma), sitio
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dres, *_):
-        q, e, stats, g = ctx.saved_tensors
-        lead, gshape, bshape = ctx.meta
-        N, d = q.shape
-        dev = q.device
+    def backward(ctx, dy, dres, _):
+        sitio, g = ctx.saved_tensors
+        forma, N, d, m, s = ctx.meta
+        dev, q = sitio.device, sitio.data_ptr()
         bf16 = dy.dtype == torch.bfloat16
-        dyc = _a16(_c(dy) if bf16 else _c(dy, torch.float32)).view(N, d)
-        dr = None if dres is None else _a16(_c(dres, torch.float32)).view(N, d)
-        if _norma8_propia(d):
-            dx = torch.empty((N, d), dtype=torch.float32, device=dev)
-            dp = torch.empty((2 * d,), dtype=torch.float32, device=dev)
+        dy = _a16(_c(dy) if bf16 else _c(dy, torch.float32))
+        dres = _a16(_c(dres, torch.float32))
+        if _norma8_propia(d) and g.data_ptr() % 16 == 0:
+            dx = torch.empty(forma, dtype=torch.float32, device=dev)
             wsb = query('asrn_norm8_bwd_workspace', N, d)
+            dp = torch.empty((2, d), dtype=torch.float32, device=dev)
             ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
-            call('asrn_norm8_bwd', ptr(q), ptr(e), ptr(g), ptr(stats), N, d, ptr(dyc), int(bf16), ptr(dr), ptr(dx), ptr(dp),
-                 ptr(ws), wsb, stream_of(dev))
-            return dx.view(*lead, d), dp[:d].view(gshape), dp[d:].view(bshape), None, None
-        xh = (leer8(q, e) - stats[:, :1]) * stats[:, 1:]
-        f = dyc.float()
+            _en(dev, 'asrn_norm8_bwd', q, q + s, ptr(g), q + m, N, d, ptr(dy), int(bf16), ptr(dres), ptr(dx), ptr(dp), ptr(ws), wsb)
+            dg, db = dp.unbind(0)
+            return dx, dg, db, None, None
+        mu, rstd = sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1)
+        xh = (_leer8(q, q + s, N, d, dev, torch.float32) - mu) * rstd
+        f = dy.float().view(N, d)
         p = f * g
-        dx = stats[:, 1:] * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True))
-        dx = dx if dr is None else dx + dr
-        return dx.view(*lead, d), (f * xh).sum(0).view(gshape), f.sum(0).view(bshape), None, None
+        dx = rstd * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True)) + dres.view(N, d)
+        return dx.view(forma), (f * xh).sum(0), f.sum(0), None, None
 
 
 def _norma8_propia(d):
@@ -1757,22 +1789,25 @@ def _a16(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _norma8_leer(ts, dtype, k=1, L=None):
-    """norma8's output again, (N, d k): the columns of a causal window of k tokens over texts of L (k = 1: as it was)."""
-    q, e, stats, g, b = ts
-    N, d = q.shape
-    g, b = _c(g.detach(), torch.float32), _c(b.detach(), torch.float32)
-    L = N if L is None else L
-    if _norma8_propia(d) and not (g.data_ptr() | b.data_ptr()) % 16:
-        out = torch.empty((N, d * k), dtype=dtype, device=q.device)
-        call('asrn_norm8_read', ptr(q), ptr(e), ptr(g), ptr(b), ptr(stats), N // L if L else 0, L, d, k,
-             int(dtype == torch.bfloat16), ptr(out), stream_of(q.device))
-        return out
-    y = (leer8(q, e) - stats[:, :1]) * stats[:, 1:] * g + b
-    if k == 1:
-        return y.to(dtype)
-    zp = F.pad(y.view(-1, L, d), (0, 0, k - 1, 0)).unfold(1, k, 1)
-    return zp.reshape(N, d * k).to(dtype)
+def _leer_norma8(N, d, k=1, L=None):
+    """leer for norma8's output, (N, d k): the columns of a causal window of k tokens over texts of L (k = 1: as it was)."""
+    m, s, _ = _partes8(N, d, datos=2)
+
+    def leer(ts, dtype):
+        sitio, g, b = ts
+        q, dev = sitio.data_ptr(), sitio.device
+        g, b = _c(g.detach(), torch.float32), _c(b.detach(), torch.float32)
+        if _norma8_propia(d) and not (g.data_ptr() | b.data_ptr()) % 16:
+            out = torch.empty((N, d * k), dtype=dtype, device=dev)
+            _en(dev, 'asrn_norm8_read', q, q + s, ptr(g), ptr(b), q + m, 1 if L is None else N // L, L or N, d, k,
+                int(dtype == torch.bfloat16), ptr(out))
+            return out
+        mu, rstd = sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1)
+        y = (_leer8(q, q + s, N, d, dev, torch.float32) - mu) * rstd * g + b
+        if k == 1:
+            return y.to(dtype)
+        return F.pad(y.view(-1, L, d), (0, 0, k - 1, 0)).unfold(1, k, 1).reshape(N, d * k).to(dtype)
+    return leer
 
 
 def norma8(ln, x, dtype):
@@ -1785,12 +1820,14 @@ def norma8(ln, x, dtype):
             and torch.is_grad_enabled() and ln.elementwise_affine and ln.bias is not None
             and tuple(ln.normalized_shape) == (d,)):
         return *norma_residual(ln, x, dtype), None
-    y, x, q, e, stats = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
-    return y, x, Guardado8(_norma8_leer, (q, e, stats, ln.weight, ln.bias))
+    y, x, sitio = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
+    return y, x, Guardado8(_leer_norma8(x.numel() // d, d), (sitio, ln.weight, ln.bias))
 
 
 def ventana8(z, k, dtype, guardado):
     """(ventana_causal(z, k, dtype), what lineal8 reads those columns from) for the output z (B, L, d) fp32 of norma8 and
     what norma8 kept."""
-    L = z.shape[1]
-    return ventana_causal(z, k, dtype), guardado and Guardado8(lambda ts, dt: _norma8_leer(ts, dt, k, L), guardado.tensores)
+    if guardado is None:
+        return ventana_causal(z, k, dtype), None
+    B, L, d = z.shape
+    return ventana_causal(z, k, dtype), Guardado8(_leer_norma8(B * L, d, k, L), guardado.tensores)
