@@ -18,8 +18,8 @@
 namespace asrn {
 
 constexpr int kPfThreads = 256;
-constexpr int kPfUnroll = 8;
-constexpr int kPfPiece = kPfUnroll * kPfThreads;       // tokens a workgroup sums, all loads in flight at once
+constexpr int kPfUnroll = 2;
+constexpr int kPfPiece = 4 * kPfUnroll * kPfThreads;       // tokens a workgroup sums, all loads in flight at once
 constexpr int kPfLossThreads = 1024;
 
 struct PfPart { double sum; double n; };
@@ -34,28 +34,33 @@ struct PfArgs {
   const float* g; float* dlp;
 };
 
+// ROW: a text's tokens lie next to each other and are read 4 at a time
+template <bool ROW>
 __global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
   __shared__ PfPart red[kPfThreads / kWave];
   const int64_t row = blockIdx.x / a.pieces, t0 = (int64_t)(blockIdx.x % a.pieces) * kPfPiece;
   const int64_t t1 = t0 + kPfPiece < a.L ? t0 + kPfPiece : a.L;
   double s = 0.0;
   int n = 0;
-  for (int64_t tb = t0 + threadIdx.x; tb < t1; tb += kPfUnroll * kPfThreads) {
-    float x[kPfUnroll], r[kPfUnroll];
-    bool m[kPfUnroll];
+  const bool ref = a.ref.p && !a.ref_rows;
+  float x[kPfUnroll][4], r[kPfUnroll][4];
+  uint32_t m[kPfUnroll];
 #pragma unroll
-    for (int u = 0; u < kPfUnroll; ++u) {
-      const int64_t t = tb + u * kPfThreads, tc = t < t1 ? t : tb;
-      m[u] = a.mask.on(row, tc) && t < t1;
-      x[u] = a.lp.at(row, tc);
-      r[u] = a.ref.p && !a.ref_rows ? a.ref.at(row, tc) : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < kPfUnroll; ++u) {     // selected, not multiplied: what a mask hides may be infinite or NaN
-      s += m[u] ? (double)x[u] - (double)r[u] : 0.0;
-      n += m[u];
-    }
+  for (int u = 0; u < kPfUnroll; ++u) {
+    const int64_t t = t0 + 4 * (threadIdx.x + u * kPfThreads);
+    const int k = t1 - t >= 4 ? 4 : t1 > t ? (int)(t1 - t) : 0;
+    m[u] = a.mask.on4<ROW>(row, t, k);
+    a.lp.four<ROW>(row, t, k, 0.f, x[u]);
+    if (ref) a.ref.four<ROW>(row, t, k, 0.f, r[u]);
   }
+#pragma unroll
+  for (int u = 0; u < kPfUnroll; ++u)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {             // selected, not multiplied: what a mask hides may be infinite or NaN
+      const bool on = m[u] >> (8 * k) & 0xffu;
+      s += on ? (double)x[u][k] - (ref ? (double)r[u][k] : 0.0) : 0.0;
+      n += on;
+    }
   s = wave_sum_d(s);
   double c = wave_sum_d((double)n);
   if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = PfPart{s, c};
@@ -124,11 +129,25 @@ __global__ __launch_bounds__(kPfLossThreads) void k_pref_loss(PfArgs a) {
   }
 }
 
+template <bool ROW>
 __global__ __launch_bounds__(kPfThreads) void k_pref_bwd(PfArgs a) {
   const int64_t row = blockIdx.x / a.pieces, t0 = (int64_t)(blockIdx.x % a.pieces) * kPfPiece;
   const float c = a.coef[row] * *a.g;
   const int64_t t1 = t0 + kPfPiece < a.L ? t0 + kPfPiece : a.L;
-  for (int64_t t = t0 + threadIdx.x; t < t1; t += kPfThreads) a.dlp[row * a.L + t] = a.mask.on(row, t) ? c : 0.f;
+  for (int64_t t = t0 + 4 * threadIdx.x; t < t1; t += 4 * kPfThreads) {
+    const int n = t1 - t < 4 ? (int)(t1 - t) : 4;
+    const uint32_t m = a.mask.on4<ROW>(row, t, n);
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = m >> (8 * k) & 0xffu ? c : 0.f;
+    if (n == 4) {
+      __builtin_memcpy(a.dlp + row * a.L + t, v, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < n) a.dlp[row * a.L + t + k] = v[k];
+    }
+  }
 }
 
 }  // namespace asrn
@@ -172,7 +191,9 @@ extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, c
   a.part = (PfPart*)workspace; a.pieces = (uint32_t)pf_pieces(L); a.lanes = lanes_for(a.pieces);
   a.loss = loss; a.reward = rewards; a.coef = coef;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(k_pref_rows, dim3((unsigned)(a.pieces * 2 * P)), dim3(kPfThreads), 0, st, a);
+  const dim3 grid((unsigned)(a.pieces * 2 * P)), block(kPfThreads);
+  if (a.lp.row() && a.mask.row() && (a.ref_rows || a.ref.row())) hipLaunchKernelGGL(k_pref_rows<true>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(k_pref_rows<false>, grid, block, 0, st, a);
   if (check_launch("asrn_preference_fwd")) return 1;
   hipLaunchKernelGGL(k_pref_loss, dim3(1), dim3(kPfLossThreads), 0, st, a);
   return check_launch("asrn_preference_fwd");
@@ -187,6 +208,8 @@ extern "C" int asrn_preference_bwd(const float* coef, const float* g, const uint
   if (mask) a.mask = Strided{mask, mask_strides[0], mask_strides[1]};
   a.P = P; a.L = L; a.coef = const_cast<float*>(coef); a.g = g; a.dlp = dlp;
   a.pieces = (uint32_t)pf_pieces(L);
-  hipLaunchKernelGGL(k_pref_bwd, dim3((unsigned)(a.pieces * 2 * P)), dim3(kPfThreads), 0, (hipStream_t)stream, a);
+  const dim3 grid((unsigned)(a.pieces * 2 * P)), block(kPfThreads);
+  if (a.mask.row()) hipLaunchKernelGGL(k_pref_bwd<true>, grid, block, 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(k_pref_bwd<false>, grid, block, 0, (hipStream_t)stream, a);
   return check_launch("asrn_preference_bwd");
 }

@@ -13,6 +13,32 @@ struct Strided {
   __device__ __forceinline__ bool on(int64_t b, int64_t t) const {
     return !p || reinterpret_cast<const uint8_t*>(p)[b * sb + t * st] != 0;
   }
+  // n <= 4 tokens from t (the rest as `other`). ROW: tokens adjacent, read as one vector from any element's address
+  template <bool ROW>
+  __device__ __forceinline__ void four(int64_t b, int64_t t, int n, float other, float* x) const {
+    if (ROW && n == 4) {
+      __builtin_memcpy(x, reinterpret_cast<const float*>(p) + b * sb + t, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = k < n ? at(b, t + k) : other;
+    }
+  }
+  // the mask of n <= 4 tokens from t, a byte each (the rest 0)
+  template <bool ROW>
+  __device__ __forceinline__ uint32_t on4(int64_t b, int64_t t, int n) const {
+    uint32_t w = 0;
+    if (!p) {
+      w = 0x01010101u;
+    } else if (ROW && n == 4) {
+      __builtin_memcpy(&w, reinterpret_cast<const uint8_t*>(p) + b * sb + t, 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < n) w |= (uint32_t)reinterpret_cast<const uint8_t*>(p)[b * sb + (t + k) * st] << (8 * k);
+    }
+    return n == 4 ? w : n > 0 ? w & ((1u << (8 * n)) - 1u) : 0u;
+  }
+  bool row() const { return !p || st == 1; }
 };
 
 // sums of doubles over the wave, in a fixed order: DPP rotations within each row of 16 lanes (no LDS), the rows by lane
