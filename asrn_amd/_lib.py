@@ -159,6 +159,23 @@ def load(path=LIB_PATH):
     return lib
 
 
+_nodos = None
+
+
+def nodos():
+    """The C++ autograd nodes (csrc/nodos.cpp), over the entry points of the library that load() opened."""
+    global _nodos
+    if _nodos is None:
+        lib = load()
+        try:
+            from . import _nodos as modulo
+        except ImportError as e:
+            raise ASRNHipError(f'asrn_amd/_nodos.so is missing or does not load: build it with `python -m asrn_amd.build` ({e})')
+        modulo.iniciar(lambda nombre: ctypes.cast(getattr(lib, nombre), _P).value, ASRNHipError)
+        _nodos = modulo
+    return _nodos
+
+
 def ptr(t):
     """Device pointer of a tensor (None -> NULL)."""
     return None if t is None else ctypes.c_void_p(t.data_ptr())

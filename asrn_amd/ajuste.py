@@ -8,35 +8,22 @@ texts and the clipped policy loss, each with its gradient, on the library's kern
 The reference package has no counterpart; the functions stand beside the model's loss (ops.cross_entropy). GPU only.
 Nothing waits on the host, so a step over them can be captured in a HIP graph.
 """
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import ptr, query
-from .ops import _dev, _en
+from ._lib import nodos
+from .ops import _dev
 
 TIPOS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # the kernels' logits
 FORMAS = ('sigmoide', 'ipo', 'bisagra')
 REDUCCIONES = ('fichas', 'textos')
 
 
-def _denso(g):
-    """An upstream gradient as contiguous fp32."""
-    return (g if g.dtype == torch.float32 else g.float()).contiguous()
-
-
 def _mismo_gpu(quien, dev, **tensores):
     for n, t in tensores.items():
         if t is not None and t.device != dev:
             raise ValueError(f'{quien}: {n} is on {t.device}, the rest on {dev}')
-
-
-def _pasos(*ts):
-    """The row and token strides of (B, L) tensors (0, 0 for None) as the C array the kernels' entry points take."""
-    s = [v for t in ts for v in ((0, 0) if t is None else t.stride())]
-    return (ctypes.c_int64 * len(s))(*s)
 
 
 def _mascara(quien, m, forma, dev):
@@ -70,57 +57,6 @@ def _numero(quien, nombre, v, minimo, maximo=math.inf, abierto=False):
 # log-probabilities of given tokens
 # ---------------------------------------------------------------------------------------------------------------------
 
-def _filas(x):
-    """logits (..., V) as (row count, L, stride over b, stride over t) for rows b L + t read in place, and the tensor
-    they are read from: a (B, L, V) slice needs no copy, more leading axes are flattened."""
-    V = x.shape[-1]
-    if x.stride(-1) != 1 and V > 1:
-        x = x.contiguous()
-    if x.dim() > 3:
-        x = x.reshape(-1, *x.shape[-2:])
-    if x.dim() == 1:
-        return 1, 1, 0, 0, x
-    if x.dim() == 2:
-        return x.shape[0], x.shape[0], 0, x.stride(0), x
-    return x.shape[0] * x.shape[1], x.shape[1], x.stride(0), x.stride(1), x
-
-
-class LogProbabilidades(torch.autograd.Function):
-    """asrn_token_logp_fwd/bwd: (log-probabilities, entropies or None) of rows of logits, fp32; the gradient comes back
-    in the logits' dtype."""
-
-    @staticmethod
-    def forward(ctx, logits, y, ignorar, inv_t, entropia):
-        dev, V = logits.device, logits.shape[-1]
-        filas, L, sb, st, x = _filas(logits)
-        t = y.reshape(-1)
-        lp = torch.empty(y.shape, dtype=torch.float32, device=dev)
-        stats = torch.empty((filas, 2), dtype=torch.float32, device=dev)
-        H = torch.empty(y.shape, dtype=torch.float32, device=dev) if entropia else None
-        if filas:
-            _en(dev, 'asrn_token_logp_fwd', ptr(x), TIPOS[x.dtype], filas, L, V, sb, st, ptr(t), ignorar, inv_t, ptr(lp),
-                    ptr(H), ptr(stats))
-        ctx.save_for_backward(x, t, stats, H)
-        ctx.meta = (filas, L, sb, st, ignorar, inv_t, logits.shape)
-        ctx.set_materialize_grads(False)
-        return lp, H
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, gh):
-        x, t, stats, H = ctx.saved_tensors
-        filas, L, sb, st, ignorar, inv_t, forma = ctx.meta
-        if g is None and gh is None:
-            return None, None, None, None, None
-        g = None if g is None else _denso(g)
-        gh = None if gh is None else _denso(gh)
-        dx = torch.empty(forma, dtype=x.dtype, device=x.device)
-        if filas:
-            _en(x.device, 'asrn_token_logp_bwd', ptr(x), TIPOS[x.dtype], filas, L, forma[-1], sb, st, ptr(t), ignorar, inv_t,
-                    ptr(stats), ptr(H), ptr(g), ptr(gh), ptr(dx))
-        return dx, None, None, None, None
-
-
 def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False):
     """log softmax(logits / temperatura) at the tokens y, in fp32: logits (..., V) fp32, bf16 or fp16, read as they are
     through their strides (no fp32 copy), y (...) integers. 0 where y == ignorar, and no gradient there; NaN for a token
@@ -138,52 +74,20 @@ def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False)
         raise ValueError(f'{quien}: {y.numel()} tokens (up to 2**31 - 1)')
     _mismo_gpu(quien, dev, y=y)
     T = _numero(quien, 'temperatura', temperatura, 1e-6, 1e6)
-    lp, H = LogProbabilidades.apply(logits, y.to(torch.int64), int(ignorar), 1.0 / T, bool(entropia))
+    x, t = logits, y.to(torch.int64).contiguous()
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if x.dim() > 3:                                  # more leading axes are flattened; a (B, L, V) slice needs no copy
+        x, t = x.reshape(-1, *x.shape[-2:]), t.view(-1, t.shape[-1])
+    lp, H = nodos().logp(x, t, TIPOS[x.dtype], int(ignorar), 1.0 / T, bool(entropia))
+    if logits.dim() > 3:
+        lp, H = lp.view(y.shape), H if H is None else H.view(y.shape)
     return (lp, H) if entropia else lp
 
 
 # ---------------------------------------------------------------------------------------------------------------------
 # the preference loss
 # ---------------------------------------------------------------------------------------------------------------------
-
-class Preferencia(torch.autograd.Function):
-    """asrn_preference_fwd/bwd: (loss, rewards) of lp (2P, L); the gradient of a row is one coefficient, kept from the
-    forward."""
-
-    @staticmethod
-    def forward(ctx, lp, fijos):
-        m, ref, forma, beta, suavizado, margen, por_longitud = fijos      # constants: no autograd around them
-        dev = lp.device
-        P, L = lp.shape[0] // 2, lp.shape[1]
-        perdida = torch.empty((), dtype=torch.float32, device=dev)
-        rec = torch.empty((2 * P,), dtype=torch.float32, device=dev)
-        wsb = query('asrn_preference_workspace', P, L)
-        ws = torch.empty((max(wsb, 0) + 8 * P,), dtype=torch.uint8, device=dev)
-        coef = ws.data_ptr() + max(wsb, 0)           # the rows' coefficients, kept for the backward, behind the workspace
-        por_fila = ref is not None and ref.dim() == 1
-        ref_pasos = None if ref is None else (ctypes.c_int64 * 2)(ref.stride(0), 0) if por_fila else _pasos(ref)
-        _en(dev, 'asrn_preference_fwd', ptr(lp), _pasos(lp), ptr(ref), ref_pasos, int(por_fila), ptr(m),
-                None if m is None else _pasos(m), P, L, FORMAS.index(forma), beta, suavizado, margen, int(por_longitud),
-                ptr(perdida), ptr(rec), coef, ptr(ws), wsb)
-        ctx.save_for_backward(ws, m)
-        ctx.meta = (P, L, max(wsb, 0))
-        ctx.mark_non_differentiable(rec)
-        ctx.set_materialize_grads(False)
-        return perdida, rec
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        ws, m = ctx.saved_tensors
-        P, L, wsb = ctx.meta
-        if g is None:
-            return None, None
-        dlp = torch.empty((2 * P, L), dtype=torch.float32, device=ws.device)
-        gc = _denso(g)
-        _en(ws.device, 'asrn_preference_bwd', ws.data_ptr() + wsb, ptr(gc), ptr(m), None if m is None else _pasos(m), P, L,
-                ptr(dlp))
-        return dlp, None
-
 
 def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', suavizado=0.0, margen=0.0,
                         por_longitud=False):
@@ -215,54 +119,12 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
     if suavizado and tipo != 'sigmoide':
         raise ValueError(f"{quien}: suavizado belongs to tipo='sigmoide'")
     margen = _numero(quien, 'margen', margen, -math.inf)
-    return Preferencia.apply(_f32(lp), (m, ref, tipo, beta, suavizado, margen, bool(por_longitud)))
+    return nodos().preferencia(_f32(lp), m, ref, FORMAS.index(tipo), beta, suavizado, margen, bool(por_longitud))
 
 
 # ---------------------------------------------------------------------------------------------------------------------
 # the policy loss
 # ---------------------------------------------------------------------------------------------------------------------
-
-class Politica(torch.autograd.Function):
-    """asrn_policy_fwd/bwd: (loss, statistics) of lp and the entropies H (B, L); the tokens' gradients before the
-    reduction are kept from the forward, in fp32."""
-
-    @staticmethod
-    def forward(ctx, lp, H, fijos):
-        A, vieja, ref, m, lo, hi, tope, beta, peso, por_texto = fijos     # constants: no autograd around them
-        dev = lp.device
-        B, L = lp.shape
-        perdida = torch.empty((), dtype=torch.float32, device=dev)
-        datos = torch.empty((4,), dtype=torch.float32, device=dev)
-        # one buffer: the workspace, then what the backward needs: the texts' divisors and the tokens' gradients
-        wsb = query('asrn_policy_workspace', B, L)
-        fin = max(wsb, 0)
-        ws = torch.empty((fin + 4 * B + (4 * B * L if ctx.needs_input_grad[0] else 0),), dtype=torch.uint8, device=dev)
-        div = ws.data_ptr() + fin
-        crudo = div + 4 * B if ctx.needs_input_grad[0] else None
-        _en(dev, 'asrn_policy_fwd', ptr(lp), ptr(A), ptr(vieja), ptr(ref), ptr(H), ptr(m), _pasos(lp, A, vieja, ref, H, m),
-                B, L, lo, hi, tope, beta, peso, int(por_texto), crudo, ptr(perdida), ptr(datos), div, ptr(ws), wsb)
-        ctx.save_for_backward(ws, m)
-        ctx.meta = (B, L, peso, fin)
-        ctx.mark_non_differentiable(datos)
-        ctx.set_materialize_grads(False)
-        return perdida, datos
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        ws, m = ctx.saved_tensors
-        B, L, peso, fin = ctx.meta
-        if g is None:
-            return None, None, None
-        dev = ws.device
-        dlp = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
-        dH = torch.empty((B, L), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-        gc = _denso(g)
-        div = ws.data_ptr() + fin
-        _en(dev, 'asrn_policy_bwd', div + 4 * B, div, ptr(gc), ptr(m), None if m is None else _pasos(m), B, L, peso, ptr(dlp),
-            ptr(dH))
-        return dlp, dH, None
-
 
 def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope=None, lp_ref=None, beta=0.0,
                      entropia=None, peso_entropia=0.0, reduccion='fichas'):
@@ -302,8 +164,8 @@ def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope
         raise ValueError(f'{quien}: peso_entropia={peso} needs entropia')
     if reduccion not in REDUCCIONES:
         raise ValueError(f'{quien}: reduccion={reduccion!r}: one of {REDUCCIONES}')
-    return Politica.apply(_f32(lp), _f32(entropia), (_fijo(ventaja), _fijo(lp_vieja), _fijo(lp_ref), m, lo, hi, tope, beta,
-                                                     peso, reduccion == 'textos'))
+    return nodos().politica(_f32(lp), _f32(entropia), _fijo(ventaja), _fijo(lp_vieja), _fijo(lp_ref), m, lo, hi, tope, beta, peso,
+                            reduccion == 'textos')
 
 
 token_log_probs, preference_loss, policy_loss = log_probabilidades, perdida_preferencia, perdida_politica

@@ -1,4 +1,5 @@
-"""Builds libasrn_hip.so (the C-ABI library of HIP kernels for gfx950) in-tree with hipcc.
+"""Builds libasrn_hip.so (the C-ABI library of HIP kernels for gfx950) in-tree with hipcc, and _nodos.so (autograd nodes
+in C++ over its entry points, host code only) with the C++ compiler against the installed PyTorch.
 
     python -m asrn_amd.build            # or asrn_amd.build.build()
 
@@ -14,6 +15,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libasrn_hip.so')
+NODOS = os.path.join(HERE, '_nodos.so')
 SOURCES = ['errors.hip', 'bucket_sort.hip', 'ngram.hip', 'scan.hip', 'candidates.hip', 'decode.hip',
            'decode_produce.hip', 'gate.hip', 'context.hip', 'hidden.hip', 'reduce.hip', 'small_gemm.hip', 'gemm.hip', 'blocks.hip',
            'phi.hip', 'sampling.hip', 'block_step.hip', 'cross_entropy.hip', 'conv_window.hip',
@@ -33,11 +35,30 @@ def hipcc():
     raise RuntimeError('hipcc not found: the ASRN HIP library needs ROCm')
 
 
+def orden_nodos(salida):
+    """The command that compiles csrc/nodos.cpp into `salida`."""
+    import sysconfig
+
+    import torch
+    raiz = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    return [os.environ.get('CXX') or shutil.which('g++') or os.path.join(rocm, 'llvm', 'bin', 'clang++'),
+            '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', f'-I{INCLUDE}',
+            f"-I{os.path.join(raiz, 'include')}", f"-I{os.path.join(raiz, 'include', 'torch', 'csrc', 'api', 'include')}",
+            f"-I{os.path.join(rocm, 'include')}", f"-I{sysconfig.get_paths()['include']}", os.path.join(CSRC, 'nodos.cpp'),
+            '-o', salida, f"-L{os.path.join(raiz, 'lib')}", '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip', '-ltorch_hip',
+            '-ltorch_python']
+
+
 def build(verbose=False, jobs=None):
-    """Compiles every source (in parallel) and links the shared library atomically. Raises on any error."""
+    """Compiles every source (in parallel), links the shared library and places it and the nodes atomically. Raises on any
+    error."""
     cc = hipcc()
     with tempfile.TemporaryDirectory(prefix='asrn_build_') as tmp:
-        procs = []
+        tmp_nodos = os.path.join(tmp, '_nodos.so')
+        procs = [('nodos.cpp', subprocess.Popen(orden_nodos(tmp_nodos), stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                                text=True))]
         objs = []
         for src in SOURCES:
             obj = os.path.join(tmp, src.replace('.hip', '.o'))
@@ -54,14 +75,15 @@ def build(verbose=False, jobs=None):
             elif verbose and out.strip():
                 print(out)
         if errors:
-            raise RuntimeError('hipcc failed:\n' + '\n'.join(errors))
+            raise RuntimeError('compiling failed:\n' + '\n'.join(errors))
         tmp_lib = os.path.join(tmp, 'libasrn_hip.so')
         cmd = [cc, '-shared', '-fPIC', f'--offload-arch={ARCH}', *objs, '-o', tmp_lib]
         r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         if r.returncode != 0:
             raise RuntimeError('link failed:\n' + r.stdout)
-        shutil.copyfile(tmp_lib, LIB + '.tmp')
-        os.replace(LIB + '.tmp', LIB)
+        for hecho, sitio in ((tmp_lib, LIB), (tmp_nodos, NODOS)):
+            shutil.copyfile(hecho, sitio + '.tmp')
+            os.replace(sitio + '.tmp', sitio)
     return LIB
 
 

@@ -13,7 +13,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, query, stream_of
+from ._lib import call, nodos, ptr, query, stream_of
 from .lineal import column_sums, gemm, lineal8, weight_grad
 
 I32 = torch.int32
@@ -1623,11 +1623,6 @@ def _partes8(N, d, datos=0):
     return m, s, s + N * -(-d // GRUPO8)
 
 
-def _sitio8(N, d, dev, datos=0):
-    m, s, fin = _partes8(N, d, datos)
-    return torch.empty((fin,), dtype=torch.uint8, device=dev), m, s
-
-
 def guardar8(x):
     """x (..., d) fp32 or bf16 in 8 bits: (codes int8 (N, d), scale bytes uint8 (N, ceil(d / 32))). Per 32 neighbouring
     channels the smallest 2^e with max |x| <= 127 2^e (-126 <= e <= 121; the byte is e + 127) and the integers nearest to
@@ -1660,47 +1655,6 @@ def _leer8(q, e, N, d, dev, dtype, gelu=False):
     return out
 
 
-class Gelu8(torch.autograd.Function):
-    """asrn_gelu8_fwd/bwd: gelu(u), or h + gelu(u) (h fp32; gelu rounds to u's dtype first, as the separate ops do), with
-    u kept in 8 bits for the backward; returns also what is kept."""
-
-    @staticmethod
-    def forward(ctx, u, h):
-        dev, forma, bf16 = u.device, u.shape, u.dtype == torch.bfloat16
-        d = forma[-1]
-        u, N = u.contiguous(), u.numel() // d
-        sitio, _, s = _sitio8(N, d, dev)
-        if h is None:
-            out = torch.empty(forma, dtype=u.dtype, device=dev)
-        else:
-            h = h.contiguous()
-            out = torch.empty(forma, dtype=torch.float32, device=dev)
-        q = sitio.data_ptr()
-        _en(dev, 'asrn_gelu8_fwd', ptr(u), int(bf16), ptr(h), N, d, ptr(out), q, q + s)
-        ctx.save_for_backward(sitio)
-        ctx.meta = (bf16, forma, N, d, s)
-        ctx.mark_non_differentiable(sitio)
-        ctx.set_materialize_grads(False)
-        return out, sitio
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        sitio, = ctx.saved_tensors
-        bf16, forma, N, d, s = ctx.meta
-        if g is None:
-            return None, None
-        gu = None
-        if ctx.needs_input_grad[0]:
-            gc = g.contiguous()
-            if gc.dtype not in (torch.float32, torch.bfloat16):
-                gc = gc.float()
-            gu = torch.empty(forma, dtype=torch.bfloat16 if bf16 else torch.float32, device=sitio.device)
-            q = sitio.data_ptr()
-            _en(sitio.device, 'asrn_gelu8_bwd', q, q + s, ptr(gc), int(gc.dtype == torch.bfloat16), N, d, int(bf16), ptr(gu))
-        return gu, g if ctx.needs_input_grad[1] else None
-
-
 def _gelu8_ok(u):
     return u.is_cuda and u.dtype in (torch.float32, torch.bfloat16) and u.dim() >= 1 and u.numel() > 0 and torch.is_grad_enabled()
 
@@ -1718,7 +1672,7 @@ def gelu8(u):
     dtype: (F.gelu(u), None)."""
     if not _gelu8_ok(u):
         return F.gelu(u), None
-    y, sitio = Gelu8.apply(u, None)
+    y, sitio = nodos().gelu8(u, None)
     d = u.shape[-1]
     return y, Guardado8(_leer_gelu8(u.numel() // d, d), (sitio,))
 
@@ -1726,13 +1680,13 @@ def gelu8(u):
 def suma_gelu8(h, u):
     """h + F.gelu(u) with u kept in 8 bits: h fp32 of u's shape; else the separate ops, gelu8 among them."""
     if _gelu8_ok(u) and h.dtype == torch.float32 and h.shape == u.shape and h.device == u.device:
-        return Gelu8.apply(u, h)[0]
+        return nodos().gelu8(u, h)[0]
     return h + gelu8(u)[0]
 
 
 class Norma8(torch.autograd.Function):
-    """NormaResidual that keeps x in 8 bits (and (mean, rstd) per row, of x itself): asrn_norm8_fwd/bwd where d is a
-    multiple of 4 up to 1024, else the same with torch's LayerNorm and asrn_pack8. Returns also what is kept."""
+    """norma8's op for the widths that asrn_norm8_fwd does not take (no multiple of 4, or past 1024): torch's LayerNorm and
+    asrn_pack8, the same values kept in the same places."""
 
     @staticmethod
     def forward(ctx, x, gamma, beta, eps, dtype):
@@ -1740,53 +1694,33 @@ class Norma8(torch.autograd.Function):
         d = forma[-1]
         x2, N = x.contiguous(), x.numel() // d
         g, b = _c(gamma, torch.float32), _c(beta, torch.float32)
-        sitio, m, s = _sitio8(N, d, dev, datos=2)
+        m, s, fin = _partes8(N, d, datos=2)
+        sitio = torch.empty((fin,), dtype=torch.uint8, device=dev)
+        y, mu, rstd = torch.native_layer_norm(x2, (d,), g, b, eps)
+        sitio[m:m + 8 * N].view(torch.float32).view(N, 2).copy_(torch.cat([mu.view(N, 1), rstd.view(N, 1)], 1))
         q = sitio.data_ptr()
-        if _norma8_propia(d) and not (x2.data_ptr() | g.data_ptr() | b.data_ptr()) % 16:
-            y = torch.empty(forma, dtype=dtype, device=dev)
-            _en(dev, 'asrn_norm8_fwd', ptr(x2), ptr(g), ptr(b), N, d, eps, int(dtype == torch.bfloat16), ptr(y), q + m, q, q + s)
-        else:
-            y, mu, rstd = torch.native_layer_norm(x2, (d,), g, b, eps)
-            y = y.to(dtype)
-            sitio[m:m + 8 * N].view(torch.float32).view(N, 2).copy_(torch.cat([mu.view(N, 1), rstd.view(N, 1)], 1))
-            _en(dev, 'asrn_pack8', ptr(x2), 0, N, d, q, q + s)
+        _en(dev, 'asrn_pack8', ptr(x2), 0, N, d, q, q + s)
         ctx.save_for_backward(sitio, g)
         ctx.meta = (forma, N, d, m, s)
         ctx.mark_non_differentiable(sitio)
-        return y, x2.view(forma), sitio
+        return y.to(dtype), x2.view(forma), sitio
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dres, _):
         sitio, g = ctx.saved_tensors
         forma, N, d, m, s = ctx.meta
-        dev, q = sitio.device, sitio.data_ptr()
-        bf16 = dy.dtype == torch.bfloat16
-        dy = _a16(_c(dy) if bf16 else _c(dy, torch.float32))
-        dres = _a16(_c(dres, torch.float32))
-        if _norma8_propia(d) and g.data_ptr() % 16 == 0:
-            dx = torch.empty(forma, dtype=torch.float32, device=dev)
-            wsb = query('asrn_norm8_bwd_workspace', N, d)
-            dp = torch.empty((2, d), dtype=torch.float32, device=dev)
-            ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
-            _en(dev, 'asrn_norm8_bwd', q, q + s, ptr(g), q + m, N, d, ptr(dy), int(bf16), ptr(dres), ptr(dx), ptr(dp), ptr(ws), wsb)
-            dg, db = dp.unbind(0)
-            return dx, dg, db, None, None
+        q = sitio.data_ptr()
         mu, rstd = sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1)
-        xh = (_leer8(q, q + s, N, d, dev, torch.float32) - mu) * rstd
-        f = dy.float().view(N, d)
+        xh = (_leer8(q, q + s, N, d, sitio.device, torch.float32) - mu) * rstd
+        f = dy.float().reshape(N, d)
         p = f * g
-        dx = rstd * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True)) + dres.view(N, d)
+        dx = rstd * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True)) + dres.reshape(N, d)
         return dx.view(forma), (f * xh).sum(0), f.sum(0), None, None
 
 
 def _norma8_propia(d):
     return d % 4 == 0 and d <= 1024
-
-
-def _a16(t):
-    """t, copied if its rows lie off the 16-byte boundary that the kernels read from."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _leer_norma8(N, d, k=1, L=None):
@@ -1820,7 +1754,10 @@ def norma8(ln, x, dtype):
             and torch.is_grad_enabled() and ln.elementwise_affine and ln.bias is not None
             and tuple(ln.normalized_shape) == (d,)):
         return *norma_residual(ln, x, dtype), None
-    y, x, sitio = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
+    if _norma8_propia(d):
+        y, x, sitio = nodos().norma8(x, ln.weight, ln.bias, ln.eps, dtype == torch.bfloat16)
+    else:
+        y, x, sitio = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
     return y, x, Guardado8(_leer_norma8(x.numel() // d, d), (sitio, ln.weight, ln.bias))
 
 
