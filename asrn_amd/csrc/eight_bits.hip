@@ -24,7 +24,8 @@ namespace asrn {
 constexpr int kE8Threads = 256;
 constexpr int kE8Waves = kE8Threads / kWave;
 constexpr int kE8Group = 32;
-constexpr int kE8MaxD4 = 4;                   // the LayerNorm's widths: d <= 1024
+constexpr int kE8MaxD = 8192;                 // the LayerNorm's widths
+constexpr int kE8WaveD = 1024;                // up to this a wave takes a row, past it a workgroup
 
 typedef __bf16 e8_b2 __attribute__((ext_vector_type(2)));
 typedef float e8_f2 __attribute__((ext_vector_type(2)));
@@ -237,9 +238,17 @@ struct N8Args {
   void* y; float2* stats; uint32_t* q; uint8_t* e; int groups;      // q as words of 4 channels
   const void* dy; const float* dres; float* dx; float* partial;
   int64_t L; int k;
+  int per;                                    // backward: rows of a workgroup
 };
 constexpr int kN8FwdRows = 2;                 // rows a wave has in flight
-constexpr int kN8BwdRows = 32;                // rows a backward's workgroup takes
+// Rows a backward's workgroup takes: enough workgroups for two a CU, as long as each has 8 rows at least (its partial row
+// of parameter gradients costs as much as 2 rows), 32 at most (us with 32 always / so: 1505 x 260 11.0 / 7.7, 4096 x 2048
+// 54.8 / 23.2, 4096 x 8192 258 / 107)
+constexpr int kN8BwdLeast = 8, kN8BwdMost = 32, kN8BwdGroups = 512;
+static int n8_bwd_rows(int64_t rows) {
+  const int64_t per = (rows + kN8BwdGroups - 1) / kN8BwdGroups;
+  return per <= kN8BwdLeast ? kN8BwdLeast : per >= kN8BwdMost ? kN8BwdMost : (int)((per + 7) / 8 * 8);
+}
 
 __device__ __forceinline__ float n8_dot(const float4& a, const float4& b) { return a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w; }
 template <bool B16>
@@ -256,6 +265,25 @@ template <bool B16>
 __device__ __forceinline__ void n8_store(void* p, int64_t quad, const float4& v) {
   if constexpr (B16) reinterpret_cast<uint2*>(p)[quad] = make_uint2(e8_pack_bf16(v.x, v.y), e8_pack_bf16(v.z, v.w));
   else reinterpret_cast<float4*>(p)[quad] = v;
+}
+
+// the 4 channels c of a row: y, the codes and, by a group's first lane, the scale's byte. All lanes of a wave call it, so
+// that a group's 8 lanes meet; x is 0 past the row (the last group's scale is that of its own channels)
+template <bool O16>
+__device__ __forceinline__ void n8_row_out(const N8Args& a, int64_t r, int c, const float4& t, float mean, float rstd) {
+  uint32_t top = e8_abs(t.x);
+  top = e8_abs(t.y) > top ? e8_abs(t.y) : top;
+  top = e8_abs(t.z) > top ? e8_abs(t.z) : top;
+  top = e8_abs(t.w) > top ? e8_abs(t.w) : top;
+  const uint32_t byte = e8_byte(max_of8(top));
+  const int d4 = a.d >> 2;
+  if (c < d4) {
+    const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], b = reinterpret_cast<const float4*>(a.beta)[c];
+    n8_store<O16>(a.y, r * d4 + c, make_float4((t.x - mean) * rstd * w.x + b.x, (t.y - mean) * rstd * w.y + b.y,
+                                               (t.z - mean) * rstd * w.z + b.z, (t.w - mean) * rstd * w.w + b.w));
+    a.q[r * d4 + c] = e8_quad(t, e8_inverse(byte));
+    if ((c & 7) == 0) a.e[r * a.groups + (c >> 3)] = (uint8_t)byte;
+  }
 }
 
 template <int D4, bool O16>
@@ -288,22 +316,7 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_fwd(N8Args a) {
       }
     const float rstd = rsqrtf(wave_sum_u(v) * inv_d + a.eps);
 #pragma unroll
-    for (int k = 0; k < D4; ++k) {
-      const int c = lane + kWave * k;
-      const float4 t = x[u][k];               // 0 past the row: the last group's scale is that of its own channels
-      uint32_t top = e8_abs(t.x);
-      top = e8_abs(t.y) > top ? e8_abs(t.y) : top;
-      top = e8_abs(t.z) > top ? e8_abs(t.z) : top;
-      top = e8_abs(t.w) > top ? e8_abs(t.w) : top;
-      const uint32_t byte = e8_byte(max_of8(top));
-      if (c < d4) {
-        const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], b = reinterpret_cast<const float4*>(a.beta)[c];
-        n8_store<O16>(a.y, r * d4 + c, make_float4((t.x - mean) * rstd * w.x + b.x, (t.y - mean) * rstd * w.y + b.y,
-                                                   (t.z - mean) * rstd * w.z + b.z, (t.w - mean) * rstd * w.w + b.w));
-        a.q[r * d4 + c] = e8_quad(t, e8_inverse(byte));
-        if ((lane & 7) == 0) a.e[r * a.groups + (c >> 3)] = (uint8_t)byte;
-      }
-    }
+    for (int k = 0; k < D4; ++k) n8_row_out<O16>(a, r, lane + kWave * k, x[u][k], mean, rstd);
     if (lane == 0) a.stats[r] = make_float2(mean, rstd);
   }
 }
@@ -313,7 +326,7 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_bwd(N8Args a) {
   __shared__ float4 red[kE8Waves][2 * D4 * kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, d4 = a.d >> 2;
   const float inv_d = 1.f / (float)a.d;
-  const int64_t r0 = (int64_t)blockIdx.x * kN8BwdRows + wave * (kN8BwdRows / kE8Waves);
+  const int64_t r0 = (int64_t)blockIdx.x * a.per + wave * (a.per / kE8Waves);
   float4 gw[D4], gb[D4], w[D4];
 #pragma unroll
   for (int k = 0; k < D4; ++k) {
@@ -322,7 +335,7 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_bwd(N8Args a) {
     if (c < d4) w[k] = reinterpret_cast<const float4*>(a.gamma)[c];
   }
   constexpr int U = 2;                        // rows in flight
-  for (int b = 0; b < kN8BwdRows / kE8Waves; b += U) {
+  for (int b = 0; b < a.per / kE8Waves; b += U) {
     uint32_t q[U][D4], e[U][D4];
     float4 dy[U][D4], dr[U][D4];
     float2 st[U];
@@ -394,6 +407,114 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_bwd(N8Args a) {
       v.x += red[i][src].x; v.y += red[i][src].y; v.z += red[i][src].z; v.w += red[i][src].w;
     }
     out[c] = v;
+  }
+}
+
+// Rows past 1,024 channels: a workgroup takes a row, 4 channels a thread and step, and the sums over the row go through
+// LDS. The backward's threads keep their own channels' parameter gradients over the workgroup's rows, so nothing is joined
+// at the end (4096 x 2048 bf16: forward 11.8 us, backward 23.2 us).
+__device__ __forceinline__ float2 n8_block_sums(float a, float b, float2* red) {
+  a = wave_sum_u(a);
+  b = wave_sum_u(b);
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x >> 6] = make_float2(a, b);
+  __syncthreads();
+  float2 r = red[0];
+#pragma unroll
+  for (int w = 1; w < kE8Waves; ++w) {
+    r.x += red[w].x;
+    r.y += red[w].y;
+  }
+  return r;
+}
+
+template <int D4, bool O16>
+__global__ __launch_bounds__(kE8Threads) void k_norm8_fwd_wide(N8Args a) {
+  __shared__ float2 red[2][kE8Waves];
+  const int tid = threadIdx.x, d4 = a.d >> 2;
+  const int64_t r = blockIdx.x;
+  const float inv_d = 1.f / (float)a.d;
+  float4 x[D4];
+  float s = 0.f, v = 0.f;
+#pragma unroll
+  for (int k = 0; k < D4; ++k) {
+    const int c = tid + kE8Threads * k;
+    x[k] = c < d4 ? reinterpret_cast<const float4*>(a.x)[r * d4 + c] : make_float4(0.f, 0.f, 0.f, 0.f);
+    s += (x[k].x + x[k].y) + (x[k].z + x[k].w);
+  }
+  const float mean = n8_block_sums(s, 0.f, red[0]).x * inv_d;
+#pragma unroll
+  for (int k = 0; k < D4; ++k)
+    if (tid + kE8Threads * k < d4) {
+      const float4 c = make_float4(x[k].x - mean, x[k].y - mean, x[k].z - mean, x[k].w - mean);
+      v += n8_dot(c, c);
+    }
+  const float rstd = rsqrtf(n8_block_sums(v, 0.f, red[1]).x * inv_d + a.eps);
+#pragma unroll
+  for (int k = 0; k < D4; ++k) n8_row_out<O16>(a, r, tid + kE8Threads * k, x[k], mean, rstd);
+  if (tid == 0) a.stats[r] = make_float2(mean, rstd);
+}
+
+template <int D4, bool D16>
+__global__ __launch_bounds__(kE8Threads) void k_norm8_bwd_wide(N8Args a) {
+  __shared__ float2 red[2][kE8Waves];
+  const int tid = threadIdx.x, d4 = a.d >> 2;
+  const float inv_d = 1.f / (float)a.d;
+  const int64_t r0 = (int64_t)blockIdx.x * a.per, r1 = r0 + a.per < a.rows ? r0 + a.per : a.rows;
+  float4 gw[D4], gb[D4];
+#pragma unroll
+  for (int k = 0; k < D4; ++k) gw[k] = gb[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t r = r0; r < r1; ++r) {
+    uint32_t q[D4], e[D4];
+    float4 xh[D4], g[D4], dr[D4];
+    const float2 st = a.stats[r];
+#pragma unroll
+    for (int k = 0; k < D4; ++k) {
+      const int c = tid + kE8Threads * k;
+      q[k] = e[k] = 0u;
+      g[k] = dr[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < d4) {
+        q[k] = a.q[r * d4 + c];
+        e[k] = a.e[r * a.groups + (c >> 3)];
+        g[k] = n8_load<D16>(a.dy, r * d4 + c);
+        if (a.dres) dr[k] = reinterpret_cast<const float4*>(a.dres)[r * d4 + c];
+      }
+    }
+    float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < D4; ++k) {
+      const int c = tid + kE8Threads * k;
+      xh[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < d4) {
+        const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], d = g[k], t = e8_open(q[k], e8_scale(e[k]));
+        xh[k] = make_float4((t.x - st.x) * st.y, (t.y - st.x) * st.y, (t.z - st.x) * st.y, (t.w - st.x) * st.y);
+        gw[k].x += d.x * xh[k].x; gw[k].y += d.y * xh[k].y; gw[k].z += d.z * xh[k].z; gw[k].w += d.w * xh[k].w;
+        gb[k].x += d.x; gb[k].y += d.y; gb[k].z += d.z; gb[k].w += d.w;
+        g[k] = make_float4(d.x * w.x, d.y * w.y, d.z * w.z, d.w * w.w);
+        m1 += (g[k].x + g[k].y) + (g[k].z + g[k].w);
+        m2 += n8_dot(g[k], xh[k]);
+      }
+    }
+    // two buffers in turn: a wave may be a row ahead of the slowest, never two
+    const float2 m = n8_block_sums(m1, m2, red[r & 1]);
+    m1 = m.x * inv_d;
+    m2 = m.y * inv_d;
+#pragma unroll
+    for (int k = 0; k < D4; ++k) {
+      const int c = tid + kE8Threads * k;
+      if (c < d4)
+        reinterpret_cast<float4*>(a.dx)[r * d4 + c] =
+            make_float4(st.y * (g[k].x - m1 - xh[k].x * m2) + dr[k].x, st.y * (g[k].y - m1 - xh[k].y * m2) + dr[k].y,
+                        st.y * (g[k].z - m1 - xh[k].z * m2) + dr[k].z, st.y * (g[k].w - m1 - xh[k].w * m2) + dr[k].w);
+    }
+  }
+  float4* out = reinterpret_cast<float4*>(a.partial) + (int64_t)blockIdx.x * 2 * d4;
+#pragma unroll
+  for (int k = 0; k < D4; ++k) {
+    const int c = tid + kE8Threads * k;
+    if (c < d4) {
+      out[c] = gw[k];
+      out[d4 + c] = gb[k];
+    }
   }
 }
 
@@ -482,8 +603,8 @@ static int e8_setup(E8Args& a, int64_t rows, int64_t d, const char* what) {
   return 0;
 }
 static int n8_check(const N8Args& a, const char* what) {
-  ASRN_REQUIRE(a.rows >= 0 && a.d > 0 && a.d % 4 == 0 && a.d <= 4 * kE8MaxD4 * kWave && a.rows < (int64_t(1) << 31),
-               "%s: bad sizes rows=%lld d=%d (a multiple of 4, <= %d)", what, (long long)a.rows, a.d, 4 * kE8MaxD4 * kWave);
+  ASRN_REQUIRE(a.rows >= 0 && a.d > 0 && a.d % 4 == 0 && a.d <= kE8MaxD && a.rows < (int64_t(1) << 31),
+               "%s: bad sizes rows=%lld d=%d (a multiple of 4, <= %d)", what, (long long)a.rows, a.d, kE8MaxD);
   return 0;
 }
 static bool e8_aligned(const void* p, unsigned to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -564,16 +685,19 @@ extern "C" int asrn_gelu8_bwd(const int8_t* q, const uint8_t* e, const void* dy,
   return check_launch("asrn_gelu8_bwd");
 }
 
+#define N8_ONE(KERNEL, D4, B16)                                                           \
+  if (B16) hipLaunchKernelGGL((KERNEL<D4, true>), grid, block, 0, st, a);                 \
+  else hipLaunchKernelGGL((KERNEL<D4, false>), grid, block, 0, st, a)
 #define N8_SWITCH(KERNEL, B16)                                                            \
   switch ((a.d + 4 * kWave - 1) / (4 * kWave)) {                                          \
-    case 1: if (B16) hipLaunchKernelGGL((KERNEL<1, true>), grid, block, 0, st, a);        \
-            else hipLaunchKernelGGL((KERNEL<1, false>), grid, block, 0, st, a); break;    \
-    case 2: if (B16) hipLaunchKernelGGL((KERNEL<2, true>), grid, block, 0, st, a);        \
-            else hipLaunchKernelGGL((KERNEL<2, false>), grid, block, 0, st, a); break;    \
-    case 3: if (B16) hipLaunchKernelGGL((KERNEL<3, true>), grid, block, 0, st, a);        \
-            else hipLaunchKernelGGL((KERNEL<3, false>), grid, block, 0, st, a); break;    \
-    default: if (B16) hipLaunchKernelGGL((KERNEL<4, true>), grid, block, 0, st, a);       \
-             else hipLaunchKernelGGL((KERNEL<4, false>), grid, block, 0, st, a); break;   \
+    case 1: N8_ONE(KERNEL, 1, B16); break;                                                \
+    case 2: N8_ONE(KERNEL, 2, B16); break;                                                \
+    case 3: N8_ONE(KERNEL, 3, B16); break;                                                \
+    case 4: N8_ONE(KERNEL, 4, B16); break;                                                \
+    default:                                                                              \
+      if (a.d <= 2048) { N8_ONE(KERNEL##_wide, 2, B16); }                                 \
+      else if (a.d <= 4096) { N8_ONE(KERNEL##_wide, 4, B16); }                            \
+      else { N8_ONE(KERNEL##_wide, 8, B16); }                                             \
   }
 
 extern "C" int asrn_norm8_fwd(const float* x, const float* gamma, const float* beta, int64_t rows, int32_t d, float eps,
@@ -588,17 +712,17 @@ extern "C" int asrn_norm8_fwd(const float* x, const float* gamma, const float* b
   ASRN_REQUIRE(e8_aligned(x, 16) && e8_aligned(gamma, 16) && e8_aligned(beta, 16) && e8_aligned(y, out_bf16 ? 8 : 16) &&
                    e8_aligned(q, 4) && e8_aligned(stats, 8),
                "asrn_norm8_fwd: rows and parameters must be 16-byte aligned (8 for bf16)");
-  const int64_t per = kE8Waves * kN8FwdRows;
+  const int64_t per = d <= kE8WaveD ? kE8Waves * kN8FwdRows : 1;
   const dim3 grid((unsigned)((rows + per - 1) / per)), block(kE8Threads);
   hipStream_t st = (hipStream_t)stream;
   N8_SWITCH(k_norm8_fwd, out_bf16)
   return check_launch("asrn_norm8_fwd");
 }
 
-static int64_t n8_bwd_groups(int64_t rows) { return rows > 0 ? (rows + kN8BwdRows - 1) / kN8BwdRows : 1; }
+static int64_t n8_bwd_groups(int64_t rows) { return rows > 0 ? (rows + n8_bwd_rows(rows) - 1) / n8_bwd_rows(rows) : 1; }
 
 extern "C" int64_t asrn_norm8_bwd_workspace(int64_t rows, int32_t d) {
-  if (rows < 0 || d <= 0 || d > 4 * kE8MaxD4 * kWave || rows >= (int64_t(1) << 31)) return -1;
+  if (rows < 0 || d <= 0 || d > kE8MaxD || rows >= (int64_t(1) << 31)) return -1;
   const int64_t groups = n8_bwd_groups(rows), part = (groups * 2 * d * 4 + 255) / 256 * 256;
   const int64_t sums = asrn_column_sums_workspace(groups, 2 * (int64_t)d);
   return sums < 0 ? -1 : part + sums;
@@ -610,7 +734,7 @@ extern "C" int asrn_norm8_bwd(const int8_t* q, const uint8_t* e, const float* ga
   N8Args a{};
   a.gamma = gamma; a.rows = rows; a.d = d; a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
   a.q = reinterpret_cast<uint32_t*>(const_cast<int8_t*>(q)); a.e = const_cast<uint8_t*>(e); a.groups = e8_groups(d);
-  a.dy = dy; a.dres = dres; a.dx = dx; a.partial = (float*)workspace;
+  a.dy = dy; a.dres = dres; a.dx = dx; a.partial = (float*)workspace; a.per = n8_bwd_rows(rows);
   if (n8_check(a, "asrn_norm8_bwd")) return 1;
   const int64_t need = asrn_norm8_bwd_workspace(rows, d);
   ASRN_REQUIRE(need >= 0 && workspace && workspace_bytes >= need && e8_aligned(workspace, 256),

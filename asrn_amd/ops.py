@@ -1685,7 +1685,7 @@ def suma_gelu8(h, u):
 
 
 class Norma8(torch.autograd.Function):
-    """norma8's op for the widths that asrn_norm8_fwd does not take (no multiple of 4, or past 1024): torch's LayerNorm and
+    """norma8's op for the widths that asrn_norm8_fwd does not take (no multiple of 4, or past 8192): torch's LayerNorm and
     asrn_pack8, the same values kept in the same places."""
 
     @staticmethod
@@ -1720,7 +1720,7 @@ class Norma8(torch.autograd.Function):
 
 
 def _norma8_propia(d):
-    return d % 4 == 0 and d <= 1024
+    return d % 4 == 0 and d <= 8192
 
 
 def _leer_norma8(N, d, k=1, L=None):

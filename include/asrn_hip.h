@@ -704,7 +704,7 @@ int asrn_policy_bwd(const float* raw, const float* weight, const float* g, const
  * norm8_fwd: asrn_layer_norm_fwd with x's q, e. norm8_bwd: asrn_layer_norm_bwd with x read from q, e: xhat =
  * (q 2^e - mean) rstd. norm8_read: y formed again from q, e and stats as the columns of a causal window of k tokens,
  * out (B, L, d k), out[b, t, c k + j] = y[b, t + j - (k - 1), c], 0 before a row's start, 1 <= k <= 16. norm8: d a
- * multiple of 4, <= 1024, rows 16-byte aligned (8 for bf16); workspace: asrn_norm8_bwd_workspace bytes, 256-byte
+ * multiple of 4, <= 8192, rows 16-byte aligned (8 for bf16); workspace: asrn_norm8_bwd_workspace bytes, 256-byte
  * aligned. */
 int asrn_pack8(const void* x, int32_t x_bf16, int64_t rows, int64_t d, int8_t* q, uint8_t* e, void* stream);
 int asrn_unpack8(const int8_t* q, const uint8_t* e, int64_t rows, int64_t d, int32_t gelu, int32_t out_bf16, void* out,

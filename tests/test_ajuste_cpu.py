@@ -72,11 +72,11 @@ def test_eight_bit_checks(lib):
     _mal(lib, lib.asrn_gelu8_fwd(16, 1, N, 4, 32, N, 16, 16, N), 'null pointer')
     _mal(lib, lib.asrn_gelu8_bwd(16, 16, N, 1, 4, 32, 1, 16, N), 'null pointer')
     _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 30, 1e-5, 0, 16, 16, 16, 16, N), 'multiple of 4')
-    _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 1028, 1e-5, 0, 16, 16, 16, 16, N), 'multiple of 4')
+    _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 8196, 1e-5, 0, 16, 16, 16, 16, N), 'multiple of 4')
     _mal(lib, lib.asrn_norm8_fwd(16, 16, 16, 4, 32, 0.0, 0, 16, 16, 16, 16, N), 'eps')
     _mal(lib, lib.asrn_norm8_fwd(24, 16, 16, 4, 32, 1e-5, 0, 16, 16, 16, 16, N), 'aligned')
     need = lib.asrn_norm8_bwd_workspace(100, 64)
-    assert need >= 4 * 2 * 64 * 4 and lib.asrn_norm8_bwd_workspace(-1, 64) == -1 and lib.asrn_norm8_bwd_workspace(1, 4096) == -1
+    assert need >= 4 * 2 * 64 * 4 and lib.asrn_norm8_bwd_workspace(-1, 64) == -1 and lib.asrn_norm8_bwd_workspace(1, 8196) == -1
     _mal(lib, lib.asrn_norm8_bwd(16, 16, 16, 16, 100, 64, 16, 0, N, 16, 16, 256, need - 1, N), 'workspace')
     _mal(lib, lib.asrn_norm8_read(16, 16, 16, 16, 16, 2, 5, 64, 17, 0, 16, N), 'k=17')
     _mal(lib, lib.asrn_norm8_read(16, 16, 16, 16, 16, 2, 5, 62, 4, 0, 16, N), 'multiple of 4')

@@ -148,7 +148,7 @@ def norma64(x, w, b, eps):
 
 
 @pytest.mark.parametrize('forma,d', [((1,), 4), ((3, 11), 64), ((2, 33), 260), ((70,), 768), ((9,), 1024), ((5,), 1028),
-                                     ((2, 3), 2048), ((7,), 10), ((33000,), 16)])
+                                     ((2, 3), 2048), ((35,), 2052), ((3,), 4096), ((33,), 8192), ((2,), 8200), ((7,), 10), ((33000,), 16)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_norm(forma, d, dtype):
     g = torch.Generator(device=DEV).manual_seed(d)
@@ -182,7 +182,7 @@ def test_norm(forma, d, dtype):
         dentro(guardado.leer(guardado.tensores, dt), yr, n * U * (1 + yr.abs() + (mu * s).abs().view(-1, 1)) + torch.finfo(dt).eps / 2 * yr.abs())
 
 
-@pytest.mark.parametrize('B,L,d,k', [(2, 9, 64, 4), (3, 5, 20, 3), (1, 1, 8, 4), (2, 3, 36, 16), (2, 40, 12, 5), (1, 6, 10, 4), (2, 4, 1028, 2), (2, 7, 64, 1)])
+@pytest.mark.parametrize('B,L,d,k', [(2, 9, 64, 4), (3, 5, 20, 3), (1, 1, 8, 4), (2, 3, 36, 16), (2, 40, 12, 5), (1, 6, 10, 4), (2, 4, 1028, 2), (1, 3, 8196, 4), (2, 7, 64, 1)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_window(B, L, d, k, dtype):
     """The columns formed again against the window of the LayerNorm's output formed again."""
