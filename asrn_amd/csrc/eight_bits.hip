@@ -103,7 +103,7 @@ __device__ __forceinline__ E8Place e8_place(const E8Args& a, int64_t i) {
     p.row = 0; p.c0 = 0; p.n = 8; p.at = 8 * i; p.group = i >> 2;
   } else {
     const uint32_t per = 4u * (uint32_t)a.groups;
-    p.row = a.lanes < (int64_t(1) << 32) ? (int64_t)((uint32_t)i / per) : i / per;
+    p.row = (uint32_t)i / per;                // lanes < 2^32
     p.c0 = 8 * (int)(i - p.row * per);
     p.n = a.d - p.c0 < 0 ? 0 : a.d - p.c0 > 8 ? 8 : a.d - p.c0;
     p.at = p.row * a.d + p.c0;
@@ -528,7 +528,7 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_run(N8Args a) {
   const int64_t runs = (a.L + kN8Run - 1) / kN8Run, texts = a.rows / a.L;
   const int64_t i = (int64_t)blockIdx.x * kE8Threads + threadIdx.x;
   if (i >= texts * runs * d4) return;
-  const int64_t run = texts * runs * d4 < (int64_t(1) << 32) ? (int64_t)((uint32_t)i / (uint32_t)d4) : i / d4;
+  const int64_t run = (uint32_t)i / (uint32_t)d4;       // lanes < 2^32
   const int c = (int)(i - run * d4);
   const int64_t b = (uint32_t)run / (uint32_t)runs, t0 = (run - b * runs) * kN8Run, r0 = b * a.L;
   const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], z = reinterpret_cast<const float4*>(a.beta)[c];
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_read(N8Args a) {
   const int d4 = a.d >> 2;
   const int64_t i = (int64_t)blockIdx.x * kE8Threads + threadIdx.x;
   if (i >= a.rows * d4) return;
-  const int64_t r = a.rows * d4 < (int64_t(1) << 32) ? (int64_t)((uint32_t)i / (uint32_t)d4) : i / d4;
+  const int64_t r = (uint32_t)i / (uint32_t)d4;         // lanes < 2^32
   const int c = (int)(i - r * d4);
   const int64_t t = (uint32_t)r % (uint32_t)a.L;       // rows, L < 2^31
   const float4 w = reinterpret_cast<const float4*>(a.gamma)[c], b = reinterpret_cast<const float4*>(a.beta)[c];
@@ -592,6 +592,9 @@ __global__ __launch_bounds__(kE8Threads) void k_norm8_read(N8Args a) {
   }
 }
 
+// a launch has fewer than 2^32 threads
+constexpr int64_t kE8Lanes = (int64_t(1) << 32) - kE8Threads;
+
 static int e8_groups(int64_t d) { return (int)((d + kE8Group - 1) / kE8Group); }
 
 static int e8_setup(E8Args& a, int64_t rows, int64_t d, const char* what) {
@@ -599,11 +602,12 @@ static int e8_setup(E8Args& a, int64_t rows, int64_t d, const char* what) {
                    (rows == 0 || d < (int64_t(1) << 38) / rows),
                "%s: bad sizes rows=%lld d=%lld", what, (long long)rows, (long long)d);
   a.rows = rows; a.d = (int)d; a.groups = e8_groups(d); a.lanes = rows * a.groups * 4;
-  ASRN_REQUIRE((a.lanes + kE8Threads - 1) / kE8Threads < (int64_t(1) << 31), "%s: too many values", what);
+  ASRN_REQUIRE(a.lanes <= kE8Lanes, "%s: too many values (%lld x %lld)", what, (long long)rows, (long long)d);
   return 0;
 }
 static int n8_check(const N8Args& a, const char* what) {
-  ASRN_REQUIRE(a.rows >= 0 && a.d > 0 && a.d % 4 == 0 && a.d <= kE8MaxD && a.rows < (int64_t(1) << 31),
+  ASRN_REQUIRE(a.rows >= 0 && a.d > 0 && a.d % 4 == 0 && a.d <= kE8MaxD &&
+                   a.rows <= (a.d <= kE8WaveD ? kE8Lanes / 32 : kE8Lanes / kE8Threads),
                "%s: bad sizes rows=%lld d=%d (a multiple of 4, <= %d)", what, (long long)a.rows, a.d, kE8MaxD);
   return 0;
 }
@@ -775,7 +779,7 @@ extern "C" int asrn_norm8_read(const int8_t* q, const uint8_t* e, const float* g
   const bool run = k == 1 || k == 4;
   const int64_t lanes = (run ? B * ((L + kN8Run - 1) / kN8Run) : a.rows) * (d / 4);
   const int64_t blocks = (lanes + kE8Threads - 1) / kE8Threads;
-  ASRN_REQUIRE(blocks < (int64_t(1) << 31), "asrn_norm8_read: too many values");
+  ASRN_REQUIRE(lanes <= kE8Lanes, "asrn_norm8_read: too many values");
   hipStream_t st = (hipStream_t)stream;
   if (run) {
     const dim3 grid((unsigned)blocks), block(kE8Threads);

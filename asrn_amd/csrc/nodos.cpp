@@ -12,7 +12,6 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -79,22 +78,11 @@ void pasos(const Opcional& t, int64_t* s) {
   s[0] = t ? t->stride(0) : 0;
   s[1] = t ? t->stride(1) : 0;
 }
-// A backward's results as they are, or, where the backward itself is recorded, as values whose own gradient is refused:
-// the kernels have no second derivative.
-variable_list una_vez(variable_list&& r) {
-  if (!at::GradMode::is_enabled()) return std::move(r);
-  for (auto& t : r)
-    if (t.defined()) t = t.detach().requires_grad_(true);
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      "trying to differentiate twice a function that was marked with once_differentiable", (int64_t)r.size());
-  variable_list defined, wrapped;
-  for (auto& t : r)
-    if (t.defined()) defined.push_back(t);
-  wrapped = (*error)(variable_list(defined));
-  size_t k = 0;
-  for (auto& t : r)
-    if (t.defined()) t = wrapped[k++];
-  return std::move(r);
+// The kernels have no second derivative: a backward that is itself recorded is refused, whatever the recording is for (a
+// delayed error would be passed over where the second gradient also has another path).
+void una_vez(const char* que) {
+  if (at::GradMode::is_enabled())
+    throw Fallo(std::string(que) + ": its gradient cannot be recorded (create_graph=True), the kernels have no second derivative");
 }
 
 // ---- log-probabilities of given tokens -----------------------------------------------------------------------------------
@@ -124,6 +112,7 @@ struct LogProbabilidades : Function<LogProbabilidades> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("log_probabilidades");
     Tensor gl = g[0], gh = g.size() > 1 ? g[1] : Tensor();
     if (!gl.defined() && !gh.defined()) return {Tensor(), Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
@@ -136,7 +125,7 @@ struct LogProbabilidades : Function<LogProbabilidades> {
       vale(lib.logp_bwd(ptr(x), (int32_t)n[0], n[1], n[2], n[3], n[4], n[5], s[1].data_ptr<int64_t>(), n[6],
                         (float)ctx->saved_data["t"].toDouble(), f32(s[2]), s.size() > 3 ? f32(s[3]) : nullptr, f32(gl), f32(gh),
                         ptr(dx), en.st), "asrn_token_logp_bwd");
-    return una_vez({dx, Tensor(), Tensor()});
+    return {dx, Tensor(), Tensor()};
   }
 };
 
@@ -190,6 +179,7 @@ struct Preferencia : Function<Preferencia> {
     return {perdida, rec};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("perdida_preferencia");
     if (!g[0].defined()) return {Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
@@ -200,7 +190,7 @@ struct Preferencia : Function<Preferencia> {
     pasos(m, sm);
     vale(lib.pref_bwd(reinterpret_cast<float*>(static_cast<char*>(s[0].data_ptr()) + n[2]), f32(gd), u8(m), sm, n[0], n[1], f32(dlp),
                       en.st), "asrn_preference_bwd");
-    return una_vez({dlp, Tensor()});
+    return {dlp, Tensor()};
   }
 };
 
@@ -244,6 +234,7 @@ struct Politica : Function<Politica> {
     return {perdida, datos};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("perdida_politica");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
@@ -259,7 +250,7 @@ struct Politica : Function<Politica> {
     pasos(m, sm);
     vale(lib.pol_bwd(div + B, div, f32(gd), u8(m), sm, B, L, ctx->saved_data["w"].toDouble(), f32(dlp), f32(dH), en.st),
          "asrn_policy_bwd");
-    return una_vez({dlp, dH, Tensor()});
+    return {dlp, dH, Tensor()};
   }
 };
 
@@ -301,6 +292,7 @@ struct Gelu8 : Function<Gelu8> {
     return {y, sitio};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("gelu8");
     if (!g[0].defined()) return {Tensor(), Tensor()};
     const variable_list s = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
@@ -311,7 +303,7 @@ struct Gelu8 : Function<Gelu8> {
       du = vacio(ctx->saved_data["f"].toIntVector(), s[0], n[3] ? at::kBFloat16 : at::kFloat);
       vale(lib.gelu8_bwd(q_de(s[0]), e_de(s[0], n[2]), ptr(dy), es16(dy), n[0], n[1], (int32_t)n[3], ptr(du), en.st), "asrn_gelu8_bwd");
     }
-    return una_vez({du, n[4] && ctx->needs_input_grad(1) ? g[0] : Tensor()});
+    return {du, n[4] && ctx->needs_input_grad(1) ? g[0] : Tensor()};
   }
 };
 
@@ -340,10 +332,11 @@ struct Norma8 : Function<Norma8> {
     return {y, xc.view(x.sizes()), sitio};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("norma8");
     const variable_list s = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
     const auto forma = ctx->saved_data["f"].toIntVector();
-    if (!g[0].defined()) return una_vez({g[1], Tensor(), Tensor(), Tensor(), Tensor()});       // the residual path alone
+    if (!g[0].defined()) return {g[1], Tensor(), Tensor(), Tensor(), Tensor()};       // the residual path alone
     En en(s[0]);
     const Tensor dy = alineado(es16(g[0]) ? g[0].contiguous() : denso(g[0]));
     const Tensor dr = g[1].defined() ? alineado(denso(g[1])) : Tensor();
@@ -351,7 +344,7 @@ struct Norma8 : Function<Norma8> {
     Tensor dx = vacio(forma, s[0]), dp = vacio({2, n[1]}, s[0]), ws = vacio({wsb < 0 ? 0 : wsb}, s[0], at::kByte);
     vale(lib.norm8_bwd(q_de(s[0]), e_de(s[0], n[3]), f32(s[1]), reinterpret_cast<float*>(e_de(s[0], n[2])), n[0], (int32_t)n[1],
                        ptr(dy), es16(dy), f32(dr), f32(dx), f32(dp), ptr(ws), wsb, en.st), "asrn_norm8_bwd");
-    return una_vez({dx, dp.select(0, 0), dp.select(0, 1), Tensor(), Tensor()});
+    return {dx, dp.select(0, 0), dp.select(0, 1), Tensor(), Tensor()};
   }
 };
 

@@ -226,7 +226,7 @@ using namespace asrn;
 
 static int64_t po_pieces(int64_t L) { return L > 0 ? (L + kPoPiece - 1) / kPoPiece : 1; }
 static bool po_sizes(int64_t B, int64_t L) {
-  return B >= 1 && B < (int64_t(1) << 31) && L >= 0 && L < (int64_t(1) << 31) && B * po_pieces(L) < (int64_t(1) << 31);
+  return B >= 1 && B < (int64_t(1) << 31) && L >= 0 && L < (int64_t(1) << 31) && B * po_pieces(L) < (int64_t(1) << 24);   // a launch has fewer than 2^32 threads
 }
 static int po_check(int64_t B, int64_t L, const char* what) {
   ASRN_REQUIRE(po_sizes(B, L), "%s: bad sizes B=%lld L=%lld", what, (long long)B, (long long)L);

@@ -156,7 +156,7 @@ using namespace asrn;
 
 static int64_t pf_pieces(int64_t L) { return L > 0 ? (L + kPfPiece - 1) / kPfPiece : 1; }
 static bool pf_sizes(int64_t P, int64_t L) {
-  return P >= 1 && P < (int64_t(1) << 30) && L >= 0 && L < (int64_t(1) << 31) && 2 * P * pf_pieces(L) < (int64_t(1) << 31);
+  return P >= 1 && P < (int64_t(1) << 30) && L >= 0 && L < (int64_t(1) << 31) && 2 * P * pf_pieces(L) < (int64_t(1) << 24);   // a launch has fewer than 2^32 threads
 }
 static int pf_check(int64_t P, int64_t L, const char* what) {
   ASRN_REQUIRE(pf_sizes(P, L), "%s: bad sizes P=%lld L=%lld", what, (long long)P, (long long)L);

@@ -268,23 +268,27 @@ static int lp_check(const LpArgs& a, int32_t type, const char* what) {
                    a.sb >= 0 && a.st >= 0 && a.rows % a.L == 0,
                "%s: bad sizes rows=%lld L=%lld V=%lld strides %lld, %lld", what, (long long)a.rows, (long long)a.L,
                (long long)a.V, (long long)a.sb, (long long)a.st);
+  // a launch has fewer than 2^32 threads: 64 a row for short vocabularies, else 256 or 1,024
+  ASRN_REQUIRE(a.rows < (int64_t(1) << (a.V <= 2048 ? 26 : 22)), "%s: too many rows (%lld)", what, (long long)a.rows);
   ASRN_REQUIRE(a.inv_t > 0.f && a.inv_t < INFINITY, "%s: the temperature's inverse must be positive and finite", what);
   return 0;
 }
+
+// Vectors of a row up to which a wave takes it, four rows a workgroup (16384 x 256 fp32 backward: 18 us with 256 threads a
+// row, 7 with a wave; 16384 x 8000 bf16, 1000 vectors, stays with 256). Rows up to which a workgroup has 1,024 threads in
+// the forward and a row is split over several in the backward: four workgroups a CU (512 x 50304 bf16: forward 13 us)
+constexpr int64_t kLpWave = 512, kLpGroups = 1024;
 
 template <int T, bool ENT>
 static void lp_fwd(const LpArgs& a, hipStream_t st) {
   const int64_t nvec = a.V / LpType<T>::E;
 #define ASRN_LP(TPR, ROWS)                                                                             \
   hipLaunchKernelGGL((k_logp_fwd<T, TPR, ENT>), dim3((unsigned)((a.rows + ROWS - 1) / ROWS)), dim3(TPR * ROWS), 0, st, a)
-  if (nvec <= 512) ASRN_LP(64, 4);
-  else if (nvec <= 2048 || a.rows > 1024) ASRN_LP(256, 1);
+  if (nvec <= kLpWave) ASRN_LP(64, 4);
+  else if (nvec <= 2048 || a.rows > kLpGroups) ASRN_LP(256, 1);
   else ASRN_LP(1024, 1);
 #undef ASRN_LP
 }
-
-// workgroups a backward's grid should have at least, by splitting the rows: four a CU
-constexpr int64_t kLpGroups = 1024;
 
 }  // namespace asrn
 
@@ -329,7 +333,7 @@ extern "C" int asrn_token_logp_bwd(const void* logits, int32_t type, int64_t row
   int64_t splits = (kLpGroups + rows - 1) / rows, most = (V + round - 1) / round;
   splits = splits < most ? splits : most;
   a.splits = (int)(splits < 1 ? 1 : splits > 65535 ? 65535 : splits);
-  const bool corto = V / (type == kLpF32 ? 4 : 8) <= 512;          // a wave a row, as in the forward
+  const bool corto = V / (type == kLpF32 ? 4 : 8) <= kLpWave;
   const dim3 grid((unsigned)(corto ? (rows + 3) / 4 : rows), (unsigned)a.splits), block(256);
   hipStream_t st = (hipStream_t)stream;
 #define ASRN_LP_B2(T, TH)                                                               \

@@ -237,6 +237,8 @@ class _Lineal8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        if torch.is_grad_enabled():
+            raise RuntimeError('lineal8: its gradient cannot be recorded (create_graph=True)')
         wc, *guardados = ctx.saved_tensors
         tipos, leer, dt, n = ctx.meta
         return (*_gradientes(g, wc, lambda: leer(guardados, dt), tipos, ctx.needs_input_grad), *(None,) * (2 + n))

@@ -10,7 +10,6 @@ import math
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, nodos, ptr, query, stream_of
@@ -1706,8 +1705,9 @@ class Norma8(torch.autograd.Function):
         return y.to(dtype), x2.view(forma), sitio
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dres, _):
+        if torch.is_grad_enabled():
+            raise RuntimeError('norma8: its gradient cannot be recorded (create_graph=True)')
         sitio, g = ctx.saved_tensors
         forma, N, d, m, s = ctx.meta
         q = sitio.data_ptr()

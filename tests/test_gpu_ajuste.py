@@ -165,6 +165,27 @@ def test_logp_differences():
         assert abs((dx.double() * d).sum() - num) <= 1e-6 * (dx.double() * d).abs().sum() + 1e-8
 
 
+def test_logp_past_32_bits():
+    """More than 2^31 logits: the last rows against the same rows alone, bit for bit, gradient included."""
+    filas, V = 43_001, 50_304
+    x = torch.empty(filas, V, dtype=torch.bfloat16, device=DEV).fill_(0.5)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    cola = (2 * torch.randn(5, V, generator=g, device=DEV)).bfloat16()
+    x[-5:] = cola
+    y = torch.full((filas,), 7, device=DEV)
+    y[-5:] = torch.randint(0, V, (5,), generator=g, device=DEV)
+    y[:20_000] = -100
+    x.requires_grad_()
+    lp = asrn_amd.log_probabilidades(x, y)
+    dx, = torch.autograd.grad(lp, x, torch.ones_like(lp))
+    c = torch.cat([x.detach()[:1200], cola]).requires_grad_()        # past 1,024 rows: the same kernels
+    yc = torch.cat([torch.full((1200,), 7, device=DEV), y[-5:]])
+    l2 = asrn_amd.log_probabilidades(c, yc)
+    d2, = torch.autograd.grad(l2, c, torch.ones_like(l2))
+    assert torch.equal(lp[-5:], l2[-5:]) and torch.equal(dx[-5:], d2[-5:]) and torch.equal(lp[20_000:20_010], l2[:10])
+    assert (lp[:20_000] == 0).all() and (dx[19_990:20_000] == 0).all()
+
+
 def test_logp_gradients_of_one_output_and_expanded():
     x = torch.randn(2, 3, 50, device=DEV).requires_grad_()
     y = torch.randint(0, 50, (2, 3), device=DEV)
@@ -242,6 +263,43 @@ def test_preference_long_texts_and_strides():
         e, er, ed = preferencia_exacta(lp, mm, ref, 0.1, 'sigmoide', 0.0, 0.0, False)
         assert abs(perdida.double() - e) <= U * e.abs() + 1e-12 * L and ((rec.double() - er).abs() <= U * er.abs() + 1e-12 * L).all()
         assert ((dlp.double() - ed).abs() <= 4 * U * ed.abs() + 1e-13 * L).all()
+
+
+def test_losses_of_very_many_texts():
+    """Tens of thousands of one-token texts, and gradients against central differences of the float64 definitions."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    lp = (-torch.rand(70_000, 1, generator=g, device=DEV)).requires_grad_()
+    perdida, rec = asrn_amd.perdida_preferencia(lp)
+    e, er, ed = preferencia_exacta(lp, None, None, 0.1, 'sigmoide', 0.0, 0.0, False)
+    d, = torch.autograd.grad(perdida, lp)
+    assert abs(perdida.double() - e) <= 2 * U and (rec.double() - er).abs().max() <= U and ((d.double() - ed).abs() <= 3 * U * ed.abs()).all()
+    A = torch.randn(70_000, generator=g, device=DEV)
+    old = lp.detach() + 0.1
+    for reduccion in ajuste.REDUCCIONES:
+        perdida, est = asrn_amd.perdida_politica(lp, A, old, reduccion=reduccion)
+        (e, ee, ed), tam = politica_exacta(lp, A, old, None, 0.2, 0.2, None, None, 0.0, None, 0.0, reduccion)
+        d, = torch.autograd.grad(perdida, lp)
+        assert abs(perdida.double() - e) <= U * e.abs() + EXP * tam[0].sum() and ((d.double() - ed).abs() <= 6 * U * ed.abs() + EXP * tam[0]).all()
+
+
+def test_losses_differences():
+    """The gradients along random directions against central differences of the float64 definitions, away from the clips'
+    and the hinge's corners (the step is far smaller than any token's distance from them)."""
+    g = torch.Generator(device=DEV).manual_seed(12)
+    lp = (-torch.rand(6, 33, generator=g, device=DEV)).requires_grad_()
+    old, A = lp.detach() + 0.3 * torch.randn(6, 33, generator=g, device=DEV), torch.randn(6, 33, generator=g, device=DEV)
+    m = torch.rand(6, 33, generator=g, device=DEV) < 0.7
+    casos = [(asrn_amd.perdida_preferencia(lp, m, old, beta=0.3, tipo=t)[0],
+              lambda v, t=t: preferencia_exacta(v, m, old, 0.3, t, 0.0, 0.0, False)[0]) for t in ajuste.FORMAS]
+    casos.append((asrn_amd.perdida_politica(lp, A, old, m, lp_ref=old, beta=0.1)[0],
+                  lambda v: politica_exacta(v, A, old, m, 0.2, 0.2, None, old, 0.1, None, 0.0, 'fichas')[0][0]))
+    for perdida, f in casos:
+        dlp, = torch.autograd.grad(perdida, lp)
+        for _ in range(2):
+            d = torch.randn(6, 33, generator=g, device=DEV).double()
+            v = lp.detach().double()
+            num = (f(v + 1e-6 * d) - f(v - 1e-6 * d)) / 2e-6
+            assert abs((dlp.double() * d).sum() - num) <= 1e-6 * (dlp.double() * d).abs().sum() + 1e-8
 
 
 def test_preference_degenerate():

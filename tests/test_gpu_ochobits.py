@@ -391,6 +391,26 @@ def test_refusals():
     assert ops.guardar8(torch.zeros(0, 40, device=DEV))[0].shape == (0, 40)
 
 
+def test_past_32_bits():
+    """More than 2^31 values: the last rows against the same rows alone."""
+    N, d = 70_001, 30_720
+    u = torch.zeros(N, d, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    cola = torch.randn(3, d, generator=g, device=DEV).bfloat16()
+    u[-3:] = cola
+    q, e = ops.guardar8(u)
+    q2, e2 = ops.guardar8(cola)
+    assert torch.equal(q[-3:], q2) and torch.equal(e[-3:], e2) and (q[-4] == 0).all()
+    assert torch.equal(ops.leer8(q, e, torch.bfloat16)[-3:], ops.leer8(q2, e2, torch.bfloat16))
+
+
+def test_second_gradients_are_refused():
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    for y in (ops.gelu8(x)[0], ops.norma8(torch.nn.LayerNorm(64).to(DEV), x, torch.float32)[0]):
+        with pytest.raises(RuntimeError, match='create_graph'):
+            torch.autograd.grad((y * y).sum() + (x ** 3).sum(), x, create_graph=True)
+
+
 def test_strided_inputs_and_offsets():
     """Inputs that are slices, and rows off a 16-byte boundary."""
     base = torch.randn(2, 9, 130, device=DEV)
