@@ -111,9 +111,18 @@ class PasoGrafado:
     The first `calentar` calls are ordinary steps, run on a side stream (they build AdamW's state and the layers'
     workspaces); the next call captures one step and every later call replays it. A step with a non-finite loss or
     gradient norm changes nothing (the fused AdamW's found_inf), salto = 1. bf16 or fp32; no recomputation (checkpoint
-    'no' or 'ocho'), no torch.compile, no accumulation. grabar=False runs every step eagerly (the same arithmetic; also on the CPU)."""
+    'no' or 'ocho'), no torch.compile, no accumulation. grabar=False runs every step eagerly (the same arithmetic; also on
+    the CPU).
 
-    def __init__(self, modelo, optimizador, lote, largo, precision='bf16', recorte=1.0, calentar=3, grabar=None):
+    perdida: the step's loss from the logits, y and the tensors of `extras`, a scalar (default: entropia). The extras are
+    per-step inputs like x and y, given here for their shapes and to each call for their values:
+
+        pref = lambda logits, y, ref: perdida_preferencia(log_probabilidades(logits, y), y != -100, ref)[0]
+        paso = PasoGrafado(modelo, opt, 2 * pares, largo, perdida=pref, extras=(ref,))
+        perdida, norma, salto = paso(x, y, lr=..., extras=(ref,))"""
+
+    def __init__(self, modelo, optimizador, lote, largo, precision='bf16', recorte=1.0, calentar=3, grabar=None,
+                 perdida=None, extras=()):
         base = _base(modelo)
         disp = next(base.parameters()).device
         grabar = (disp.type == 'cuda') if grabar is None else bool(grabar)
@@ -131,6 +140,8 @@ class PasoGrafado:
         self.params = [p for p in base.parameters() if p.requires_grad]
         self.x = torch.zeros((lote, largo), dtype=torch.long, device=disp)
         self.y = torch.zeros_like(self.x)
+        self.perdida = entropia if perdida is None else perdida
+        self.extras = [torch.zeros_like(t, device=disp, requires_grad=False) for t in extras]
         self.lrs = []
         if grabar:
             # the rate lives in device tensors, so a schedule needs no new capture
@@ -143,7 +154,7 @@ class PasoGrafado:
     def _uno(self):
         with autocast(self.precision, self.disp, cache=not self.grabar):
             logits = self.modelo(self.x)
-        perdida = entropia(logits, self.y)
+        perdida = self.perdida(logits, self.y, *self.extras)
         perdida.backward()
         recorte = ops.recortar_gradientes(self.params, self.recorte, perdida)
         if recorte is None:
@@ -186,10 +197,15 @@ class PasoGrafado:
         with torch.cuda.graph(self.grafo):
             self.salida = self._uno()
 
-    def __call__(self, x, y, lr=None):
-        """x, y (lote, largo) -> (loss, gradient norm, skipped) as device tensors."""
+    def __call__(self, x, y, lr=None, extras=()):
+        """x, y (lote, largo) and the extras of this step -> (loss, gradient norm, skipped) as device tensors."""
+        if len(extras) != len(self.extras) or any(a.shape != b.shape for a, b in zip(extras, self.extras)):
+            raise ValueError(f'PasoGrafado: extras {[tuple(t.shape) for t in extras]} against '
+                             f'{[tuple(t.shape) for t in self.extras]}')
         self.x.copy_(x, non_blocking=True)
         self.y.copy_(y, non_blocking=True)
+        for a, b in zip(self.extras, extras):
+            a.copy_(b, non_blocking=True)
         if lr is not None:
             self._poner_lr(lr)
         if not self.grabar:

@@ -251,6 +251,8 @@ def test_block(d, mezcla, k, bits):
         out.append((y.detach(), *torch.autograd.grad(y, [h, *b.parameters()], gy)))
     assert torch.allclose(out[0][0], out[1][0], rtol=1e-5, atol=1e-5) if bits == 32 else \
         (out[0][0] - out[1][0]).norm() <= 2e-3 * out[0][0].norm()
+    if d % 4 == 0 and d <= 1024:                     # where both modes run the library's LayerNorm: the same bits
+        assert torch.equal(out[0][0], out[1][0])
     for a, c in zip(out[0][1:], out[1][1:]):
         assert (a - c).norm() <= 0.04 * a.norm() + 1e-6
 
@@ -344,6 +346,47 @@ def test_graphed_step(precision):
             assert salto.item() == 0
         perdidas.append(fila)
     assert all(abs(a - b) <= (1e-5 if precision == 'fp32' else 2e-3) * abs(b) for a, b in zip(*perdidas)), perdidas
+
+
+def _pref(logits, y, ref):
+    return asrn_amd.perdida_preferencia(asrn_amd.log_probabilidades(logits, y), y != -100, ref, beta=0.3)[0]
+
+
+def _pol(logits, y, A, vieja):
+    lp, H = asrn_amd.log_probabilidades(logits, y, entropia=True)
+    return asrn_amd.perdida_politica(lp, A, vieja, y != -100, lp_ref=vieja, beta=0.04, entropia=H, peso_entropia=0.01,
+                                     reduccion='textos')[0]
+
+
+@pytest.mark.parametrize('cual', ['preferencia', 'politica'])
+@pytest.mark.parametrize('checkpoint', ['no', 'ocho'])
+def test_graphed_fine_tuning(cual, checkpoint):
+    """PasoGrafado with the preference or the policy loss and its per-step inputs: replays equal the eager steps."""
+    g = torch.Generator().manual_seed(7)
+    P, L = 2, 40
+    pasos = []
+    for _ in range(7):
+        x = torch.randint(0, 61, (2 * P, L + 1), generator=g).to(DEV)
+        y = x[:, 1:].clone()
+        y[:, :9] = -100
+        y[1, 20:] = -100
+        pasos.append((x[:, :-1], y, torch.randn(2 * P, generator=g).to(DEV), (-3 * torch.rand(2 * P, L, generator=g)).to(DEV)))
+    perdidas = []
+    for grabar in (True, False):
+        m = _modelo(checkpoint)
+        opt = asrn_amd.crear_optimizador(m, 1e-3, capturable=grabar)
+        de = (lambda p: (p[3],)) if cual == 'preferencia' else (lambda p: p[2:])
+        paso = asrn_amd.PasoGrafado(m, opt, 2 * P, L, precision='fp32', grabar=grabar, perdida=_pref if cual == 'preferencia' else _pol,
+                                    extras=de(pasos[0]))
+        with pytest.raises(ValueError, match='extras'):
+            paso(*pasos[0][:2], lr=1e-3)
+        fila = []
+        for p in pasos:
+            perdida, _, salto = paso(*p[:2], lr=1e-3, extras=de(p))
+            fila.append(perdida.item())
+            assert salto.item() == 0
+        perdidas.append(fila)
+    assert all(abs(a - b) <= 2e-5 * (1 + abs(b)) for a, b in zip(*perdidas)), perdidas
 
 
 def test_fine_tuning_step():
