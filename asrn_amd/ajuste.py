@@ -20,19 +20,24 @@ FORMAS = ('sigmoide', 'ipo', 'bisagra')
 REDUCCIONES = ('fichas', 'textos')
 
 
-def _mismo_gpu(quien, dev, **tensores):
+def _igual(quien, lp, **tensores):
+    """Floating tensors of lp's shape on its device, or None."""
     for n, t in tensores.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f'{quien}: {n} is on {t.device}, the rest on {dev}')
+        if t is not None:
+            if t.shape != lp.shape or not t.is_floating_point():
+                raise ValueError(f'{quien}: {n} {tuple(t.shape)} of {t.dtype} against lp {tuple(lp.shape)}')
+            if t.device != lp.device:
+                raise ValueError(f'{quien}: {n} is on {t.device}, the rest on {lp.device}')
 
 
 def _mascara(quien, m, forma, dev):
     """A (B, L) mask as bytes (nonzero keeps the token), or None."""
     if m is None:
         return None
-    if tuple(m.shape) != tuple(forma):
+    if m.shape != forma:
         raise ValueError(f'{quien}: mascara {tuple(m.shape)} against {tuple(forma)} tokens')
-    _mismo_gpu(quien, dev, mascara=m)
+    if m.device != dev:
+        raise ValueError(f'{quien}: mascara is on {m.device}, the rest on {dev}')
     return (m if m.dtype == torch.bool else m != 0).view(torch.uint8)
 
 
@@ -64,7 +69,7 @@ def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False)
     is 0. The gradient is in the logits' dtype. Sums are held in fp32, as cross_entropy's."""
     quien = 'log_probabilidades'
     dev = _dev(logits)
-    if logits.dim() < 1 or tuple(logits.shape[:-1]) != tuple(y.shape):
+    if logits.dim() < 1 or logits.shape[:-1] != y.shape:
         raise ValueError(f'{quien}: logits {tuple(logits.shape)} against tokens {tuple(y.shape)}')
     if logits.dtype not in TIPOS:
         raise ValueError(f'{quien}: logits of {logits.dtype} (fp32, bf16 or fp16 are taken)')
@@ -72,7 +77,8 @@ def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False)
         raise ValueError(f'{quien}: a vocabulary of {logits.shape[-1]} tokens and token ids of {y.dtype}')
     if y.numel() >= 1 << 31:
         raise ValueError(f'{quien}: {y.numel()} tokens (up to 2**31 - 1)')
-    _mismo_gpu(quien, dev, y=y)
+    if y.device != dev:
+        raise ValueError(f'{quien}: y is on {y.device}, the logits on {dev}')
     T = _numero(quien, 'temperatura', temperatura, 1e-6, 1e6)
     x, t = logits, y.to(torch.int64).contiguous()
     if x.stride(-1) != 1 and x.shape[-1] > 1:
@@ -108,9 +114,10 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
         raise ValueError(f'{quien}: lp {tuple(lp.shape)} of {lp.dtype}: (2P, L) log-probabilities, P >= 1, are needed')
     m = _mascara(quien, mascara, lp.shape, dev)
     if ref is not None:
-        if tuple(ref.shape) not in (tuple(lp.shape), (lp.shape[0],)) or not ref.is_floating_point():
-            raise ValueError(f'{quien}: ref {tuple(ref.shape)} of {ref.dtype} against lp {tuple(lp.shape)}')
-        _mismo_gpu(quien, dev, ref=ref)
+        if ref.dim() != 1:
+            _igual(quien, lp, ref=ref)
+        elif ref.shape[0] != lp.shape[0] or not ref.is_floating_point() or ref.device != dev:
+            raise ValueError(f'{quien}: ref {tuple(ref.shape)} of {ref.dtype} on {ref.device} against lp {tuple(lp.shape)} on {dev}')
         ref = _fijo(ref)
     if tipo not in FORMAS:
         raise ValueError(f'{quien}: tipo={tipo!r}: one of {FORMAS}')
@@ -146,12 +153,9 @@ def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope
     dev = _dev(lp)
     if lp.dim() != 2 or lp.shape[0] < 1 or not lp.is_floating_point():
         raise ValueError(f'{quien}: lp {tuple(lp.shape)} of {lp.dtype}: (B, L) log-probabilities, B >= 1, are needed')
-    if tuple(ventaja.shape) == (lp.shape[0],):
+    if ventaja.dim() == 1 and ventaja.shape[0] == lp.shape[0]:
         ventaja = ventaja[:, None].expand(lp.shape)
-    for n, t in (('ventaja', ventaja), ('lp_vieja', lp_vieja), ('lp_ref', lp_ref), ('entropia', entropia)):
-        if t is not None and (tuple(t.shape) != tuple(lp.shape) or not t.is_floating_point()):
-            raise ValueError(f'{quien}: {n} {tuple(t.shape)} of {t.dtype} against lp {tuple(lp.shape)}')
-    _mismo_gpu(quien, dev, ventaja=ventaja, lp_vieja=lp_vieja, lp_ref=lp_ref, entropia=entropia)
+    _igual(quien, lp, ventaja=ventaja, lp_vieja=lp_vieja, lp_ref=lp_ref, entropia=entropia)
     m = _mascara(quien, mascara, lp.shape, dev)
     lo, hi = recorte if isinstance(recorte, (tuple, list)) and len(recorte) == 2 else (recorte, recorte)
     lo, hi = _numero(quien, 'recorte', lo, 0.0, 1.0), _numero(quien, 'recorte', hi, 0.0)

@@ -12,6 +12,8 @@
 //                 the piece's count, loss, clipped tokens, KL to old (r - 1 - d) and to the reference, and entropy.
 //   k_pol_loss    one workgroup: the pieces' sums in a fixed order, the loss, the statistics, each text's divisor.
 //   k_pol_bwd     the gradients over their divisor times the loss's own gradient.
+// 160 texts of 20,001 tokens with every term: 21.6 + 6.6 + 9.1 us, the first at 3.8 TB/s beside its arithmetic; short
+// batches are bound by launches (5.6 + 4.2 + 3.4 us).
 #include <math.h>
 
 #include "common.h"

@@ -7,9 +7,11 @@
 //   k_pref_rows  a row in pieces of 2,048 tokens, one workgroup each: the masked sum and the count of a piece. Long rows
 //                and few rows alike spread over the chip; the sums are in double (a long text's log-probability is a
 //                small difference of large sums), each piece's in a fixed order.
-//   k_pref_loss  one workgroup, a pair a thread: the pieces added in order, the loss, the rewards and the coefficients.
+//   k_pref_loss  one workgroup, a pair a group of lanes, one lane a piece: the pieces added in a fixed order, the loss, the
+//                rewards and the coefficients.
 //   k_pref_bwd   d lp = m g c, written once.
-// HBM-bound for long batches (9 to 13 bytes a token each way), launches for short ones.
+// Bound by launches for short batches (2.8 + 2.8 + 2.2 us); 24 pairs of 50,001 tokens take 5.4 + 6.1 + 5.5 us (the first
+// reads 21.6 MB; 8.4 us with 4-byte loads).
 #include <math.h>
 
 #include "common.h"

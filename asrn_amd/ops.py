@@ -1637,15 +1637,14 @@ def guardar8(x):
     return q, e
 
 
-def leer8(q, e, dtype=torch.float32, gelu=False):
-    """The values that guardar8's codes and scales stand for (gelu: their GELU), (N, d) fp32 or bf16. The values fit bf16
-    exactly."""
+def leer8(q, e, dtype=torch.float32):
+    """The values that guardar8's codes and scales stand for, (N, d) fp32 or bf16: they fit bf16 exactly."""
     dev = _dev(q, e)
     if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() != 2 or e.device != dev or \
             tuple(e.shape) != (q.shape[0], -(-q.shape[1] // GRUPO8)) or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f'leer8: codes {tuple(q.shape)} of {q.dtype} with scales {tuple(e.shape)} of {e.dtype} to {dtype}')
     q, e = q.contiguous(), e.contiguous()
-    return _leer8(q.data_ptr(), e.data_ptr(), *q.shape, dev, dtype, gelu)
+    return _leer8(q.data_ptr(), e.data_ptr(), *q.shape, dev, dtype)
 
 
 def _leer8(q, e, N, d, dev, dtype, gelu=False):

@@ -358,11 +358,12 @@ def politica_exacta(lp, A, vieja, m, lo, hi, tope, ref, beta, H, peso, reduccion
     return (loss.detach(), est, *torch.autograd.grad(loss, [v] + ([] if h is None else [h]))), tam
 
 
-# The policy kernel's exponentials are fp32's, all else double. exp: expf within one step (2 U) and the factor of its
-# argument's rounding, 3 U; expm1: one step, and its argument rounded (U (1 + |q|) of the result for |q| < 4): 7 U; exp q -
-# 1 - q: its series' few roundings (4 U) up to |q| = 1/2, past it expm1's 2 U times expm1 / kl <= 4.4, 9 U, and the
-# argument's. So a token's loss is within 3 U r |A| + 12 U beta kl and its gradient within 3 U r |A| + 7 U beta |expm1 q|
-# (here with the divisor: tam), the statistics within 12 U of themselves, before the last roundings.
+# The policy kernel's exponentials are fp32's, all else double. Up to |d| = 1 the series for exp d - 1 - d: its eleven
+# steps shrink, so their roundings and the argument's come to 5 U of it, and of exp d - 1 and exp d (1 + d and it, in
+# double) to less. Past it expf within one step (2 U) and the factor of its argument's rounding, 3 U of exp d, so 3 U e /
+# |e - 1| <= 4.8 U of exp d - 1 and 3 U e / (e - 2) <= 11.4 U of exp d - 1 - d (the worst at d = 1). So a token's loss is
+# within 3 U r |A| + 12 U beta kl and its gradient within 3 U r |A| + 7 U beta |expm1 q| (here with the divisor: tam), the
+# statistics within 12 U of themselves, before the last roundings.
 EXP, EXPM1, KL = 3 * U, 7 * U, 12 * U
 
 
