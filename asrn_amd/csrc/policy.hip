@@ -11,9 +11,10 @@
 //   k_pol_tokens  pieces of 2,048 tokens of a text, one workgroup each: the per-token gradient (not yet divided), and
 //                 the piece's count, loss, clipped tokens, KL to old (r - 1 - d) and to the reference, and entropy.
 //   k_pol_loss    one workgroup: the pieces' sums in a fixed order, the loss, the statistics, each text's divisor.
+//   k_pol_few     the two in one launch for a few short texts.
 //   k_pol_bwd     the gradients over their divisor times the loss's own gradient.
 // 160 texts of 20,001 tokens with every term: 21.6 + 6.6 + 9.1 us, the first at 3.8 TB/s beside its arithmetic; short
-// batches are bound by launches (5.6 + 4.2 + 3.4 us).
+// batches are bound by launches (4 texts of 50: 6.2 and 3.4 us).
 #include <math.h>
 
 #include "common.h"
@@ -71,70 +72,73 @@ __device__ __forceinline__ PoExp po_terms(double d) {
   return PoExp{e1, e1 - d};
 }
 
-// ROW: every text's tokens lie next to each other and are read 4 at a time (3.2 M tokens: 33 -> 23 us)
+// n <= 4 tokens of a text from t: their gradients, and what they add to a lane's sums. ROW: every text's tokens lie next to
+// each other and are read 4 at a time (3.2 M tokens: 33 -> 23 us)
+struct PoLane { double s[kPoSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0}; int kept = 0, clipped = 0; };
+template <bool ROW>
+__device__ __forceinline__ void po_four(const PoArgs& a, int64_t row, int64_t t, int n, PoLane& z) {
+  float lp[4], old[4], adv[4], ref[4], ent[4], raw[4];
+  const uint32_t m = a.mask.on4<ROW>(row, t, n);
+  a.lp.four<ROW>(row, t, n, 0.f, lp);
+  if (a.adv.st == 0) adv[0] = adv[1] = adv[2] = adv[3] = a.adv.at(row, 0);
+  else a.adv.four<ROW>(row, t, n, 0.f, adv);
+  if (a.old.p) a.old.four<ROW>(row, t, n, 0.f, old);
+  if (a.ref.p) a.ref.four<ROW>(row, t, n, 0.f, ref);
+  if (a.ent.p) a.ent.four<ROW>(row, t, n, 0.f, ent);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    double dl = 0.0;
+    if (u < n && (m >> (8 * u) & 0xffu)) {    // what a mask hides may be infinite or NaN: nothing of it is used
+      const double A = adv[u], d = a.old.p ? (double)lp[u] - (double)old[u] : (double)(lp[u] - lp[u]);
+      const PoExp x = po_terms(d);
+      const double rA = fma(x.e1, A, A);
+      const bool cap = a.cap > 0.0 && A < 0.0 && d > a.log_cap;
+      const bool out = cap || (A > 0.0 && d > a.log_hi) || (A < 0.0 && d < a.log_lo);
+      double l = -(out ? (cap ? a.cap : A > 0.0 ? a.hi : a.lo) * A : rA);
+      dl = out ? 0.0 : -rA;
+      ++z.kept;
+      z.clipped += out;
+      z.s[3] += x.kl;
+      if (a.ref.p) {
+        const PoExp q = po_terms((double)ref[u] - (double)lp[u]);
+        if (a.beta != 0.0) {
+          l = fma(a.beta, q.kl, l);
+          dl = fma(-a.beta, q.e1, dl);
+        }
+        z.s[4] += q.kl;
+      }
+      if (a.ent.p) {
+        l = fma(-a.w_ent, (double)ent[u], l);
+        z.s[5] += (double)ent[u];
+      }
+      z.s[1] += l;
+    }
+    raw[u] = (float)dl;
+  }
+  if (a.raw) {
+    if (n == 4) {
+      __builtin_memcpy(a.raw + row * a.L + t, raw, 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < n) a.raw[row * a.L + t + u] = raw[u];
+    }
+  }
+}
+
 template <bool ROW>
 __global__ __launch_bounds__(kPoThreads) void k_pol_tokens(PoArgs a) {
   __shared__ double red[kPoThreads / kWave][kPoSums];
   const int64_t row = blockIdx.x / a.pieces, t0 = (int64_t)(blockIdx.x % a.pieces) * kPoPiece;
   const int64_t t1 = t0 + kPoPiece < a.L ? t0 + kPoPiece : a.L;
-  double s[kPoSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-  int kept = 0, clipped = 0;
-  for (int64_t t = t0 + 4 * threadIdx.x; t < t1; t += 4 * kPoThreads) {
-    const int n = t1 - t < 4 ? (int)(t1 - t) : 4;
-    float lp[4], old[4], adv[4], ref[4], ent[4], raw[4];
-    const uint32_t m = a.mask.on4<ROW>(row, t, n);
-    a.lp.four<ROW>(row, t, n, 0.f, lp);
-    if (a.adv.st == 0) adv[0] = adv[1] = adv[2] = adv[3] = a.adv.at(row, 0);
-    else a.adv.four<ROW>(row, t, n, 0.f, adv);
-    if (a.old.p) a.old.four<ROW>(row, t, n, 0.f, old);
-    if (a.ref.p) a.ref.four<ROW>(row, t, n, 0.f, ref);
-    if (a.ent.p) a.ent.four<ROW>(row, t, n, 0.f, ent);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      double dl = 0.0;
-      if (m >> (8 * u) & 0xffu) {             // what a mask hides may be infinite or NaN: nothing of it is used
-        const double A = adv[u], d = a.old.p ? (double)lp[u] - (double)old[u] : (double)(lp[u] - lp[u]);
-        const PoExp x = po_terms(d);
-        const double rA = fma(x.e1, A, A);
-        const bool cap = a.cap > 0.0 && A < 0.0 && d > a.log_cap;
-        const bool out = cap || (A > 0.0 && d > a.log_hi) || (A < 0.0 && d < a.log_lo);
-        double l = -(out ? (cap ? a.cap : A > 0.0 ? a.hi : a.lo) * A : rA);
-        dl = out ? 0.0 : -rA;
-        ++kept;
-        clipped += out;
-        s[3] += x.kl;
-        if (a.ref.p) {
-          const PoExp q = po_terms((double)ref[u] - (double)lp[u]);
-          if (a.beta != 0.0) {
-            l = fma(a.beta, q.kl, l);
-            dl = fma(-a.beta, q.e1, dl);
-          }
-          s[4] += q.kl;
-        }
-        if (a.ent.p) {
-          l = fma(-a.w_ent, (double)ent[u], l);
-          s[5] += (double)ent[u];
-        }
-        s[1] += l;
-      }
-      raw[u] = (float)dl;
-    }
-    if (a.raw) {
-      if (n == 4) {
-        __builtin_memcpy(a.raw + row * a.L + t, raw, 16);
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (u < n) a.raw[row * a.L + t + u] = raw[u];
-      }
-    }
-  }
-  s[0] = kept;
-  s[2] = clipped;
+  PoLane z;
+  for (int64_t t = t0 + 4 * threadIdx.x; t < t1; t += 4 * kPoThreads) po_four<ROW>(a, row, t, t1 - t < 4 ? (int)(t1 - t) : 4, z);
+  z.s[0] = z.kept;
+  z.s[2] = z.clipped;
 #pragma unroll
   for (int k = 0; k < kPoSums; ++k) {
-    s[k] = wave_sum_d(s[k]);
-    if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave][k] = s[k];
+    const double v = wave_sum_d(z.s[k]);
+    if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave][k] = v;
   }
   __syncthreads();
   if (threadIdx.x < kPoSums) {
@@ -144,10 +148,58 @@ __global__ __launch_bounds__(kPoThreads) void k_pol_tokens(PoArgs a) {
   }
 }
 
-__global__ __launch_bounds__(kPoLossThreads) void k_pol_loss(PoArgs a) {
-  __shared__ double red[kPoLossThreads / kWave][kPoSums + 2];
+// The end of the loss over a workgroup of TH threads: s is a lane's share of the sums, then of the texts' means and of
+// the texts with tokens; weight[b] holds a text's own count (at least 1) and becomes its divisor.
+template <int TH>
+__device__ __forceinline__ void po_finish(const PoArgs& a, double* s) {
+  __shared__ double red[TH / kWave][kPoSums + 2];
   __shared__ double sums[kPoSums + 2];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < kPoSums + 2; ++k) {
+    s[k] = wave_sum_d(s[k]);
+    if (lane == 0) red[wave][k] = s[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < kPoSums + 2) {            // a sum a thread, the waves in order
+    double v = 0.0;
+    for (int w = 0; w < TH / kWave; ++w) v += red[w][threadIdx.x];
+    sums[threadIdx.x] = v;
+  }
+  __syncthreads();
+  const double n = sums[0], nt = sums[kPoSums + 1];
+  if (threadIdx.x == 0) *a.loss = (float)(a.by_text ? sums[kPoSums] / nt : sums[1] / n);   // no token at all: 0 / 0
+  if (threadIdx.x < 4) a.stats[threadIdx.x] = (float)(sums[2 + threadIdx.x] / n);
+  for (int64_t b = threadIdx.x; b < a.B; b += TH)
+    a.weight[b] = (float)(a.by_text ? (double)a.weight[b] * nt : n);
+}
+
+// Few short texts in one launch: a wave a text, and the workgroup the loss (us in two launches / in one: 4 x 50 8.7 / 6.2,
+// 8 x 512 8.3 / 7.9, 16 x 256, two texts a wave, 8.3 / 8.7)
+constexpr int kPoFew = 8, kPoShort = 512, kPoFewThreads = kPoFew * kWave;
+template <bool ROW>
+__global__ __launch_bounds__(kPoFewThreads) void k_pol_few(PoArgs a) {
+  const int lane = threadIdx.x & (kWave - 1);
+  double s[kPoSums + 2] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+  const int64_t b = threadIdx.x / kWave;
+  if (b < a.B) {
+    PoLane z;
+    for (int64_t t = 4 * lane; t < a.L; t += 4 * kWave) po_four<ROW>(a, b, t, a.L - t < 4 ? (int)(a.L - t) : 4, z);
+    z.s[0] = z.kept;
+    z.s[2] = z.clipped;
+#pragma unroll
+    for (int k = 0; k < kPoSums; ++k) s[k] = z.s[k];
+    const double n = wave_sum_d(z.s[0]), loss = wave_sum_d(z.s[1]);
+    if (lane == 0) {
+      a.weight[b] = (float)(n > 0.0 ? n : 1.0);
+      s[kPoSums] += n > 0.0 ? loss / n : 0.0;
+      s[kPoSums + 1] += n > 0.0 ? 1.0 : 0.0;
+    }
+  }
+  po_finish<kPoFewThreads>(a, s);
+}
+
+__global__ __launch_bounds__(kPoLossThreads) void k_pol_loss(PoArgs a) {
   double s[kPoSums + 2] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};     // ..., the texts' means, texts with tokens
   const int g = a.lanes, part = threadIdx.x & (g - 1);
   // whole waves stay in the loop: a lane past the texts sums the last one again and keeps nothing
@@ -173,23 +225,7 @@ __global__ __launch_bounds__(kPoLossThreads) void k_pol_loss(PoArgs a) {
     s[kPoSums] += n > 0.0 ? loss / n : 0.0;
     s[kPoSums + 1] += n > 0.0 ? 1.0 : 0.0;
   }
-#pragma unroll
-  for (int k = 0; k < kPoSums + 2; ++k) {
-    s[k] = wave_sum_d(s[k]);
-    if (lane == 0) red[wave][k] = s[k];
-  }
-  __syncthreads();
-  if (threadIdx.x < kPoSums + 2) {            // a sum a thread, the waves in order
-    double v = 0.0;
-    for (int w = 0; w < kPoLossThreads / kWave; ++w) v += red[w][threadIdx.x];
-    sums[threadIdx.x] = v;
-  }
-  __syncthreads();
-  const double n = sums[0], nt = sums[kPoSums + 1];
-  if (threadIdx.x == 0) *a.loss = (float)(a.by_text ? sums[kPoSums] / nt : sums[1] / n);   // no token at all: 0 / 0
-  if (threadIdx.x < 4) a.stats[threadIdx.x] = (float)(sums[2 + threadIdx.x] / n);
-  for (int64_t b = threadIdx.x; b < a.B; b += kPoLossThreads)
-    a.weight[b] = (float)(a.by_text ? (double)a.weight[b] * nt : n);
+  po_finish<kPoLossThreads>(a, s);
 }
 
 template <bool ROW>
@@ -268,7 +304,13 @@ extern "C" int asrn_policy_fwd(const float* lp, const float* advantage, const fl
   a.loss = loss; a.stats = stats; a.weight = weight;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(a.pieces * B)), block(kPoThreads);
-  if (a.lp.row() && (a.adv.row() || a.adv.st == 0) && a.old.row() && a.ref.row() && a.ent.row() && a.mask.row())
+  const bool rows = a.lp.row() && (a.adv.row() || a.adv.st == 0) && a.old.row() && a.ref.row() && a.ent.row() && a.mask.row();
+  if (B <= kPoFew && L <= kPoShort) {
+    if (rows) hipLaunchKernelGGL(k_pol_few<true>, dim3(1), dim3(kPoFewThreads), 0, st, a);
+    else hipLaunchKernelGGL(k_pol_few<false>, dim3(1), dim3(kPoFewThreads), 0, st, a);
+    return check_launch("asrn_policy_fwd");
+  }
+  if (rows)
     hipLaunchKernelGGL(k_pol_tokens<true>, grid, block, 0, st, a);
   else
     hipLaunchKernelGGL(k_pol_tokens<false>, grid, block, 0, st, a);

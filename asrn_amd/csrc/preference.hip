@@ -9,8 +9,9 @@
 //                small difference of large sums), each piece's in a fixed order.
 //   k_pref_loss  one workgroup, a pair a group of lanes, one lane a piece: the pieces added in a fixed order, the loss, the
 //                rewards and the coefficients.
+//   k_pref_few   the two in one launch for a few short texts.
 //   k_pref_bwd   d lp = m g c, written once.
-// Bound by launches for short batches (2.8 + 2.8 + 2.2 us); 24 pairs of 50,001 tokens take 5.4 + 6.1 + 5.5 us (the first
+// Bound by launches for short batches (one pair of 60: 3.4 and 2.2 us); 24 pairs of 50,001 tokens take 5.4 + 6.1 + 5.5 us (the first
 // reads 21.6 MB; 8.4 us with 4-byte loads).
 #include <math.h>
 
@@ -36,7 +37,22 @@ struct PfArgs {
   const float* g; float* dlp;
 };
 
-// ROW: a text's tokens lie next to each other and are read 4 at a time
+// adds n <= 4 tokens of a text from t. ROW: a text's tokens lie next to each other and are read 4 at a time
+template <bool ROW>
+__device__ __forceinline__ void pf_four(const PfArgs& a, int64_t row, int64_t t, int n, double& s, int& count) {
+  const bool ref = a.ref.p && !a.ref_rows;
+  float x[4], r[4];
+  const uint32_t m = a.mask.on4<ROW>(row, t, n);
+  a.lp.four<ROW>(row, t, n, 0.f, x);
+  if (ref) a.ref.four<ROW>(row, t, n, 0.f, r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {               // selected, not multiplied: what a mask hides may be infinite or NaN
+    const bool on = m >> (8 * k) & 0xffu;
+    s += on ? (double)x[k] - (ref ? (double)r[k] : 0.0) : 0.0;
+    count += on;
+  }
+}
+
 template <bool ROW>
 __global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
   __shared__ PfPart red[kPfThreads / kWave];
@@ -44,25 +60,11 @@ __global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
   const int64_t t1 = t0 + kPfPiece < a.L ? t0 + kPfPiece : a.L;
   double s = 0.0;
   int n = 0;
-  const bool ref = a.ref.p && !a.ref_rows;
-  float x[kPfUnroll][4], r[kPfUnroll][4];
-  uint32_t m[kPfUnroll];
 #pragma unroll
   for (int u = 0; u < kPfUnroll; ++u) {
     const int64_t t = t0 + 4 * (threadIdx.x + u * kPfThreads);
-    const int k = t1 - t >= 4 ? 4 : t1 > t ? (int)(t1 - t) : 0;
-    m[u] = a.mask.on4<ROW>(row, t, k);
-    a.lp.four<ROW>(row, t, k, 0.f, x[u]);
-    if (ref) a.ref.four<ROW>(row, t, k, 0.f, r[u]);
+    pf_four<ROW>(a, row, t, t1 - t >= 4 ? 4 : t1 > t ? (int)(t1 - t) : 0, s, n);
   }
-#pragma unroll
-  for (int u = 0; u < kPfUnroll; ++u)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {             // selected, not multiplied: what a mask hides may be infinite or NaN
-      const bool on = m[u] >> (8 * k) & 0xffu;
-      s += on ? (double)x[u][k] - (ref ? (double)r[u][k] : 0.0) : 0.0;
-      n += on;
-    }
   s = wave_sum_d(s);
   double c = wave_sum_d((double)n);
   if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = PfPart{s, c};
@@ -79,49 +81,36 @@ __global__ __launch_bounds__(kPfThreads) void k_pref_rows(PfArgs a) {
 // log(1 + exp(-|h|)) + max(-h, 0) = -log sigma(h)
 __device__ __forceinline__ double neg_log_sigma(double h) { return log1p(exp(-fabs(h))) + (h < 0.0 ? -h : h != h ? h : 0.0); }
 
-__global__ __launch_bounds__(kPfLossThreads) void k_pref_loss(PfArgs a) {
-  __shared__ double red[kPfLossThreads / kWave];
-  double total = 0.0;
-  const int g = a.lanes, lane = threadIdx.x & (g - 1);
-  // whole waves stay in the loop: a lane past the pairs sums the last pair again and writes nothing
-  for (int64_t i0 = threadIdx.x / g; i0 - (threadIdx.x / g) < a.P; i0 += kPfLossThreads / g) {
-    const int64_t i = i0 < a.P ? i0 : a.P - 1;
-    double R[2], div[2];
-    for (int k = 0; k < 2; ++k) {
-      const int64_t row = i + k * a.P;
-      double s = 0.0, n = 0.0;
-      for (uint32_t p = lane; p < a.pieces; p += g) {
-        const PfPart q = a.part[row * a.pieces + p];
-        s += q.sum;
-        n += q.n;
-      }
-      s = group_sum_d(s, g);
-      n = group_sum_d(n, g);
-      if (a.ref.p && a.ref_rows) s -= (double)a.ref.at(row, 0);
-      div[k] = a.mean && n > 1.0 ? n : 1.0;     // an empty answer: a sum of nothing, divided by 1
-      R[k] = s / div[k];
-    }
-    if (lane != 0 || i0 >= a.P) continue;
-    a.reward[i] = (float)(a.beta * R[0]);
-    a.reward[i + a.P] = (float)(a.beta * R[1]);
-    const double h = a.beta * (R[0] - R[1]) - a.margin;
-    double v, dh;
-    if (a.kind == 0) {
-      v = (1.0 - a.smooth) * neg_log_sigma(h) + (a.smooth != 0.0 ? a.smooth * neg_log_sigma(-h) : 0.0);
-      dh = a.smooth - 1.0 / (1.0 + exp(h));
-    } else if (a.kind == 1) {
-      const double q = (h - 0.5) / a.beta;
-      v = q * q;
-      dh = 2.0 * q / a.beta;
-    } else {
-      v = h < 1.0 ? 1.0 - h : h != h ? h : 0.0;
-      dh = h < 1.0 ? -1.0 : h != h ? h : 0.0;
-    }
-    total += v;
-    const double c = dh * a.beta / (double)a.P;
-    a.coef[i] = (float)(c / div[0]);
-    a.coef[i + a.P] = (float)(-c / div[1]);
+// pair i from its rows' sums (chosen, rejected): the rewards and coefficients; returns its loss
+__device__ __forceinline__ double pf_pair(const PfArgs& a, int64_t i, const PfPart* q) {
+  double R[2], div[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const double s = q[k].sum - (a.ref.p && a.ref_rows ? (double)a.ref.at(i + k * a.P, 0) : 0.0);
+    div[k] = a.mean && q[k].n > 1.0 ? q[k].n : 1.0;           // an empty answer: a sum of nothing, divided by 1
+    R[k] = s / div[k];
+    a.reward[i + k * a.P] = (float)(a.beta * R[k]);
   }
+  const double h = a.beta * (R[0] - R[1]) - a.margin;
+  double v, dh;
+  if (a.kind == 0) {
+    v = (1.0 - a.smooth) * neg_log_sigma(h) + (a.smooth != 0.0 ? a.smooth * neg_log_sigma(-h) : 0.0);
+    dh = a.smooth - 1.0 / (1.0 + exp(h));
+  } else if (a.kind == 1) {
+    const double w = (h - 0.5) / a.beta;
+    v = w * w;
+    dh = 2.0 * w / a.beta;
+  } else {
+    v = h < 1.0 ? 1.0 - h : h != h ? h : 0.0;
+    dh = h < 1.0 ? -1.0 : h != h ? h : 0.0;
+  }
+  const double c = dh * a.beta / (double)a.P;
+  a.coef[i] = (float)(c / div[0]);
+  a.coef[i + a.P] = (float)(-c / div[1]);
+  return v;
+}
+__device__ __forceinline__ void pf_finish(const PfArgs& a, double total) {
+  __shared__ double red[kPfLossThreads / kWave];
   total = wave_sum_d(total);
   if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = total;
   __syncthreads();
@@ -129,6 +118,52 @@ __global__ __launch_bounds__(kPfLossThreads) void k_pref_loss(PfArgs a) {
     for (int w = 1; w < kPfLossThreads / kWave; ++w) total += red[w];
     *a.loss = (float)(total / (double)a.P);
   }
+}
+
+__global__ __launch_bounds__(kPfLossThreads) void k_pref_loss(PfArgs a) {
+  double total = 0.0;
+  const int g = a.lanes, lane = threadIdx.x & (g - 1);
+  // whole waves stay in the loop: a lane past the pairs sums the last pair again and writes nothing
+  for (int64_t i0 = threadIdx.x / g; i0 - (threadIdx.x / g) < a.P; i0 += kPfLossThreads / g) {
+    const int64_t i = i0 < a.P ? i0 : a.P - 1;
+    PfPart q[2];
+    for (int k = 0; k < 2; ++k) {
+      double s = 0.0, n = 0.0;
+      for (uint32_t p = lane; p < a.pieces; p += g) {
+        const PfPart x = a.part[(i + k * a.P) * a.pieces + p];
+        s += x.sum;
+        n += x.n;
+      }
+      q[k] = PfPart{group_sum_d(s, g), group_sum_d(n, g)};
+    }
+    if (lane == 0 && i0 < a.P) total += pf_pair(a, i, q);
+  }
+  pf_finish(a, total);
+}
+
+// Few short texts in one launch: a wave a text, then a thread a pair (us in two launches / in one: 1 pair x 60 5.5 / 3.4, 8 x
+// 512 5.5 / 4.7, 32 x 128, four texts a wave, 6.0 / 8.0)
+constexpr int kPfFew = kPfLossThreads / kWave, kPfShort = 512;    // texts, tokens
+template <bool ROW>
+__global__ __launch_bounds__(kPfLossThreads) void k_pref_few(PfArgs a) {
+  __shared__ PfPart part[kPfFew];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t row = threadIdx.x / kWave;
+  if (row < 2 * a.P) {
+    double s = 0.0;
+    int n = 0;
+    for (int64_t t = 4 * lane; t < a.L; t += 4 * kWave) pf_four<ROW>(a, row, t, a.L - t < 4 ? (int)(a.L - t) : 4, s, n);
+    s = wave_sum_d(s);
+    const double c = wave_sum_d((double)n);
+    if (lane == 0) part[row] = PfPart{s, c};
+  }
+  __syncthreads();
+  double total = 0.0;
+  if (threadIdx.x < a.P) {
+    const PfPart q[2] = {part[threadIdx.x], part[threadIdx.x + a.P]};
+    total = pf_pair(a, threadIdx.x, q);
+  }
+  pf_finish(a, total);
 }
 
 template <bool ROW>
@@ -194,7 +229,13 @@ extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, c
   a.loss = loss; a.reward = rewards; a.coef = coef;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(a.pieces * 2 * P)), block(kPfThreads);
-  if (a.lp.row() && a.mask.row() && (a.ref_rows || a.ref.row())) hipLaunchKernelGGL(k_pref_rows<true>, grid, block, 0, st, a);
+  const bool rows = a.lp.row() && a.mask.row() && (a.ref_rows || a.ref.row());
+  if (2 * P <= kPfFew && L <= kPfShort) {
+    if (rows) hipLaunchKernelGGL(k_pref_few<true>, dim3(1), dim3(kPfLossThreads), 0, st, a);
+    else hipLaunchKernelGGL(k_pref_few<false>, dim3(1), dim3(kPfLossThreads), 0, st, a);
+    return check_launch("asrn_preference_fwd");
+  }
+  if (rows) hipLaunchKernelGGL(k_pref_rows<true>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(k_pref_rows<false>, grid, block, 0, st, a);
   if (check_launch("asrn_preference_fwd")) return 1;
   hipLaunchKernelGGL(k_pref_loss, dim3(1), dim3(kPfLossThreads), 0, st, a);

@@ -221,7 +221,7 @@ def preferencia_exacta(lp, m, ref, beta, tipo, suavizado, margen, por_longitud):
     return loss.detach(), (beta * R).detach(), torch.autograd.grad(loss, v)[0]
 
 
-@pytest.mark.parametrize('P,L', [(1, 1), (1, 60), (3, 257), (2, 4096), (2, 4097), (5, 9001), (300, 33)])
+@pytest.mark.parametrize('P,L', [(1, 1), (1, 60), (3, 257), (8, 512), (8, 513), (9, 100), (2, 4096), (2, 4097), (5, 9001), (300, 33)])
 @pytest.mark.parametrize('tipo,suavizado,margen,por_longitud', [
     ('sigmoide', 0.0, 0.0, False), ('sigmoide', 0.1, 0.3, True), ('ipo', 0.0, 0.0, True), ('ipo', 0.0, -0.2, False),
     ('bisagra', 0.0, 0.0, False), ('bisagra', 0.0, 0.5, True)])
@@ -367,7 +367,7 @@ def politica_exacta(lp, A, vieja, m, lo, hi, tope, ref, beta, H, peso, reduccion
 EXP, EXPM1, KL = 3 * U, 7 * U, 12 * U
 
 
-@pytest.mark.parametrize('B,L', [(1, 1), (2, 50), (3, 2048), (3, 2049), (2, 7001), (700, 9)])
+@pytest.mark.parametrize('B,L', [(1, 1), (2, 50), (8, 512), (8, 513), (9, 100), (3, 2048), (3, 2049), (2, 7001), (700, 9)])
 @pytest.mark.parametrize('ventaja', ['fichas', 'textos'])
 @pytest.mark.parametrize('tope,kl,entropia,vieja', [(None, False, False, True), (1.5, True, True, True),
                                                     (None, True, False, False)])
