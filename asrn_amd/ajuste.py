@@ -75,8 +75,6 @@ def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False)
         raise ValueError(f'{quien}: logits of {logits.dtype} (fp32, bf16 or fp16 are taken)')
     if logits.shape[-1] < 1 or y.is_floating_point() or y.is_complex() or y.dtype == torch.bool:
         raise ValueError(f'{quien}: a vocabulary of {logits.shape[-1]} tokens and token ids of {y.dtype}')
-    if y.numel() >= 1 << 31:
-        raise ValueError(f'{quien}: {y.numel()} tokens (up to 2**31 - 1)')
     if y.device != dev:
         raise ValueError(f'{quien}: y is on {y.device}, the logits on {dev}')
     T = _numero(quien, 'temperatura', temperatura, 1e-6, 1e6)

@@ -268,8 +268,8 @@ static int lp_check(const LpArgs& a, int32_t type, const char* what) {
                    a.sb >= 0 && a.st >= 0 && a.rows % a.L == 0,
                "%s: bad sizes rows=%lld L=%lld V=%lld strides %lld, %lld", what, (long long)a.rows, (long long)a.L,
                (long long)a.V, (long long)a.sb, (long long)a.st);
-  // a launch has fewer than 2^32 threads: 64 a row for short vocabularies, else 256 or 1,024
-  ASRN_REQUIRE(a.rows < (int64_t(1) << (a.V <= 2048 ? 26 : 22)), "%s: too many rows (%lld)", what, (long long)a.rows);
+  // a launch has fewer than 2^32 threads: 64 a row for short vocabularies, else 256 (1,024 for up to 1,024 rows)
+  ASRN_REQUIRE(a.rows < (int64_t(1) << (a.V <= 2048 ? 26 : 24)), "%s: too many rows (%lld)", what, (long long)a.rows);
   ASRN_REQUIRE(a.inv_t > 0.f && a.inv_t < INFINITY, "%s: the temperature's inverse must be positive and finite", what);
   return 0;
 }

@@ -27,6 +27,8 @@ def test_token_logp_checks(lib):
     _mal(lib, f(0, 4, 2, 0, 20, 10), 'bad sizes')
     _mal(lib, f(0, 4, 2, 10, -20, 10), 'bad sizes')
     _mal(lib, f(0, 1 << 31, 1, 10, 20, 10), 'bad sizes')
+    _mal(lib, f(0, 1 << 26, 1, 10, 20, 10), 'too many rows')
+    _mal(lib, f(1, 1 << 24, 1, 5000, 5000, 5000), 'too many rows')
     _mal(lib, f(0, 4, 2, 10, 20, 10), 'null pointer')
     assert f(0, 0, 2, 10, 20, 10) == 0                      # no rows: no launch
     _mal(lib, lib.asrn_token_logp_fwd(N, 0, 4, 2, 10, 20, 10, N, -100, 0.0, N, N, N, N), 'temperature')

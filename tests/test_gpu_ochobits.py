@@ -447,6 +447,31 @@ def test_past_32_bits():
     assert torch.equal(ops.leer8(q, e, torch.bfloat16)[-3:], ops.leer8(q2, e2, torch.bfloat16))
 
 
+@pytest.mark.parametrize('d', [64, 2048, 10])
+def test_one_output_or_input_alone(d):
+    """Gradients of one output only, and of one input only."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    ln = torch.nn.LayerNorm(d).to(DEV)
+    x, gy = r(9, d).requires_grad_(), r(9, d)
+    y, a, _ = ops.norma8(ln, x, torch.float32)
+    solo = torch.autograd.grad(y, (x, ln.weight), gy, retain_graph=True)
+    cero = torch.autograd.grad((y, a), (x, ln.weight), (gy, torch.zeros_like(gy)), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(solo, cero))
+    dx, dw = torch.autograd.grad(a, (x, ln.weight), gy, allow_unused=True)
+    assert torch.equal(dx, gy) and (dw is None or (dw == 0).all())
+    y, a, _ = ops.norma8(ln, x.detach(), torch.float32)
+    assert torch.allclose(torch.autograd.grad(y, ln.bias, gy)[0], gy.sum(0), atol=1e-4)
+    u, h = r(9, d), r(9, d).requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.suma_gelu8(h, u), h, gy)[0], gy)
+    s = ops.suma_gelu8(h.detach(), u.requires_grad_())
+    assert torch.equal(torch.autograd.grad(s, u, gy)[0], torch.autograd.grad(ops.gelu8(u)[0], u, gy)[0])
+    w = r(3, d)
+    e, guardado = ops.gelu8(u)
+    y = lineal8(e, w, None, guardado)                # a weight without a gradient: nothing is read back
+    assert torch.allclose(torch.autograd.grad(y, e, torch.ones_like(y))[0], w.sum(0).expand(9, d), atol=1e-5)
+
+
 def test_second_gradients_are_refused():
     x = torch.randn(4, 64, device=DEV, requires_grad=True)
     for y in (ops.gelu8(x)[0], ops.norma8(torch.nn.LayerNorm(64).to(DEV), x, torch.float32)[0]):
