@@ -1647,10 +1647,15 @@ def leer8(q, e, dtype=torch.float32):
     return _leer8(q.data_ptr(), e.data_ptr(), *q.shape, dev, dtype)
 
 
+def _leido(forma, dtype, dev):
+    """Room for what the kernels read back, which they write in fp32 or bf16: other dtypes are rounded from fp32."""
+    return torch.empty(forma, dtype=torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, device=dev)
+
+
 def _leer8(q, e, N, d, dev, dtype, gelu=False):
-    out = torch.empty((N, d), dtype=dtype, device=dev)
+    out = _leido((N, d), dtype, dev)
     _en(dev, 'asrn_unpack8', q, e, N, d, int(gelu), int(dtype == torch.bfloat16), ptr(out))
-    return out
+    return out.to(dtype)
 
 
 def _gelu8_ok(u):
@@ -1731,10 +1736,10 @@ def _leer_norma8(N, d, k=1, L=None):
         q, dev = sitio.data_ptr(), sitio.device
         g, b = _c(g.detach(), torch.float32), _c(b.detach(), torch.float32)
         if _norma8_propia(d) and not (g.data_ptr() | b.data_ptr()) % 16:
-            out = torch.empty((N, d * k), dtype=dtype, device=dev)
+            out = _leido((N, d * k), dtype, dev)
             _en(dev, 'asrn_norm8_read', q, q + s, ptr(g), ptr(b), q + m, 1 if L is None else N // L, L or N, d, k,
                 int(dtype == torch.bfloat16), ptr(out))
-            return out
+            return out.to(dtype)
         mu, rstd = sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1)
         y = (_leer8(q, q + s, N, d, dev, torch.float32) - mu) * rstd * g + b
         if k == 1:

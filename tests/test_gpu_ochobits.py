@@ -500,3 +500,31 @@ def test_strided_inputs_and_offsets():
         f = gy.double()
         ref = s * (f - f.mean(-1, keepdim=True) - xh * (f * xh).mean(-1, keepdim=True)) + f
         assert (dx - ref).abs().max() <= 1e-5 * (1 + s.max())
+
+
+@pytest.mark.parametrize('d', [64, 30])
+@pytest.mark.parametrize('dt', [torch.float16, torch.float64])
+def test_products_in_other_dtypes(d, dt):
+    """Products in fp16 (autocast) and fp64 after ops that kept fp32 inputs: the weight gradient is lineal's on the values
+    read back, rounded to the product's dtype."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(2, 9, d, generator=g, device=DEV)
+    w = torch.randn(8, d, generator=g, device=DEV)
+    ln = torch.nn.LayerNorm(d).to(DEV)
+
+    def gw(op, y, peso, *resto):
+        peso = peso.detach().to(torch.float64 if dt == torch.float64 else torch.float32).requires_grad_()
+        with torch.autocast('cuda', dtype=torch.float16, enabled=dt == torch.float16):
+            z = op(y.double() if dt == torch.float64 else y, peso, None, *resto)
+        assert z.dtype == dt
+        return torch.autograd.grad(z, peso, torch.ones_like(z))[0]
+
+    for y, guardado in (ops.gelu8(x.clone().requires_grad_()), ops.norma8(ln, x, torch.float32)[::2]):
+        leido = guardado.leer(guardado.tensores, dt)
+        assert leido.dtype == dt and torch.equal(leido, guardado.leer(guardado.tensores, torch.float32).to(dt))
+        assert torch.equal(gw(lineal8, y, w, guardado), gw(lineal, leido.float().view(x.shape), w))
+    z, _, guardado = ops.norma8(ln, x, torch.float32)
+    cols, guardado = ops.ventana8(z, 3, torch.float32, guardado)
+    w3 = torch.randn(8, 3 * d, generator=g, device=DEV)
+    leido = guardado.leer(guardado.tensores, dt)
+    assert torch.equal(gw(lineal8, cols, w3, guardado), gw(lineal, leido.float().view(cols.shape), w3))
