@@ -257,6 +257,9 @@ def lineal8(x, w, b, guardado):
     ops.ventana8 or ops.gelu8 returned with x (None: lineal itself). The product and x's gradient are lineal's."""
     if guardado is None or not torch.is_grad_enabled():
         return lineal(x, w, b)
+    N, d = guardado.forma
+    if x.shape[-1] != d or x.numel() != N * d:
+        raise ValueError(f'lineal8: x {tuple(x.shape)} and rows ({N}, {d}) kept of another tensor')
     dev = x.device.type
     dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else x.dtype
     return _Lineal8.apply(x, w, b, dt, guardado.leer, *guardado.tensores)

@@ -1596,10 +1596,10 @@ GRUPO8 = 32                   # neighbouring channels that share a scale
 
 class Guardado8:
     """What norma8, ventana8 or gelu8 keep of their input, for lineal8: leer(tensores, dtype) gives the rows of their
-    output (N, d), formed again from the 8 bits."""
+    output, `forma` (N, d), formed again from the 8 bits."""
 
-    def __init__(self, leer, tensores):
-        self.leer, self.tensores = leer, tuple(tensores)
+    def __init__(self, leer, tensores, forma):
+        self.leer, self.tensores, self.forma = leer, tuple(tensores), forma
 
 
 _corriente = torch._C._cuda_getCurrentRawStream       # a stream's handle without the Python object around it
@@ -1676,8 +1676,8 @@ def gelu8(u):
     if not _gelu8_ok(u):
         return F.gelu(u), None
     y, sitio = nodos().gelu8(u, None)
-    d = u.shape[-1]
-    return y, Guardado8(_leer_gelu8(u.numel() // d, d), (sitio,))
+    forma = (u.numel() // u.shape[-1], u.shape[-1])
+    return y, Guardado8(_leer_gelu8(*forma), (sitio,), forma)
 
 
 def suma_gelu8(h, u):
@@ -1754,6 +1754,9 @@ def norma8(ln, x, dtype):
     the deviation of x itself. The output is norma_residual's; the gradients of x and the parameters are those at the
     8-bit values. x fp32, dtype fp32 or bf16. Without gradients, off the GPU or for another ln: norma_residual and None."""
     d = x.shape[-1]
+    for p in (ln.weight, ln.bias):
+        if p is not None and p.device != x.device:           # its address means nothing to a kernel on x's device
+            raise ValueError(f'norma8: x is on {x.device}, the LayerNorm on {p.device}')
     if not (x.is_cuda and x.dtype == torch.float32 and x.numel() > 0 and dtype in (torch.float32, torch.bfloat16)
             and torch.is_grad_enabled() and ln.elementwise_affine and ln.bias is not None
             and tuple(ln.normalized_shape) == (d,)):
@@ -1762,13 +1765,18 @@ def norma8(ln, x, dtype):
         y, x, sitio = nodos().norma8(x, ln.weight, ln.bias, ln.eps, dtype == torch.bfloat16)
     else:
         y, x, sitio = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
-    return y, x, Guardado8(_leer_norma8(x.numel() // d, d), (sitio, ln.weight, ln.bias))
+    N = x.numel() // d
+    return y, x, Guardado8(_leer_norma8(N, d), (sitio, ln.weight, ln.bias), (N, d))
 
 
 def ventana8(z, k, dtype, guardado):
     """(ventana_causal(z, k, dtype), what lineal8 reads those columns from) for the output z (B, L, d) fp32 of norma8 and
     what norma8 kept."""
+    if z.dim() != 3 or z.dtype != torch.float32 or dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f'ventana8: z {tuple(z.shape)} of {z.dtype} to {dtype}: (B, L, d) fp32 to fp32 or bf16 is needed')
     if guardado is None:
         return ventana_causal(z, k, dtype), None
     B, L, d = z.shape
-    return ventana_causal(z, k, dtype), Guardado8(_leer_norma8(B * L, d, k, L), guardado.tensores)
+    if guardado.forma != (B * L, d) or len(guardado.tensores) != 3:
+        raise ValueError(f'ventana8: z {tuple(z.shape)} and rows {guardado.forma} that norma8 did not keep for it')
+    return ventana_causal(z, k, dtype), Guardado8(_leer_norma8(B * L, d, k, L), guardado.tensores, (B * L, d * k))

@@ -528,3 +528,24 @@ def test_products_in_other_dtypes(d, dt):
     w3 = torch.randn(8, 3 * d, generator=g, device=DEV)
     leido = guardado.leer(guardado.tensores, dt)
     assert torch.equal(gw(lineal8, cols, w3, guardado), gw(lineal, leido.float().view(cols.shape), w3))
+
+
+def test_what_was_kept_belongs_to_its_tensor():
+    """ventana8 and lineal8 refuse what an op kept of a tensor of another size, norma8 parameters on another device."""
+    x = torch.randn(2, 9, 64, device=DEV)
+    w = torch.randn(8, 64, device=DEV, requires_grad=True)
+    ln = torch.nn.LayerNorm(64).to(DEV)
+    z, _, guardado = ops.norma8(ln, x, torch.float32)
+    y, del_gelu = ops.gelu8(x.requires_grad_())
+    for otro in (torch.randn(2, 10, 64, device=DEV), torch.randn(1, 9, 64, device=DEV), torch.randn(4, 9, 32, device=DEV)):
+        with pytest.raises(ValueError, match='ventana8'):
+            ops.ventana8(otro, 3, torch.float32, guardado)
+        with pytest.raises(ValueError, match='lineal8'):
+            lineal8(otro, w, None, guardado)
+    for args in ((z, 3, torch.float32, del_gelu), (z, 3, torch.float16, guardado), (z.bfloat16(), 3, torch.bfloat16, guardado),
+                 (z.view(18, 64), 3, torch.float32, guardado), (z, 3, torch.float16, None)):
+        with pytest.raises(ValueError, match='ventana8'):
+            ops.ventana8(*args)
+    with pytest.raises(ValueError, match='norma8'):
+        ops.norma8(torch.nn.LayerNorm(64), x, torch.float32)
+    assert lineal8(y, w, None, del_gelu).shape == (2, 9, 8)
