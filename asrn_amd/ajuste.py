@@ -145,8 +145,8 @@ def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope
     mascara (B, L): nonzero on the answers' tokens (None: all); what it hides is not used, NaN and infinities included.
     reduccion: 'fichas' averages over the masked tokens, 'textos' over the texts' own means (texts without tokens left
     out); NaN when no token is left. The gradient goes to lp and entropia; the rest are constants. Statistics (means over
-    the masked tokens): [share of clipped tokens, r - 1 - log r, exp(q) - 1 - q, H]. Everything per token and every sum
-    is formed in double."""
+    the masked tokens): [share of clipped tokens, r - 1 - log r, exp(q) - 1 - q, H]. Differences, products and
+    sums are formed in double, exponentials to fp32's accuracy."""
     quien = 'perdida_politica'
     dev = _dev(lp)
     if lp.dim() != 2 or lp.shape[0] < 1 or not lp.is_floating_point():

@@ -12,12 +12,14 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
 #include <stdexcept>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "asrn_hip.h"
 
@@ -353,6 +355,17 @@ std::tuple<Tensor, Tensor, Tensor> norma8(const Tensor& x, const Tensor& gamma, 
   return {r[0], r[1], r[2]};
 }
 
+// Whether a graph recorded on the default stream still holds one of these leaves' accumulators. A backward inside a
+// capture would run it on that stream, which no capture may wait for.
+bool hojas_en_uso(const std::vector<Tensor>& hojas) {
+  for (const Tensor& t : hojas) {
+    const auto nodo = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto corriente = nodo ? nodo->stream() : std::nullopt;
+    if (corriente && corriente->id() == 0) return true;
+  }
+  return false;
+}
+
 // direccion(name): the address of an entry point of the opened library; error: the class of its failures
 void iniciar(const py::function& direccion, py::object error) {
   const auto de = [&](auto& f, const char* nombre) {
@@ -388,6 +401,7 @@ void iniciar(const py::function& direccion, py::object error) {
 PYBIND11_MODULE(_nodos, m) {
   using Libre = py::call_guard<py::gil_scoped_release>;
   m.def("iniciar", &iniciar);
+  m.def("hojas_en_uso", &hojas_en_uso);
   m.def("logp", &logp);
   m.def("preferencia", &preferencia, Libre());
   m.def("politica", &politica, Libre());

@@ -16,6 +16,7 @@ import warnings
 import torch
 
 from . import archivo, ops
+from ._lib import nodos
 from .modelo import _base
 
 # the suffix and gate parameters of each ASRN layer learn this many times faster (asrn/nucleo.py:2188-2189)
@@ -191,6 +192,10 @@ class PasoGrafado:
         return r
 
     def _capturar(self):
+        # a graph of an eager call that still lives would take the captured backward to the default stream
+        if nodos().hojas_en_uso(self.params):
+            raise RuntimeError('PasoGrafado: the step cannot be captured while an eager graph of the parameters lives '
+                               '(a loss, logits or scores kept from a call outside torch.no_grad()): drop or detach it')
         # gradients start as None: inside the graph they are assigned, not accumulated
         self.opt.zero_grad(set_to_none=True)
         self.grafo = torch.cuda.CUDAGraph()

@@ -681,7 +681,7 @@ int asrn_preference_bwd(const float* coef, const float* g, const uint8_t* mask, 
  * *loss = the mean over the masked tokens, or over the texts' means (by_text); stats (4) = means over the tokens of
  * [clipped, r - 1 - d, exp q - 1 - q, H]; raw (B, L, or null) = each token's gradient with respect to lp, weight (B) =
  * what a text's tokens are divided by. bwd: dlp (B, L) = *g raw / weight, dentropy (B, L) = -*g entropy_weight /
- * weight (either null), 0 where masked. In double, fixed order. workspace: asrn_policy_workspace(B, L) bytes, 16-byte
+ * weight (either null), 0 where masked. Sums in double, fixed order. workspace: asrn_policy_workspace(B, L) bytes, 16-byte
  * aligned (-1: sizes refused). */
 int64_t asrn_policy_workspace(int64_t B, int64_t L);
 int asrn_policy_fwd(const float* lp, const float* advantage, const float* old_lp, const float* ref_lp,

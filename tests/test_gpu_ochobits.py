@@ -389,6 +389,28 @@ def test_graphed_fine_tuning(cual, checkpoint):
     assert all(abs(a - b) <= 2e-5 * (1 + abs(b)) for a, b in zip(*perdidas)), perdidas
 
 
+def test_graphed_step_refuses_a_living_eager_graph():
+    """A score kept with its graph holds the parameters' accumulators on the default stream: the capture is refused, and
+    runs once the score is dropped."""
+    from asrn_amd._lib import nodos
+    x = torch.randint(0, 61, (2, 31), generator=torch.Generator().manual_seed(3)).to(DEV)
+    m = _modelo('no')
+    opt = asrn_amd.crear_optimizador(m, 1e-3, capturable=True)
+    paso = asrn_amd.PasoGrafado(m, opt, 2, 30, precision='fp32', calentar=1)
+    paso(x[:, :-1], x[:, 1:], lr=1e-3)
+    assert not nodos().hojas_en_uso(paso.params)
+    lp = m.log_probabilidades(x[:, :-1], x[:, 1:])
+    assert nodos().hojas_en_uso(paso.params)
+    with pytest.raises(RuntimeError, match='eager graph'):
+        paso(x[:, :-1], x[:, 1:], lr=1e-3)
+    esperada = -lp.detach().mean()
+    del lp
+    assert not nodos().hojas_en_uso(paso.params)
+    for _ in range(3):
+        perdida, _, salto = paso(x[:, :-1], x[:, 1:], lr=0.0)
+        assert abs(perdida.item() - esperada.item()) <= 1e-5 * esperada.item() and salto.item() == 0
+
+
 def test_fine_tuning_step():
     """The operators together, as a fine-tuning step runs them: a reference's scores, then preference and policy steps on
     a model in 8 bits. The losses and gradients are finite, every parameter moves, and the step in 8 bits takes the same
