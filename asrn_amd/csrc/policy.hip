@@ -40,13 +40,19 @@ struct PoArgs {
   const float* g; float* dlp; float* dent;
 };
 
-// exp d within two steps of fp32: expf of d rounded, and the rounding's own factor; past fp32's range the square of the
-// half's (the double exp's registers would cost half the waves)
+// exp d over double's range to a few steps of fp32: expf of d rounded, and the rounding's own factor; past fp32's range the
+// square of the half's (two steps) or, from 160 on, the eighth power of the eighth's (eight steps; the double exp's
+// registers would cost half the waves)
 __device__ __forceinline__ double po_exp(double d) {
   const float f = (float)d;
-  const bool far = f > 80.f;
-  const double e = expf(far ? 0.5f * f : f), rest = d - (double)f;
-  return (far ? e * e : e) * (fabs(rest) < 1.0 ? 1.0 + rest : 1.0);   // infinite d: expf's answer; NaN: NaN
+  double e = expf(f > 160.f ? 0.125f * f : f > 80.f ? 0.5f * f : f);
+  const double rest = d - (double)f;
+  if (f > 80.f) e *= e;
+  if (f > 160.f) {
+    e *= e;
+    e *= e;
+  }
+  return e * (fabs(rest) < 1.0 ? 1.0 + rest : 1.0);             // infinite d: expf's answer; NaN: NaN
 }
 // exp d - 1 (first) and exp d - 1 - d (second), each to a few steps of fp32 at every d: up to |d| = 1 from the second
 // one's series, where the difference would cancel (the first term left out is 2^-32 of the sum), past it from exp d
@@ -91,7 +97,8 @@ __device__ __forceinline__ void po_four(const PoArgs& a, int64_t row, int64_t t,
     if (u < n && (m >> (8 * u) & 0xffu)) {    // what a mask hides may be infinite or NaN: nothing of it is used
       const double A = adv[u], d = a.old.p ? (double)lp[u] - (double)old[u] : (double)(lp[u] - lp[u]);
       const PoExp x = po_terms(d);
-      const double rA = fma(x.e1, A, A);
+      // an advantage of 0 takes nothing from any finite d, also where exp d passes double's range
+      const double rA = fma(A == 0.0 && fabs(d) < INFINITY ? 0.0 : x.e1, A, A);
       const bool cap = a.cap > 0.0 && A < 0.0 && d > a.log_cap;
       const bool out = cap || (A > 0.0 && d > a.log_hi) || (A < 0.0 && d < a.log_lo);
       double l = -(out ? (cap ? a.cap : A > 0.0 ? a.hi : a.lo) * A : rA);

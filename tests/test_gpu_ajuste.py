@@ -425,6 +425,34 @@ def test_policy_borders():
     assert abs(perdida.item() - (0.0 + 0.0 - 1.2 + 0.8) / 4) <= 1e-7 and (d == 0).all()
 
 
+@pytest.mark.parametrize('B', [1, 9])                   # one launch, and the tokens' own
+def test_policy_far_ratios(B):
+    """Ratios past fp32's range, against float64: nothing of them under an advantage of 0 (at any finite d, 64 bits' own
+    range passed too), finite under one that is small enough, and in a KL term of a small weight."""
+    lp = torch.tensor([[177.0, 178.0, 300.0, 709.0, 800.0, 3e38, -3e38, 0.5]] * B, device=DEV, requires_grad=True)
+    A = torch.zeros(B, 8, device=DEV)
+    A[:, -1] = -1.0
+    perdida, est = asrn_amd.perdida_politica(lp, A, torch.zeros_like(lp))
+    d, = torch.autograd.grad(perdida, lp)
+    e = math.exp(0.5) / 8
+    assert abs(perdida.item() - e) <= 2 * EXP * e and (d[:, :-1] == 0).all() and ((d[:, -1] - e / B).abs() <= 6 * U * e).all()
+    assert torch.isfinite(est[:1]).all()
+    # exp d for d > 160 is the eighth power of expf's, each within a step (2 U): 16 U, and the loss's own rounding
+    for v in (161.0, 177.75, 178.0, 185.3):
+        lp = torch.full((B, 3), v, device=DEV, requires_grad=True)
+        A = torch.full((B,), -1e-43, device=DEV)         # subnormal: r A is finite in fp32
+        perdida, _ = asrn_amd.perdida_politica(lp, A, torch.zeros_like(lp))
+        d, = torch.autograd.grad(perdida, lp)
+        e = math.exp(lp[0, 0].item()) * -A[0].double().item()
+        assert abs(perdida.item() - e) <= 18 * U * e and ((d.double() * 3 * B - e).abs() <= 22 * U * e).all(), v
+    for q, beta in ((170.0, 1e-60), (178.0, 1e-60), (300.0, 1e-120), (700.0, 1e-290)):
+        lp = torch.zeros(B, 2, device=DEV, requires_grad=True)
+        perdida, _ = asrn_amd.perdida_politica(lp, torch.zeros(B, device=DEV), lp_ref=torch.full((B, 2), q, device=DEV), beta=beta)
+        d, = torch.autograd.grad(perdida, lp)
+        e = beta * (math.expm1(q) - q)
+        assert abs(perdida.item() - e) <= 18 * U * e and ((d.double() * 2 * B + e).abs() <= 22 * U * e).all(), q
+
+
 def test_policy_strides_and_masks():
     g = torch.Generator(device=DEV).manual_seed(5)
     B, L = 6, 3001
