@@ -1596,10 +1596,10 @@ GRUPO8 = 32                   # neighbouring channels that share a scale
 
 class Guardado8:
     """What norma8, ventana8 or gelu8 keep of their input, for lineal8: leer(tensores, dtype) gives the rows of their
-    output, `forma` (N, d), formed again from the 8 bits."""
+    output, `forma` (N, d), formed again from the 8 bits. norma: norma8's own, the one that ventana8 reads."""
 
-    def __init__(self, leer, tensores, forma):
-        self.leer, self.tensores, self.forma = leer, tuple(tensores), forma
+    def __init__(self, leer, tensores, forma, norma=False):
+        self.leer, self.tensores, self.forma, self.norma = leer, tuple(tensores), forma, norma
 
 
 _corriente = torch._C._cuda_getCurrentRawStream       # a stream's handle without the Python object around it
@@ -1766,7 +1766,7 @@ def norma8(ln, x, dtype):
     else:
         y, x, sitio = Norma8.apply(x, ln.weight, ln.bias, ln.eps, dtype)
     N = x.numel() // d
-    return y, x, Guardado8(_leer_norma8(N, d), (sitio, ln.weight, ln.bias), (N, d))
+    return y, x, Guardado8(_leer_norma8(N, d), (sitio, ln.weight, ln.bias), (N, d), norma=True)
 
 
 def ventana8(z, k, dtype, guardado):
@@ -1777,6 +1777,6 @@ def ventana8(z, k, dtype, guardado):
     if guardado is None:
         return ventana_causal(z, k, dtype), None
     B, L, d = z.shape
-    if guardado.forma != (B * L, d) or len(guardado.tensores) != 3:
+    if guardado.forma != (B * L, d) or not guardado.norma:
         raise ValueError(f'ventana8: z {tuple(z.shape)} and rows {guardado.forma} that norma8 did not keep for it')
     return ventana_causal(z, k, dtype), Guardado8(_leer_norma8(B * L, d, k, L), guardado.tensores, (B * L, d * k))

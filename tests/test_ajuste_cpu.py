@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import asrn_amd
-from asrn_amd import _lib
+from asrn_amd import _lib, ops
 
 N = None
 
@@ -94,3 +94,15 @@ def test_public_names_refuse_cpu_tensors():
               lambda: asrn_amd.preference_loss(lp), lambda: asrn_amd.policy_loss(lp, lp)):
         with pytest.raises(RuntimeError, match='GPU only'):
             f()
+
+
+def test_window_reads_only_what_norma8_kept():
+    """The columns of a window have rows of another width than the ones kept: reading them as norma8's would leave their
+    buffers."""
+    leer = lambda ts, dt: pytest.fail('read')
+    t = (torch.zeros(1), torch.zeros(4), torch.zeros(4))
+    z = torch.zeros(2, 5, 12)
+    for guardado in (ops.Guardado8(leer, t, (10, 12)), ops.Guardado8(leer, t[:1], (10, 12)),
+                     ops.Guardado8(leer, t, (10, 4), norma=True)):
+        with pytest.raises(ValueError, match='did not keep'):
+            ops.ventana8(z, 3, torch.float32, guardado)

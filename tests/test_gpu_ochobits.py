@@ -571,3 +571,13 @@ def test_what_was_kept_belongs_to_its_tensor():
     with pytest.raises(ValueError, match='norma8'):
         ops.norma8(torch.nn.LayerNorm(64), x, torch.float32)
     assert lineal8(y, w, None, del_gelu).shape == (2, 9, 8)
+
+
+def test_window_of_a_window_is_refused():
+    """What ventana8 itself returns goes to lineal8, not back into ventana8."""
+    ln = torch.nn.LayerNorm(64).to(DEV)
+    z, _, guardado = ops.norma8(ln, torch.randn(2, 9, 64, device=DEV), torch.float32)
+    for k in (1, 3):
+        cols, gc = ops.ventana8(z, k, torch.float32, guardado)
+        with pytest.raises(ValueError, match='did not keep'):
+            ops.ventana8(cols, k, torch.float32, gc)
