@@ -260,6 +260,8 @@ def lineal8(x, w, b, guardado):
     N, d = guardado.forma
     if x.shape[-1] != d or x.numel() != N * d:
         raise ValueError(f'lineal8: x {tuple(x.shape)} and rows ({N}, {d}) kept of another tensor')
+    if any(t.device != x.device for t in guardado.tensores):     # the weight gradient's kernels read both
+        raise ValueError(f'lineal8: x is on {x.device}, the rows kept on {guardado.tensores[0].device}')
     dev = x.device.type
     dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else x.dtype
     return _Lineal8.apply(x, w, b, dt, guardado.leer, *guardado.tensores)

@@ -1779,4 +1779,6 @@ def ventana8(z, k, dtype, guardado):
     B, L, d = z.shape
     if guardado.forma != (B * L, d) or not guardado.norma:
         raise ValueError(f'ventana8: z {tuple(z.shape)} and rows {guardado.forma} that norma8 did not keep for it')
+    if guardado.tensores[0].device != z.device:
+        raise ValueError(f'ventana8: z is on {z.device}, the rows kept on {guardado.tensores[0].device}')
     return ventana_causal(z, k, dtype), Guardado8(_leer_norma8(B * L, d, k, L), guardado.tensores, (B * L, d * k))

@@ -4,6 +4,7 @@ import torch
 
 import asrn_amd
 from asrn_amd import _lib, ops
+from asrn_amd.lineal import lineal8
 
 N = None
 
@@ -106,3 +107,14 @@ def test_window_reads_only_what_norma8_kept():
                      ops.Guardado8(leer, t, (10, 4), norma=True)):
         with pytest.raises(ValueError, match='did not keep'):
             ops.ventana8(z, 3, torch.float32, guardado)
+
+
+def test_what_was_kept_on_another_device_is_refused():
+    """The weight gradient reads the product's gradient and the kept rows in one kernel: they must be on one device."""
+    leer = lambda ts, dt: pytest.fail('read')
+    t = tuple(torch.zeros(4, device='meta') for _ in range(3))
+    x, w = torch.zeros(2, 5, 4), torch.zeros(3, 4, requires_grad=True)
+    with pytest.raises(ValueError, match='kept on meta'):
+        lineal8(x, w, None, ops.Guardado8(leer, t, (10, 4)))
+    with pytest.raises(ValueError, match='kept on meta'):
+        ops.ventana8(x, 3, torch.float32, ops.Guardado8(leer, t, (10, 4), norma=True))
