@@ -1715,12 +1715,13 @@ class Norma8(torch.autograd.Function):
         sitio, g = ctx.saved_tensors
         forma, N, d, m, s = ctx.meta
         q = sitio.data_ptr()
-        mu, rstd = sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1)
-        xh = (_leer8(q, q + s, N, d, sitio.device, torch.float32) - mu) * rstd
-        f = dy.float().reshape(N, d)
-        p = f * g
-        dx = rstd * (p - p.mean(1, keepdim=True) - xh * (p * xh).mean(1, keepdim=True)) + dres.reshape(N, d)
-        return dx.view(forma), (f * xh).sum(0), f.sum(0), None, None
+        mu, rstd = (t.contiguous() for t in sitio[m:m + 8 * N].view(torch.float32).view(N, 2).split(1, 1))
+        # torch's LayerNorm backward on the 8-bit values: its sums over the rows clear nothing with a memset, as torch's
+        # sum does over many rows, so a captured step may hold it
+        dx, dg, db = torch.ops.aten.native_layer_norm_backward(
+            dy.float().reshape(N, d).contiguous(), _leer8(q, q + s, N, d, sitio.device, torch.float32), (d,), mu, rstd, g,
+            torch.empty_like(g), (True, True, True))
+        return (dx + dres.reshape(N, d)).view(forma), dg, db, None, None
 
 
 def _norma8_propia(d):

@@ -581,3 +581,34 @@ def test_window_of_a_window_is_refused():
         cols, gc = ops.ventana8(z, k, torch.float32, guardado)
         with pytest.raises(ValueError, match='did not keep'):
             ops.ventana8(cols, k, torch.float32, gc)
+
+
+@pytest.mark.parametrize('N,d', [(40_000, 66), (3, 8198)])
+def test_other_widths_in_a_graph(N, d):
+    """The widths that torch's LayerNorm runs: a captured backward replays as the eager one, step after step."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    ln = torch.nn.LayerNorm(d).to(DEV)
+    x, gy = r(N, d).requires_grad_(), r(N, d)
+
+    def paso():
+        y, a, _ = ops.norma8(ln, x, torch.float32)
+        return [y.detach(), *torch.autograd.grad((y, a), (x, ln.weight, ln.bias), (gy, gy))]
+
+    lado = torch.cuda.Stream()
+    lado.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(lado):
+        paso()
+    torch.cuda.current_stream().wait_stream(lado)
+    torch.cuda.synchronize()
+    grafo = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(grafo):
+        salida = paso()
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(r(N, d))
+            gy.copy_(r(N, d))
+        grafo.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(salida, paso()):
+            assert torch.equal(a, b)
