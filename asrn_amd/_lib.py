@@ -117,6 +117,7 @@ SIGNATURES = {
     'asrn_decode_produce': (ctypes.c_int, [_P] * 4 + [_I64, _I32] + [_P] * 9 + [_I32] * 4 + [_P, _P, _F32, _P, _P, _F32,
                                                                                               _F32, _P, _P, _I32]
                             + [_P] * 6 + [_I64, _I64, _P, _P, _P, _I64, _P]),
+    'asrn_graph_memsets': (_I64, [_P]),
     'asrn_token_logp_fwd': (ctypes.c_int, [_P, _I32] + [_I64] * 5 + [_P, _I64, _F32, _P, _P, _P, _P]),
     'asrn_token_logp_bwd': (ctypes.c_int, [_P, _I32] + [_I64] * 5 + [_P, _I64, _F32] + [_P] * 6),
     'asrn_preference_workspace': (_I64, [_I64, _I64]),

@@ -16,7 +16,7 @@ import warnings
 import torch
 
 from . import archivo, ops
-from ._lib import nodos
+from ._lib import nodos, query
 from .modelo import _base
 
 # the suffix and gate parameters of each ASRN layer learn this many times faster (asrn/nucleo.py:2188-2189)
@@ -196,11 +196,27 @@ class PasoGrafado:
         if nodos().hojas_en_uso(self.params):
             raise RuntimeError('PasoGrafado: the step cannot be captured while an eager graph of the parameters lives '
                                '(a loss, logits or scores kept from a call outside torch.no_grad()): drop or detach it')
+        # a loss of the caller's may record memsets (a torch sum over many values does), which ModeloASRN._una_corriente
+        # keeps out of steps on one stream: such a step is captured again on two, before any replay
+        ajena = self.perdida is not entropia
+        grafo, salida = self._grabado(guardar=ajena)
+        if ajena and query('asrn_graph_memsets', grafo.raw_cuda_graph()) != 0:
+            del grafo, salida
+            antes = getattr(self.modelo, 'permite_una_corriente', True)
+            self.modelo.permite_una_corriente = False
+            try:
+                grafo, salida = self._grabado()
+            finally:
+                self.modelo.permite_una_corriente = antes
+        self.grafo, self.salida = grafo, salida
+
+    def _grabado(self, guardar=False):
         # gradients start as None: inside the graph they are assigned, not accumulated
         self.opt.zero_grad(set_to_none=True)
-        self.grafo = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.grafo):
-            self.salida = self._uno()
+        grafo = torch.cuda.CUDAGraph(keep_graph=guardar)
+        with torch.cuda.graph(grafo):
+            salida = self._uno()
+        return grafo, salida
 
     def __call__(self, x, y, lr=None, extras=()):
         """x, y (lote, largo) and the extras of this step -> (loss, gradient norm, skipped) as device tensors."""

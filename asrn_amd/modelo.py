@@ -214,6 +214,8 @@ class ModeloASRN(nn.Module):
     protecciones: the ASRN
     layers' Protecciones (group A by default); the remaining keywords are CapaASRNEstable's."""
 
+    permite_una_corriente = True       # False: no step keeps its ASRN layers on one stream (PasoGrafado's captures)
+
     def __init__(self, V, d=64, n_capas=2, largo_cada=2, ff=None, k=4, init_profundo=None, checkpoint=False,
                  dropout=0.0, mezcla='conv', memoria_max=1024, protecciones=None, **opciones_capa):
         super().__init__()
@@ -255,7 +257,7 @@ class ModeloASRN(nn.Module):
         (16 x 1024 tokens, d 64). So only steps without such ops: torch does not sort the tokens (up to
         ops.FICHAS_EN_FILA of them, or the library's gradient), the blocks are the fused 'conv' ones ('memoria' sums its
         parameters' gradients in torch, with a cleared counter) and d is one the fused kernels take."""
-        return (E.numel() <= UNA_CORRIENTE and E.shape[-1] <= 1024
+        return (self.permite_una_corriente and E.numel() <= UNA_CORRIENTE and E.shape[-1] <= 1024
                 and (x.numel() <= ops.FICHAS_EN_FILA or ops.incrustar_ok(self.emb, x))
                 and all(type(b) is BloqueLocal and b.mezcla == 'conv' for b in self.bloques))
 

@@ -26,6 +26,10 @@ const char* asrn_hip_last_error(void);
 /* ABI version of this library (increments on any signature change). */
 int32_t asrn_hip_abi_version(void);
 
+/* The memset nodes of a captured graph (hipGraph_t), -1 for none or one that cannot be read. Such a node is not safe in a
+ * graph without branches whose replays are queued back to back: a step that holds one keeps two streams. */
+int64_t asrn_graph_memsets(void* graph);
+
 /* ---- a1 + a2: sign hash and stable bucket sort ------------------------------------------------------------------
  * Replaces CapaASRN._ids (asrn/nucleo.py:661-664), `ids.argsort(dim=-1, stable=True)` and `torch.gather(ids, 1,
  * orden)` (asrn/estable.py:282-283, 288-291).

@@ -118,3 +118,16 @@ def test_what_was_kept_on_another_device_is_refused():
         lineal8(x, w, None, ops.Guardado8(leer, t, (10, 4)))
     with pytest.raises(ValueError, match='kept on meta'):
         ops.ventana8(x, 3, torch.float32, ops.Guardado8(leer, t, (10, 4), norma=True))
+
+
+def test_graph_memsets_without_a_graph(lib):
+    assert lib.asrn_graph_memsets(N) == -1 and 'no graph' in lib.asrn_hip_last_error().decode()
+
+
+def test_one_stream_can_be_switched_off():
+    m = asrn_amd.crear_modelo(61, 64, 2, semilla=1).train()
+    x = torch.zeros(1, 8, dtype=torch.long)
+    E = m.emb(x)
+    assert m._una_corriente(E, x)
+    m.permite_una_corriente = False
+    assert not m._una_corriente(E, x)

@@ -612,3 +612,38 @@ def test_other_widths_in_a_graph(N, d):
         torch.cuda.synchronize()
         for a, b in zip(salida, paso()):
             assert torch.equal(a, b)
+
+
+def _grande(logits, y):
+    """A loss with a torch sum over all logits, which many workgroups share: torch clears their counter with a memset."""
+    return asrn_amd.log_probabilidades(logits, y).mean() * -1 + 1e-3 * (logits.float() ** 2).sum() / y.numel()
+
+
+def _propia(logits, y):
+    return -asrn_amd.log_probabilidades(logits, y).mean()
+
+
+@pytest.mark.parametrize('perdida,una', [(_grande, False), (_propia, True)])
+def test_graphed_losses_with_memsets_keep_two_streams(perdida, una):
+    """A captured step whose loss records a memset branches, and its replays, with eager work between, equal ordinary
+    steps; one without memsets stays on one stream."""
+    V, B, L = 997, 4, 250
+    g = torch.Generator().manual_seed(9)
+    lotes = [torch.randint(0, V, (B, L + 1), generator=g).to(DEV) for _ in range(7)]
+    filas = []
+    for grabar in (True, False):
+        m = asrn_amd.crear_modelo(V, 64, 4, semilla=5).to(DEV).train()
+        vistas = []
+        m.largos[0].register_forward_pre_hook(lambda c, a, kw: vistas.append(kw.get('una_corriente', False)), with_kwargs=True)
+        opt = asrn_amd.crear_optimizador(m, 1e-3, capturable=grabar)
+        paso = asrn_amd.PasoGrafado(m, opt, B, L, precision='fp32', calentar=1, grabar=grabar, perdida=perdida)
+        fila = []
+        for x in lotes:
+            p, _, salto = paso(x[:, :-1], x[:, 1:], lr=1e-3)
+            fila.append(p.item())
+            assert salto.item() == 0 and torch.rand(1 << 16, device=DEV).sum() > 0
+        filas.append(fila)
+        if grabar:
+            assert vistas[-1] == una and m.permite_una_corriente
+            assert una or vistas[1] is True           # the capture that was dropped
+    assert all(abs(a - b) <= 2e-5 * (1 + abs(b)) for a, b in zip(*filas)), filas
