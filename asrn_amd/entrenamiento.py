@@ -226,7 +226,7 @@ class PasoGrafado:
         self.x.copy_(x, non_blocking=True)
         self.y.copy_(y, non_blocking=True)
         for a, b in zip(self.extras, extras):
-            a.copy_(b, non_blocking=True)
+            a.copy_(b.detach(), non_blocking=True)      # values: a graph behind an extra stays the caller's
         if lr is not None:
             self._poner_lr(lr)
         if not self.grabar:

@@ -131,3 +131,21 @@ def test_one_stream_can_be_switched_off():
     assert m._una_corriente(E, x)
     m.permite_una_corriente = False
     assert not m._una_corriente(E, x)
+
+
+def test_extras_are_values():
+    """An extra that carries a graph: its values are copied, nothing flows back through it and no step keeps its graph."""
+    torch.manual_seed(2)
+    fuente = torch.nn.Parameter(torch.randn(2, 7))
+    m = torch.nn.Sequential(torch.nn.Embedding(11, 8), torch.nn.Linear(8, 11))
+    opt = torch.optim.SGD(m.parameters(), lr=0.1)
+    perdida = lambda logits, y, ref: ((torch.log_softmax(logits, -1).gather(-1, y[..., None])[..., 0] - ref) ** 2).mean()
+    paso = asrn_amd.PasoGrafado(m, opt, 2, 7, precision='fp32', grabar=False, perdida=perdida, extras=(fuente * 2,))
+    x = torch.randint(0, 11, (2, 8))
+    for i in range(3):
+        extra = fuente * (i + 1)
+        antes = [p.detach().clone() for p in m.parameters()]
+        valor, _, salto = paso(x[:, :-1], x[:, 1:], lr=0.1, extras=(extra,))
+        e = paso.extras[0]
+        assert not e.requires_grad and e.grad_fn is None and torch.equal(e, extra) and fuente.grad is None
+        assert salto == 0 and any(not torch.equal(a, b) for a, b in zip(antes, m.parameters()))
