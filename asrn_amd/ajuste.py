@@ -105,7 +105,8 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
     rejected ones (log_probabilidades); mascara (2P, L): nonzero on the answers' tokens (None: all); ref: the reference
     model's, (2P, L) a token or (2P,) summed a text already, or None for none. The gradient goes to lp; mascara and ref
     are constants. What the mask hides is not used, NaN and infinities included; a text without tokens has R = 0 (less
-    its ref sum). Sums are held in double."""
+    its ref sum). Sums are held in double; lp and a ref a token are taken in fp32 (fp64 ones are rounded to it), the sums
+    (2P,) in fp32 or fp64 as they come."""
     quien = 'perdida_preferencia'
     dev = _dev(lp)
     if lp.dim() != 2 or lp.shape[0] < 2 or lp.shape[0] % 2 or not lp.is_floating_point():
@@ -116,7 +117,7 @@ def perdida_preferencia(lp, mascara=None, ref=None, beta=0.1, tipo='sigmoide', s
             _igual(quien, lp, ref=ref)
         elif ref.shape[0] != lp.shape[0] or not ref.is_floating_point() or ref.device != dev:
             raise ValueError(f'{quien}: ref {tuple(ref.shape)} of {ref.dtype} on {ref.device} against lp {tuple(lp.shape)} on {dev}')
-        ref = _fijo(ref)
+        ref = ref.detach() if ref.dim() == 1 and ref.dtype == torch.float64 else _fijo(ref)
     if tipo not in FORMAS:
         raise ValueError(f'{quien}: tipo={tipo!r}: one of {FORMAS}')
     beta = _numero(quien, 'beta', beta, 0.0, abierto=True)
@@ -145,8 +146,8 @@ def perdida_politica(lp, ventaja, lp_vieja=None, mascara=None, recorte=0.2, tope
     mascara (B, L): nonzero on the answers' tokens (None: all); what it hides is not used, NaN and infinities included.
     reduccion: 'fichas' averages over the masked tokens, 'textos' over the texts' own means (texts without tokens left
     out); NaN when no token is left. The gradient goes to lp and entropia; the rest are constants. Statistics (means over
-    the masked tokens): [share of clipped tokens, r - 1 - log r, exp(q) - 1 - q, H]. Differences, products and
-    sums are formed in double, exponentials to fp32's accuracy."""
+    the masked tokens): [share of clipped tokens, r - 1 - log r, exp(q) - 1 - q, H]. Inputs are taken in fp32 (fp64
+    ones are rounded to it); their differences, products and sums are formed in double, exponentials to fp32's accuracy."""
     quien = 'perdida_politica'
     dev = _dev(lp)
     if lp.dim() != 2 or lp.shape[0] < 1 or not lp.is_floating_point():

@@ -166,13 +166,13 @@ struct Preferencia : Function<Preferencia> {
     // one buffer: the workspace, then the rows' coefficients, which the backward needs
     Tensor perdida = vacio({}, lp), rec = vacio({2 * P}, lp), ws = vacio({fin + 8 * P}, lp, at::kByte);
     char* w = static_cast<char*>(ws.data_ptr());
-    const bool por_fila = f.ref && f.ref->dim() == 1;
+    const int32_t por_fila = !f.ref || f.ref->dim() != 1 ? 0 : f.ref->scalar_type() == at::kDouble ? 2 : 1;
     int64_t sl[2], sr[2] = {0, 0}, sm[2];
     pasos(lp, sl);
     pasos(f.m, sm);
     if (por_fila) sr[0] = f.ref->stride(0);
     else pasos(f.ref, sr);
-    vale(lib.pref_fwd(f32(lp), sl, f32(f.ref), sr, por_fila, u8(f.m), sm, P, L, f.forma, f.beta, f.suavizado, f.margen, f.media,
+    vale(lib.pref_fwd(f32(lp), sl, ptr(f.ref), sr, por_fila, u8(f.m), sm, P, L, f.forma, f.beta, f.suavizado, f.margen, f.media,
                       f32(perdida), f32(rec), reinterpret_cast<float*>(w + fin), w, wsb, en.st), "asrn_preference_fwd");
     ctx->save_for_backward(f.m ? variable_list{ws, *f.m} : variable_list{ws});
     ctx->saved_data["n"] = std::vector<int64_t>{P, L, fin};

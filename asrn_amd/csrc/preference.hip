@@ -28,7 +28,7 @@ constexpr int kPfLossThreads = 1024;
 struct PfPart { double sum; double n; };
 
 struct PfArgs {
-  Strided lp, ref, mask;                    // ref.p null: none; ref_rows: one sum a row (ref.st unused)
+  Strided lp, ref, mask;                    // ref.p null: none; ref_rows: one sum a row (ref.st unused), 2: in double
   int64_t P, L;
   int32_t ref_rows, kind, mean;
   double beta, smooth, margin;
@@ -86,10 +86,13 @@ __device__ __forceinline__ double pf_pair(const PfArgs& a, int64_t i, const PfPa
   double R[2], div[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const double s = q[k].sum - (a.ref.p && a.ref_rows ? (double)a.ref.at(i + k * a.P, 0) : 0.0);
+    double s = q[k].sum;
+    const int64_t row = i + k * a.P;
+    if (a.ref.p && a.ref_rows)
+      s -= a.ref_rows == 2 ? reinterpret_cast<const double*>(a.ref.p)[row * a.ref.sb] : (double)a.ref.at(row, 0);
     div[k] = a.mean && q[k].n > 1.0 ? q[k].n : 1.0;           // an empty answer: a sum of nothing, divided by 1
     R[k] = s / div[k];
-    a.reward[i + k * a.P] = (float)(a.beta * R[k]);
+    a.reward[row] = (float)(a.beta * R[k]);
   }
   const double h = a.beta * (R[0] - R[1]) - a.margin;
   double v, dh;
@@ -205,13 +208,14 @@ extern "C" int64_t asrn_preference_workspace(int64_t P, int64_t L) {
   return 2 * P * pf_pieces(L) * (int64_t)sizeof(PfPart);
 }
 
-extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const float* ref,
+extern "C" int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const void* ref,
                                    const int64_t* ref_strides, int32_t ref_rows, const uint8_t* mask,
                                    const int64_t* mask_strides, int64_t P, int64_t L, int32_t kind, double beta,
                                    double smoothing, double margin, int32_t mean, float* loss, float* rewards,
                                    float* coef, void* workspace, int64_t workspace_bytes, void* stream) {
   if (pf_check(P, L, "asrn_preference_fwd")) return 1;
   ASRN_REQUIRE(kind >= 0 && kind <= 2, "asrn_preference_fwd: kind=%d (0 sigmoid, 1 ipo, 2 hinge)", kind);
+  ASRN_REQUIRE(ref_rows >= 0 && ref_rows <= 2, "asrn_preference_fwd: ref_rows=%d (0 to 2)", ref_rows);
   ASRN_REQUIRE(beta > 0.0 && beta < INFINITY && smoothing >= 0.0 && smoothing <= 1.0 && margin == margin,
                "asrn_preference_fwd: beta=%g (positive) smoothing=%g (0 to 1) margin=%g", beta, smoothing, margin);
   ASRN_REQUIRE((lp || L == 0) && lp_strides && loss && rewards && coef && (!ref || ref_strides) && (!mask || mask_strides),

@@ -663,14 +663,14 @@ int asrn_token_logp_bwd(const void* logits, int32_t type, int64_t rows, int64_t 
 
 /* ---- fine-tuning: the preference loss ------------------------------------------------------------------------------
  * No counterpart in the reference. lp (2P, L): rows 0 .. P-1 the chosen texts, P .. 2P-1 the rejected ones; mask
- * (2P, L) bytes or null; ref null, (2P, L), or (2P) sums with ref_rows. lp_strides, ref_strides, mask_strides: host
+ * (2P, L) bytes or null; ref null, (2P, L) fp32, or (2P) sums with ref_rows (1: fp32, 2: fp64). lp_strides, ref_strides, mask_strides: host
  * arrays of the row and token strides in elements. R_i = the masked sum of lp - ref (mean: over the masked count, at
  * least 1), h_i = beta (R_i - R_{P+i}) - margin; kind 0: -(1 - smoothing) log sigma(h) - smoothing log sigma(-h),
  * 1: ((h - 1/2) / beta)^2, 2: max(0, 1 - h). *loss = the mean over the pairs, rewards (2P) = beta R, coef (2P) =
  * d loss / d lp of a row's masked tokens. Sums in double, in a fixed order. bwd: dlp (2P, L) dense = *g coef, 0 where
  * masked. workspace: asrn_preference_workspace(P, L) bytes, 16-byte aligned (-1: sizes refused). */
 int64_t asrn_preference_workspace(int64_t P, int64_t L);
-int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const float* ref, const int64_t* ref_strides,
+int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const void* ref, const int64_t* ref_strides,
                         int32_t ref_rows, const uint8_t* mask, const int64_t* mask_strides, int64_t P, int64_t L,
                         int32_t kind, double beta, double smoothing, double margin, int32_t mean, float* loss,
                         float* rewards, float* coef, void* workspace, int64_t workspace_bytes, void* stream);

@@ -149,3 +149,8 @@ def test_extras_are_values():
         e = paso.extras[0]
         assert not e.requires_grad and e.grad_fn is None and torch.equal(e, extra) and fuente.grad is None
         assert salto == 0 and any(not torch.equal(a, b) for a, b in zip(antes, m.parameters()))
+
+
+def test_preference_reference_sums_check(lib):
+    for filas in (-1, 3):
+        _mal(lib, lib.asrn_preference_fwd(16, 16, 16, 16, filas, N, N, 1, 5, 0, 0.1, 0.0, 0.0, 0, 16, 16, 16, 16, 0, N), 'ref_rows')

@@ -265,6 +265,23 @@ def test_preference_long_texts_and_strides():
         assert ((dlp.double() - ed).abs() <= 4 * U * ed.abs() + 1e-13 * L).all()
 
 
+@pytest.mark.parametrize('P,L', [(1, 3), (9, 600)])
+def test_preference_sums_in_float64(P, L):
+    """The reference's sums in fp64 (also strided): their digits past fp32's reach the difference of large sums."""
+    g = torch.Generator(device=DEV).manual_seed(P)
+    lp = (-8e4 / L * (1 + 1e-3 * torch.rand(2 * P, L, generator=g, device=DEV))).requires_grad_()
+    ref = lp.detach().double().sum(1) + 3e-3 * torch.randn(2 * P, generator=g, device=DEV).double()
+    for r in (ref, torch.stack([ref, ref + 1], 1)[:, 0]):
+        perdida, rec = asrn_amd.perdida_preferencia(lp, None, r, beta=50.0)
+        d, = torch.autograd.grad(perdida, lp)
+        e, er, ed = preferencia_exacta(lp, None, r, 50.0, 'sigmoide', 0.0, 0.0, False)
+        # double sums of L values of 8e4 in all: (L + 2) half steps of double, times beta
+        s = 50 * 8e4 * (L + 2) * 2.0 ** -53 * 2
+        assert abs(perdida.double() - e) <= U * e.abs() + 2 * s and ((rec.double() - er).abs() <= U * er.abs() + s).all()
+        assert ((d.double() - ed).abs() <= 4 * U * ed.abs() + 50 * s).all()
+    assert abs(perdida.item() - math.log(2)) > 1e-4     # what fp32 sums would leave
+
+
 def test_losses_of_very_many_texts():
     """Tens of thousands of one-token texts, and gradients against central differences of the float64 definitions."""
     g = torch.Generator(device=DEV).manual_seed(11)
