@@ -1576,12 +1576,17 @@ def suma_gelu_norma(ln, h, c, dtype):
     return norma_residual(ln, h + F.gelu(c), dtype)
 
 
+def _norma_propia(d):
+    """The widths of the library's LayerNorm (asrn_layer_norm_fwd)."""
+    return d % 4 == 0 and d <= 1024
+
+
 def norma_residual(ln, x, dtype):
     """(LayerNorm ln of x in `dtype`, x for the residual path): the library's fused LayerNorm for fp32 x on the GPU
     with d a multiple of 4 up to 1024, else ln(x) (cast to dtype) and x itself."""
     d = x.shape[-1]
-    if x.is_cuda and x.dtype == torch.float32 and dtype in (torch.float32, torch.bfloat16) and d % 4 == 0 and \
-            d <= 1024 and ln.elementwise_affine and ln.bias is not None and tuple(ln.normalized_shape) == (d,):
+    if x.is_cuda and x.dtype == torch.float32 and dtype in (torch.float32, torch.bfloat16) and _norma_propia(d) and \
+            ln.elementwise_affine and ln.bias is not None and tuple(ln.normalized_shape) == (d,):
         return NormaResidual.apply(x, ln.weight, ln.bias, ln.eps, dtype)
     y = ln(x)
     return (y if y.dtype == dtype else y.to(dtype)), x
@@ -1753,14 +1758,17 @@ def norma8(ln, x, dtype):
     """(LayerNorm ln of x in `dtype`, x for the residual path, what lineal8 and ventana8 read the first from):
     norma_residual whose backward reads x back from 8 bits (guardar8's format) instead of keeping it, with the mean and
     the deviation of x itself. The output is norma_residual's; the gradients of x and the parameters are those at the
-    8-bit values. x fp32, dtype fp32 or bf16. Without gradients, off the GPU or for another ln: norma_residual and None."""
+    8-bit values. x fp32, dtype fp32 or bf16. Without gradients, off the GPU or for another ln (one whose call
+    norma_residual makes and that is no plain nn.LayerNorm, or has hooks): norma_residual and None."""
     d = x.shape[-1]
-    for p in (ln.weight, ln.bias):
+    pesos = getattr(ln, 'weight', None), getattr(ln, 'bias', None)
+    for p in pesos:
         if p is not None and p.device != x.device:           # its address means nothing to a kernel on x's device
             raise ValueError(f'norma8: x is on {x.device}, the LayerNorm on {p.device}')
     if not (x.is_cuda and x.dtype == torch.float32 and x.numel() > 0 and dtype in (torch.float32, torch.bfloat16)
-            and torch.is_grad_enabled() and ln.elementwise_affine and ln.bias is not None
-            and tuple(ln.normalized_shape) == (d,)):
+            and torch.is_grad_enabled() and all(p is not None for p in pesos) and getattr(ln, 'elementwise_affine', False)
+            and tuple(ln.normalized_shape) == (d,)
+            and (_norma_propia(d) or type(ln) is torch.nn.LayerNorm and sin_ganchos(ln))):
         return *norma_residual(ln, x, dtype), None
     if _norma8_propia(d):
         y, x, sitio = nodos().norma8(x, ln.weight, ln.bias, ln.eps, dtype == torch.bfloat16)

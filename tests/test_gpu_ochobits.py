@@ -647,3 +647,20 @@ def test_graphed_losses_with_memsets_keep_two_streams(perdida, una):
             assert vistas[-1] == una and m.permite_una_corriente
             assert una or vistas[1] is True           # the capture that was dropped
     assert all(abs(a - b) <= 2e-5 * (1 + abs(b)) for a, b in zip(*filas)), filas
+
+
+@pytest.mark.parametrize('d', [64, 66, 1028])
+def test_norms_with_hooks_or_of_other_kinds(d):
+    """norma8 of what norma_residual calls as a module: its hooks and its own forward run, and nothing is kept."""
+    x = torch.randn(3, d, device=DEV, requires_grad=True)
+    con_gancho, propia, otra = torch.nn.LayerNorm(d).to(DEV), torch.nn.LayerNorm(d).to(DEV), torch.nn.RMSNorm(d).to(DEV)
+    con_gancho.register_forward_hook(lambda m, i, o: 2 * o)
+    propia.forward = lambda t: t + 1
+    # up to 1,024 channels, multiples of 4, norma_residual fuses any affine LayerNorm (and asks for its bias)
+    for ln in [con_gancho, propia] + [otra] * (d == 66):
+        y, a, guardado = ops.norma8(ln, x, torch.float32)
+        y0, a0 = ops.norma_residual(ln, x, torch.float32)
+        assert torch.equal(y, y0) and torch.equal(a, a0) and (guardado is None) == (d != 64)
+    assert ops.norma8(otra.cpu(), x.cpu(), torch.float32)[2] is None
+    assert ops.norma8(torch.nn.LayerNorm(d, bias=False).to(DEV), x, torch.float32)[2] is None
+    assert ops.norma8(torch.nn.LayerNorm(d).to(DEV), x, torch.float32)[2] is not None
