@@ -1767,7 +1767,7 @@ def norma8(ln, x, dtype):
             raise ValueError(f'norma8: x is on {x.device}, the LayerNorm on {p.device}')
     if not (x.is_cuda and x.dtype == torch.float32 and x.numel() > 0 and dtype in (torch.float32, torch.bfloat16)
             and torch.is_grad_enabled() and all(p is not None for p in pesos) and getattr(ln, 'elementwise_affine', False)
-            and tuple(ln.normalized_shape) == (d,)
+            and tuple(ln.normalized_shape) == (d,) and ln.eps > 0
             and (_norma_propia(d) or type(ln) is torch.nn.LayerNorm and sin_ganchos(ln))):
         return *norma_residual(ln, x, dtype), None
     if _norma8_propia(d):

@@ -664,3 +664,11 @@ def test_norms_with_hooks_or_of_other_kinds(d):
     assert ops.norma8(otra.cpu(), x.cpu(), torch.float32)[2] is None
     assert ops.norma8(torch.nn.LayerNorm(d, bias=False).to(DEV), x, torch.float32)[2] is None
     assert ops.norma8(torch.nn.LayerNorm(d).to(DEV), x, torch.float32)[2] is not None
+
+
+def test_norm_without_eps():
+    """asrn_norm8_fwd takes a positive eps only; a LayerNorm with 0 runs as without 8 bits."""
+    ln = torch.nn.LayerNorm(64, eps=0.0).to(DEV)
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    y, _, guardado = ops.norma8(ln, x, torch.float32)
+    assert guardado is None and torch.equal(y, ops.norma_residual(ln, x, torch.float32)[0])
