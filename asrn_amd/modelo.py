@@ -126,8 +126,9 @@ class BloqueLocal(nn.Module):
 
     def forward(self, h, ocho=False):
         """ocho: what the backward needs is kept in 8 bits (_en_ocho) where the block's products run in fp32 or bf16 on
-        the GPU; the output is the same."""
-        if ocho and h.is_cuda and h.dtype == torch.float32 and _dtype_producto(h) in (torch.float32, torch.bfloat16):
+        the GPU and its feed-forward is this class's; the output is the same."""
+        if ocho and h.is_cuda and h.dtype == torch.float32 and _dtype_producto(h) in (torch.float32, torch.bfloat16) and \
+                type(self)._ff is BloqueLocal._ff and '_ff' not in vars(self):
             return self._en_ocho(h)
         # the LayerNorms run fused (ops.norma_residual): ln2's output comes out in the feed-forward's dtype, and the
         # residual path's gradient joins each LayerNorm's backward

@@ -672,3 +672,15 @@ def test_norm_without_eps():
     x = torch.randn(3, 64, device=DEV, requires_grad=True)
     y, _, guardado = ops.norma8(ln, x, torch.float32)
     assert guardado is None and torch.equal(y, ops.norma_residual(ln, x, torch.float32)[0])
+
+
+@pytest.mark.parametrize('como', ['subclase', 'instancia'])
+def test_block_with_its_own_feed_forward(como):
+    """A block whose feed-forward was replaced runs it, with 8 bits asked for or not."""
+    b = _bloque(64)
+    if como == 'subclase':
+        b.__class__ = type('Otro', (asrn_amd.BloqueLocal,), {'_ff': lambda s, y: 3 * asrn_amd.BloqueLocal._ff(s, y)})
+    else:
+        b._ff = lambda y: torch.zeros_like(y)
+    h = torch.randn(2, 9, 64, device=DEV, requires_grad=True)
+    assert torch.equal(b(h), b(h, ocho=True))
