@@ -82,7 +82,8 @@ def log_probabilidades(logits, y, ignorar=-100, temperatura=1.0, entropia=False)
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         x = x.contiguous()
     if x.dim() > 3:                                  # more leading axes are flattened; a (B, L, V) slice needs no copy
-        x, t = x.reshape(-1, *x.shape[-2:]), t.view(-1, t.shape[-1])
+        n = math.prod(x.shape[:-2])
+        x, t = x.reshape(n, *x.shape[-2:]), t.view(n, t.shape[-1])
     lp, H = nodos().logp(x, t, TIPOS[x.dtype], int(ignorar), 1.0 / T, bool(entropia))
     if logits.dim() > 3:
         lp, H = lp.view(y.shape), H if H is None else H.view(y.shape)

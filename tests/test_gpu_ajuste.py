@@ -118,6 +118,13 @@ def test_logp_strides(cual, dtype):
                   dx.reshape(-1, V))
 
 
+@pytest.mark.parametrize('forma', [(2, 3, 0), (0, 3, 4), (2, 0, 4), (0, 0, 0, 0)])
+def test_logp_many_axes_without_tokens(forma):
+    x = torch.randn(*forma, 5, device=DEV, requires_grad=True)
+    lp, H = asrn_amd.log_probabilidades(x, torch.zeros(forma, dtype=torch.long, device=DEV), entropia=True)
+    assert lp.shape == H.shape == forma and torch.autograd.grad(lp.sum() + H.sum(), x)[0].shape == x.shape
+
+
 @pytest.mark.parametrize('dtype', TIPOS)
 def test_logp_extremes(dtype):
     """Infinities, the type's ends, NaN and targets outside the vocabulary, against torch's log_softmax."""
