@@ -666,10 +666,12 @@ def test_norms_with_hooks_or_of_other_kinds(d):
     assert ops.norma8(torch.nn.LayerNorm(d).to(DEV), x, torch.float32)[2] is not None
 
 
-def test_norm_without_eps():
-    """asrn_norm8_fwd takes a positive eps only; a LayerNorm with 0 runs as without 8 bits."""
-    ln = torch.nn.LayerNorm(64, eps=0.0).to(DEV)
-    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+@pytest.mark.parametrize('d', [66, 1028])
+def test_norm_without_eps(d):
+    """The library's kernels take a positive eps only; at widths that torch's LayerNorm runs without 8 bits, 0 runs with
+    them too."""
+    ln = torch.nn.LayerNorm(d, eps=0.0).to(DEV)
+    x = torch.randn(3, d, device=DEV, requires_grad=True)
     y, _, guardado = ops.norma8(ln, x, torch.float32)
     assert guardado is None and torch.equal(y, ops.norma_residual(ln, x, torch.float32)[0])
 
