@@ -1607,7 +1607,10 @@ class Guardado8:
         self.leer, self.tensores, self.forma, self.norma = leer, tuple(tensores), forma, norma
 
 
-_corriente = torch._C._cuda_getCurrentRawStream       # a stream's handle without the Python object around it
+def _corriente(i):
+    """The handle of device i's current stream, without the Python object around it. Looked up here: a PyTorch without a
+    GPU build does not have it, and the package is imported there too."""
+    return torch._C._cuda_getCurrentRawStream(i)
 
 
 def _en(dev, nombre, *args):

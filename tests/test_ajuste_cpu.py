@@ -1,4 +1,8 @@
 """The fine-tuning entry points' argument checks, which fail before any device work, and the public names."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -11,7 +15,6 @@ N = None
 
 @pytest.fixture(scope='module')
 def lib():
-    import os
     if not os.path.exists(_lib.LIB_PATH):
         pytest.skip('libasrn_hip.so not built (run `python -m asrn_amd.build`)')
     return _lib.load()
@@ -154,3 +157,14 @@ def test_extras_are_values():
 def test_preference_reference_sums_check(lib):
     for filas in (-1, 3):
         _mal(lib, lib.asrn_preference_fwd(16, 16, 16, 16, filas, N, N, 1, 5, 0, 0.1, 0.0, 0.0, 0, 16, 16, 16, 16, 0, N), 'ref_rows')
+
+
+def test_import_without_a_gpu_build_of_torch():
+    """A CPU build of PyTorch has no streams; the package is still imported there (file formats, the model on the CPU)."""
+    prog = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if 'RawStream' in n]: delattr(torch._C, n)\n"
+            "import asrn_amd\n"
+            "print(asrn_amd.crear_modelo(11, 64, 2, semilla=1).num_parametros())")
+    raiz = os.path.dirname(os.path.dirname(os.path.abspath(asrn_amd.__file__)))
+    r = subprocess.run([sys.executable, '-c', prog], cwd=raiz, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and int(r.stdout) > 0, r.stderr
