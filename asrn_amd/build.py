@@ -51,21 +51,34 @@ def orden_nodos(salida):
             '-ltorch_python']
 
 
+def _colocar(hecho, sitio):
+    shutil.copyfile(hecho, sitio + '.tmp')
+    os.replace(sitio + '.tmp', sitio)
+
+
+def _salida(cmd):
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
 def build(verbose=False, jobs=None):
     """Compiles every source (in parallel), links the shared library and places it and the nodes atomically. Raises on any
-    error."""
+    error. The library needs hipcc alone: it is placed also where the nodes cannot be compiled (PyTorch's, Python's or
+    HIP's C++ headers missing), and the error says so."""
     cc = hipcc()
     with tempfile.TemporaryDirectory(prefix='asrn_build_') as tmp:
         tmp_nodos = os.path.join(tmp, '_nodos.so')
-        procs = [('nodos.cpp', subprocess.Popen(orden_nodos(tmp_nodos), stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
-                                                text=True))]
+        try:
+            nodos, error_nodos = _salida(orden_nodos(tmp_nodos)), None
+        except (ImportError, OSError) as e:
+            nodos, error_nodos = None, str(e)
+        procs = []
         objs = []
         for src in SOURCES:
             obj = os.path.join(tmp, src.replace('.hip', '.o'))
             cmd = [cc, *COMMON, *PER_FILE.get(src, []), '-c', os.path.join(CSRC, src), '-o', obj]
             if verbose:
                 print(' '.join(cmd), flush=True)
-            procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+            procs.append((src, _salida(cmd)))
             objs.append(obj)
         errors = []
         for src, p in procs:
@@ -74,16 +87,25 @@ def build(verbose=False, jobs=None):
                 errors.append(f'--- {src} ---\n{out}')
             elif verbose and out.strip():
                 print(out)
+        if nodos is not None:
+            out, _ = nodos.communicate()
+            if nodos.returncode != 0:
+                error_nodos = out
+            elif verbose and out.strip():
+                print(out)
         if errors:
-            raise RuntimeError('compiling failed:\n' + '\n'.join(errors))
+            raise RuntimeError('hipcc failed:\n' + '\n'.join(errors))
         tmp_lib = os.path.join(tmp, 'libasrn_hip.so')
         cmd = [cc, '-shared', '-fPIC', f'--offload-arch={ARCH}', *objs, '-o', tmp_lib]
         r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         if r.returncode != 0:
             raise RuntimeError('link failed:\n' + r.stdout)
-        for hecho, sitio in ((tmp_lib, LIB), (tmp_nodos, NODOS)):
-            shutil.copyfile(hecho, sitio + '.tmp')
-            os.replace(sitio + '.tmp', sitio)
+        _colocar(tmp_lib, LIB)
+        if error_nodos is not None:
+            if os.path.exists(NODOS):         # nodes of another build may call this library by other signatures
+                os.remove(NODOS)
+            raise RuntimeError(f'{LIB} is built; the autograd nodes are not (csrc/nodos.cpp):\n{error_nodos}')
+        _colocar(tmp_nodos, NODOS)
     return LIB
 
 

@@ -168,3 +168,29 @@ def test_import_without_a_gpu_build_of_torch():
     raiz = os.path.dirname(os.path.dirname(os.path.abspath(asrn_amd.__file__)))
     r = subprocess.run([sys.executable, '-c', prog], cwd=raiz, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and int(r.stdout) > 0, r.stderr
+
+
+def _compilador(ruta, rc):
+    """A stand-in for a compiler: writes the file after -o and ends with rc."""
+    ruta.write_text(f'#!{sys.executable}\nimport sys\na = sys.argv\nopen(a[a.index("-o") + 1], "w").write(a[-1])\nsys.exit({rc})\n')
+    ruta.chmod(0o755)
+    return str(ruta)
+
+
+@pytest.mark.parametrize('falla', ['no', 'nodos', 'sin_cxx', 'hipcc'])
+def test_build_places_the_library_without_the_nodes(tmp_path, monkeypatch, falla):
+    """The C ABI needs hipcc alone: nodes that do not compile are reported after the library is in its place."""
+    from asrn_amd import build
+    cc = _compilador(tmp_path / 'cc', int(falla == 'hipcc'))
+    monkeypatch.setattr(build, 'hipcc', lambda: cc)
+    monkeypatch.setenv('CXX', str(tmp_path / 'none') if falla == 'sin_cxx' else _compilador(tmp_path / 'cxx', int(falla == 'nodos')))
+    monkeypatch.setattr(build, 'LIB', str(tmp_path / 'lib.so'))
+    monkeypatch.setattr(build, 'NODOS', str(tmp_path / 'nodos.so'))
+    if falla in ('nodos', 'sin_cxx'):
+        (tmp_path / 'nodos.so').write_text('of an earlier build')
+    if falla == 'no':
+        assert build.build() == build.LIB
+    else:
+        with pytest.raises(RuntimeError, match='hipcc failed' if falla == 'hipcc' else 'autograd nodes are not'):
+            build.build()
+    assert os.path.exists(build.LIB) == (falla != 'hipcc') and os.path.exists(build.NODOS) == (falla == 'no')
