@@ -16,7 +16,7 @@ import warnings
 import torch
 
 from . import archivo, ops
-from ._lib import nodos, query
+from ._lib import ASRNHipError, nodos, query
 from .modelo import _base
 
 # the suffix and gate parameters of each ASRN layer learn this many times faster (asrn/nucleo.py:2188-2189)
@@ -191,9 +191,15 @@ class PasoGrafado:
         self.hechos += 1
         return r
 
+    def _hojas_en_uso(self):
+        try:
+            return nodos().hojas_en_uso(self.params)
+        except ASRNHipError:                         # a library built without the nodes: the ordinary step needs none
+            return False
+
     def _capturar(self):
         # a graph of an eager call that still lives would take the captured backward to the default stream
-        if nodos().hojas_en_uso(self.params):
+        if self._hojas_en_uso():
             raise RuntimeError('PasoGrafado: the step cannot be captured while an eager graph of the parameters lives '
                                '(a loss, logits or scores kept from a call outside torch.no_grad()): drop or detach it')
         # a loss of the caller's may record memsets (a torch sum over many values does), which ModeloASRN._una_corriente

@@ -686,3 +686,22 @@ def test_block_with_its_own_feed_forward(como):
         b._ff = lambda y: torch.zeros_like(y)
     h = torch.randn(2, 9, 64, device=DEV, requires_grad=True)
     assert torch.equal(b(h), b(h, ocho=True))
+
+
+def test_graphed_step_without_the_nodes(monkeypatch):
+    """A library that was built alone: the ordinary captured step runs as before."""
+    from asrn_amd import _lib
+
+    def faltan():
+        raise _lib.ASRNHipError('_nodos.so is missing')
+
+    monkeypatch.setattr('asrn_amd.entrenamiento.nodos', faltan)
+    monkeypatch.setattr('asrn_amd.ops.nodos', faltan)
+    x = torch.randint(0, 61, (2, 31), generator=torch.Generator().manual_seed(3)).to(DEV)
+    filas = []
+    for grabar in (True, False):
+        m = _modelo('no')
+        opt = asrn_amd.crear_optimizador(m, 1e-3, capturable=grabar)
+        paso = asrn_amd.PasoGrafado(m, opt, 2, 30, precision='fp32', calentar=1, grabar=grabar)
+        filas.append([paso(x[:, :-1], x[:, 1:], lr=1e-3)[0].item() for _ in range(4)])
+    assert all(abs(a - b) <= 1e-5 * abs(b) for a, b in zip(*filas))
