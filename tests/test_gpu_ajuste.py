@@ -588,3 +588,26 @@ def test_side_stream():
         otra = paso()
     torch.cuda.current_stream().wait_stream(lado)
     assert all(torch.equal(a, b) for a, b in zip(base, otra))
+
+
+@pytest.mark.parametrize('B,L', [(4, 50), (6, 5001)])
+def test_losses_on_a_side_stream(B, L):
+    """Both losses and their gradients on another stream, work before them on it: the default stream's bits."""
+    g = torch.Generator(device=DEV).manual_seed(B)
+    lp0 = -torch.rand(B, L, generator=g, device=DEV)
+    old, A = lp0 + 0.1 * torch.randn(B, L, generator=g, device=DEV), torch.randn(B, generator=g, device=DEV)
+    m = torch.rand(B, L, generator=g, device=DEV) < 0.6
+
+    def paso():
+        lp = (lp0 * 2 - lp0).requires_grad_()        # written on the current stream
+        a, rec = asrn_amd.perdida_preferencia(lp, m, old)
+        b, est = asrn_amd.perdida_politica(lp, A, old, m, lp_ref=old, beta=0.1)
+        return [t.detach() for t in (a, rec, b, est, *torch.autograd.grad(a + b, lp))]
+
+    base = paso()
+    torch.cuda.synchronize()
+    lado = torch.cuda.Stream()
+    with torch.cuda.stream(lado):
+        otra = paso()
+    lado.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(base, otra))

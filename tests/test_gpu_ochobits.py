@@ -705,3 +705,56 @@ def test_graphed_step_without_the_nodes(monkeypatch):
         paso = asrn_amd.PasoGrafado(m, opt, 2, 30, precision='fp32', calentar=1, grabar=grabar)
         filas.append([paso(x[:, :-1], x[:, 1:], lr=1e-3)[0].item() for _ in range(4)])
     assert all(abs(a - b) <= 1e-5 * abs(b) for a, b in zip(*filas))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_gelu_types_and_values(dtype):
+    """The output and the gradient come in the input's type; in bf16 the output is F.gelu's bit for bit, in fp32 both are
+    within their roundings of the definition."""
+    u = (2.5 * torch.randn(37, 64, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV)).to(dtype).requires_grad_()
+    y, _ = ops.gelu8(u)
+    du, = torch.autograd.grad(y, u, torch.ones_like(y))
+    assert y.dtype == dtype and du.dtype == dtype
+    if dtype == torch.bfloat16:
+        assert torch.equal(y, F.gelu(u))
+    else:
+        dentro(y.detach(), F.gelu(u.detach()), 8 * U * (1 + u.detach().abs().double()))
+
+
+@pytest.mark.parametrize('mezcla', ['conv', 'memoria'])
+@pytest.mark.parametrize('bits', [16, 32])
+def test_block_with_dropout(mezcla, bits):
+    """Active dropout from the same seed: the output of the block without 8 bits, its gradients within the 8 bits' share."""
+    b = _bloque(64, mezcla, dropout=0.3)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    h = torch.randn(3, 50, 64, generator=g, device=DEV, requires_grad=True)
+    gy = torch.randn(3, 50, 64, generator=g, device=DEV)
+    out = []
+    for ocho in (False, True):
+        torch.manual_seed(11)
+        with torch.autocast('cuda', torch.bfloat16, enabled=bits == 16):
+            y = b(h, ocho=ocho)
+        out.append((y.detach(), *torch.autograd.grad(y, [h, *b.parameters()], gy)))
+    assert torch.allclose(out[0][0], out[1][0], rtol=1e-5, atol=1e-5) if bits == 32 else \
+        (out[0][0] - out[1][0]).norm() <= 2e-3 * out[0][0].norm()
+    for a, c in zip(out[0][1:], out[1][1:]):
+        assert (a - c).norm() <= 0.04 * a.norm() + 1e-6
+
+
+def test_block_on_a_side_stream():
+    """A block in 8 bits on another stream, its input written there: the default stream's output and gradients."""
+    b = _bloque(256)
+    h0 = torch.randn(3, 50, 256, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+
+    def paso():
+        h = (h0 * 2 - h0).requires_grad_()
+        y = b(h, ocho=True)
+        return [y.detach(), *torch.autograd.grad(y, [h, *b.parameters()], h0)]
+
+    base = paso()
+    torch.cuda.synchronize()
+    lado = torch.cuda.Stream()
+    with torch.cuda.stream(lado):
+        otra = paso()
+    lado.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(base, otra))
