@@ -14,8 +14,10 @@
 //   k_norm8_read the LayerNorm's output again, as the columns of a causal window of k tokens (k = 1: as it was).
 //   k_gelu8_fwd  gelu(u) [+ h], and u's 8 bits: 8 channels a lane.
 //   k_gelu8_bwd  d u = gelu'(u8) d y;   k_gelu8_read gelu(u8);   k_pack8, k_unpack8 the format alone.
-// All are bound by HBM (16384 x 768 bf16: LayerNorm 16 and 25 us, 5.5-5.7 TB/s; 16384 x 1536 bf16: the GELU's gradient 21
-// us, 6.0 TB/s) but the GELU's forward in bf16, by erff's instructions (28 us, 4.5 TB/s).
+// All are bound by HBM (16384 x 768 bf16: LayerNorm 16 and 25 us, 5.5-5.7 TB/s, read back 10 and, as a window of 4, 24;
+// 16384 x 1536 bf16: the GELU's gradient 21 us, 6.1 TB/s, read back 17, 20 with nothing of it in a cache) but the GELU's
+// forward in bf16, by erff's instructions (27 us, 4.7 TB/s), and the LayerNorm's backward past 4,096 channels, whose 222
+// registers leave 2 waves a SIMD (4096 x 8192: 100 us for 370 MB).
 #include <math.h>
 
 #include "common.h"
@@ -65,8 +67,9 @@ __device__ __forceinline__ uint32_t max_of8(uint32_t v) { return dpp_max<0x141>(
 // ---- GELU ----------------------------------------------------------------------------------------------------------
 // exact GELU, as torch forms it in fp32
 __device__ __forceinline__ float e8_gelu(float x) { return x * 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
-// For the values read back: Phi(-|x|) = e p with e = exp(-x^2 / 2), from Abramowitz and Stegun's 7.1.26 (erfc within
-// 1.5e-7, and its tail, which is taken without a subtraction, within 1e-5 of itself). One exponential and one reciprocal
+// For the values read back: Phi(-|x|) = e p with e = exp(-x^2 / 2), from Abramowitz and Stegun's 7.1.26: erfc within 1.5e-7,
+// so Phi within 7e-8 at every x. Of itself the vanishing tail is less exact the further out: 5e-5 at |x| = 3, 5e-4 at 4,
+// 1e-2 at 8, where it weighs nothing beside the 8 bits' own rounding. One exponential and one reciprocal
 // serve the value and the derivative: with m = Phi(-|x|) - |x| phi(x), gelu = max(x, 0) - |x| Phi(-|x|) and gelu' = m
 // below 0, 1 - m above (erff's two branches cost about twice the instructions, and these kernels run out of them first)
 __device__ __forceinline__ float e8_tail(float x, float* e) {
@@ -187,8 +190,8 @@ __device__ __forceinline__ void e8_read(const E8Args& a, const E8Place& p, float
 }
 
 enum { kE8Gelu = 0, kE8Pack = 1 };
-// u -> out = gelu(u) [+ h], and u's 8 bits (kE8Pack: the bits alone). Every lane of a group reaches the group's maximum
-// (lanes past the tensor repeat its last group's values and write nothing).
+// u -> out = gelu(u) [+ h], and u's 8 bits (kE8Pack: the bits alone). Every lane of a group reaches the group's maximum:
+// the four enter or leave together, and channels past a row's end count as 0.
 template <bool B16, int OP, bool ADD, bool WHOLE>
 __global__ __launch_bounds__(kE8Threads) void k_gelu8_fwd(E8Args a) {
   const int64_t i = (int64_t)blockIdx.x * kE8Threads + threadIdx.x;

@@ -11,8 +11,10 @@
 //                rewards and the coefficients.
 //   k_pref_few   the two in one launch for a few short texts.
 //   k_pref_bwd   d lp = m g c, written once.
-// Bound by launches for short batches (one pair of 60: 3.4 and 2.2 us); 24 pairs of 50,001 tokens take 5.4 + 6.1 + 5.5 us (the first
-// reads 21.6 MB; 8.4 us with 4-byte loads).
+// Bound by launches for short batches (one pair of 60: 3.0 and 2.1 us); 24 pairs of 50,001 tokens take 5.4 + 6.3 + 5.2 us
+// (the first reads 21.6 MB; 8.4 us with 4-byte loads). k_pref_loss is one workgroup at any size, each step's loads waiting
+// for the ones before: 3 to 5 us up to 2,048 pieces, then 1.4 us a thousand, which past 16,000 texts of one piece is as long
+// as k_pref_rows.
 #include <math.h>
 
 #include "common.h"

@@ -647,7 +647,7 @@ int asrn_gelu_norm_bwd(const float* x, const void* c, int32_t c_bf16, const floa
 
 /* ---- fine-tuning: log-probabilities of given tokens -------------------------------------------------------------
  * No counterpart in the reference (beside its loss, asrn/nucleo.py:1108). logits in fp32, bf16 or fp16 (type 0, 1, 2),
- * row r of `rows` (< 2^31, a multiple of L) starting at element (r / L) stride_b + (r % L) stride_t, its V values
+ * row r of `rows` (a multiple of L, < 2^24, or < 2^26 for V <= 2048) starting at element (r / L) stride_b + (r % L) stride_t, its V values
  * adjacent; no alignment beyond the elements'. target (rows) int64. With z = (x - max x) inv_temperature:
  * fwd: logp (rows) = z[target] - log sum exp z, entropy (rows, or null) = -sum p log p, both 0 where target ==
  * ignore_index (the row is not read), logp NaN for a target outside [0, V); stats (rows, 2) for the backward.
@@ -668,7 +668,8 @@ int asrn_token_logp_bwd(const void* logits, int32_t type, int64_t rows, int64_t 
  * least 1), h_i = beta (R_i - R_{P+i}) - margin; kind 0: -(1 - smoothing) log sigma(h) - smoothing log sigma(-h),
  * 1: ((h - 1/2) / beta)^2, 2: max(0, 1 - h). *loss = the mean over the pairs, rewards (2P) = beta R, coef (2P) =
  * d loss / d lp of a row's masked tokens. Sums in double, in a fixed order. bwd: dlp (2P, L) dense = *g coef, 0 where
- * masked. workspace: asrn_preference_workspace(P, L) bytes, 16-byte aligned (-1: sizes refused). */
+ * masked. workspace: asrn_preference_workspace(P, L) bytes, 16-byte aligned (-1: sizes refused: 2P texts in pieces of
+ * 2,048 tokens, at least one each, must be fewer than 2^24 pieces). */
 int64_t asrn_preference_workspace(int64_t P, int64_t L);
 int asrn_preference_fwd(const float* lp, const int64_t* lp_strides, const void* ref, const int64_t* ref_strides,
                         int32_t ref_rows, const uint8_t* mask, const int64_t* mask_strides, int64_t P, int64_t L,
@@ -686,7 +687,7 @@ int asrn_preference_bwd(const float* coef, const float* g, const uint8_t* mask, 
  * [clipped, r - 1 - d, exp q - 1 - q, H]; raw (B, L, or null) = each token's gradient with respect to lp, weight (B) =
  * what a text's tokens are divided by. bwd: dlp (B, L) = *g raw / weight, dentropy (B, L) = -*g entropy_weight /
  * weight (either null), 0 where masked. Sums in double, fixed order. workspace: asrn_policy_workspace(B, L) bytes, 16-byte
- * aligned (-1: sizes refused). */
+ * aligned (-1: sizes refused: B texts in pieces of 2,048 tokens, fewer than 2^24 as above). */
 int64_t asrn_policy_workspace(int64_t B, int64_t L);
 int asrn_policy_fwd(const float* lp, const float* advantage, const float* old_lp, const float* ref_lp,
                     const float* entropy, const uint8_t* mask, const int64_t* strides, int64_t B, int64_t L,
