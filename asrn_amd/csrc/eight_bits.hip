@@ -68,8 +68,8 @@ __device__ __forceinline__ uint32_t max_of8(uint32_t v) { return dpp_max<0x141>(
 // exact GELU, as torch forms it in fp32
 __device__ __forceinline__ float e8_gelu(float x) { return x * 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
 // For the values read back: Phi(-|x|) = e p with e = exp(-x^2 / 2), from Abramowitz and Stegun's 7.1.26: erfc within 1.5e-7,
-// so Phi within 7e-8 at every x. Of itself the vanishing tail is less exact the further out: 5e-5 at |x| = 3, 5e-4 at 4,
-// 1e-2 at 8, where it weighs nothing beside the 8 bits' own rounding. One exponential and one reciprocal
+// so Phi within 8e-8 at every x before fp32's roundings. Of itself the vanishing tail is less exact the further out: 5e-5
+// at |x| = 3, 5e-4 at 4, 1e-2 at 8, where it weighs nothing beside the 8 bits' own rounding. One exponential and one reciprocal
 // serve the value and the derivative: with m = Phi(-|x|) - |x| phi(x), gelu = max(x, 0) - |x| Phi(-|x|) and gelu' = m
 // below 0, 1 - m above (erff's two branches cost about twice the instructions, and these kernels run out of them first)
 __device__ __forceinline__ float e8_tail(float x, float* e) {

@@ -758,3 +758,19 @@ def test_block_on_a_side_stream():
         otra = paso()
     lado.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(base, otra))
+
+
+def test_graphed_loss_with_memsets_and_dropout():
+    """A step captured twice whose model draws: every replay draws anew, and its loss is an eager step's but for the draw."""
+    V, B, L = 997, 4, 250
+    x = torch.randint(0, V, (B, L + 1), generator=torch.Generator().manual_seed(9)).to(DEV)
+    m = asrn_amd.crear_modelo(V, 64, 4, semilla=5, dropout=0.3).to(DEV).train()
+    opt = asrn_amd.crear_optimizador(m, 1e-3, capturable=True)
+    paso = asrn_amd.PasoGrafado(m, opt, B, L, precision='fp32', calentar=1, perdida=_grande)
+    vals = []
+    for _ in range(5):
+        p, _, salto = paso(x[:, :-1], x[:, 1:], lr=0.0)
+        vals.append(p.item())
+        assert salto.item() == 0
+    eager = _grande(m(x[:, :-1]), x[:, 1:]).item()
+    assert len(set(vals)) == 5 and all(abs(v - eager) <= 0.1 * abs(eager) for v in vals), (vals, eager)
