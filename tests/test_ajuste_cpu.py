@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import asrn_amd
-from asrn_amd import _lib, ops
+from asrn_amd import _lib
+from asrn_amd import ops
 from asrn_amd.lineal import lineal8
 
 N = None
@@ -15,6 +16,7 @@ N = None
 
 @pytest.fixture(scope='module')
 def lib():
+    import os
     if not os.path.exists(_lib.LIB_PATH):
         pytest.skip('libasrn_hip.so not built (run `python -m asrn_amd.build`)')
     return _lib.load()
