@@ -9,6 +9,8 @@ The public names mirror the reference package (KIROKOWA/ASRN, asrn/__init__.py:4
   - training: crear_optimizador, tasa_aprendizaje, PasoGrafado, entrenar / train, evaluar / evaluate;
   - fine-tuning losses: log_probabilidades / token_log_probs, perdida_preferencia / preference_loss,
     perdida_politica / policy_loss;
+  - a local block's operators with a state a channel: conv_canal / channel_conv, paso_conv_canal / channel_conv_step,
+    escaneo_selectivo / selective_scan, paso_selectivo / selective_step;
   - files: guardar / save, cargar / load (the reference's format, v83 on);
   - generation: escribir / generate (the loop on the device), EscritorModelo / ModelWriter (the model's O(1) step),
     EscritorCapa / LayerWriter (one layer's);
@@ -29,6 +31,8 @@ from .escritura import EscritorCapa, LayerWriter
 from .generacion import EscritorModelo, escribir
 from .modelo import TALLAS, BloqueLocal, ConfigASRN, ModeloASRN, crear_desde_config, crear_modelo
 from .ops import escaneo
+from .selectiva import (channel_conv, channel_conv_step, conv_canal, escaneo_selectivo, paso_conv_canal, paso_selectivo,
+                        selective_scan, selective_step)
 
 __version__ = '0.2.0'
 
@@ -44,4 +48,5 @@ __all__ = ['ASRNLayer', 'CapaASRNEstable', 'ASRNCoreLayer', 'CapaASRN', 'Protecc
            'tasa_aprendizaje', 'PasoGrafado', 'entrenar', 'train', 'evaluar', 'evaluate', 'guardar', 'save',
            'cargar', 'load', 'escribir', 'generate', 'EscritorModelo', 'ModelWriter', 'EscritorCapa', 'LayerWriter',
            'log_probabilidades', 'token_log_probs', 'perdida_preferencia', 'preference_loss', 'perdida_politica',
-           'policy_loss', 'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']
+           'policy_loss', 'conv_canal', 'channel_conv', 'paso_conv_canal', 'channel_conv_step', 'escaneo_selectivo',
+           'selective_scan', 'paso_selectivo', 'selective_step', 'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']

@@ -1,4 +1,5 @@
-// Autograd nodes, in C++, of the fine-tuning losses and of the activations in 8 bits: they allocate, launch the library's
+// Autograd nodes, in C++, of the fine-tuning losses, of the activations in 8 bits and of a local block's operators with a
+// state a channel: they allocate, launch the library's
 // entry points on torch's current stream and keep what the backward needs. These operators' kernels take a few
 // microseconds, and a node written in Python costs more than they do: its backward runs Python on the autograd thread
 // (a log-probability's forward and backward over 200 rows: 95 us a pass, 48 with these).
@@ -52,6 +53,16 @@ struct Biblioteca {
   decltype(&asrn_norm8_fwd) norm8_fwd;
   decltype(&asrn_norm8_bwd) norm8_bwd;
   decltype(&asrn_norm8_bwd_workspace) norm8_ws;
+  decltype(&asrn_channel_conv_fwd) conv_fwd;
+  decltype(&asrn_channel_conv_bwd_workspace) conv_ws;
+  decltype(&asrn_channel_conv_bwd) conv_bwd;
+  decltype(&asrn_channel_conv_step) conv_paso;
+  decltype(&asrn_selective_checks) sel_marcas;
+  decltype(&asrn_selective_fwd_workspace) sel_ws;
+  decltype(&asrn_selective_fwd) sel_fwd;
+  decltype(&asrn_selective_bwd_workspace) sel_bwd_ws;
+  decltype(&asrn_selective_bwd) sel_bwd;
+  decltype(&asrn_selective_step) sel_paso;
 } lib;
 
 void vale(int rc, const char* que) {
@@ -355,6 +366,164 @@ std::tuple<Tensor, Tensor, Tensor> norma8(const Tensor& x, const Tensor& gamma, 
   return {r[0], r[1], r[2]};
 }
 
+// ---- a local block's operators with a state a channel ---------------------------------------------------------------------
+int32_t tipo_de(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
+// the channels next to each other: the kernels read the other axes through their strides
+Tensor por_canal(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor como(const Tensor& g, const Tensor& x) {       // a gradient in x's type, dense
+  return g.scalar_type() == x.scalar_type() && g.is_contiguous() ? g : g.to(x.scalar_type()).contiguous();
+}
+Tensor f32_o_nada(const Tensor& t) { return t.defined() ? denso(t) : t; }
+Tensor o_nada(const Opcional& t) { return t ? *t : Tensor(); }
+Tensor espacio(int64_t n, const Tensor& x) { return vacio({n < 0 ? 0 : n}, x, at::kByte); }
+bool con_gradiente(std::initializer_list<const Tensor*> ts) {
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : ts)
+      if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+void sin_gradiente(const char* que, std::initializer_list<const Tensor*> ts) {
+  if (con_gradiente(ts)) throw Fallo(std::string(que) + ": a token's step has no gradient: call it under torch.no_grad()");
+}
+
+// z (B, L, d), w (d, k) or (d, 1, k), b (d) or undefined
+struct ConvCanal : Function<ConvCanal> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& w, const Opcional& sesgo, int64_t act) {
+    En en(z);
+    const Tensor b = o_nada(sesgo);
+    const Tensor zc = por_canal(z), wc = denso(w), bc = f32_o_nada(b);
+    Tensor y = vacio(z.sizes(), z, z.scalar_type());
+    vale(lib.conv_fwd(ptr(zc), tipo_de(z), zc.stride(0), zc.stride(1), f32(wc), f32(bc), z.size(0), z.size(1), (int32_t)z.size(2),
+                      (int32_t)w.size(-1), (int32_t)act, ptr(y), en.st), "asrn_channel_conv_fwd");
+    ctx->save_for_backward({zc, w, b});
+    ctx->saved_data["a"] = act;
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("conv_canal");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &z = s[0], &w = s[1], &b = s[2];
+    En en(z);
+    const int64_t B = z.size(0), L = z.size(1), d = z.size(2), k = w.size(-1), wsb = lib.conv_ws(B, L, (int32_t)d, (int32_t)k);
+    const Tensor gy = como(g[0], z), wc = denso(w), bc = f32_o_nada(b);
+    Tensor dz = vacio(z.sizes(), z, z.scalar_type()), ws = espacio(wsb, z);
+    Tensor dp = B * L ? vacio({k + 1, d}, z) : at::zeros({k + 1, d}, z.options().dtype(at::kFloat));
+    vale(lib.conv_bwd(ptr(z), tipo_de(z), z.stride(0), z.stride(1), f32(wc), f32(bc), ptr(gy), B, L, (int32_t)d, (int32_t)k,
+                      (int32_t)ctx->saved_data["a"].toInt(), ptr(dz), f32(dp), ptr(ws), wsb, en.st), "asrn_channel_conv_bwd");
+    return {dz, dp.narrow(0, 0, k).t().view_as(w).to(w.scalar_type()),
+            b.defined() ? dp.select(0, k).to(b.scalar_type()) : Tensor(), Tensor()};
+  }
+};
+
+Tensor conv_canal(const Tensor& z, const Tensor& w, const Opcional& b, int64_t act) {
+  return ConvCanal::apply(z, w, b, act)[0];
+}
+
+// z (B, d), ventana (B, d, k - 1) dense -> y and the next window, the same tensor or a new one
+std::pair<Tensor, Tensor> paso_conv_canal(const Tensor& z, const Tensor& ventana, const Tensor& w, const Opcional& b, int64_t act,
+                                          bool en_sitio) {
+  sin_gradiente("paso_conv_canal", {&z, &ventana, &w});
+  En en(z);
+  const Tensor zc = por_canal(z), wc = denso(w), bc = f32_o_nada(o_nada(b));
+  Tensor y = vacio(z.sizes(), z, z.scalar_type()), sig = en_sitio ? ventana : at::empty_like(ventana);
+  vale(lib.conv_paso(ptr(zc), tipo_de(z), zc.stride(0), ptr(ventana), ptr(sig), f32(wc), f32(bc), z.size(0), (int32_t)z.size(1),
+                     (int32_t)w.size(-1), (int32_t)act, ptr(y), en.st), "asrn_channel_conv_step");
+  return {y, sig};
+}
+
+// u, dl, z (B, L, d), Bm, C (B, L, N) of one type; A (d, N), D, sesgo (d), h0 (B, d, N); D, z, sesgo, h0 may be undefined
+struct Selectivo : Function<Selectivo> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& u, const Tensor& dl, const Tensor& A, const Tensor& Bm,
+                               const Tensor& C, const Opcional& D_, const Opcional& z_, const Opcional& sesgo_,
+                               const Opcional& h0_, bool softplus, bool guarda, bool estado) {
+    En en(u);
+    const Tensor D = o_nada(D_), z = o_nada(z_), sesgo = o_nada(sesgo_), h0 = o_nada(h0_);
+    const int64_t B = u.size(0), L = u.size(1), d = u.size(2), N = A.size(1), wsb = lib.sel_ws(B, L, (int32_t)d, (int32_t)N);
+    const Tensor uc = por_canal(u), dc = por_canal(dl), Bc = por_canal(Bm), Cc = por_canal(C), zc = por_canal(z);
+    const Tensor Ac = denso(A), Dc = f32_o_nada(D), sc = f32_o_nada(sesgo), hc = f32_o_nada(h0);
+    Tensor y = vacio(u.sizes(), u, u.scalar_type()), ws = espacio(wsb, u), fin, marcas;
+    if (estado)      // no tokens: the state that came
+      fin = B * L ? vacio({B, d, N}, u) : hc.defined() ? hc.clone() : at::zeros({B, d, N}, u.options().dtype(at::kFloat));
+    if (guarda) marcas = vacio({B, lib.sel_marcas(L), d, N}, u);
+    int64_t st[10];
+    pasos(uc, st);
+    pasos(dc, st + 2);
+    pasos(Bc, st + 4);
+    pasos(Cc, st + 6);
+    pasos(zc.defined() ? Opcional(zc) : std::nullopt, st + 8);
+    vale(lib.sel_fwd(ptr(uc), ptr(dc), ptr(Bc), ptr(Cc), ptr(zc), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(hc), B, L,
+                     (int32_t)d, (int32_t)N, softplus, ptr(y), f32(fin), f32(marcas), ptr(ws), wsb, en.st), "asrn_selective_fwd");
+    ctx->save_for_backward({uc, dc, A, Bc, Cc, D, zc, sesgo, marcas});
+    ctx->saved_data["n"] = std::vector<int64_t>{softplus, h0.defined() ? (int64_t)h0.scalar_type() : -1};
+    ctx->set_materialize_grads(false);
+    return estado ? variable_list{y, fin} : variable_list{y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("escaneo_selectivo");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &u = s[0], &dl = s[1], &A = s[2], &Bm = s[3], &C = s[4], &D = s[5], &z = s[6], &sesgo = s[7], &marcas = s[8];
+    const Tensor gfin = g.size() > 1 ? f32_o_nada(g[1]) : Tensor();
+    variable_list r(12);
+    if (!g[0].defined() && !gfin.defined()) return r;
+    const auto n = ctx->saved_data["n"].toIntVector();
+    En en(u);
+    const auto tipo = u.scalar_type();
+    const Tensor gy = g[0].defined() ? como(g[0], u) : at::zeros(u.sizes(), u.options());
+    const int64_t B = u.size(0), L = u.size(1), d = u.size(2), N = A.size(1), wsb = lib.sel_bwd_ws(B, L, (int32_t)d, (int32_t)N);
+    const Tensor Ac = denso(A), Dc = f32_o_nada(D), sc = f32_o_nada(sesgo);
+    Tensor du = vacio(u.sizes(), u, tipo), ddl = vacio(u.sizes(), u, tipo), dB = vacio(Bm.sizes(), u, tipo),
+           dC = vacio(C.sizes(), u, tipo), dz = z.defined() ? vacio(u.sizes(), u, tipo) : Tensor(), dh, ws = espacio(wsb, u);
+    Tensor dp = B * L ? vacio({d * N + 2 * d}, u) : at::zeros({d * N + 2 * d}, u.options().dtype(at::kFloat));
+    if (n[1] >= 0)
+      dh = B * L ? vacio({B, d, N}, u) : gfin.defined() ? gfin.clone() : at::zeros({B, d, N}, u.options().dtype(at::kFloat));
+    int64_t st[12];
+    pasos(u, st);
+    pasos(dl, st + 2);
+    pasos(Bm, st + 4);
+    pasos(C, st + 6);
+    pasos(z.defined() ? Opcional(z) : std::nullopt, st + 8);
+    pasos(gy, st + 10);
+    vale(lib.sel_bwd(ptr(u), ptr(dl), ptr(Bm), ptr(C), ptr(z), ptr(gy), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(marcas),
+                     f32(gfin), B, L, (int32_t)d, (int32_t)N, (int32_t)n[0], ptr(du), ptr(ddl), ptr(dB), ptr(dC), ptr(dz), f32(dp),
+                     f32(dh), ptr(ws), wsb, en.st), "asrn_selective_bwd");
+    r[0] = du;
+    r[1] = ddl;
+    r[2] = dp.narrow(0, 0, d * N).view({d, N}).to(A.scalar_type());
+    r[3] = dB;
+    r[4] = dC;
+    if (D.defined()) r[5] = dp.narrow(0, d * N, d).to(D.scalar_type());
+    r[6] = dz;
+    if (sesgo.defined()) r[7] = dp.narrow(0, d * N + d, d).to(sesgo.scalar_type());
+    if (dh.defined()) r[8] = dh.to((at::ScalarType)n[1]);
+    return r;
+  }
+};
+
+std::pair<Tensor, Opcional> selectivo(const Tensor& u, const Tensor& dl, const Tensor& A, const Tensor& Bm, const Tensor& C,
+                                      const Opcional& D, const Opcional& z, const Opcional& sesgo, const Opcional& h0,
+                                      bool softplus, bool estado) {
+  const Tensor Dt = o_nada(D), zt = o_nada(z), st = o_nada(sesgo), ht = o_nada(h0);
+  const variable_list r = Selectivo::apply(u, dl, A, Bm, C, D, z, sesgo, h0, softplus,
+                                           con_gradiente({&u, &dl, &A, &Bm, &C, &Dt, &zt, &st, &ht}), estado);
+  return {r[0], estado ? Opcional(r[1]) : std::nullopt};
+}
+
+// u, dl, z (B, d), Bm, C (B, N), h (B, d, N) fp32 dense -> y and the next state, the same tensor or a new one
+std::pair<Tensor, Tensor> paso_selectivo(const Tensor& u, const Tensor& dl, const Tensor& A, const Tensor& Bm, const Tensor& C,
+                                         const Tensor& h, const Opcional& D, const Opcional& z, const Opcional& sesgo,
+                                         bool softplus, bool en_sitio) {
+  const Tensor zt = o_nada(z);
+  sin_gradiente("paso_selectivo", {&u, &dl, &A, &Bm, &C, &h, &zt});
+  En en(u);
+  const Tensor uc = por_canal(u), dc = por_canal(dl), Bc = por_canal(Bm), Cc = por_canal(C), zc = por_canal(zt);
+  const Tensor Ac = denso(A), Dc = f32_o_nada(o_nada(D)), sc = f32_o_nada(o_nada(sesgo));
+  Tensor y = vacio(u.sizes(), u, u.scalar_type()), sig = en_sitio ? h : at::empty_like(h);
+  const int64_t st[5] = {uc.stride(0), dc.stride(0), Bc.stride(0), Cc.stride(0), zc.defined() ? zc.stride(0) : 0};
+  vale(lib.sel_paso(ptr(uc), ptr(dc), ptr(Bc), ptr(Cc), ptr(zc), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(h), f32(sig),
+                    u.size(0), (int32_t)u.size(1), (int32_t)A.size(1), softplus, ptr(y), en.st), "asrn_selective_step");
+  return {y, sig};
+}
+
 // Whether a graph recorded on the default stream still holds one of these leaves' accumulators. A backward inside a
 // capture would run it on that stream, which no capture may wait for.
 bool hojas_en_uso(const std::vector<Tensor>& hojas) {
@@ -385,6 +554,16 @@ void iniciar(const py::function& direccion, py::object error) {
   de(lib.norm8_fwd, "asrn_norm8_fwd");
   de(lib.norm8_bwd, "asrn_norm8_bwd");
   de(lib.norm8_ws, "asrn_norm8_bwd_workspace");
+  de(lib.conv_fwd, "asrn_channel_conv_fwd");
+  de(lib.conv_ws, "asrn_channel_conv_bwd_workspace");
+  de(lib.conv_bwd, "asrn_channel_conv_bwd");
+  de(lib.conv_paso, "asrn_channel_conv_step");
+  de(lib.sel_marcas, "asrn_selective_checks");
+  de(lib.sel_ws, "asrn_selective_fwd_workspace");
+  de(lib.sel_fwd, "asrn_selective_fwd");
+  de(lib.sel_bwd_ws, "asrn_selective_bwd_workspace");
+  de(lib.sel_bwd, "asrn_selective_bwd");
+  de(lib.sel_paso, "asrn_selective_step");
   static PyObject* clase;                     // held to the process's end
   clase = error.release().ptr();
   py::register_exception_translator([](std::exception_ptr p) {
@@ -407,4 +586,8 @@ PYBIND11_MODULE(_nodos, m) {
   m.def("politica", &politica, Libre());
   m.def("gelu8", &gelu8, Libre());
   m.def("norma8", &norma8, Libre());
+  m.def("conv_canal", &conv_canal, Libre());
+  m.def("paso_conv_canal", &paso_conv_canal, Libre());
+  m.def("selectivo", &selectivo, Libre());
+  m.def("paso_selectivo", &paso_selectivo, Libre());
 }

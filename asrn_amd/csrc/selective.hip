@@ -1,0 +1,694 @@
+// The selective state space scan. For texts b, tokens t, channels c and states n:
+//   delta = softplus(dl + bias) (or dl + bias),   h_t = exp(delta_t A) h_{t-1} + delta_t u_t B_t,
+//   y_t = (sum_n C_t h_t + D u_t) silu(z_t)
+// with A (d, N), B and C shared by the channels, h in fp32. Its backward and one token's step.
+//
+// A wave takes 64 channels of one text. For the tokens' values lane l is channel l; for the states a lane holds 4
+// neighbouring channels (quad q = l / 4) by a quarter of the states (l % 4): what the channels share (B, C) and what the
+// states share (delta, delta u) comes from LDS as vectors, the sum over the states is one exchange within the quad that
+// leaves channel l in lane l again, and the sums over the channels that the backward needs (dB, dC) begin inside a lane.
+// A wave's LDS is its own: no barriers in the forward.
+// Every channel and state has its own decay, so there is no matrix product in it: an exponential and about four
+// multiply-adds a token, channel and state bound the forward.
+// Texts too few to fill the card are cut into chunks: each chunk's end state from a zero state and its sum of delta
+// first, then the chunks' start states one after the other (exp(A sum delta) carries a state over a chunk), then all chunks
+// at once. The backward does the same from the end with the states' gradients. A chunk is a multiple of kCheck
+// tokens, where the forward of a training step leaves its state: the backward forms the states in between again in
+// registers. Partial sums are added in a fixed order; the chunks are a function of the sizes alone.
+#include <type_traits>
+
+#include "types.h"
+
+namespace asrn {
+
+constexpr int kCheck = 8;         // tokens between two kept states; also the tile of the backward
+constexpr int kTile = 16;         // tokens that the forward stages at once
+constexpr int kMaxWaves = 4;      // of a workgroup, 64 channels each
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Selective {
+  const void *u, *dl, *z, *Bm, *Cm, *gy;                       // z may be null
+  int64_t ub, ut, dlb, dlt, zb, zt, Bb, Bt, Cb, Ct, gb, gt;    // strides of texts and tokens in elements
+  const float *A, *D, *bias, *h0;                              // D, bias, h0 may be null
+  void* y;
+  float* hend;                    // (B, d, N) or null
+  float* check;                   // (B, ceil(L / kCheck), d, N) or null
+  float* carry;                   // (B, chunks - 1, d, N): end states from zero, then the chunks' start states
+  float* total;                   // (B, chunks, d): sums of delta
+  int64_t B, L, chunk;
+  int d, N, chunks, softplus;
+  // backward
+  const float* ghend;             // (B, d, N) or null
+  void *du, *ddl, *dz;
+  float* dh0;                     // (B, d, N) or null
+  float* bc;                      // (blocks, B L, 2, N): dB and dC of a workgroup's channels
+  float* part;                    // (B chunks, d N + 2 d): dA, dD, dbias
+};
+
+// softplus(x) = max(x, 0) + log1p(exp(-|x|)); log1p(e) = 2 atanh(e / (2 + e)), whose series ends at s^15 / 15 of s <= 1/3
+__device__ __forceinline__ float softplus(float x) {
+  const float e = exp_fast(-fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+  float p = fmaf(q, 1.f / 15, 1.f / 13);
+  p = fmaf(q, p, 1.f / 11);
+  p = fmaf(q, p, 1.f / 9);
+  p = fmaf(q, p, 1.f / 7);
+  p = fmaf(q, p, 1.f / 5);
+  p = fmaf(q, p, 1.f / 3);
+  p = fmaf(q * s, p, s);
+  return fmaxf(x, 0.f) + 2.f * p;
+}
+
+// DPP within a quad: lane ^ 1 and lane ^ 2
+__device__ __forceinline__ float quad_xor1(float v) { return dpp<0xB1>(v); }
+__device__ __forceinline__ float quad_xor2(float v) { return dpp<0x4E>(v); }
+
+// v[i] of channel i of the quad's four, partial over the quad's lanes -> lane i's sum of v[i]
+__device__ __forceinline__ float quad_scatter(const float (&v)[4], int lane) {
+  const bool b0 = lane & 1, b1 = lane & 2;
+  const float r0 = (b0 ? v[1] : v[0]) + quad_xor1(b0 ? v[0] : v[1]);
+  const float r1 = (b0 ? v[3] : v[2]) + quad_xor1(b0 ? v[2] : v[3]);
+  return (b1 ? r1 : r0) + quad_xor2(b1 ? r0 : r1);
+}
+
+// What one wave's lanes write to LDS is read by its other lanes: in order in the hardware, and for the compiler here.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// x[0 .. NPL) of LDS, NPL in {2, 4, 8}
+template <int NPL>
+__device__ __forceinline__ void lds_vec(const float* p, float (&x)[NPL]) {
+  if constexpr (NPL == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x; x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NPL / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  }
+}
+
+// A wave's place: its text, its channels from c0 on, lane l's own channel c, the lane's quad's channels q .. q + 3 and its
+// states n0 .. n0 + NPL - 1
+struct Place {
+  int lane, wave, c, q, n0;
+  bool live;
+};
+template <int NPL>
+__device__ __forceinline__ Place place_of(const Selective& s) {
+  Place p;
+  p.lane = lane_id();
+  p.wave = threadIdx.x >> 6;
+  const int c0 = ((int)blockIdx.x * (int)(blockDim.x >> 6) + p.wave) * 64;
+  p.c = c0 + p.lane;
+  p.q = c0 + (p.lane & ~3);
+  p.n0 = (p.lane & 3) * NPL;
+  p.live = p.c < s.d;
+  return p;
+}
+
+// the lane's 4 x NPL values of a (d, N) array; `none` outside it
+template <int NPL>
+__device__ __forceinline__ void load_state(const float* x, const Selective& s, const Place& p, float (&h)[4][NPL],
+                                           float scale = 1.f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      h[i][j] = x && p.q + i < s.d && p.n0 + j < s.N ? scale * x[(int64_t)(p.q + i) * s.N + p.n0 + j] : 0.f;
+}
+template <int NPL>
+__device__ __forceinline__ void store_state(float* x, const Selective& s, const Place& p, const float (&h)[4][NPL]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (p.q + i < s.d && p.n0 + j < s.N) x[(int64_t)(p.q + i) * s.N + p.n0 + j] = h[i][j];
+}
+
+// B and C of TT tokens from t on, n padded with zeros to NP = 4 NPL: a wave's registers, then its LDS
+template <typename T, int NPL, int TT>
+struct Shared {
+  static constexpr int NP = 4 * NPL, E = (TT * NP + 63) / 64;
+  float x[E];
+  __device__ __forceinline__ void load(const void* X, int64_t sb, int64_t st, int64_t b, int64_t t, int64_t t1, int N, int lane) {
+    const T* p = static_cast<const T*>(X) + b * sb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = lane + 64 * e, r = i / NP, n = i % NP;
+      x[e] = r < TT && t + r < t1 && n < N ? (float)p[(t + r) * st + n] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(float* l, int lane) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (TT * NP % 64 == 0 || lane + 64 * e < TT * NP) l[lane + 64 * e] = x[e];
+  }
+};
+
+template <typename T, int TT>
+__device__ __forceinline__ void load_channel(const void* X, int64_t sb, int64_t st, int64_t b, int64_t t, int64_t t1, const Place& p,
+                                             float (&x)[TT]) {
+  const T* q = static_cast<const T*>(X) + b * sb + p.c;
+#pragma unroll
+  for (int r = 0; r < TT; ++r) x[r] = p.live && t + r < t1 ? (float)q[(t + r) * st] : 0.f;
+}
+
+// The forward over one chunk. LOCAL: its end state from zero and its sum of delta only.
+template <typename T, int NPL, bool LOCAL>
+__global__ __launch_bounds__(64 * kMaxWaves) void k_selective(Selective s) {
+  constexpr int NP = 4 * NPL, TT = kTile;
+  __shared__ float lds[kMaxWaves][TT * (128 + 2 * NP)];
+  const Place p = place_of<NPL>(s);
+  const int64_t b = blockIdx.z, chunk = blockIdx.y, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
+  float* sd = lds[p.wave];
+  float *su = sd + TT * 64, *sB = su + TT * 64, *sC = sB + TT * NP;
+  const int64_t dN = (int64_t)s.d * s.N, checks = (s.L + kCheck - 1) / kCheck;
+  float A2[4][NPL], h[4][NPL];
+  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL>(LOCAL ? nullptr : chunk ? s.carry + (b * (s.chunks - 1) + chunk - 1) * dN : s.h0 ? s.h0 + b * dN : nullptr,
+                  s, p, h);
+  const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
+  float sum = 0.f;
+  float u[TT], dl[TT], z[TT];
+  Shared<T, NPL, TT> mb, mc;
+  auto load = [&](int64_t t) {
+    load_channel<T, TT>(s.u, s.ub, s.ut, b, t, t1, p, u);
+    load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
+    mb.load(s.Bm, s.Bb, s.Bt, b, t, t1, s.N, p.lane);
+    if (!LOCAL) {
+      if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
+      mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+    }
+  };
+  load(t0);
+  for (int64_t t = t0; t < t1; t += TT) {
+    wave_lds_fence();
+    float du[TT], g[TT];              // D u and the gate of this tile, u and z being loaded for the next
+#pragma unroll
+    for (int r = 0; r < TT; ++r) {
+      const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
+      sd[r * 64 + p.lane] = delta;
+      su[r * 64 + p.lane] = delta * u[r];
+      if (LOCAL && t + r < t1) sum += delta;
+      if (!LOCAL) {
+        du[r] = D * u[r];
+        g[r] = s.z ? z[r] * sigmoid(z[r]) : 1.f;
+      }
+    }
+    mb.store(sB, p.lane);
+    if (!LOCAL) mc.store(sC, p.lane);
+    wave_lds_fence();
+    if (t + TT < t1) load(t + TT);
+#pragma unroll
+    for (int r = 0; r < TT; ++r) {
+      if (t + r >= t1) continue;                  // uniform
+      if (!LOCAL && s.check && (r % kCheck) == 0) store_state<NPL>(s.check + (b * checks + (t + r) / kCheck) * dN, s, p, h);
+      float dt[4], x[4], B[NPL], C[NPL], y[4];
+      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+      lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
+      lds_vec<NPL>(sB + r * NP + p.n0, B);
+      if (!LOCAL) lds_vec<NPL>(sC + r * NP + p.n0, C);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+          h[i][j] = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2[i][j]), h[i][j], x[i] * B[j]);
+          if (!LOCAL) y[i] = fmaf(h[i][j], C[j], y[i]);
+        }
+      }
+      if (!LOCAL) {
+        const float v = (quad_scatter(y, p.lane) + du[r]) * g[r];
+        if (p.live) static_cast<T*>(s.y)[(b * s.L + t + r) * s.d + p.c] = (T)v;
+      }
+    }
+  }
+  if (LOCAL) {
+    store_state<NPL>(s.carry + (b * (s.chunks - 1) + chunk) * dN, s, p, h);
+    if (p.live) s.total[(b * s.chunks + chunk) * s.d + p.c] = sum;
+  } else if (s.hend && chunk == s.chunks - 1) {
+    store_state<NPL>(s.hend + b * dN, s, p, h);
+  }
+}
+
+// The chunks' start states, in place of their end states from zero: carry[j] = the state that chunk j + 1 starts from.
+__global__ __launch_bounds__(256) void k_selective_carry(Selective s) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, dN = (int64_t)s.d * s.N;
+  if (i >= s.B * dN) return;
+  const int64_t b = i / dN, e = i % dN, c = e / s.N;
+  const float A2 = s.A[e] * kLog2e;
+  float h = s.h0 ? s.h0[b * dN + e] : 0.f;
+  float* x = s.carry + b * (s.chunks - 1) * dN + e;
+  const float* w = s.total + b * s.chunks * s.d + c;
+#pragma unroll 4
+  for (int j = 0; j < s.chunks - 1; ++j) {
+    h = fmaf(__builtin_amdgcn_exp2f(A2 * w[(int64_t)j * s.d]), h, x[j * dN]);
+    x[j * dN] = h;
+  }
+}
+
+// The backward's: carry[j] holds the gradient that chunk j + 1 passes to the state before it from a zero gradient at its
+// end, and becomes that of the state that chunk j ends in.
+__global__ __launch_bounds__(256) void k_selective_carry_bwd(Selective s) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, dN = (int64_t)s.d * s.N;
+  if (i >= s.B * dN) return;
+  const int64_t b = i / dN, e = i % dN, c = e / s.N;
+  const float A2 = s.A[e] * kLog2e;
+  float g = s.ghend ? s.ghend[b * dN + e] : 0.f;
+  float* x = s.carry + b * (s.chunks - 1) * dN + e;
+  const float* w = s.total + b * s.chunks * s.d + c;
+#pragma unroll 4
+  for (int j = s.chunks - 2; j >= 0; --j) {
+    g = fmaf(__builtin_amdgcn_exp2f(A2 * w[(int64_t)(j + 1) * s.d]), g, x[j * dN]);
+    x[j * dN] = g;
+  }
+}
+
+// What a chunk passes back to the state before it, from a zero gradient at its end, and its sum of delta.
+template <typename T, int NPL>
+__global__ __launch_bounds__(64 * kMaxWaves) void k_selective_local_bwd(Selective s) {
+  constexpr int NP = 4 * NPL, TT = kTile;
+  __shared__ float lds[kMaxWaves][TT * (128 + NP)];
+  const Place p = place_of<NPL>(s);
+  const int64_t b = blockIdx.z, chunk = blockIdx.y + 1, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
+  float* sd = lds[p.wave];
+  float *sg = sd + TT * 64, *sC = sg + TT * 64;
+  const int64_t dN = (int64_t)s.d * s.N;
+  float A2[4][NPL], g[4][NPL];
+  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL>(nullptr, s, p, g);
+  const float bias = s.bias && p.live ? s.bias[p.c] : 0.f;
+  float sum = 0.f;
+  float gy[TT], dl[TT], z[TT];
+  Shared<T, NPL, TT> mc;
+  auto load = [&](int64_t t) {
+    load_channel<T, TT>(s.gy, s.gb, s.gt, b, t, t1, p, gy);
+    load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
+    if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
+    mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+  };
+  int64_t t = t0 + (t1 - t0 - 1) / TT * TT;
+  load(t);
+  for (; t >= t0; t -= TT) {
+    wave_lds_fence();
+#pragma unroll
+    for (int r = 0; r < TT; ++r) {
+      const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
+      sd[r * 64 + p.lane] = delta;
+      sg[r * 64 + p.lane] = s.z ? gy[r] * z[r] * sigmoid(z[r]) : gy[r];
+      if (t + r < t1) sum += delta;
+    }
+    mc.store(sC, p.lane);
+    wave_lds_fence();
+    if (t > t0) load(t - TT);
+#pragma unroll
+    for (int r = TT - 1; r >= 0; --r) {
+      if (t + r >= t1) continue;                  // uniform
+      float dt[4], x[4], C[NPL];
+      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+      lds_vec<4>(sg + r * 64 + (p.lane & ~3), x);
+      lds_vec<NPL>(sC + r * NP + p.n0, C);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+          g[i][j] = fmaf(x[i], C[j], g[i][j]) * __builtin_amdgcn_exp2f(dt[i] * A2[i][j]);
+    }
+  }
+  store_state<NPL>(s.carry + (b * (s.chunks - 1) + chunk - 1) * dN, s, p, g);
+  if (p.live) s.total[(b * s.chunks + chunk) * s.d + p.c] = sum;
+}
+
+// The backward over one chunk, kCheck tokens at a time from its end: the states of those tokens again from the kept one, then
+// with G_t, the gradient of h_t, from the last to the first:
+//   G_t += gy_t C_t;  dC_t += gy_t h_t;  dB_t += G_t delta_t u_t;  d(delta u) = sum G_t B_t;
+//   w = G_t exp(delta_t A) h_{t-1};  dA += w delta_t;  d delta += sum w A;  G_{t-1} = G_t exp(delta_t A)
+// dB and dC are summed over the lane's 4 channels, then over a row of 16 lanes; the rows' and waves' sums through LDS.
+template <typename T, int NPL>
+__global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s) {
+  constexpr int NP = 4 * NPL, TT = kCheck;
+  constexpr int NJ = (NPL + 3) / 4;               // values of dB (and of dC) that a lane leaves of its row's sums
+  __shared__ float lds[kMaxWaves][TT * (192 + 2 * NP)];
+  __shared__ float red[TT][2][kMaxWaves * 4][NP];
+  const Place p = place_of<NPL>(s);
+  const int waves = blockDim.x >> 6;
+  const int64_t b = blockIdx.z, chunk = blockIdx.y, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
+  float* sd = lds[p.wave];
+  float *su = sd + TT * 64, *sg = su + TT * 64, *sB = sg + TT * 64, *sC = sB + TT * NP;
+  const int64_t dN = (int64_t)s.d * s.N, checks = (s.L + kCheck - 1) / kCheck;
+  float A2[4][NPL], dA[4][NPL], G[4][NPL];
+  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL>(nullptr, s, p, dA);
+  load_state<NPL>(chunk + 1 < s.chunks ? s.carry + (b * (s.chunks - 1) + chunk) * dN : s.ghend ? s.ghend + b * dN : nullptr, s, p,
+                  G);
+  const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
+  float dD = 0.f, dbias = 0.f;
+  const int row = p.lane >> 4, cq = (p.lane >> 2) & 3;
+  for (int64_t t = t0 + (t1 - t0 - 1) / TT * TT; t >= t0; t -= TT) {
+    float h[TT + 1][4][NPL];
+    load_state<NPL>(s.check + (b * checks + t / kCheck) * dN, s, p, h[0]);
+    float u[TT], dl[TT], z[TT], gy[TT];
+    {
+      Shared<T, NPL, TT> mb, mc;
+      load_channel<T, TT>(s.u, s.ub, s.ut, b, t, t1, p, u);
+      load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
+      if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
+      load_channel<T, TT>(s.gy, s.gb, s.gt, b, t, t1, p, gy);
+      mb.load(s.Bm, s.Bb, s.Bt, b, t, t1, s.N, p.lane);
+      mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+      wave_lds_fence();
+#pragma unroll
+      for (int r = 0; r < TT; ++r) {
+        const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
+        sd[r * 64 + p.lane] = delta;
+        su[r * 64 + p.lane] = delta * u[r];
+        sg[r * 64 + p.lane] = s.z ? gy[r] * z[r] * sigmoid(z[r]) : gy[r];
+      }
+      mb.store(sB, p.lane);
+      mc.store(sC, p.lane);
+      wave_lds_fence();
+    }
+#pragma unroll
+    for (int r = 0; r < TT; ++r) {                // past the text's end delta u is 0 and the state no longer matters
+      float dt[4], x[4], B[NPL];
+      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+      lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
+      lds_vec<NPL>(sB + r * NP + p.n0, B);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+          h[r + 1][i][j] = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2[i][j]), h[r][i][j], x[i] * B[j]);
+    }
+#pragma unroll
+    for (int r = TT - 1; r >= 0; --r) {
+      if (t + r >= t1) continue;                  // uniform
+      float dt[4], x[4], g[4], B[NPL], C[NPL], y[4], dx[4], dd[4], dB[NPL], dC[NPL];
+      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+      lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
+      lds_vec<4>(sg + r * 64 + (p.lane & ~3), g);
+      lds_vec<NPL>(sB + r * NP + p.n0, B);
+      lds_vec<NPL>(sC + r * NP + p.n0, C);
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) dB[j] = dC[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = dx[i] = dd[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+          const float G1 = fmaf(g[i], C[j], G[i][j]);
+          y[i] = fmaf(h[r + 1][i][j], C[j], y[i]);
+          dC[j] = fmaf(g[i], h[r + 1][i][j], dC[j]);
+          dB[j] = fmaf(G1, x[i], dB[j]);
+          dx[i] = fmaf(G1, B[j], dx[i]);
+          G[i][j] = G1 * __builtin_amdgcn_exp2f(dt[i] * A2[i][j]);
+          const float w = G[i][j] * h[r][i][j];
+          dd[i] = fmaf(w, A2[i][j], dd[i]);
+          dA[i][j] = fmaf(w, dt[i], dA[i][j]);
+        }
+      }
+      const float ys = quad_scatter(y, p.lane), ds = quad_scatter(dx, p.lane), dds = quad_scatter(dd, p.lane);
+      const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane];
+      float ddl = fmaf(dds, kLn2, ds * u[r]);
+      if (s.softplus) ddl *= sigmoid(dl[r] + bias);
+      dbias += ddl;
+      dD = fmaf(gg, u[r], dD);
+      if (p.live) {
+        const int64_t o = (b * s.L + t + r) * s.d + p.c;
+        static_cast<T*>(s.du)[o] = (T)fmaf(ds, delta, gg * D);
+        static_cast<T*>(s.ddl)[o] = (T)ddl;
+        if (s.z) {
+          const float q = sigmoid(z[r]);
+          static_cast<T*>(s.dz)[o] = (T)(gy[r] * fmaf(D, u[r], ys) * q * (1.f + z[r] * (1.f - q)));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {             // over the row's quads
+        dB[j] += dpp<0x128>(dB[j]);
+        dC[j] += dpp<0x128>(dC[j]);
+        dB[j] += dpp<0x124>(dB[j]);
+        dC[j] += dpp<0x124>(dC[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < NJ; ++k) {              // quad cq of the row leaves values 4 k + cq
+        float vb = dB[4 * k], vc = dC[4 * k];
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+          if (4 * k + j < NPL) {
+            vb = cq == j ? dB[4 * k + j] : vb;
+            vc = cq == j ? dC[4 * k + j] : vc;
+          }
+        if (4 * k + cq < NPL) {
+          red[r][0][p.wave * 4 + row][p.n0 + 4 * k + cq] = vb;
+          red[r][1][p.wave * 4 + row][p.n0 + 4 * k + cq] = vc;
+        }
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < TT * 2 * s.N; e += blockDim.x) {
+      const int r = e / (2 * s.N), k = e / s.N % 2, n = e % s.N;
+      if (t + r < t1) {
+        float v = 0.f;
+        for (int w = 0; w < 4 * waves; ++w) v += red[r][k][w][n];
+        s.bc[((blockIdx.x * s.B + b) * s.L + t + r) * 2 * s.N + k * s.N + n] = v;
+      }
+    }
+    __syncthreads();
+  }
+  float* part = s.part + (b * s.chunks + chunk) * (dN + 2 * s.d);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (p.q + i < s.d && p.n0 + j < s.N) part[(int64_t)(p.q + i) * s.N + p.n0 + j] = dA[i][j];
+  if (p.live) {
+    part[dN + p.c] = dD;
+    part[dN + s.d + p.c] = dbias;
+  }
+  if (s.dh0 && chunk == 0) store_state<NPL>(s.dh0 + b * dN, s, p, G);
+}
+
+// dB and dC: the workgroups' sums in order, in the tensors' type
+template <typename T>
+__global__ __launch_bounds__(256) void k_selective_shared(const float* bc, int blocks, int64_t rows, int N, T* dB, T* dC) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = rows * 2 * N;
+  if (i >= n) return;
+  float v = 0.f;
+  for (int k = 0; k < blocks; ++k) v += bc[k * n + i];
+  const int64_t row = i / (2 * N);
+  const int e = (int)(i % (2 * N));
+  if (e < N) dB[row * N + e] = (T)v;
+  else dC[row * N + e - N] = (T)v;
+}
+
+// One token: 4 lanes a channel, each every fourth state.
+template <typename T>
+__global__ __launch_bounds__(256) void k_selective_step(Selective s, const float* h, float* next) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, q = i >> 2, b = q / s.d;
+  const int ng = (int)(i & 3), c = (int)(q % s.d);
+  const bool live = b < s.B;                      // whole quads: the exchange below stays within one
+  const int64_t bb = live ? b : 0;
+  float dl = (float)static_cast<const T*>(s.dl)[bb * s.dlb + c] + (s.bias ? s.bias[c] : 0.f);
+  const float u = (float)static_cast<const T*>(s.u)[bb * s.ub + c], delta = s.softplus ? softplus(dl) : dl;
+  const T *Bm = static_cast<const T*>(s.Bm) + bb * s.Bb, *Cm = static_cast<const T*>(s.Cm) + bb * s.Cb;
+  const float* hr = h + (bb * s.d + c) * s.N;
+  float* hw = next + (bb * s.d + c) * s.N;
+  float y = 0.f;
+  for (int n = ng; n < s.N; n += 4) {
+    const float a = __builtin_amdgcn_exp2f(delta * (s.A[(int64_t)c * s.N + n] * kLog2e));
+    const float x = fmaf(a, hr[n], delta * u * (float)Bm[n]);
+    if (live) hw[n] = x;
+    y = fmaf(x, (float)Cm[n], y);
+  }
+  y += quad_xor1(y);
+  y += quad_xor2(y);
+  if (live && ng == 0) {
+    if (s.D) y = fmaf(s.D[c], u, y);
+    if (s.z) {
+      const float z = (float)static_cast<const T*>(s.z)[b * s.zb + c];
+      y *= z * sigmoid(z);
+    }
+    static_cast<T*>(s.y)[q] = (T)y;
+  }
+}
+
+// Waves of 64 channels a workgroup: at most kMaxWaves, spread evenly
+static void grid_of(int d, int& waves, int& blocks) {
+  const int n = (d + 63) / 64;
+  blocks = (n + kMaxWaves - 1) / kMaxWaves;
+  waves = (n + blocks - 1) / blocks;
+  blocks = (n + waves - 1) / waves;
+}
+
+constexpr int kWantWaves = 2048;    // 2 a SIMD
+// Chunks of a text: as many as fill the card, of at least kMinChunk tokens (a chunk's tokens are walked twice when there
+// are several).
+constexpr int kMinChunk = 64;
+static int64_t chunk_of(int64_t B, int64_t L, int d) {
+  const int64_t waves = B * ((d + 63) / 64);
+  int64_t n = kWantWaves / waves;
+  if (n < 2) return (L + kTile - 1) / kTile * kTile;
+  int64_t c = (L + n - 1) / n;
+  if (c < kMinChunk) c = kMinChunk;
+  return (c + kTile - 1) / kTile * kTile;
+}
+static int chunks_of(int64_t B, int64_t L, int d) {
+  const int64_t c = chunk_of(B, L, d);
+  return c > 0 ? (int)((L + c - 1) / c) : 0;
+}
+
+static int check(const Selective& s, int32_t type, const char* what) {
+  ASRN_REQUIRE(type_ok(type), "%s: type %d", what, type);
+  ASRN_REQUIRE(s.B >= 0 && s.L >= 0 && s.d >= 1 && s.d < (1 << 22) && s.N >= 1 && s.N <= 32,
+               "%s: bad sizes B=%lld L=%lld d=%d N=%d (1 <= N <= 32)", what, (long long)s.B, (long long)s.L, s.d, s.N);
+  ASRN_REQUIRE(s.B < 65536 && s.L < ((int64_t)1 << 30) && s.B * s.L < ((int64_t)1 << 36), "%s: too many tokens", what);
+  return 0;
+}
+
+template <typename F>
+static int with_states(int N, F&& f) {
+  if (N <= 8) return f(std::integral_constant<int, 2>{});
+  if (N <= 16) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 8>{});
+}
+
+static int64_t carry_bytes(int64_t B, int chunks, int64_t d, int64_t N) {
+  return chunks > 1 ? (B * ((chunks - 1) * d * N + chunks * d) * 4 + 255) / 256 * 256 : 0;
+}
+
+}  // namespace asrn
+
+using namespace asrn;
+
+extern "C" int64_t asrn_selective_checks(int64_t L) { return L < 0 ? -1 : (L + kCheck - 1) / kCheck; }
+
+extern "C" int64_t asrn_selective_fwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N) {
+  if (B < 0 || L < 0 || d < 1 || N < 1) return -1;
+  if (B == 0 || L == 0) return 0;
+  return carry_bytes(B, chunks_of(B, L, d), d, N);
+}
+
+extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z,
+                                  int32_t type, const int64_t* strides, const float* A, const float* D, const float* bias,
+                                  const float* h0, int64_t B, int64_t L, int32_t d, int32_t N, int32_t softplus, void* y,
+                                  float* hend, float* checks, void* workspace, int64_t workspace_bytes, void* stream) {
+  Selective s = {};
+  s.u = u; s.dl = delta; s.Bm = B_; s.Cm = C_; s.z = z;
+  s.A = A; s.D = D; s.bias = bias; s.h0 = h0; s.y = y; s.hend = hend; s.check = checks;
+  s.B = B; s.L = L; s.d = d; s.N = N; s.softplus = softplus;
+  if (check(s, type, "asrn_selective_fwd")) return 1;
+  if (B == 0 || L == 0) return 0;
+  ASRN_REQUIRE(u && delta && B_ && C_ && A && y && strides, "asrn_selective_fwd: null pointer");
+  s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
+  s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9];
+  s.chunk = chunk_of(B, L, d);
+  s.chunks = chunks_of(B, L, d);
+  ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_fwd: too many chunks");
+  const int64_t need = carry_bytes(B, s.chunks, d, N);
+  if (need) {
+    ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
+                 "asrn_selective_fwd: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                 (long long)workspace_bytes);
+    s.carry = (float*)workspace;
+    s.total = s.carry + B * (s.chunks - 1) * (int64_t)d * N;
+  }
+  int waves, blocks;
+  grid_of(d, waves, blocks);
+  hipStream_t st = (hipStream_t)stream;
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    return with_states(N, [&](auto npl) {
+      constexpr int NPL = decltype(npl)::value;
+      if (s.chunks > 1) {
+        hipLaunchKernelGGL((k_selective<T, NPL, true>), dim3(blocks, s.chunks - 1, B), dim3(64 * waves), 0, st, s);
+        hipLaunchKernelGGL(k_selective_carry, dim3((unsigned)((B * d * N + 255) / 256)), dim3(256), 0, st, s);
+      }
+      hipLaunchKernelGGL((k_selective<T, NPL, false>), dim3(blocks, s.chunks, B), dim3(64 * waves), 0, st, s);
+      return check_launch("asrn_selective_fwd");
+    });
+  });
+}
+
+static int64_t bc_floats(int64_t B, int64_t L, int d, int N) {
+  int waves, blocks;
+  grid_of(d, waves, blocks);
+  return (blocks * B * L * 2 * N + 63) / 64 * 64;
+}
+
+extern "C" int64_t asrn_selective_bwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N) {
+  if (B < 0 || L < 0 || d < 1 || N < 1) return -1;
+  if (B == 0 || L == 0) return 0;
+  const int chunks = chunks_of(B, L, d);
+  return carry_bytes(B, chunks, d, N) + bc_floats(B, L, d, N) * 4 + B * chunks * ((int64_t)d * N + 2 * d) * 4;
+}
+
+extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z,
+                                  const void* dy, int32_t type, const int64_t* strides, const float* A, const float* D,
+                                  const float* bias, const float* checks, const float* dhend, int64_t B, int64_t L, int32_t d,
+                                  int32_t N, int32_t softplus, void* du, void* ddelta, void* dB, void* dC, void* dz,
+                                  float* dparams, float* dh0, void* workspace, int64_t workspace_bytes, void* stream) {
+  Selective s = {};
+  s.u = u; s.dl = delta; s.Bm = B_; s.Cm = C_; s.z = z; s.gy = dy;
+  s.A = A; s.D = D; s.bias = bias; s.check = const_cast<float*>(checks); s.ghend = dhend;
+  s.du = du; s.ddl = ddelta; s.dz = dz; s.dh0 = dh0;
+  s.B = B; s.L = L; s.d = d; s.N = N; s.softplus = softplus;
+  if (check(s, type, "asrn_selective_bwd")) return 1;
+  if (B == 0 || L == 0) return 0;
+  ASRN_REQUIRE(u && delta && B_ && C_ && A && dy && checks && strides && du && ddelta && dB && dC && dparams && (!z || dz),
+               "asrn_selective_bwd: null pointer");
+  s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
+  s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9]; s.gb = strides[10]; s.gt = strides[11];
+  s.chunk = chunk_of(B, L, d);
+  s.chunks = chunks_of(B, L, d);
+  ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_bwd: too many chunks");
+  const int64_t need = asrn_selective_bwd_workspace(B, L, d, N), groups = B * s.chunks, cols = (int64_t)d * N + 2 * d;
+  ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
+               "asrn_selective_bwd: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+               (long long)workspace_bytes);
+  ASRN_REQUIRE(groups < (1 << 30) && cols < (1 << 30), "asrn_selective_bwd: too many chunks");
+  s.carry = (float*)workspace;
+  s.total = s.carry + B * (s.chunks - 1) * (int64_t)d * N;
+  s.bc = (float*)((char*)workspace + carry_bytes(B, s.chunks, d, N));
+  s.part = s.bc + bc_floats(B, L, d, N);
+  int waves, blocks;
+  grid_of(d, waves, blocks);
+  hipStream_t st = (hipStream_t)stream;
+  const int rc = with_type(type, [&](auto t) {
+    using T = decltype(t);
+    return with_states(N, [&](auto npl) {
+      constexpr int NPL = decltype(npl)::value;
+      if (s.chunks > 1) {
+        hipLaunchKernelGGL((k_selective_local_bwd<T, NPL>), dim3(blocks, s.chunks - 1, B), dim3(64 * waves), 0, st, s);
+        hipLaunchKernelGGL(k_selective_carry_bwd, dim3((unsigned)((B * d * N + 255) / 256)), dim3(256), 0, st, s);
+      }
+      hipLaunchKernelGGL((k_selective_bwd<T, NPL>), dim3(blocks, s.chunks, B), dim3(64 * waves), 0, st, s);
+      hipLaunchKernelGGL((k_selective_shared<T>), dim3((unsigned)((B * L * 2 * N + 255) / 256)), dim3(256), 0, st, s.bc, blocks,
+                         B * L, N, (T*)dB, (T*)dC);
+      return check_launch("asrn_selective_bwd");
+    });
+  });
+  return rc ? rc : group_sums(s.part, (int)groups, (int)cols, dparams, st);
+}
+
+extern "C" int asrn_selective_step(const void* u, const void* delta, const void* B_, const void* C_, const void* z,
+                                   int32_t type, const int64_t* strides, const float* A, const float* D, const float* bias,
+                                   const float* h, float* next, int64_t B, int32_t d, int32_t N, int32_t softplus, void* y,
+                                   void* stream) {
+  Selective s = {};
+  s.u = u; s.dl = delta; s.Bm = B_; s.Cm = C_; s.z = z;
+  s.A = A; s.D = D; s.bias = bias; s.y = y;
+  s.B = B; s.L = 1; s.d = d; s.N = N; s.softplus = softplus;
+  if (check(s, type, "asrn_selective_step")) return 1;
+  if (B == 0) return 0;
+  ASRN_REQUIRE(u && delta && B_ && C_ && A && y && h && next && strides, "asrn_selective_step: null pointer");
+  s.ub = strides[0]; s.dlb = strides[1]; s.Bb = strides[2]; s.Cb = strides[3]; s.zb = strides[4];
+  return with_type(type, [&](auto t) {
+    hipLaunchKernelGGL((k_selective_step<decltype(t)>), dim3((unsigned)((B * d * 4 + 255) / 256)), dim3(256), 0,
+                       (hipStream_t)stream, s, h, next);
+    return check_launch("asrn_selective_step");
+  });
+}

@@ -727,6 +727,53 @@ int asrn_norm8_bwd(const int8_t* q, const uint8_t* e, const float* gamma, const 
 int asrn_norm8_read(const int8_t* q, const uint8_t* e, const float* gamma, const float* beta, const float* stats, int64_t B,
                     int64_t L, int32_t d, int32_t k, int32_t out_bf16, void* out, void* stream);
 
+/* ---- a local block's causal convolution of each channel ------------------------------------------------------------
+ * The reference's per-channel convolution of a 'memoria' block (asrn/nucleo.py:969-1014) with its bias and activation in
+ * one pass. Values in fp32, bf16 or fp16 (type 0, 1, 2); z (B, L, d) with its texts and tokens stride_b and stride_t
+ * elements apart and its channels adjacent, no alignment beyond the element's; w (d, k) and bias (d, or null) fp32,
+ * 1 <= k <= 16; act 0 none, 1 GELU (erf), 2 SiLU; fp32 sums.
+ * fwd: y (B, L, d) dense = act(bias[c] + sum_j w[c, j] z[b, t - (k - 1) + j, c]), zeros before a text's start.
+ * bwd: dy dense; dz (B, L, d) dense; dparams (k + 1, d): dw[c, j] at (j, c), then dbias; summed in a fixed order.
+ * workspace: asrn_channel_conv_bwd_workspace bytes (-1: bad sizes), 16-byte aligned. B L = 0 writes nothing.
+ * step: one token, z (B, d), rows stride_b apart; window (B, d, k - 1) dense, the values before it, oldest first; next (the
+ * same buffer, or another) gets the window after it. */
+int asrn_channel_conv_fwd(const void* z, int32_t type, int64_t stride_b, int64_t stride_t, const float* w, const float* bias,
+                          int64_t B, int64_t L, int32_t d, int32_t k, int32_t act, void* y, void* stream);
+int64_t asrn_channel_conv_bwd_workspace(int64_t B, int64_t L, int32_t d, int32_t k);
+int asrn_channel_conv_bwd(const void* z, int32_t type, int64_t stride_b, int64_t stride_t, const float* w, const float* bias,
+                          const void* dy, int64_t B, int64_t L, int32_t d, int32_t k, int32_t act, void* dz, float* dparams,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int asrn_channel_conv_step(const void* z, int32_t type, int64_t stride_b, const void* window, void* next, const float* w,
+                           const float* bias, int64_t B, int32_t d, int32_t k, int32_t act, void* y, void* stream);
+
+/* ---- selective state space scan ------------------------------------------------------------------------------------
+ * No counterpart in the reference (beside its affine scan, asrn/nucleo.py:188-196). u, delta, z (B, L, d; z may be null)
+ * and B_, C_ (B, L, N) in fp32, bf16 or fp16 (type 0, 1, 2), all of one type, the last axis adjacent, texts and tokens
+ * through strides (host array in elements: text and token stride of u, delta, B_, C_, z, and for the backward dy). A (d, N),
+ * D, bias (d, or null) fp32; states (B, d, N) fp32 dense. D_t = softplus(delta + bias) (softplus 0: delta + bias),
+ *   h_t = exp(D_t A) h_{t-1} + D_t u_t B_t,  y_t = (sum_n C_t h_t + D u_t) silu(z_t)   (without z: no gate)
+ * from h0 (null: zeros). fwd: y (B, L, d) dense; hend (or null) the last state; checks (or null; B x
+ * asrn_selective_checks(L) x d x N) the states that the backward starts from. bwd: dhend (or null) the last state's
+ * gradient; du, ddelta, dz (with z), dB, dC dense in the inputs' type; dparams = dA (d, N), then dD (d), then dbias (d); dh0
+ * (or null). Sums in a fixed order. workspaces 16-byte aligned, of the stated sizes (-1: bad sizes). B L = 0 writes nothing.
+ * step: one token; strides (host) = the rows' of u, delta, B_, C_, z; next (the same buffer, or another) gets the state.
+ * Requires 1 <= N <= 32, d < 2^22, B < 2^16, L < 2^30, B L < 2^36. */
+int64_t asrn_selective_checks(int64_t L);
+int64_t asrn_selective_fwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N);
+int asrn_selective_fwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z, int32_t type,
+                       const int64_t* strides, const float* A, const float* D, const float* bias, const float* h0, int64_t B,
+                       int64_t L, int32_t d, int32_t N, int32_t softplus, void* y, float* hend, float* checks, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int64_t asrn_selective_bwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N);
+int asrn_selective_bwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z, const void* dy,
+                       int32_t type, const int64_t* strides, const float* A, const float* D, const float* bias,
+                       const float* checks, const float* dhend, int64_t B, int64_t L, int32_t d, int32_t N, int32_t softplus,
+                       void* du, void* ddelta, void* dB, void* dC, void* dz, float* dparams, float* dh0, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int asrn_selective_step(const void* u, const void* delta, const void* B_, const void* C_, const void* z, int32_t type,
+                        const int64_t* strides, const float* A, const float* D, const float* bias, const float* h, float* next,
+                        int64_t B, int32_t d, int32_t N, int32_t softplus, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
