@@ -140,7 +140,7 @@ SIGNATURES = {
     'asrn_channel_conv_bwd': (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _I64,
                                              _P]),
     'asrn_channel_conv_step': (ctypes.c_int, [_P, _I32, _I64, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P]),
-    'asrn_selective_checks': (_I64, [_I64]),
+    'asrn_selective_checks': (_I64, [_I64, _I64, _I32, _I32]),
     'asrn_selective_fwd_workspace': (_I64, [_I64, _I64, _I32, _I32]),
     'asrn_selective_fwd': (ctypes.c_int, [_P] * 5 + [_I32] + [_P] * 5 + [_I64, _I64, _I32, _I32, _I32] + [_P] * 4 + [_I64, _P]),
     'asrn_selective_bwd_workspace': (_I64, [_I64, _I64, _I32, _I32]),

@@ -370,6 +370,8 @@ std::tuple<Tensor, Tensor, Tensor> norma8(const Tensor& x, const Tensor& gamma, 
 int32_t tipo_de(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
 // the channels next to each other: the kernels read the other axes through their strides
 Tensor por_canal(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// a scan's (B, L, .): its tokens within the kernels' 32-bit offsets too
+Tensor cercanas(const Tensor& t) { return t.defined() && t.stride(1) >= (1 << 24) ? t.contiguous() : por_canal(t); }
 Tensor como(const Tensor& g, const Tensor& x) {       // a gradient in x's type, dense
   return g.scalar_type() == x.scalar_type() && g.is_contiguous() ? g : g.to(x.scalar_type()).contiguous();
 }
@@ -439,12 +441,12 @@ struct Selectivo : Function<Selectivo> {
     En en(u);
     const Tensor D = o_nada(D_), z = o_nada(z_), sesgo = o_nada(sesgo_), h0 = o_nada(h0_);
     const int64_t B = u.size(0), L = u.size(1), d = u.size(2), N = A.size(1), wsb = lib.sel_ws(B, L, (int32_t)d, (int32_t)N);
-    const Tensor uc = por_canal(u), dc = por_canal(dl), Bc = por_canal(Bm), Cc = por_canal(C), zc = por_canal(z);
+    const Tensor uc = cercanas(u), dc = cercanas(dl), Bc = cercanas(Bm), Cc = cercanas(C), zc = cercanas(z);
     const Tensor Ac = denso(A), Dc = f32_o_nada(D), sc = f32_o_nada(sesgo), hc = f32_o_nada(h0);
     Tensor y = vacio(u.sizes(), u, u.scalar_type()), ws = espacio(wsb, u), fin, marcas;
     if (estado)      // no tokens: the state that came
       fin = B * L ? vacio({B, d, N}, u) : hc.defined() ? hc.clone() : at::zeros({B, d, N}, u.options().dtype(at::kFloat));
-    if (guarda) marcas = vacio({B, lib.sel_marcas(L), d, N}, u);
+    if (guarda) marcas = vacio({lib.sel_marcas(B, L, (int32_t)d, (int32_t)N)}, u);
     int64_t st[10];
     pasos(uc, st);
     pasos(dc, st + 2);

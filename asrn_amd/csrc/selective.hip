@@ -32,10 +32,10 @@ struct Selective {
   const float *A, *D, *bias, *h0;                              // D, bias, h0 may be null
   void* y;
   float* hend;                    // (B, d, N) or null
-  float* check;                   // (B, ceil(L / kCheck), d, N) or null
-  float* carry;                   // (B, chunks - 1, d, N): end states from zero, then the chunks' start states
+  float* check;                   // (B, ceil(L / kCheck), own) or null
+  float* carry;                   // (B, chunks - 1, own): end states from zero, then the chunks' start states
   float* total;                   // (B, chunks, d): sums of delta
-  int64_t B, L, chunk;
+  int64_t B, L, chunk, own;       // own: floats of a state as the lanes hold it
   int d, N, chunks, softplus;
   // backward
   const float* ghend;             // (B, d, N) or null
@@ -91,26 +91,26 @@ __device__ __forceinline__ void lds_vec(const float* p, float (&x)[NPL]) {
   }
 }
 
-// A wave's place: its text, its channels from c0 on, lane l's own channel c, the lane's quad's channels q .. q + 3 and its
-// states n0 .. n0 + NPL - 1
+// A wave's place: its 64 channels' number, lane l's own channel c, the lane's quad's channels q .. q + 3 and its states
+// n0 .. n0 + NPL - 1
 struct Place {
-  int lane, wave, c, q, n0;
+  int lane, wave, group, c, q, n0;
   bool live;
 };
 template <int NPL>
 __device__ __forceinline__ Place place_of(const Selective& s) {
   Place p;
   p.lane = lane_id();
-  p.wave = threadIdx.x >> 6;
-  const int c0 = ((int)blockIdx.x * (int)(blockDim.x >> 6) + p.wave) * 64;
-  p.c = c0 + p.lane;
-  p.q = c0 + (p.lane & ~3);
+  p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  p.group = (int)blockIdx.x * (int)(blockDim.x >> 6) + p.wave;
+  p.c = p.group * 64 + p.lane;
+  p.q = p.group * 64 + (p.lane & ~3);
   p.n0 = (p.lane & 3) * NPL;
   p.live = p.c < s.d;
   return p;
 }
 
-// the lane's 4 x NPL values of a (d, N) array; `none` outside it
+// the lane's 4 x NPL values of a (d, N) array, 0 outside it
 template <int NPL>
 __device__ __forceinline__ void load_state(const float* x, const Selective& s, const Place& p, float (&h)[4][NPL],
                                            float scale = 1.f) {
@@ -129,17 +129,61 @@ __device__ __forceinline__ void store_state(float* x, const Selective& s, const 
       if (p.q + i < s.d && p.n0 + j < s.N) x[(int64_t)(p.q + i) * s.N + p.n0 + j] = h[i][j];
 }
 
-// B and C of TT tokens from t on, n padded with zeros to NP = 4 NPL: a wave's registers, then its LDS
+// The kernels' own states (kept ones, carries) lie as the lanes hold them: per 64 channels 4 NPL x 64 floats, in vectors of
+// V of a lane, padded channels and states among them (0).
+template <int NPL>
+struct Own {
+  static constexpr int V = NPL < 4 ? NPL : 4, G = 4 * NPL / V;
+  typedef float FV __attribute__((ext_vector_type(V)));
+  static __device__ __forceinline__ void load(const float* x, const Place& p, float (&h)[4][NPL]) {
+    const FV* v = reinterpret_cast<const FV*>(x) + (int64_t)p.group * 64 * G;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const FV w = v[(unsigned)(g * 64 + p.lane)];
+#pragma unroll
+      for (int k = 0; k < V; ++k) h[g * V / NPL][g * V % NPL + k] = w[k];
+    }
+  }
+  static __device__ __forceinline__ void store(float* x, const Place& p, const float (&h)[4][NPL]) {
+    FV* v = reinterpret_cast<FV*>(x) + (int64_t)p.group * 64 * G;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      FV w;
+#pragma unroll
+      for (int k = 0; k < V; ++k) w[k] = h[g * V / NPL][g * V % NPL + k];
+      v[(unsigned)(g * 64 + p.lane)] = w;
+    }
+  }
+  // the channel and the state of the i-th float
+  static __device__ __forceinline__ void where(int64_t i, int64_t& c, int& n) {
+    const int k = (int)(i % V), lane = (int)(i / V % 64), g = (int)(i / (V * 64) % G);
+    c = i / (V * 64 * G) * 64 + (lane & ~3) + g * V / NPL;
+    n = (lane & 3) * NPL + g * V % NPL + k;
+  }
+};
+
+// the tokens of a tile of TT that begins at t of a chunk that ends at t1
+template <int TT>
+__device__ __forceinline__ int tokens_of(int64_t t, int64_t t1) {
+  const int n = __builtin_amdgcn_readfirstlane((int)(t1 - t));       // opaque: compared as 64 bits, each use would fill a mask
+  return n < TT ? n : TT;
+}
+
+// B or C of TT tokens from t on, the states padded with zeros to NP = 4 NPL: a wave's registers, then its LDS. Tokens past
+// the chunk's end repeat its last.
 template <typename T, int NPL, int TT>
 struct Shared {
   static constexpr int NP = 4 * NPL, E = (TT * NP + 63) / 64;
   float x[E];
-  __device__ __forceinline__ void load(const void* X, int64_t sb, int64_t st, int64_t b, int64_t t, int64_t t1, int N, int lane) {
-    const T* p = static_cast<const T*>(X) + b * sb;
+  __device__ __forceinline__ void load(const T* X, int64_t st, int64_t t, int64_t t1, int N, int lane) {
+    const T* p = X + t * st;
+    const int last = tokens_of<TT>(t, t1) - 1;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = lane + 64 * e, r = i / NP, n = i % NP;
-      x[e] = r < TT && t + r < t1 && n < N ? (float)p[(t + r) * st + n] : 0.f;
+      const int i = lane + 64 * e, n = i % NP;
+      const int r = i / NP < last ? i / NP : last;
+      const float v = (float)p[(unsigned)(r * (int)st + (n < N ? n : 0))];
+      x[e] = n < N ? v : 0.f;
     }
   }
   __device__ __forceinline__ void store(float* l, int lane) const {
@@ -149,12 +193,54 @@ struct Shared {
   }
 };
 
+// A text's rows of channels from one token on, lane l at its channel: the row as the scalar offset of a buffer access (an
+// address a row would fill the scalar registers). Lanes without a channel lie past the buffer's end: they read 0, so that
+// their states stay 0 and nothing of theirs enters a sum, and what they store is dropped.
+constexpr unsigned kBufferBytes = 1u << 30;
+template <typename T>
+struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned at, step;
+  __device__ __forceinline__ Rows(const T* row, int64_t st, const Place& p)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, kBufferBytes, 0x00027000)),
+        at(p.live ? p.c * (unsigned)sizeof(T) : kBufferBytes),
+        // opaque: its multiples are formed where they are used, not kept over the tiles
+        step(__builtin_amdgcn_readfirstlane((unsigned)st * (unsigned)sizeof(T))) {}
+  __device__ __forceinline__ T load(unsigned row) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, row, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rsrc, at, row, 0));
+  }
+  __device__ __forceinline__ void store(T v, unsigned row) const {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, at, row, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, at, row, 0);
+  }
+};
+
+// lane l's channel of TT tokens from t on, of a text's rows; past the chunk's end its last token again
 template <typename T, int TT>
-__device__ __forceinline__ void load_channel(const void* X, int64_t sb, int64_t st, int64_t b, int64_t t, int64_t t1, const Place& p,
-                                             float (&x)[TT]) {
-  const T* q = static_cast<const T*>(X) + b * sb + p.c;
+__device__ __forceinline__ void load_channel(const T* rows, int64_t st, int64_t t, int64_t t1, const Place& p, T (&x)[TT]) {
+  const Rows<T> q(rows + t * st, st, p);
+  const int last = tokens_of<TT>(t, t1) - 1;
+  unsigned row = 0;
 #pragma unroll
-  for (int r = 0; r < TT; ++r) x[r] = p.live && t + r < t1 ? (float)q[(t + r) * st] : 0.f;
+  for (int r = 0; r < TT; ++r) {
+    x[r] = q.load(row);
+    row += r < last ? q.step : 0u;
+  }
+}
+
+__device__ __forceinline__ float decay(float delta, float A2) { return __builtin_amdgcn_exp2f(delta * A2); }
+
+// delta of a lane's TT tokens
+template <typename T, int TT>
+__device__ __forceinline__ void step_sizes(const T (&dl)[TT], float bias, bool sp, float (&delta)[TT]) {
+  if (sp) {
+#pragma unroll
+    for (int r = 0; r < TT; ++r) delta[r] = softplus((float)dl[r] + bias);
+  } else {
+#pragma unroll
+    for (int r = 0; r < TT; ++r) delta[r] = (float)dl[r] + bias;
+  }
 }
 
 // The forward over one chunk. LOCAL: its end state from zero and its sum of delta only.
@@ -167,46 +253,59 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective(Selective s) {
   float* sd = lds[p.wave];
   float *su = sd + TT * 64, *sB = su + TT * 64, *sC = sB + TT * NP;
   const int64_t dN = (int64_t)s.d * s.N, checks = (s.L + kCheck - 1) / kCheck;
+  const T *pu = static_cast<const T*>(s.u) + b * s.ub, *pd = static_cast<const T*>(s.dl) + b * s.dlb,
+          *pz = static_cast<const T*>(s.z) + b * s.zb, *pB = static_cast<const T*>(s.Bm) + b * s.Bb,
+          *pC = static_cast<const T*>(s.Cm) + b * s.Cb;
+  T* py = static_cast<T*>(s.y) + b * s.L * s.d;
+  const bool gate = s.z != nullptr;
   float A2[4][NPL], h[4][NPL];
   load_state<NPL>(s.A, s, p, A2, kLog2e);
-  load_state<NPL>(LOCAL ? nullptr : chunk ? s.carry + (b * (s.chunks - 1) + chunk - 1) * dN : s.h0 ? s.h0 + b * dN : nullptr,
-                  s, p, h);
+  if (!LOCAL && chunk) Own<NPL>::load(s.carry + (b * (s.chunks - 1) + chunk - 1) * s.own, p, h);
+  else load_state<NPL>(!LOCAL && s.h0 ? s.h0 + b * dN : nullptr, s, p, h);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
   float sum = 0.f;
-  float u[TT], dl[TT], z[TT];
+  T u[TT], dl[TT], z[TT];
   Shared<T, NPL, TT> mb, mc;
   auto load = [&](int64_t t) {
-    load_channel<T, TT>(s.u, s.ub, s.ut, b, t, t1, p, u);
-    load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
-    mb.load(s.Bm, s.Bb, s.Bt, b, t, t1, s.N, p.lane);
+    load_channel<T, TT>(pu, s.ut, t, t1, p, u);
+    load_channel<T, TT>(pd, s.dlt, t, t1, p, dl);
+    mb.load(pB, s.Bt, t, t1, s.N, p.lane);
     if (!LOCAL) {
-      if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
-      mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+      if (gate) load_channel<T, TT>(pz, s.zt, t, t1, p, z);
+      mc.load(pC, s.Ct, t, t1, s.N, p.lane);
     }
   };
   load(t0);
   for (int64_t t = t0; t < t1; t += TT) {
     wave_lds_fence();
-    float du[TT], g[TT];              // D u and the gate of this tile, u and z being loaded for the next
+    float delta[TT], du[TT], g[TT];   // du, g: D u and the gate of this tile, while u and z are loaded for the next
+    const int left = tokens_of<TT>(t, t1);
+    step_sizes<T, TT>(dl, bias, s.softplus != 0, delta);
+    if (left < TT)                    // past the chunk's end a delta of 0 leaves the state as it is
+#pragma unroll
+      for (int r = 0; r < TT; ++r)
+        if (r >= left) {
+          delta[r] = 0.f;
+          u[r] = (T)0.f;
+        }
 #pragma unroll
     for (int r = 0; r < TT; ++r) {
-      const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
-      sd[r * 64 + p.lane] = delta;
-      su[r * 64 + p.lane] = delta * u[r];
-      if (LOCAL && t + r < t1) sum += delta;
-      if (!LOCAL) {
-        du[r] = D * u[r];
-        g[r] = s.z ? z[r] * sigmoid(z[r]) : 1.f;
+      sd[r * 64 + p.lane] = delta[r];
+      su[r * 64 + p.lane] = delta[r] * (float)u[r];
+      if (LOCAL) {
+        sum += delta[r];
+      } else {
+        du[r] = D * (float)u[r];
+        g[r] = gate ? (float)z[r] * sigmoid((float)z[r]) : 1.f;
       }
     }
     mb.store(sB, p.lane);
     if (!LOCAL) mc.store(sC, p.lane);
     wave_lds_fence();
     if (t + TT < t1) load(t + TT);
-#pragma unroll
-    for (int r = 0; r < TT; ++r) {
-      if (t + r >= t1) continue;                  // uniform
-      if (!LOCAL && s.check && (r % kCheck) == 0) store_state<NPL>(s.check + (b * checks + (t + r) / kCheck) * dN, s, p, h);
+    const Rows<T> out(py + t * s.d, s.d, p);
+    auto step = [&](int r) {
+      if (!LOCAL && s.check && (r % kCheck) == 0 && r < left) Own<NPL>::store(s.check + (b * checks + (t + r) / kCheck) * s.own, p, h);
       float dt[4], x[4], B[NPL], C[NPL], y[4];
       lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
       lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
@@ -217,54 +316,48 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective(Selective s) {
         y[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-          h[i][j] = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2[i][j]), h[i][j], x[i] * B[j]);
+          h[i][j] = fmaf(decay(dt[i], A2[i][j]), h[i][j], x[i] * B[j]);
           if (!LOCAL) y[i] = fmaf(h[i][j], C[j], y[i]);
         }
       }
       if (!LOCAL) {
         const float v = (quad_scatter(y, p.lane) + du[r]) * g[r];
-        if (p.live) static_cast<T*>(s.y)[(b * s.L + t + r) * s.d + p.c] = (T)v;
+        if (r < left) out.store((T)v, r * out.step);
       }
-    }
+    };
+#pragma unroll
+    for (int r = 0; r < TT; ++r) step(r);
   }
   if (LOCAL) {
-    store_state<NPL>(s.carry + (b * (s.chunks - 1) + chunk) * dN, s, p, h);
+    Own<NPL>::store(s.carry + (b * (s.chunks - 1) + chunk) * s.own, p, h);
     if (p.live) s.total[(b * s.chunks + chunk) * s.d + p.c] = sum;
   } else if (s.hend && chunk == s.chunks - 1) {
     store_state<NPL>(s.hend + b * dN, s, p, h);
   }
 }
 
-// The chunks' start states, in place of their end states from zero: carry[j] = the state that chunk j + 1 starts from.
+// BACK false: the chunks' start states, in place of their end states from zero: carry[j] = the state that chunk j + 1 starts
+// from. BACK: carry[j] holds the gradient that chunk j + 1 passes to the state before it from a zero gradient at its end, and
+// becomes that of the state that chunk j ends in.
+template <int NPL, bool BACK>
 __global__ __launch_bounds__(256) void k_selective_carry(Selective s) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, dN = (int64_t)s.d * s.N;
-  if (i >= s.B * dN) return;
-  const int64_t b = i / dN, e = i % dN, c = e / s.N;
-  const float A2 = s.A[e] * kLog2e;
-  float h = s.h0 ? s.h0[b * dN + e] : 0.f;
-  float* x = s.carry + b * (s.chunks - 1) * dN + e;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= s.B * s.own) return;
+  const int64_t b = i / s.own, e = i % s.own;
+  int64_t c;
+  int n;
+  Own<NPL>::where(e, c, n);
+  if (c >= s.d || n >= s.N) return;               // stay 0
+  const float A2 = s.A[c * s.N + n] * kLog2e, *x0 = BACK ? s.ghend : s.h0;
+  float h = x0 ? x0[(b * s.d + c) * s.N + n] : 0.f;
+  float* x = s.carry + b * (s.chunks - 1) * s.own + e;
   const float* w = s.total + b * s.chunks * s.d + c;
-#pragma unroll 4
-  for (int j = 0; j < s.chunks - 1; ++j) {
-    h = fmaf(__builtin_amdgcn_exp2f(A2 * w[(int64_t)j * s.d]), h, x[j * dN]);
-    x[j * dN] = h;
-  }
-}
-
-// The backward's: carry[j] holds the gradient that chunk j + 1 passes to the state before it from a zero gradient at its
-// end, and becomes that of the state that chunk j ends in.
-__global__ __launch_bounds__(256) void k_selective_carry_bwd(Selective s) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, dN = (int64_t)s.d * s.N;
-  if (i >= s.B * dN) return;
-  const int64_t b = i / dN, e = i % dN, c = e / s.N;
-  const float A2 = s.A[e] * kLog2e;
-  float g = s.ghend ? s.ghend[b * dN + e] : 0.f;
-  float* x = s.carry + b * (s.chunks - 1) * dN + e;
-  const float* w = s.total + b * s.chunks * s.d + c;
-#pragma unroll 4
-  for (int j = s.chunks - 2; j >= 0; --j) {
-    g = fmaf(__builtin_amdgcn_exp2f(A2 * w[(int64_t)(j + 1) * s.d]), g, x[j * dN]);
-    x[j * dN] = g;
+  const int m = s.chunks - 1;
+#pragma unroll 8
+  for (int k = 0; k < m; ++k) {
+    const int64_t j = BACK ? m - 1 - k : k;
+    h = fmaf(decay(w[(BACK ? j + 1 : j) * s.d], A2), h, x[j * s.own]);
+    x[j * s.own] = h;
   }
 }
 
@@ -277,37 +370,52 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective_local_bwd(Selectiv
   const int64_t b = blockIdx.z, chunk = blockIdx.y + 1, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
   float* sd = lds[p.wave];
   float *sg = sd + TT * 64, *sC = sg + TT * 64;
-  const int64_t dN = (int64_t)s.d * s.N;
+  const T *pd = static_cast<const T*>(s.dl) + b * s.dlb, *pz = static_cast<const T*>(s.z) + b * s.zb,
+          *pC = static_cast<const T*>(s.Cm) + b * s.Cb, *pg = static_cast<const T*>(s.gy) + b * s.gb;
+  const bool gate = s.z != nullptr;
   float A2[4][NPL], g[4][NPL];
   load_state<NPL>(s.A, s, p, A2, kLog2e);
   load_state<NPL>(nullptr, s, p, g);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f;
   float sum = 0.f;
-  float gy[TT], dl[TT], z[TT];
+  T gy[TT], dl[TT], z[TT];
   Shared<T, NPL, TT> mc;
   auto load = [&](int64_t t) {
-    load_channel<T, TT>(s.gy, s.gb, s.gt, b, t, t1, p, gy);
-    load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
-    if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
-    mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+    load_channel<T, TT>(pg, s.gt, t, t1, p, gy);
+    load_channel<T, TT>(pd, s.dlt, t, t1, p, dl);
+    if (gate) load_channel<T, TT>(pz, s.zt, t, t1, p, z);
+    mc.load(pC, s.Ct, t, t1, s.N, p.lane);
   };
   int64_t t = t0 + (t1 - t0 - 1) / TT * TT;
   load(t);
   for (; t >= t0; t -= TT) {
     wave_lds_fence();
+    float delta[TT];
+    step_sizes<T, TT>(dl, bias, s.softplus != 0, delta);
+    const int left = tokens_of<TT>(t, t1);
+    if (left < TT)                    // past the chunk's end: no gradient, and a delta of 0 passes it on as it is
+#pragma unroll
+      for (int r = 0; r < TT; ++r)
+        if (r >= left) {
+          delta[r] = 0.f;
+          gy[r] = z[r] = (T)0.f;
+        }
 #pragma unroll
     for (int r = 0; r < TT; ++r) {
-      const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
-      sd[r * 64 + p.lane] = delta;
-      sg[r * 64 + p.lane] = s.z ? gy[r] * z[r] * sigmoid(z[r]) : gy[r];
-      if (t + r < t1) sum += delta;
+      sd[r * 64 + p.lane] = delta[r];
+      sum += delta[r];
+    }
+    if (gate) {
+#pragma unroll
+      for (int r = 0; r < TT; ++r) sg[r * 64 + p.lane] = (float)gy[r] * ((float)z[r] * sigmoid((float)z[r]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < TT; ++r) sg[r * 64 + p.lane] = (float)gy[r];
     }
     mc.store(sC, p.lane);
     wave_lds_fence();
     if (t > t0) load(t - TT);
-#pragma unroll
-    for (int r = TT - 1; r >= 0; --r) {
-      if (t + r >= t1) continue;                  // uniform
+    auto step = [&](int r) {
       float dt[4], x[4], C[NPL];
       lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
       lds_vec<4>(sg + r * 64 + (p.lane & ~3), x);
@@ -315,11 +423,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective_local_bwd(Selectiv
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-          g[i][j] = fmaf(x[i], C[j], g[i][j]) * __builtin_amdgcn_exp2f(dt[i] * A2[i][j]);
-    }
+        for (int j = 0; j < NPL; ++j) g[i][j] = fmaf(x[i], C[j], g[i][j]) * decay(dt[i], A2[i][j]);
+    };
+#pragma unroll
+    for (int r = TT - 1; r >= 0; --r) step(r);
   }
-  store_state<NPL>(s.carry + (b * (s.chunks - 1) + chunk - 1) * dN, s, p, g);
+  Own<NPL>::store(s.carry + (b * (s.chunks - 1) + chunk - 1) * s.own, p, g);
   if (p.live) s.total[(b * s.chunks + chunk) * s.d + p.c] = sum;
 }
 
@@ -332,48 +441,71 @@ template <typename T, int NPL>
 __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s) {
   constexpr int NP = 4 * NPL, TT = kCheck;
   constexpr int NJ = (NPL + 3) / 4;               // values of dB (and of dC) that a lane leaves of its row's sums
-  __shared__ float lds[kMaxWaves][TT * (192 + 2 * NP)];
+  __shared__ float lds[kMaxWaves][TT * (384 + 2 * NP)];
   __shared__ float red[TT][2][kMaxWaves * 4][NP];
   const Place p = place_of<NPL>(s);
   const int waves = blockDim.x >> 6;
   const int64_t b = blockIdx.z, chunk = blockIdx.y, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
   float* sd = lds[p.wave];
   float *su = sd + TT * 64, *sg = su + TT * 64, *sB = sg + TT * 64, *sC = sB + TT * NP;
+  float *lu = sC + TT * NP + p.lane, *ls = lu + TT * 64, *lz = ls + TT * 64;       // a lane's own
   const int64_t dN = (int64_t)s.d * s.N, checks = (s.L + kCheck - 1) / kCheck;
+  const T *pu = static_cast<const T*>(s.u) + b * s.ub, *pd = static_cast<const T*>(s.dl) + b * s.dlb,
+          *pz = static_cast<const T*>(s.z) + b * s.zb, *pB = static_cast<const T*>(s.Bm) + b * s.Bb,
+          *pC = static_cast<const T*>(s.Cm) + b * s.Cb, *pg = static_cast<const T*>(s.gy) + b * s.gb;
+  const bool gate = s.z != nullptr;
   float A2[4][NPL], dA[4][NPL], G[4][NPL];
   load_state<NPL>(s.A, s, p, A2, kLog2e);
   load_state<NPL>(nullptr, s, p, dA);
-  load_state<NPL>(chunk + 1 < s.chunks ? s.carry + (b * (s.chunks - 1) + chunk) * dN : s.ghend ? s.ghend + b * dN : nullptr, s, p,
-                  G);
+  if (chunk + 1 < s.chunks) Own<NPL>::load(s.carry + (b * (s.chunks - 1) + chunk) * s.own, p, G);
+  else load_state<NPL>(s.ghend ? s.ghend + b * dN : nullptr, s, p, G);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
   float dD = 0.f, dbias = 0.f;
   const int row = p.lane >> 4, cq = (p.lane >> 2) & 3;
   for (int64_t t = t0 + (t1 - t0 - 1) / TT * TT; t >= t0; t -= TT) {
+    const int left = tokens_of<TT>(t, t1);
     float h[TT + 1][4][NPL];
-    load_state<NPL>(s.check + (b * checks + t / kCheck) * dN, s, p, h[0]);
-    float u[TT], dl[TT], z[TT], gy[TT];
+    Own<NPL>::load(s.check + (b * checks + t / kCheck) * s.own, p, h[0]);
     {
+      T u[TT], dl[TT], z[TT], gy[TT];
       Shared<T, NPL, TT> mb, mc;
-      load_channel<T, TT>(s.u, s.ub, s.ut, b, t, t1, p, u);
-      load_channel<T, TT>(s.dl, s.dlb, s.dlt, b, t, t1, p, dl);
-      if (s.z) load_channel<T, TT>(s.z, s.zb, s.zt, b, t, t1, p, z);
-      load_channel<T, TT>(s.gy, s.gb, s.gt, b, t, t1, p, gy);
-      mb.load(s.Bm, s.Bb, s.Bt, b, t, t1, s.N, p.lane);
-      mc.load(s.Cm, s.Cb, s.Ct, b, t, t1, s.N, p.lane);
+      load_channel<T, TT>(pu, s.ut, t, t1, p, u);
+      load_channel<T, TT>(pd, s.dlt, t, t1, p, dl);
+      load_channel<T, TT>(pg, s.gt, t, t1, p, gy);
+      if (gate) load_channel<T, TT>(pz, s.zt, t, t1, p, z);
+      mb.load(pB, s.Bt, t, t1, s.N, p.lane);
+      mc.load(pC, s.Ct, t, t1, s.N, p.lane);
       wave_lds_fence();
+      float delta[TT];
+      step_sizes<T, TT>(dl, bias, s.softplus != 0, delta);
+#pragma unroll
+      for (int r = 0; r < TT; ++r) ls[r * 64] = s.softplus ? sigmoid((float)dl[r] + bias) : 1.f;
+      if (left < TT)                  // past the text's end: a delta of 0 leaves the state as it is, and no gradient enters a sum
+#pragma unroll
+        for (int r = 0; r < TT; ++r)
+          if (r >= left) {
+            delta[r] = ls[r * 64] = 0.f;
+            u[r] = gy[r] = z[r] = (T)0.f;
+          }
 #pragma unroll
       for (int r = 0; r < TT; ++r) {
-        const float x = dl[r] + bias, delta = s.softplus ? softplus(x) : x;
-        sd[r * 64 + p.lane] = delta;
-        su[r * 64 + p.lane] = delta * u[r];
-        sg[r * 64 + p.lane] = s.z ? gy[r] * z[r] * sigmoid(z[r]) : gy[r];
+        const float gf = (float)gy[r];
+        sd[r * 64 + p.lane] = delta[r];
+        su[r * 64 + p.lane] = delta[r] * (float)u[r];
+        lu[r * 64] = (float)u[r];
+        sg[r * 64 + p.lane] = gf;
+        if (gate) {
+          const float zf = (float)z[r], q = sigmoid(zf);
+          sg[r * 64 + p.lane] = gf * (zf * q);
+          lz[r * 64] = gf * (q * (1.f + zf * (1.f - q)));
+        }
       }
       mb.store(sB, p.lane);
       mc.store(sC, p.lane);
       wave_lds_fence();
     }
 #pragma unroll
-    for (int r = 0; r < TT; ++r) {                // past the text's end delta u is 0 and the state no longer matters
+    for (int r = 0; r < TT; ++r) {
       float dt[4], x[4], B[NPL];
       lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
       lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
@@ -381,12 +513,12 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-          h[r + 1][i][j] = fmaf(__builtin_amdgcn_exp2f(dt[i] * A2[i][j]), h[r][i][j], x[i] * B[j]);
+        for (int j = 0; j < NPL; ++j) h[r + 1][i][j] = fmaf(decay(dt[i], A2[i][j]), h[r][i][j], x[i] * B[j]);
     }
-#pragma unroll
-    for (int r = TT - 1; r >= 0; --r) {
-      if (t + r >= t1) continue;                  // uniform
+    wave_lds_fence();   // the values are read, and the decays formed, again: kept from above they would fill the registers
+    const int64_t o = (b * s.L + t) * s.d;
+    const Rows<T> odu(static_cast<T*>(s.du) + o, s.d, p), odl(static_cast<T*>(s.ddl) + o, s.d, p), odz(static_cast<T*>(s.dz) + o, s.d, p);
+    auto step = [&](int r) {
       float dt[4], x[4], g[4], B[NPL], C[NPL], y[4], dx[4], dd[4], dB[NPL], dC[NPL];
       lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
       lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
@@ -405,26 +537,21 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s
           dC[j] = fmaf(g[i], h[r + 1][i][j], dC[j]);
           dB[j] = fmaf(G1, x[i], dB[j]);
           dx[i] = fmaf(G1, B[j], dx[i]);
-          G[i][j] = G1 * __builtin_amdgcn_exp2f(dt[i] * A2[i][j]);
+          G[i][j] = G1 * decay(dt[i], A2[i][j]);
           const float w = G[i][j] * h[r][i][j];
           dd[i] = fmaf(w, A2[i][j], dd[i]);
           dA[i][j] = fmaf(w, dt[i], dA[i][j]);
         }
       }
       const float ys = quad_scatter(y, p.lane), ds = quad_scatter(dx, p.lane), dds = quad_scatter(dd, p.lane);
-      const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane];
-      float ddl = fmaf(dds, kLn2, ds * u[r]);
-      if (s.softplus) ddl *= sigmoid(dl[r] + bias);
+      const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane], uf = lu[r * 64];
+      const float ddl = fmaf(dds, kLn2, ds * uf) * ls[r * 64];
       dbias += ddl;
-      dD = fmaf(gg, u[r], dD);
-      if (p.live) {
-        const int64_t o = (b * s.L + t + r) * s.d + p.c;
-        static_cast<T*>(s.du)[o] = (T)fmaf(ds, delta, gg * D);
-        static_cast<T*>(s.ddl)[o] = (T)ddl;
-        if (s.z) {
-          const float q = sigmoid(z[r]);
-          static_cast<T*>(s.dz)[o] = (T)(gy[r] * fmaf(D, u[r], ys) * q * (1.f + z[r] * (1.f - q)));
-        }
+      dD = fmaf(gg, uf, dD);
+      if (r < left) {
+        odu.store((T)fmaf(ds, delta, gg * D), r * odu.step);
+        odl.store((T)ddl, r * odl.step);
+        if (gate) odz.store((T)(fmaf(D, uf, ys) * lz[r * 64]), r * odz.step);
       }
 #pragma unroll
       for (int j = 0; j < NPL; ++j) {             // over the row's quads
@@ -447,11 +574,14 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s
           red[r][1][p.wave * 4 + row][p.n0 + 4 * k + cq] = vc;
         }
       }
-    }
+      __builtin_amdgcn_sched_barrier(0);          // a step's LDS reads stay in it: the states leave few registers
+    };
+#pragma unroll
+    for (int r = TT - 1; r >= 0; --r) step(r);
     __syncthreads();
     for (int e = threadIdx.x; e < TT * 2 * s.N; e += blockDim.x) {
       const int r = e / (2 * s.N), k = e / s.N % 2, n = e % s.N;
-      if (t + r < t1) {
+      if (r < left) {
         float v = 0.f;
         for (int w = 0; w < 4 * waves; ++w) v += red[r][k][w][n];
         s.bc[((blockIdx.x * s.B + b) * s.L + t + r) * 2 * s.N + k * s.N + n] = v;
@@ -460,11 +590,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s
     __syncthreads();
   }
   float* part = s.part + (b * s.chunks + chunk) * (dN + 2 * s.d);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (p.q + i < s.d && p.n0 + j < s.N) part[(int64_t)(p.q + i) * s.N + p.n0 + j] = dA[i][j];
+  store_state<NPL>(part, s, p, dA);
   if (p.live) {
     part[dN + p.c] = dD;
     part[dN + s.d + p.c] = dbias;
@@ -492,15 +618,14 @@ __global__ __launch_bounds__(256) void k_selective_step(Selective s, const float
   const int ng = (int)(i & 3), c = (int)(q % s.d);
   const bool live = b < s.B;                      // whole quads: the exchange below stays within one
   const int64_t bb = live ? b : 0;
-  float dl = (float)static_cast<const T*>(s.dl)[bb * s.dlb + c] + (s.bias ? s.bias[c] : 0.f);
+  const float dl = (float)static_cast<const T*>(s.dl)[bb * s.dlb + c] + (s.bias ? s.bias[c] : 0.f);
   const float u = (float)static_cast<const T*>(s.u)[bb * s.ub + c], delta = s.softplus ? softplus(dl) : dl;
   const T *Bm = static_cast<const T*>(s.Bm) + bb * s.Bb, *Cm = static_cast<const T*>(s.Cm) + bb * s.Cb;
   const float* hr = h + (bb * s.d + c) * s.N;
   float* hw = next + (bb * s.d + c) * s.N;
   float y = 0.f;
   for (int n = ng; n < s.N; n += 4) {
-    const float a = __builtin_amdgcn_exp2f(delta * (s.A[(int64_t)c * s.N + n] * kLog2e));
-    const float x = fmaf(a, hr[n], delta * u * (float)Bm[n]);
+    const float x = fmaf(decay(delta, s.A[(int64_t)c * s.N + n] * kLog2e), hr[n], delta * u * (float)Bm[n]);
     if (live) hw[n] = x;
     y = fmaf(x, (float)Cm[n], y);
   }
@@ -546,6 +671,9 @@ static int check(const Selective& s, int32_t type, const char* what) {
   ASRN_REQUIRE(s.B >= 0 && s.L >= 0 && s.d >= 1 && s.d < (1 << 22) && s.N >= 1 && s.N <= 32,
                "%s: bad sizes B=%lld L=%lld d=%d N=%d (1 <= N <= 32)", what, (long long)s.B, (long long)s.L, s.d, s.N);
   ASRN_REQUIRE(s.B < 65536 && s.L < ((int64_t)1 << 30) && s.B * s.L < ((int64_t)1 << 36), "%s: too many tokens", what);
+  // a tile's tokens are addressed in 32 bits
+  for (int64_t st : {s.ut, s.dlt, s.zt, s.Bt, s.Ct, s.gt})
+    ASRN_REQUIRE(st >= 0 && st < (1 << 24), "%s: a token stride of %lld: below 2^24 is needed", what, (long long)st);
   return 0;
 }
 
@@ -556,15 +684,23 @@ static int with_states(int N, F&& f) {
   return f(std::integral_constant<int, 8>{});
 }
 
-static int64_t carry_bytes(int64_t B, int chunks, int64_t d, int64_t N) {
-  return chunks > 1 ? (B * ((chunks - 1) * d * N + chunks * d) * 4 + 255) / 256 * 256 : 0;
+// a state as the lanes of all workgroups hold it, the last ones' waves without channels among them
+static int64_t own_floats(int d, int N) {
+  int waves, blocks;
+  grid_of(d, waves, blocks);
+  return (int64_t)blocks * waves * 64 * (N <= 8 ? 8 : N <= 16 ? 16 : 32);
+}
+static int64_t carry_bytes(int64_t B, int chunks, int d, int N) {
+  return chunks > 1 ? (B * ((chunks - 1) * own_floats(d, N) + (int64_t)chunks * d) * 4 + 255) / 256 * 256 : 0;
 }
 
 }  // namespace asrn
 
 using namespace asrn;
 
-extern "C" int64_t asrn_selective_checks(int64_t L) { return L < 0 ? -1 : (L + kCheck - 1) / kCheck; }
+extern "C" int64_t asrn_selective_checks(int64_t B, int64_t L, int32_t d, int32_t N) {
+  return B < 0 || L < 0 || d < 1 || N < 1 || N > 32 ? -1 : B * ((L + kCheck - 1) / kCheck) * own_floats(d, N);
+}
 
 extern "C" int64_t asrn_selective_fwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N) {
   if (B < 0 || L < 0 || d < 1 || N < 1) return -1;
@@ -580,13 +716,16 @@ extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* 
   s.u = u; s.dl = delta; s.Bm = B_; s.Cm = C_; s.z = z;
   s.A = A; s.D = D; s.bias = bias; s.h0 = h0; s.y = y; s.hend = hend; s.check = checks;
   s.B = B; s.L = L; s.d = d; s.N = N; s.softplus = softplus;
+  if (strides) {
+    s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
+    s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9];
+  }
   if (check(s, type, "asrn_selective_fwd")) return 1;
   if (B == 0 || L == 0) return 0;
   ASRN_REQUIRE(u && delta && B_ && C_ && A && y && strides, "asrn_selective_fwd: null pointer");
-  s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
-  s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9];
   s.chunk = chunk_of(B, L, d);
   s.chunks = chunks_of(B, L, d);
+  s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_fwd: too many chunks");
   const int64_t need = carry_bytes(B, s.chunks, d, N);
   if (need) {
@@ -594,7 +733,7 @@ extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* 
                  "asrn_selective_fwd: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
                  (long long)workspace_bytes);
     s.carry = (float*)workspace;
-    s.total = s.carry + B * (s.chunks - 1) * (int64_t)d * N;
+    s.total = s.carry + B * (s.chunks - 1) * s.own;
   }
   int waves, blocks;
   grid_of(d, waves, blocks);
@@ -605,7 +744,7 @@ extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* 
       constexpr int NPL = decltype(npl)::value;
       if (s.chunks > 1) {
         hipLaunchKernelGGL((k_selective<T, NPL, true>), dim3(blocks, s.chunks - 1, B), dim3(64 * waves), 0, st, s);
-        hipLaunchKernelGGL(k_selective_carry, dim3((unsigned)((B * d * N + 255) / 256)), dim3(256), 0, st, s);
+        hipLaunchKernelGGL((k_selective_carry<NPL, false>), dim3((unsigned)((B * s.own + 255) / 256)), dim3(256), 0, st, s);
       }
       hipLaunchKernelGGL((k_selective<T, NPL, false>), dim3(blocks, s.chunks, B), dim3(64 * waves), 0, st, s);
       return check_launch("asrn_selective_fwd");
@@ -636,14 +775,17 @@ extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* 
   s.A = A; s.D = D; s.bias = bias; s.check = const_cast<float*>(checks); s.ghend = dhend;
   s.du = du; s.ddl = ddelta; s.dz = dz; s.dh0 = dh0;
   s.B = B; s.L = L; s.d = d; s.N = N; s.softplus = softplus;
+  if (strides) {
+    s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
+    s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9]; s.gb = strides[10]; s.gt = strides[11];
+  }
   if (check(s, type, "asrn_selective_bwd")) return 1;
   if (B == 0 || L == 0) return 0;
   ASRN_REQUIRE(u && delta && B_ && C_ && A && dy && checks && strides && du && ddelta && dB && dC && dparams && (!z || dz),
                "asrn_selective_bwd: null pointer");
-  s.ub = strides[0]; s.ut = strides[1]; s.dlb = strides[2]; s.dlt = strides[3]; s.Bb = strides[4]; s.Bt = strides[5];
-  s.Cb = strides[6]; s.Ct = strides[7]; s.zb = strides[8]; s.zt = strides[9]; s.gb = strides[10]; s.gt = strides[11];
   s.chunk = chunk_of(B, L, d);
   s.chunks = chunks_of(B, L, d);
+  s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_bwd: too many chunks");
   const int64_t need = asrn_selective_bwd_workspace(B, L, d, N), groups = B * s.chunks, cols = (int64_t)d * N + 2 * d;
   ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
@@ -651,7 +793,7 @@ extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* 
                (long long)workspace_bytes);
   ASRN_REQUIRE(groups < (1 << 30) && cols < (1 << 30), "asrn_selective_bwd: too many chunks");
   s.carry = (float*)workspace;
-  s.total = s.carry + B * (s.chunks - 1) * (int64_t)d * N;
+  s.total = s.carry + B * (s.chunks - 1) * s.own;
   s.bc = (float*)((char*)workspace + carry_bytes(B, s.chunks, d, N));
   s.part = s.bc + bc_floats(B, L, d, N);
   int waves, blocks;
@@ -663,7 +805,7 @@ extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* 
       constexpr int NPL = decltype(npl)::value;
       if (s.chunks > 1) {
         hipLaunchKernelGGL((k_selective_local_bwd<T, NPL>), dim3(blocks, s.chunks - 1, B), dim3(64 * waves), 0, st, s);
-        hipLaunchKernelGGL(k_selective_carry_bwd, dim3((unsigned)((B * d * N + 255) / 256)), dim3(256), 0, st, s);
+        hipLaunchKernelGGL((k_selective_carry<NPL, true>), dim3((unsigned)((B * s.own + 255) / 256)), dim3(256), 0, st, s);
       }
       hipLaunchKernelGGL((k_selective_bwd<T, NPL>), dim3(blocks, s.chunks, B), dim3(64 * waves), 0, st, s);
       hipLaunchKernelGGL((k_selective_shared<T>), dim3((unsigned)((B * L * 2 * N + 255) / 256)), dim3(256), 0, st, s.bc, blocks,

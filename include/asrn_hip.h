@@ -752,13 +752,13 @@ int asrn_channel_conv_step(const void* z, int32_t type, int64_t stride_b, const 
  * through strides (host array in elements: text and token stride of u, delta, B_, C_, z, and for the backward dy). A (d, N),
  * D, bias (d, or null) fp32; states (B, d, N) fp32 dense. D_t = softplus(delta + bias) (softplus 0: delta + bias),
  *   h_t = exp(D_t A) h_{t-1} + D_t u_t B_t,  y_t = (sum_n C_t h_t + D u_t) silu(z_t)   (without z: no gate)
- * from h0 (null: zeros). fwd: y (B, L, d) dense; hend (or null) the last state; checks (or null; B x
- * asrn_selective_checks(L) x d x N) the states that the backward starts from. bwd: dhend (or null) the last state's
+ * from h0 (null: zeros). fwd: y (B, L, d) dense; hend (or null) the last state; checks (or null;
+ * asrn_selective_checks floats, -1: bad sizes) the states that the backward starts from, in the kernels' own order. bwd: dhend (or null) the last state's
  * gradient; du, ddelta, dz (with z), dB, dC dense in the inputs' type; dparams = dA (d, N), then dD (d), then dbias (d); dh0
  * (or null). Sums in a fixed order. workspaces 16-byte aligned, of the stated sizes (-1: bad sizes). B L = 0 writes nothing.
  * step: one token; strides (host) = the rows' of u, delta, B_, C_, z; next (the same buffer, or another) gets the state.
- * Requires 1 <= N <= 32, d < 2^22, B < 2^16, L < 2^30, B L < 2^36. */
-int64_t asrn_selective_checks(int64_t L);
+ * Requires 1 <= N <= 32, d < 2^22, B < 2^16, L < 2^30, B L < 2^36, token strides below 2^24. */
+int64_t asrn_selective_checks(int64_t B, int64_t L, int32_t d, int32_t N);
 int64_t asrn_selective_fwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N);
 int asrn_selective_fwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z, int32_t type,
                        const int64_t* strides, const float* A, const float* D, const float* bias, const float* h0, int64_t B,

@@ -103,7 +103,8 @@ def test_entries_refuse(lib):
     falla(sel(B=1 << 16), 'too many')
     falla(sel(), 'null')
     assert sel(B=0) == 0 and sel(L=0) == 0
-    assert lib.asrn_selective_checks(17) == 3 and lib.asrn_selective_checks(0) == 0
+    # 5 waves of 64 channels are 2 workgroups of 3
+    assert lib.asrn_selective_checks(2, 17, 300, 9) == 2 * 3 * 6 * 64 * 16 and lib.asrn_selective_checks(2, 0, 8, 4) == 0
     assert lib.asrn_selective_fwd_workspace(0, 5, 8, 4) == 0 and lib.asrn_selective_fwd_workspace(2, 5, 0, 4) == -1
     # 12 waves fill 1/170 of the card: a long text is cut, and its chunks' states need room
     assert lib.asrn_selective_fwd_workspace(1, 1 << 15, 768, 16) > 0
