@@ -10,7 +10,7 @@ The public names mirror the reference package (KIROKOWA/ASRN, asrn/__init__.py:4
   - fine-tuning losses: log_probabilidades / token_log_probs, perdida_preferencia / preference_loss,
     perdida_politica / policy_loss;
   - a local block's operators with a state a channel: conv_canal / channel_conv, paso_conv_canal / channel_conv_step,
-    escaneo_selectivo / selective_scan, paso_selectivo / selective_step;
+    escaneo_selectivo / selective_scan, paso_selectivo / selective_step, lineal_activa / linear_act;
   - files: guardar / save, cargar / load (the reference's format, v83 on);
   - generation: escribir / generate (the loop on the device), EscritorModelo / ModelWriter (the model's O(1) step),
     EscritorCapa / LayerWriter (one layer's);
@@ -29,6 +29,7 @@ from .entrenamiento import (MULT_SUFIJO_Y_PUERTA, PESOS_SUFIJO_Y_PUERTA, PasoGra
                             evaluar, tasa_aprendizaje)
 from .escritura import EscritorCapa, LayerWriter
 from .generacion import EscritorModelo, escribir
+from .lineal import lineal_activa, linear_act
 from .modelo import TALLAS, BloqueLocal, ConfigASRN, ModeloASRN, crear_desde_config, crear_modelo
 from .ops import escaneo
 from .selectiva import (channel_conv, channel_conv_step, conv_canal, escaneo_selectivo, paso_conv_canal, paso_selectivo,
@@ -49,4 +50,4 @@ __all__ = ['ASRNLayer', 'CapaASRNEstable', 'ASRNCoreLayer', 'CapaASRN', 'Protecc
            'cargar', 'load', 'escribir', 'generate', 'EscritorModelo', 'ModelWriter', 'EscritorCapa', 'LayerWriter',
            'log_probabilidades', 'token_log_probs', 'perdida_preferencia', 'preference_loss', 'perdida_politica',
            'policy_loss', 'conv_canal', 'channel_conv', 'paso_conv_canal', 'channel_conv_step', 'escaneo_selectivo',
-           'selective_scan', 'paso_selectivo', 'selective_step', 'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']
+           'selective_scan', 'paso_selectivo', 'selective_step', 'lineal_activa', 'linear_act', 'MULT_SUFIJO_Y_PUERTA', 'PESOS_SUFIJO_Y_PUERTA', 'ops', 'cargar_biblioteca', 'load_library', 'LIB_PATH', 'ASRNHipError', '__version__']

@@ -34,7 +34,7 @@
 // Products with few tiles (weight gradients: K is the token axis) are cut along K: partial products in a workspace,
 // summed in order by a second launch. No atomics: the result is a function of the sizes alone.
 // The weight gradient's bias gradient, the column sums of A (TA), is summed from the values a tile loads anyway.
-#include "common.h"
+#include "linear_act.h"
 
 namespace asrn {
 
@@ -212,8 +212,9 @@ struct Operand {
 template <int BM, int BN, bool F32>
 constexpr int step_k() { return !F32 || BM + BN == 128 ? 64 : 32; }
 
-template <int BM, int BN, bool TA, bool TB, bool F32>
-__global__ __launch_bounds__(kGemmThr, 2) void k_gemm(Gemm g) {
+// EPI: the results go through e instead of to C (and bias)
+template <int BM, int BN, bool TA, bool TB, bool F32, bool EPI = false>
+__global__ __launch_bounds__(kGemmThr, 2) void k_gemm(Gemm g, Epilogue ep) {
   constexpr int BK = step_k<BM, BN, F32>();
   using OA = Operand<BM, TA, F32, BK>;
   using OB = Operand<BN, TB, F32, BK>;
@@ -323,6 +324,10 @@ __global__ __launch_bounds__(kGemmThr, 2) void k_gemm(Gemm g) {
           if (F32 && !(fabsf(v) < INFINITY)) {
             bad |= 1ull << ((i * NI + j) * 16 + e);
           } else {
+            if (EPI && last) {
+              ep.one<float>(m, n, v);
+              continue;
+            }
             float* o = out + (int64_t)m * ldo + n;
             if (last) v += bias;
             if (last && g.accumulate) v += *o;
@@ -384,6 +389,10 @@ __global__ __launch_bounds__(kGemmThr, 2) void k_gemm(Gemm g) {
           for (int e = 0; e < 16; ++e) {
             if (!(bad >> ((i * NI + j) * 16 + e) & 1)) continue;     // inside the matrix, and not stored above
             const int m = m0 + wm + 32 * i + 8 * (e >> 2) + 4 * lc + (e & 3);
+            if (EPI && last) {
+              ep.one<float>(m, n, acc[i][j][e]);
+              continue;
+            }
             float* o = out + (int64_t)m * ldo + n;
             float v = acc[i][j][e] + bias;
             if (last && g.accumulate) v += *o;
@@ -550,7 +559,8 @@ __global__ __launch_bounds__(kWideThr, 2) void k_gemm_wide(Gemm g) {
 // C (+)= the sum of the partial products in split order (+ bias), and the column sums behind them. A workgroup takes
 // 32 float4 columns by 8 lanes of splits; the lanes combine in order.
 constexpr int kSumCols = 32, kSumLanes = kGemmThr / kSumCols;
-__global__ __launch_bounds__(kGemmThr) void k_gemm_sum(Gemm g) {
+template <bool EPI = false>
+__global__ __launch_bounds__(kGemmThr) void k_gemm_sum(Gemm g, Epilogue ep) {
   __shared__ float4 red[kSumLanes][kSumCols];
   const int cl = threadIdx.x % kSumCols, sl = threadIdx.x / kSumCols;
   const int64_t c = ((int64_t)blockIdx.x * kSumCols + cl) * 4, mn = (int64_t)g.M * g.N;
@@ -584,6 +594,20 @@ __global__ __launch_bounds__(kGemmThr) void k_gemm_sum(Gemm g) {
     *reinterpret_cast<float4*>(g.colsum + (c - mn)) = s;
     return;
   }
+  if constexpr (EPI) {                            // any N: four results may lie in two rows
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    int64_t m = c / g.N;
+    int n = (int)(c - m * g.N);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c + k < mn) ep.one<float>(m, n, v[k]);
+      if (++n == g.N) {
+        n = 0;
+        ++m;
+      }
+    }
+    return;
+  }
   const int64_t m = c / g.N, n = c - m * g.N;
   float* o = g.C + m * g.ldc + n;
   if (g.bias) { s.x += g.bias[n]; s.y += g.bias[n + 1]; s.z += g.bias[n + 2]; s.w += g.bias[n + 3]; }
@@ -595,7 +619,8 @@ __global__ __launch_bounds__(kGemmThr) void k_gemm_sum(Gemm g) {
 }
 
 // The tail tiles: C (+)= the sum of their slabs in order (+ bias), one float4 a thread.
-__global__ __launch_bounds__(kGemmThr) void k_gemm_tail(Gemm g, int bm, int bn) {
+template <bool EPI = false>
+__global__ __launch_bounds__(kGemmThr) void k_gemm_tail(Gemm g, int bm, int bn, Epilogue ep) {
   const int e = ((int)blockIdx.x * kGemmThr + (int)threadIdx.x) * 4, size = bm * bn, tl = e / size, r = e - tl * size;
   if (tl >= g.tail) return;
   const int tile = g.tm * g.tn - g.tail + tl, m = tile / g.tn * bm + r / bn, n = tile % g.tn * bn + r % bn;
@@ -607,6 +632,13 @@ __global__ __launch_bounds__(kGemmThr) void k_gemm_tail(Gemm g, int bm, int bn) 
   for (int z = 0; z < g.tsplits; ++z) {
     const float4 v = *reinterpret_cast<const float4*>(p + z * stride);
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  if constexpr (EPI) {
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < g.N) ep.one<float>(m, n + k, v[k]);
+    return;
   }
   float* o = g.C + (int64_t)m * g.ldc + n;
   if (g.bias) { s.x += g.bias[n]; s.y += g.bias[n + 1]; s.z += g.bias[n + 2]; s.w += g.bias[n + 3]; }
@@ -683,12 +715,47 @@ static Plan plan_of(int64_t M, int64_t N, int64_t K, bool f32, int tile, int spl
 template <int BM, int BN, bool F32>
 static void launch_tile(bool ta, bool tb, const Gemm& g, unsigned grid, hipStream_t st) {
   if constexpr (!F32) {
-    hipLaunchKernelGGL((k_gemm<BM, BN, true, true, false>), dim3(grid), dim3(kGemmThr), 0, st, g);
+    hipLaunchKernelGGL((k_gemm<BM, BN, true, true, false>), dim3(grid), dim3(kGemmThr), 0, st, g, Epilogue{});
   } else {
-    if (ta && tb) hipLaunchKernelGGL((k_gemm<BM, BN, true, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g);
-    else if (tb) hipLaunchKernelGGL((k_gemm<BM, BN, false, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<BM, BN, false, false, true>), dim3(grid), dim3(kGemmThr), 0, st, g);
+    if (ta && tb) hipLaunchKernelGGL((k_gemm<BM, BN, true, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g, Epilogue{});
+    else if (tb) hipLaunchKernelGGL((k_gemm<BM, BN, false, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g, Epilogue{});
+    else hipLaunchKernelGGL((k_gemm<BM, BN, false, false, true>), dim3(grid), dim3(kGemmThr), 0, st, g, Epilogue{});
   }
+}
+
+int64_t gemm_epilogue_workspace(int64_t M, int64_t N, int64_t K) {
+  const Plan p = plan_of(M, N, K, true, 0, 0);
+  return p.splits > 1 ? p.splits * ((M * N + 3) / 4 * 4) * 4 : (int64_t)p.tail * p.tsplits * p.bm * p.bn * 4;
+}
+
+// asrn_gemm's plan for x W^T, whose results leave through the epilogue
+int gemm_epilogue(const float* x, int64_t ldx, const float* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e,
+                  void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  const char* what = "asrn_linear_act_fwd";
+  ASRN_REQUIRE(K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0,
+               "%s: fp32 operands of more than a few rows must be 16-byte aligned, K and their leading dimensions multiples of 4 "
+               "(K=%lld ldx=%lld ldw=%lld)", what, (long long)K, (long long)ldx, (long long)ldw);
+  const Plan p = plan_of(M, N, K, true, 0, 0);
+  Gemm g = {x, ldx, w, ldw, nullptr, 0, (int)M, (int)N, (int)K, nullptr, 0, nullptr, (float*)workspace, (M * N + 3) / 4 * 4,
+            p.splits, p.kper, (int)((M + p.bm - 1) / p.bm), (int)((N + p.bn - 1) / p.bn), p.tail, p.tsplits, p.tkper};
+  const int64_t total = (int64_t)g.tm * g.tn * g.splits, slabs = (int64_t)p.tail * p.tsplits;
+  ASRN_REQUIRE(total < (1 << 30), "%s: too many tiles", what);
+  const int64_t need = gemm_epilogue_workspace(M, N, K);
+  ASRN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+               "%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", what, (long long)need, (long long)workspace_bytes);
+  auto blocks = [](int64_t n) { return (n + kXcdCount - 1) / kXcdCount * kXcdCount; };
+  const unsigned grid = (unsigned)(blocks(total - p.tail) + blocks(slabs));
+  if (p.bm == 128)
+    hipLaunchKernelGGL((k_gemm<128, 128, false, false, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g, e);
+  else
+    hipLaunchKernelGGL((k_gemm<64, 64, false, false, true, true>), dim3(grid), dim3(kGemmThr), 0, st, g, e);
+  if (p.tail)
+    hipLaunchKernelGGL(k_gemm_tail<true>, dim3((unsigned)(p.tail * (p.bm * p.bn / 4 / kGemmThr))), dim3(kGemmThr), 0, st, g, p.bm,
+                       p.bn, e);
+  else if (p.splits > 1)
+    hipLaunchKernelGGL(k_gemm_sum<true>, dim3((unsigned)((g.pstride + 4 * kSumCols - 1) / (4 * kSumCols))), dim3(kGemmThr), 0, st,
+                       g, e);
+  return check_launch(what);
 }
 
 }  // namespace asrn
@@ -760,12 +827,12 @@ extern "C" int asrn_gemm(const void* A, int64_t lda, int32_t trans_a, const void
   }
   int rc = check_launch("asrn_gemm");
   if (rc == 0 && p.tail) {
-    hipLaunchKernelGGL(k_gemm_tail, dim3((unsigned)(p.tail * (p.bm * p.bn / 4 / kGemmThr))), dim3(kGemmThr), 0, st, g, p.bm,
-                       p.bn);
+    hipLaunchKernelGGL(k_gemm_tail<>, dim3((unsigned)(p.tail * (p.bm * p.bn / 4 / kGemmThr))), dim3(kGemmThr), 0, st, g, p.bm,
+                       p.bn, Epilogue{});
     return check_launch("asrn_gemm");
   }
   if (rc || p.splits == 1) return rc;
   const int64_t cols = (g.pstride + 4 * kSumCols - 1) / (4 * kSumCols);
-  hipLaunchKernelGGL(k_gemm_sum, dim3((unsigned)cols), dim3(kGemmThr), 0, st, g);
+  hipLaunchKernelGGL(k_gemm_sum<>, dim3((unsigned)cols), dim3(kGemmThr), 0, st, g, Epilogue{});
   return check_launch("asrn_gemm");
 }

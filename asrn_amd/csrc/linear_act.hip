@@ -1,0 +1,444 @@
+// A product with its epilogue: y = [res +] act(x W^T + bias), x (M, K), W (N, K), and the gradient before the activation.
+//
+// 16-bit operands run on the matrix cores (k_linear): a workgroup forms a BM x BN tile in steps of 64 k. The operands come in
+// 16-byte units of 8 k, go through registers one step ahead and lie in LDS as units whose column is exchanged by the
+// row's number, so that 8 lanes that read neighbouring rows use all banks. The matrix instruction's rows are W's, in an order
+// that leaves a lane with 16 neighbouring columns of one row of y: the epilogue reads and writes whole vectors from the
+// accumulators, with no pass through LDS. Sums are fp32; the activation's input (kept in the operands' type for the backward)
+// and y are rounded once each.
+// Few rows (k_linear_rows, one token of a few texts) read W once: see there. fp32 operands run on asrn_gemm's kernel, with
+// this epilogue.
+#include "linear_act.h"
+
+namespace asrn {
+
+typedef float fx16 __attribute__((ext_vector_type(16)));
+typedef bf16_t bfx8 __attribute__((ext_vector_type(8)));
+typedef fp16_t hx8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ fx16 mfma32(bfx8 a, bfx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ fx16 mfma32(hx8 a, hx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+struct Linear {
+  const void* x; int64_t ldx; const void* w; int64_t ldw;
+  int M, N, K;
+  Epilogue e;
+  int tm, tn;
+};
+
+// GELU for results of 16 bits: Phi(-|x|) = t p(t) exp(-x^2 / 2) with Abramowitz and Stegun's 7.1.26, erfc within 1.5e-7, one
+// exponential and one reciprocal (erff costs about twice the instructions, and the epilogue counts beside the product)
+__device__ __forceinline__ float gelu16(float x) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
+  const float z = x * 0.84932180028801904f;                        // sqrt(log2(e) / 2)
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                                   0.5f * -0.284496736f), 0.5f * 0.254829592f);
+  return fmaf(-fabsf(fminf(x, 64.f)), p * __builtin_amdgcn_exp2f(-z * z), fmaxf(x, 0.f));     // infinity stays itself
+}
+
+// V neighbouring results v of row m from column n on; whole: they lie in the matrix, and vectors of 4 in every operand
+template <typename T, int V, bool SHORT>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int N, float (&v)[V], bool whole) {
+  if (!whole) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (n + k < N) e.template one<T>(m, n + k, v[k]);
+    return;
+  }
+  if (e.bias) {
+    float b[4];
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      load_v<4>(static_cast<const T*>(e.bias) + n + k, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k + i] += b[i];
+    }
+  }
+  if (e.pre) store_v<V>(static_cast<T*>(e.pre) + m * e.ldp + n, v);
+  if (e.act == kActGelu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = SHORT ? gelu16(v[k]) : activate(v[k], kActGelu);
+  } else if (e.act == kActSilu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = activate(v[k], kActSilu);
+  }
+  if (e.res) {
+    float b[4];
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      if (e.res32) load_v<4>(static_cast<const float*>(e.res) + m * e.ldr + n + k, b);
+      else load_v<4>(static_cast<const T*>(e.res) + m * e.ldr + n + k, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k + i] += b[i];
+    }
+  }
+  if (e.y32) {
+    float* y = static_cast<float*>(e.y) + m * e.ldy + n;
+#pragma unroll
+    for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(y + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+  } else {
+    store_v<V>(static_cast<T*>(e.y) + m * e.ldy + n, v);
+  }
+}
+
+// An operand's share of a step: R rows by 64 k, units of 8 k; a thread loads U units, 8 neighbouring threads a row's 128 bytes.
+// VEC: the units are 16 bytes on their boundary (8 divides K and the row stride); else element by element.
+constexpr unsigned kPast = 1u << 31;
+template <typename T, int R, int THR, bool VEC>
+struct Units {
+  static constexpr int U = R * 8 / THR;
+  static_assert(R * 8 % THR == 0 && THR % 8 == 0, "whole units");
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned at[U], c;              // byte offsets of the rows; the thread's column of units
+  uint4 v[U];
+  // rows past the matrix repeat its last one: their results are not stored
+  __device__ __forceinline__ void start(const void* X, int64_t ld, int r0, int rows, int tid) {
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(X) + r0 * ld), 0, kPast, 0x00027000);
+    c = tid % 8;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = (tid + THR * i) / 8;
+      at[i] = (unsigned)((r0 + r < rows ? r : rows - 1 - r0) * ld + 8 * c) * (unsigned)sizeof(T);
+    }
+  }
+  // k past K reads as 0
+  __device__ __forceinline__ void load(int k0, int K) {
+    const unsigned off = (unsigned)k0 * (unsigned)sizeof(T);
+    if constexpr (VEC) {
+      const bool in = k0 + 8 * (int)c < K;
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at[i] : kPast, off, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        unsigned q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          q[j] = __builtin_amdgcn_raw_buffer_load_b16(rsrc, k0 + 8 * (int)c + j < K ? at[i] + 2 * j : kPast, off, 0);
+        v[i] = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
+      }
+    }
+  }
+  template <typename KEY>
+  __device__ __forceinline__ void store(uint4* lds, int tid, KEY key) const {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = (tid + THR * i) / 8;
+      lds[r * 8 + (c ^ key(r))] = v[i];
+    }
+  }
+};
+
+// the units' exchange: 8 rows that a quarter of a wave reads at once have 8 keys. x's rows are read in order, W's in the
+// order of w_row: lanes 0-3 and 4-7 read rows 4 q + r and 16 + 4 q + r
+__device__ __forceinline__ int x_key(int r) { return r & 7; }
+__device__ __forceinline__ int w_key(int r) { return (r & 3) | (r >> 2 & 4); }
+__device__ __forceinline__ int w_row(int i) { return (i >> 2 & 1) * 16 + (i >> 3) * 4 + (i & 3); }
+
+template <typename T, int BM, int BN, int WM, int WN, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear(Linear g) {
+  constexpr int THR = 64 * WM * WN, BK = 64, MI = BM / WM / 32, NI = BN / WN / 32;
+  typedef T TX8 __attribute__((ext_vector_type(8)));
+  __shared__ uint4 lds[2][(BM + BN) * 8];
+  // XCD i takes a contiguous range of tiles, n fastest: tiles that share rows of x share its L2
+  const int total = g.tm * g.tn, per = (total + kXcdCount - 1) / kXcdCount;
+  const int tile = (int)(blockIdx.x % kXcdCount) * per + (int)(blockIdx.x / kXcdCount);
+  if (tile >= total || (int)(blockIdx.x / kXcdCount) >= per) return;
+  const int m0 = tile / g.tn * BM, n0 = tile % g.tn * BN;
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, lr = lane & 31, lc = lane >> 5;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN), wr = w_row(lr);
+  Units<T, BM, THR, VEC> ux;
+  Units<T, BN, THR, VEC> uw;
+  ux.start(g.x, g.ldx, m0, g.M, tid);
+  uw.start(g.w, g.ldw, n0, g.N, tid);
+  fx16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  ux.load(0, g.K);
+  uw.load(0, g.K);
+  int buf = 0;
+  for (int k = 0; k < g.K; k += BK, buf ^= 1) {
+    uint4 *lx = lds[buf], *lw = lx + BM * 8;
+    ux.store(lx, tid, x_key);                     // read two steps ago: the last barrier lies between
+    uw.store(lw, tid, w_key);
+    __syncthreads();
+    if (k + BK < g.K) {
+      ux.load(k + BK, g.K);                       // in flight under this step's products
+      uw.load(k + BK, g.K);
+    }
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      TX8 fx[MI], fw[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = wm + 32 * i + lr;
+        fx[i] = __builtin_bit_cast(TX8, lx[r * 8 + ((2 * kk + lc) ^ x_key(r))]);
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int r = wn + 32 * j + wr;
+        fw[j] = __builtin_bit_cast(TX8, lw[r * 8 + ((2 * kk + lc) ^ w_key(r))]);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = mfma32(fw[j], fx[i], acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = m0 + wm + 32 * i + lr;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + wn + 32 * j + 16 * lc;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+      if (m < g.M) {
+        if (g.e.y32) finish<T, 16, false>(g.e, m, n, g.N, v, g.e.vec && n + 16 <= g.N);
+        else finish<T, 16, true>(g.e, m, n, g.N, v, g.e.vec && n + 16 <= g.N);
+      }
+    }
+  }
+}
+
+// Few rows (M <= 16): W is read once and each of its values meets every row, so the weights' bytes bound it. A wave takes 4
+// rows of W (columns of y) and all rows of x; its lanes run along k in units of 4, each with 4 x MR sums, which then
+// meet by a transposing exchange. x comes from the caches.
+template <typename T, int MR, bool VEC>
+__global__ __launch_bounds__(256) void k_linear_rows(Linear g) {
+  constexpr int NR = 4, UN = sizeof(T) == 4 ? 4 : 8;
+  __shared__ float red[4][64];
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  // the workgroup's 4 waves share 4 columns and cut k
+  const int n0 = blockIdx.x * NR, m0 = blockIdx.y * MR;
+  float acc[NR][MR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[n][m] = 0.f;
+  const T *x = static_cast<const T*>(g.x), *w = static_cast<const T*>(g.w);
+  for (int k = (wave * 64 + lane) * UN; k < g.K; k += 256 * UN) {
+    float a[NR][UN];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const T* p = w + (int64_t)(n0 + n < g.N ? n0 + n : g.N - 1) * g.ldw + k;
+      if constexpr (VEC) {
+        load_v<UN>(p, a[n]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < UN; ++j) a[n][j] = k + j < g.K ? (float)p[j] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const T* p = x + (int64_t)(m0 + m < g.M ? m0 + m : g.M - 1) * g.ldx + k;
+      float b[UN];
+      if constexpr (VEC) {
+        load_v<UN>(p, b);
+      } else {
+#pragma unroll
+        for (int j = 0; j < UN; ++j) b[j] = k + j < g.K ? (float)p[j] : 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int j = 0; j < UN; ++j) acc[n][m] = fmaf(a[n][j], b[j], acc[n][m]);
+    }
+  }
+  // sums over the lanes, one value at a time; lane n MR + m keeps its own
+  float mine = 0.f;
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const float v = wave_sum(acc[n][m]);
+      if (lane == n * MR + m) mine = v;
+    }
+  red[wave][lane] = mine;
+  __syncthreads();
+  if (wave == 0 && lane < NR * MR) {
+    const int n = n0 + lane / MR, m = m0 + lane % MR;
+    if (n < g.N && m < g.M) {
+      const float v = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+      g.e.template one<T>(m, n, v);
+    }
+  }
+}
+
+// The gradient before the activation, gp = gy act'(pre), and its column sums (the bias gradient) from the unrounded values:
+// 64 lanes of V columns by 4 rows a workgroup, a slab of rows each.
+template <typename T, typename G, int V>
+__global__ __launch_bounds__(256) void k_act_grad(const G* gy, int64_t ldg, const T* pre, int64_t ldp, int act, int64_t M, int N,
+                                                  int64_t slab, T* gp, float* part) {
+  __shared__ float red[4][64 * V];
+  const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6;
+  const int c = (blockIdx.x * 64 + cl) * V;
+  const int64_t r0 = blockIdx.y * slab, r1 = r0 + slab < M ? r0 + slab : M;
+  float s[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = 0.f;
+  if (c < N) {
+    for (int64_t r = r0 + rl; r < r1; r += 4) {
+      float g[V], p[V];
+      load_v<V>(gy + r * ldg + c, g);
+      if (act != kActNone) load_v<V>(pre + r * ldp + c, p);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (act != kActNone) g[v] *= activate_grad(p[v], act);
+        s[v] += g[v];
+      }
+      if (gp) store_v<V>(gp + r * N + c, g);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) red[rl][cl * V + v] = s[v];
+  __syncthreads();
+  if (rl == 0 && c < N && part) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = cl * V + v;
+      part[blockIdx.y * (int64_t)N + c + v] = ((red[0][i] + red[1][i]) + red[2][i]) + red[3][i];
+    }
+  }
+}
+
+template <typename T, bool VEC>
+static int launch_rows(const Linear& g, hipStream_t st) {
+  const unsigned gx = (unsigned)((g.N + 3) / 4);
+  if (g.M <= 4)
+    hipLaunchKernelGGL((k_linear_rows<T, 4, VEC>), dim3(gx, (g.M + 3) / 4), dim3(256), 0, st, g);
+  else if (g.M <= 8)
+    hipLaunchKernelGGL((k_linear_rows<T, 8, VEC>), dim3(gx, (g.M + 7) / 8), dim3(256), 0, st, g);
+  else
+    hipLaunchKernelGGL((k_linear_rows<T, 16, VEC>), dim3(gx, (g.M + 15) / 16), dim3(256), 0, st, g);
+  return check_launch("asrn_linear_act_fwd");
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+static int launch_tiles(Linear g, bool vec, hipStream_t st) {
+  g.tm = (g.M + BM - 1) / BM;
+  g.tn = (g.N + BN - 1) / BN;
+  const int64_t tiles = (int64_t)g.tm * g.tn;
+  ASRN_REQUIRE(tiles < (1 << 30), "asrn_linear_act_fwd: too many tiles");
+  const unsigned grid = (unsigned)((tiles + kXcdCount - 1) / kXcdCount * kXcdCount);
+  if (vec) hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, true>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
+  else hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, false>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
+  return check_launch("asrn_linear_act_fwd");
+}
+
+constexpr int kFewRows = 16;
+
+}  // namespace asrn
+
+using namespace asrn;
+
+static bool aligned(const void* p, int64_t ld, int bytes, int values) {
+  return ((uintptr_t)p % (uintptr_t)(bytes * values)) == 0 && ld % values == 0;
+}
+
+extern "C" int64_t asrn_linear_act_workspace(int64_t M, int64_t N, int64_t K, int32_t type) {
+  if (M < 0 || N < 0 || K < 1 || !type_ok(type)) return -1;
+  return type == 0 && M > kFewRows && N > 0 ? gemm_epilogue_workspace(M, N, K) : 0;
+}
+
+extern "C" int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t type, const void* bias,
+                                   int64_t M, int64_t N, int64_t K, int32_t act, const void* res, int64_t ldr, int32_t res_fp32,
+                                   void* pre, int64_t ldp, void* y, int64_t ldy, int32_t y_fp32, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  const char* what = "asrn_linear_act_fwd";
+  ASRN_REQUIRE(type_ok(type), "%s: type %d", what, type);
+  ASRN_REQUIRE(M >= 0 && N >= 0 && K >= 1 && M < (1 << 30) && N < (1 << 30) && K < (1 << 30) && act >= 0 && act <= 2,
+               "%s: bad sizes M=%lld N=%lld K=%lld act=%d", what, (long long)M, (long long)N, (long long)K, act);
+  if (M == 0 || N == 0) return 0;
+  ASRN_REQUIRE(x && w && y, "%s: null pointer", what);
+  ASRN_REQUIRE(ldx >= K && ldw >= K && ldy >= N && (!res || ldr >= N) && (!pre || ldp >= N) && ldx < (1 << 21) && ldw < (1 << 21),
+               "%s: leading dimensions must hold a row and x's and W's be below 2^21 (ldx=%lld ldw=%lld ldy=%lld)", what,
+               (long long)ldx, (long long)ldw, (long long)ldy);
+  const int b = type_bytes(type), by = y_fp32 ? 4 : b, br = res_fp32 ? 4 : b;
+  Linear g = {x, ldx, w, ldw, (int)M, (int)N, (int)K, {}, 0, 0};
+  g.e = {bias, res, ldr, pre, ldp, y, ldy, act, res_fp32, y_fp32, 0};
+  // vectors of the epilogue: 16 results of the operands' type, 4 of fp32 and of what it reads
+  g.e.vec = (!bias || aligned(bias, 4, b, 4)) && (!res || aligned(res, ldr, br, 4)) && (!pre || aligned(pre, ldp, b, 16)) &&
+            aligned(y, ldy, by, y_fp32 ? 4 : 16);
+  hipStream_t st = (hipStream_t)stream;
+  if (M <= kFewRows)
+    return with_type(type, [&](auto t) {
+      using T = decltype(t);
+      constexpr int un = sizeof(T) == 4 ? 4 : 8;
+      const bool vec = K % un == 0 && aligned(x, ldx, b, un) && aligned(w, ldw, b, un);
+      return vec ? launch_rows<T, true>(g, st) : launch_rows<T, false>(g, st);
+    });
+  if (type == 0) return gemm_epilogue((const float*)x, ldx, (const float*)w, ldw, M, N, K, g.e, workspace, workspace_bytes, st);
+  const bool vec = K % 8 == 0 && aligned(x, ldx, 2, 8) && aligned(w, ldw, 2, 8);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128);
+    if (t128 >= 256) return launch_tiles<T, 128, 128, 2, 2>(g, vec, st);
+    return launch_tiles<T, 64, 64, 2, 2>(g, vec, st);
+  };
+  return type == 1 ? run(bf16_t{}) : run(fp16_t{});
+}
+
+// rows of a slab: enough slabs to fill the card, 16 rows a lane at least
+static int64_t slab_of(int64_t M, int64_t N, int V) {
+  const int64_t cols = (N + 64 * V - 1) / (64 * V);
+  int64_t n = 1024 / cols;
+  if (n < 1) n = 1;
+  int64_t s = (M + n - 1) / n;
+  if (s < 64) s = 64;
+  return s;
+}
+
+extern "C" int64_t asrn_act_grad_workspace(int64_t M, int64_t N) {
+  if (M < 0 || N < 0) return -1;
+  if (M == 0 || N == 0) return 0;
+  const int64_t a = slab_of(M, N, 1), b = slab_of(M, N, 8), s = a < b ? a : b;
+  return (M + s - 1) / s * N * 4;
+}
+
+extern "C" int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const void* pre, int64_t ldp, int32_t type, int64_t M,
+                             int64_t N, int32_t act, void* gp, float* colsum, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  const char* what = "asrn_act_grad";
+  ASRN_REQUIRE(type_ok(type), "%s: type %d", what, type);
+  ASRN_REQUIRE(M >= 0 && N >= 0 && M < ((int64_t)1 << 40) && N < (1 << 30) && act >= 0 && act <= 2,
+               "%s: bad sizes M=%lld N=%lld act=%d", what, (long long)M, (long long)N, act);
+  if (M == 0 || N == 0) return 0;
+  ASRN_REQUIRE(gy && (gp || colsum) && (act == 0 || pre), "%s: null pointer", what);
+  ASRN_REQUIRE(ldg >= N && (!pre || ldp >= N), "%s: leading dimensions must hold a row", what);
+  const int b = type_bytes(type), bg = gy_fp32 ? 4 : b;
+  const int W = type == 0 ? 4 : 8;
+  const bool vec = N % W == 0 && aligned(gy, ldg, bg, W) && (!act || aligned(pre, ldp, b, W)) && (!gp || aligned(gp, N, b, W));
+  const int V = vec ? W : 1;
+  const int64_t slab = slab_of(M, N, V), slabs = (M + slab - 1) / slab;
+  ASRN_REQUIRE(slabs < 65536, "%s: too many rows", what);
+  float* part = nullptr;
+  if (colsum) {
+    ASRN_REQUIRE(workspace && !((uintptr_t)workspace & 15) && workspace_bytes >= slabs * N * 4,
+                 "%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", what, (long long)(slabs * N * 4),
+                 (long long)workspace_bytes);
+    part = (float*)workspace;
+  }
+  const dim3 grid((unsigned)((N + 64 * V - 1) / (64 * V)), (unsigned)slabs);
+  hipStream_t st = (hipStream_t)stream;
+  const int rc = with_type(type, [&](auto t) {
+    using T = decltype(t);
+    constexpr int WT = sizeof(T) == 4 ? 4 : 8;
+    auto go = [&](auto g) {
+      using G = decltype(g);
+      if (vec) hipLaunchKernelGGL((k_act_grad<T, G, WT>), grid, dim3(256), 0, st, (const G*)gy, ldg, (const T*)pre, ldp, act, M,
+                                  (int)N, slab, (T*)gp, part);
+      else hipLaunchKernelGGL((k_act_grad<T, G, 1>), grid, dim3(256), 0, st, (const G*)gy, ldg, (const T*)pre, ldp, act, M, (int)N,
+                              slab, (T*)gp, part);
+      return check_launch("asrn_act_grad");
+    };
+    return gy_fp32 ? go(float{}) : go(T{});
+  });
+  return rc || !colsum ? rc : group_sums(part, (int)slabs, (int)N, colsum, st);
+}

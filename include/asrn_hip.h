@@ -774,6 +774,24 @@ int asrn_selective_step(const void* u, const void* delta, const void* B_, const 
                         const int64_t* strides, const float* A, const float* D, const float* bias, const float* h, float* next,
                         int64_t B, int32_t d, int32_t N, int32_t softplus, void* y, void* stream);
 
+/* ---- a product with its epilogue ---------------------------------------------------------------------------------------
+ * The dense products of a local block (asrn/nucleo.py:969-1014) with what follows them: y = [res +] act(x W^T + bias).
+ * x (M, K), W (N, K), bias (N, or null) in fp32, bf16 or fp16 (type 0, 1, 2), leading dimensions in elements (below 2^21 for x
+ * and W); act 0 none, 1 GELU (erf), 2 SiLU; res (M, N, or null) and y in fp32 or in `type`; pre (or null) gets x W^T + bias in
+ * `type`, for the backward. fp32 sums, results rounded once. 16-bit operands: any sizes and addresses (8 dividing K, the leading
+ * dimensions and 16 bytes the addresses is the fast form); fp32 with M > 16: K and the leading dimensions multiples of 4, x
+ * and W 16-byte aligned. workspace: asrn_linear_act_workspace bytes, 16-byte aligned (-1: bad sizes).
+ * act_grad: gp = gy act'(pre) in `type` (or null), gy in fp32 or in `type`; colsum (or null): the fp32 sums of its columns
+ * before that rounding, in a fixed order; workspace (for colsum): asrn_act_grad_workspace bytes, 16-byte aligned.
+ * M N = 0 writes nothing. */
+int64_t asrn_linear_act_workspace(int64_t M, int64_t N, int64_t K, int32_t type);
+int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t type, const void* bias, int64_t M,
+                        int64_t N, int64_t K, int32_t act, const void* res, int64_t ldr, int32_t res_fp32, void* pre, int64_t ldp,
+                        void* y, int64_t ldy, int32_t y_fp32, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t asrn_act_grad_workspace(int64_t M, int64_t N);
+int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const void* pre, int64_t ldp, int32_t type, int64_t M, int64_t N,
+                  int32_t act, void* gp, float* colsum, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
