@@ -147,7 +147,7 @@ SIGNATURES = {
     'asrn_selective_bwd': (ctypes.c_int, [_P] * 6 + [_I32] + [_P] * 6 + [_I64, _I64, _I32, _I32, _I32] + [_P] * 8 + [_I64, _P]),
     'asrn_linear_act_workspace': (_I64, [_I64, _I64, _I64, _I32]),
     'asrn_linear_act_fwd': (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P, _I64, _P, _I64,
-                                           _I32, _P, _I64, _P]),
+                                           _I32, _I32, _P, _I64, _P]),
     'asrn_act_grad_workspace': (_I64, [_I64, _I64]),
     'asrn_act_grad': (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _I64, _I64, _I32, _P, _P, _P, _I64, _P]),
     'asrn_selective_step': (ctypes.c_int, [_P] * 5 + [_I32] + [_P] * 6 + [_I64, _I32, _I32, _I32, _P, _P]),

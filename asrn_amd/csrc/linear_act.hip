@@ -26,25 +26,10 @@ struct Linear {
   int tm, tn;
 };
 
-// GELU for results of 16 bits: Phi(-|x|) = t p(t) exp(-x^2 / 2) with Abramowitz and Stegun's 7.1.26, erfc within 1.5e-7, one
-// exponential and one reciprocal (erff costs about twice the instructions, and the epilogue counts beside the product)
-__device__ __forceinline__ float gelu16(float x) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
-  const float z = x * 0.84932180028801904f;                        // sqrt(log2(e) / 2)
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
-                                   0.5f * -0.284496736f), 0.5f * 0.254829592f);
-  return fmaf(-fabsf(fminf(x, 64.f)), p * __builtin_amdgcn_exp2f(-z * z), fmaxf(x, 0.f));     // infinity stays itself
-}
-
-// V neighbouring results v of row m from column n on; whole: they lie in the matrix, and vectors of 4 in every operand
-template <typename T, int V, bool SHORT>
-__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int N, float (&v)[V], bool whole) {
-  if (!whole) {
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (n + k < N) e.template one<T>(m, n + k, v[k]);
-    return;
-  }
+// 16 neighbouring results of row m from column n on, all in the matrix, every operand read and written in vectors of 4 or more
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, float (&v)[16]) {
+  constexpr int V = 16;
   if (e.bias) {
     float b[4];
 #pragma unroll
@@ -57,7 +42,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int 
   if (e.pre) store_v<V>(static_cast<T*>(e.pre) + m * e.ldp + n, v);
   if (e.act == kActGelu) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = SHORT ? gelu16(v[k]) : activate(v[k], kActGelu);
+    for (int k = 0; k < V; ++k) v[k] = gelu16(v[k]);
   } else if (e.act == kActSilu) {
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = activate(v[k], kActSilu);
@@ -81,19 +66,52 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int 
   }
 }
 
+// A wave's results: lane (lr, lc) holds, of 32 x 32 block (i, j), row 32 i + lr and columns 32 j + 16 lc + 0 .. 15. Where they
+// are not whole vectors in the matrix, one after the other, through LDS (16 floats a thread, whose buffers are done with).
+template <typename T, int MI, int NI, int THR>
+__device__ __forceinline__ void finish_all(const Linear& g, fx16 (&acc)[MI][NI], int m0, int n0, float* lds) {
+  const int lane = lane_id(), lr = lane & 31, lc = lane >> 5;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = m0 + 32 * i + lr;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + 32 * j + 16 * lc;
+      if (m >= g.M || n >= g.N) continue;
+      if (g.e.vec && n + 16 <= g.N) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+        finish<T>(g.e, m, n, v);
+      } else {
+        float* mine = lds + threadIdx.x;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[e * THR] = acc[i][j][e];
+        const int left = g.N - n < 16 ? g.N - n : 16;
+#pragma unroll 1
+        for (int e = 0; e < left; ++e) g.e.template one<T>(m, n + e, mine[e * THR]);
+      }
+    }
+  }
+}
+
 // An operand's share of a step: R rows by 64 k, units of 8 k; a thread loads U units, 8 neighbouring threads a row's 128 bytes.
-// VEC: the units are 16 bytes on their boundary (8 divides K and the row stride); else element by element.
+// VEC: the units are 16 bytes on their boundary (8 divides K and the row stride); else they are read wherever they lie, those
+// of the last step element by element.
 constexpr unsigned kPast = 1u << 31;
 template <typename T, int R, int THR, bool VEC>
 struct Units {
   static constexpr int U = R * 8 / THR;
   static_assert(R * 8 % THR == 0 && THR % 8 == 0, "whole units");
   __amdgpu_buffer_rsrc_t rsrc;
+  const T* base;
   unsigned at[U], c;              // byte offsets of the rows; the thread's column of units
   uint4 v[U];
   // rows past the matrix repeat its last one: their results are not stored
   __device__ __forceinline__ void start(const void* X, int64_t ld, int r0, int rows, int tid) {
-    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(X) + r0 * ld), 0, kPast, 0x00027000);
+    base = static_cast<const T*>(X) + r0 * ld;
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, kPast, 0x00027000);
     c = tid % 8;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -112,11 +130,15 @@ struct Units {
     } else {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        unsigned q[8];
+        const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at[i]) + k0;
+        if (k0 + 64 <= K) {                       // uniform
+          __builtin_memcpy(&v[i], p, 16);
+        } else {
+          unsigned q[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          q[j] = __builtin_amdgcn_raw_buffer_load_b16(rsrc, k0 + 8 * (int)c + j < K ? at[i] + 2 * j : kPast, off, 0);
-        v[i] = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
+          for (int j = 0; j < 8; ++j) q[j] = k0 + 8 * (int)c + j < K ? __builtin_bit_cast(unsigned short, p[j]) : 0u;
+          v[i] = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
+        }
       }
     }
   }
@@ -190,21 +212,107 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(Linear g) {
         for (int j = 0; j < NI; ++j) acc[i][j] = mfma32(fw[j], fx[i], acc[i][j]);
     }
   }
+  finish_all<T, MI, NI, THR>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(lds));
+}
+
+// 16 bytes a lane from memory to LDS, lane i's to l[i] (l: the same in every lane)
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rsrc, uint4* l, unsigned at, unsigned off) {
+#ifdef __HIP_DEVICE_COMPILE__                     // the host's pass does not know the 16-byte form
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)l, 16, at, off, 0, 0);
+#endif
+}
+
+// The same with the operands straight from memory to LDS, without registers in between (whole steps; a last part of one goes
+// through them). Two buffers that the compiler can tell apart: a step's loads are issued before the products of the one
+// before and waited for after them, with one barrier a step.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear_direct(Linear g) {
+  constexpr int THR = 64 * WM * WN, BK = 64, MI = BM / WM / 32, NI = BN / WN / 32, UX = BM * 8 / THR, UW = BN * 8 / THR;
+  static_assert(BM * 8 % THR == 0 && BN * 8 % THR == 0, "whole units");
+  typedef T TX8 __attribute__((ext_vector_type(8)));
+  __shared__ uint4 lds0[(BM + BN) * 8];
+  __shared__ uint4 lds1[(BM + BN) * 8];
+  const int total = g.tm * g.tn, per = (total + kXcdCount - 1) / kXcdCount;
+  const int tile = (int)(blockIdx.x % kXcdCount) * per + (int)(blockIdx.x / kXcdCount);
+  if (tile >= total || (int)(blockIdx.x / kXcdCount) >= per) return;
+  const int m0 = tile / g.tn * BM, n0 = tile % g.tn * BN;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lc = lane >> 5;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN), wr = w_row(lr);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T*>(static_cast<const T*>(g.x) + (int64_t)m0 * g.ldx), 0, kPast, 0x00027000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<T*>(static_cast<const T*>(g.w) + (int64_t)n0 * g.ldw), 0, kPast, 0x00027000);
+  unsigned ax[UX], aw[UW];        // byte offsets of the unit that lies where the thread's share of LDS does
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int m = m0 + wm + 32 * i + lr;
+  for (int i = 0; i < UX; ++i) {
+    const int r = (tid + THR * i) / 8;
+    ax[i] = (unsigned)((m0 + r < g.M ? r : g.M - 1 - m0) * g.ldx + 8 * (tid % 8 ^ x_key(r))) * 2u;
+  }
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = n0 + wn + 32 * j + 16 * lc;
-      float v[16];
+  for (int i = 0; i < UW; ++i) {
+    const int r = (tid + THR * i) / 8;
+    aw[i] = (unsigned)((n0 + r < g.N ? r : g.N - 1 - n0) * g.ldw + 8 * (tid % 8 ^ w_key(r))) * 2u;
+  }
+  auto load = [&](uint4* l, int k) __attribute__((always_inline)) {
+    const unsigned off = (unsigned)k * 2u;
+    if (k + BK <= g.K) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
-      if (m < g.M) {
-        if (g.e.y32) finish<T, 16, false>(g.e, m, n, g.N, v, g.e.vec && n + 16 <= g.N);
-        else finish<T, 16, true>(g.e, m, n, g.N, v, g.e.vec && n + 16 <= g.N);
+      for (int i = 0; i < UX; ++i)
+        to_lds(rx, l + wave * 64 + THR * i, ax[i], off);
+#pragma unroll
+      for (int i = 0; i < UW; ++i)
+        to_lds(rw, l + BM * 8 + wave * 64 + THR * i, aw[i], off);
+    } else {                                      // the last part of a step: k past K is 0
+#pragma unroll
+      for (int i = 0; i < UX; ++i) {
+        const int r = (tid + THR * i) / 8;
+        l[tid + THR * i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+            rx, k + 8 * (tid % 8 ^ x_key(r)) < g.K ? ax[i] : kPast, off, 0));
+      }
+#pragma unroll
+      for (int i = 0; i < UW; ++i) {
+        const int r = (tid + THR * i) / 8;
+        l[BM * 8 + tid + THR * i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+            rw, k + 8 * (tid % 8 ^ w_key(r)) < g.K ? aw[i] : kPast, off, 0));
       }
     }
+  };
+  fx16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  auto step = [&](uint4* l, uint4* next, int k) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);           // vmcnt(0): this wave's part of the step has arrived
+    __syncthreads();                              // everybody's has, and the other buffer's readers are done
+    if (k + BK < g.K) load(next, k + BK);
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      TX8 fx[MI], fw[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = wm + 32 * i + lr;
+        fx[i] = __builtin_bit_cast(TX8, l[r * 8 + ((2 * kk + lc) ^ x_key(r))]);
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int r = wn + 32 * j + wr;
+        fw[j] = __builtin_bit_cast(TX8, l[BM * 8 + r * 8 + ((2 * kk + lc) ^ w_key(r))]);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = mfma32(fw[j], fx[i], acc[i][j]);
+    }
+  };
+  load(lds0, 0);
+  for (int k = 0; k < g.K; k += 2 * BK) {
+    step(lds0, lds1, k);
+    if (k + BK < g.K) step(lds1, lds0, k + BK);
   }
+  finish_all<T, MI, NI, THR>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(lds0));
 }
 
 // Few rows (M <= 16): W is read once and each of its values meets every row, so the weights' bytes bound it. A wave takes 4
@@ -327,12 +435,33 @@ static int launch_tiles(Linear g, bool vec, hipStream_t st) {
   const int64_t tiles = (int64_t)g.tm * g.tn;
   ASRN_REQUIRE(tiles < (1 << 30), "asrn_linear_act_fwd: too many tiles");
   const unsigned grid = (unsigned)((tiles + kXcdCount - 1) / kXcdCount * kXcdCount);
-  if (vec) hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, true>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
+  if (vec) hipLaunchKernelGGL((k_linear_direct<T, BM, BN, WM, WN>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
   else hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, false>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
   return check_launch("asrn_linear_act_fwd");
 }
 
 constexpr int kFewRows = 16;
+
+// The tile by an estimate of the time: a start of 3 us and 4 a 768 of k (the steps wait for their loads), and for each tile that a
+// CU takes its products at 2.5 PFLOP/s times what the tile needs over that. Measured (us; 64 x 64, 128 x 128, 256 x 192,
+// 256 x 256, without an epilogue): 1024 x 768 x 768 8.2 / 12.2 / 18.5 / 23.4, 2048 x 768 x 1536 (M, K, N) 11.5 / 16.1 / 24.3 /
+// 31.3, 4096 x 1024 x 1024 16.1 / 17.9 / 28.3 / 36.0, 16384 x 768 x 1536 58 / 49 / 43 / 51, 4096 x 4096 x 4096 280 / 155 / 156 /
+// 116, 8192 x 2048 x 4096 276 / 172 / 141 / 125 (hipBLASLt's product alone: 45 at the fourth, 108 and 106 at the last two).
+static int tile_of(int64_t M, int64_t N, int64_t K) {
+  struct Tile { int bm, bn; float over; };
+  static const Tile all[] = {{64, 64, 2.5f}, {128, 128, 2.3f}, {256, 192, 1.9f}, {256, 256, 1.75f}};
+  int best = 0;
+  float least = 0.f;
+  for (const Tile& t : all) {
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const float us = 3.f + 4.f * K / 768.f + (float)((tiles + 255) / 256) * t.over * (2.f * t.bm * t.bn * K / (2.5e9f / 256));
+    if (best == 0 || us < least) {
+      least = us;
+      best = t.bm << 8 | (t.bn & 255);
+    }
+  }
+  return best;
+}
 
 }  // namespace asrn
 
@@ -349,7 +478,7 @@ extern "C" int64_t asrn_linear_act_workspace(int64_t M, int64_t N, int64_t K, in
 
 extern "C" int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t type, const void* bias,
                                    int64_t M, int64_t N, int64_t K, int32_t act, const void* res, int64_t ldr, int32_t res_fp32,
-                                   void* pre, int64_t ldp, void* y, int64_t ldy, int32_t y_fp32, void* workspace,
+                                   void* pre, int64_t ldp, void* y, int64_t ldy, int32_t y_fp32, int32_t tile, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
   const char* what = "asrn_linear_act_fwd";
   ASRN_REQUIRE(type_ok(type), "%s: type %d", what, type);
@@ -360,6 +489,8 @@ extern "C" int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, in
   ASRN_REQUIRE(ldx >= K && ldw >= K && ldy >= N && (!res || ldr >= N) && (!pre || ldp >= N) && ldx < (1 << 21) && ldw < (1 << 21),
                "%s: leading dimensions must hold a row and x's and W's be below 2^21 (ldx=%lld ldw=%lld ldy=%lld)", what,
                (long long)ldx, (long long)ldw, (long long)ldy);
+  ASRN_REQUIRE(tile == 0 || tile == (256 << 8) || tile == (256 << 8 | 192) || tile == (128 << 8 | 128) || tile == (64 << 8 | 64),
+               "%s: unknown tile %d", what, tile);
   const int b = type_bytes(type), by = y_fp32 ? 4 : b, br = res_fp32 ? 4 : b;
   Linear g = {x, ldx, w, ldw, (int)M, (int)N, (int)K, {}, 0, 0};
   g.e = {bias, res, ldr, pre, ldp, y, ldy, act, res_fp32, y_fp32, 0};
@@ -376,11 +507,15 @@ extern "C" int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, in
     });
   if (type == 0) return gemm_epilogue((const float*)x, ldx, (const float*)w, ldw, M, N, K, g.e, workspace, workspace_bytes, st);
   const bool vec = K % 8 == 0 && aligned(x, ldx, 2, 8) && aligned(w, ldw, 2, 8);
+  const int how = tile ? tile : tile_of(M, N, K);
   auto run = [&](auto t) {
     using T = decltype(t);
-    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128);
-    if (t128 >= 256) return launch_tiles<T, 128, 128, 2, 2>(g, vec, st);
-    return launch_tiles<T, 64, 64, 2, 2>(g, vec, st);
+    switch (how) {
+      case 256 << 8: return launch_tiles<T, 256, 256, 2, 4>(g, vec, st);
+      case 256 << 8 | 192: return launch_tiles<T, 256, 192, 4, 2>(g, vec, st);
+      case 128 << 8 | 128: return launch_tiles<T, 128, 128, 2, 2>(g, vec, st);
+      default: return launch_tiles<T, 64, 64, 2, 2>(g, vec, st);
+    }
   };
   return type == 1 ? run(bf16_t{}) : run(fp16_t{});
 }

@@ -315,7 +315,7 @@ def _activada(x2, w, b, act, res, tipo_y, con_pre):
     ws = torch.empty((wsb,), dtype=torch.uint8, device=x2.device) if wsb > 0 else None
     _en(x2, 'asrn_linear_act_fwd', x2.data_ptr(), max(x2.stride(0), K), w.data_ptr(), max(w.stride(0), K), TIPOS[x2.dtype], _dir(b), M,
         N, K, act, _dir(res), N if res is None else max(res.stride(0), N), int(res is not None and res.dtype == torch.float32),
-        _dir(pre), N, y.data_ptr(), N, int(tipo_y == torch.float32), _dir(ws), wsb)
+        _dir(pre), N, y.data_ptr(), N, int(tipo_y == torch.float32), 0, _dir(ws), wsb)
     return y, pre
 
 

@@ -783,11 +783,12 @@ int asrn_selective_step(const void* u, const void* delta, const void* B_, const 
  * and W 16-byte aligned. workspace: asrn_linear_act_workspace bytes, 16-byte aligned (-1: bad sizes).
  * act_grad: gp = gy act'(pre) in `type` (or null), gy in fp32 or in `type`; colsum (or null): the fp32 sums of its columns
  * before that rounding, in a fixed order; workspace (for colsum): asrn_act_grad_workspace bytes, 16-byte aligned.
+ * tile (16-bit operands): 0 by the sizes, or a tile's rows << 8 | columns (256 << 8: 256 x 256).
  * M N = 0 writes nothing. */
 int64_t asrn_linear_act_workspace(int64_t M, int64_t N, int64_t K, int32_t type);
 int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t type, const void* bias, int64_t M,
                         int64_t N, int64_t K, int32_t act, const void* res, int64_t ldr, int32_t res_fp32, void* pre, int64_t ldp,
-                        void* y, int64_t ldy, int32_t y_fp32, void* workspace, int64_t workspace_bytes, void* stream);
+                        void* y, int64_t ldy, int32_t y_fp32, int32_t tile, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t asrn_act_grad_workspace(int64_t M, int64_t N);
 int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const void* pre, int64_t ldp, int32_t type, int64_t M, int64_t N,
                   int32_t act, void* gp, float* colsum, void* workspace, int64_t workspace_bytes, void* stream);

@@ -244,3 +244,19 @@ def test_same_bits_again():
     assert torch.equal(y, y2) and torch.equal(y, asrn_amd.lineal_activa(x, w, b, 'gelu', res))
     # a row's result does not depend on the rows beside it
     assert torch.equal(y[:200], asrn_amd.lineal_activa(x[:200], w, b, 'gelu', res[:200]))
+
+
+@pytest.mark.parametrize('tile', [256 << 8, 256 << 8 | 192, 128 << 8 | 128, 64 << 8 | 64])
+@pytest.mark.parametrize('M,K,N', [(300, 128, 272), (17, 72, 40), (513, 200, 515), (260, 333, 193), (256, 64, 256)])
+@pytest.mark.parametrize('dt', [BF16, F16])
+def test_every_tile(tile, M, K, N, dt):
+    """Each tile at whole, partial and single steps and edges, with everything in the epilogue: the formula, and the same bits
+    from every tile (a result's sums have one order)."""
+    x, w, b, res = r(M, K, dt=dt), (r(N, K) * K ** -0.5).to(dt), r(N, dt=dt), r(M, N)
+    y, pre = torch.empty(M, N, device=DEV), torch.empty(M, N, device=DEV, dtype=dt)
+    _lib.call('asrn_linear_act_fwd', x.data_ptr(), K, w.data_ptr(), K, {BF16: 1, F16: 2}[dt], b.data_ptr(), M, N, K, 2, res.data_ptr(),
+              N, 1, pre.data_ptr(), N, y.data_ptr(), N, 1, tile, None, 0, torch.cuda.current_stream().cuda_stream)
+    revisar(x, w, b, 'silu', res, None, y, None)
+    p = x.double() @ w.double().t() + b.double()
+    cerca(pre, p, (K + 24) * U * (x.double().abs() @ w.double().abs().t() + b.double().abs()), 'pre')
+    assert torch.equal(y, asrn_amd.lineal_activa(x, w, b, 'silu', res))

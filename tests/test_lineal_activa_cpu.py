@@ -37,8 +37,8 @@ def test_entries_refuse():
     def falla(rc, que):
         assert rc != 0 and que in lib.asrn_hip_last_error().decode(), lib.asrn_hip_last_error().decode()
 
-    def fwd(x=64, ldx=8, ldw=8, type=0, M=20, N=8, K=8, act=0, ldy=8, ws=None, wsb=0):
-        return lib.asrn_linear_act_fwd(x, ldx, 64, ldw, type, None, M, N, K, act, None, 0, 0, None, 0, 64, ldy, 1, ws, wsb, None)
+    def fwd(x=64, ldx=8, ldw=8, type=0, M=20, N=8, K=8, act=0, ldy=8, tile=0, ws=None, wsb=0):
+        return lib.asrn_linear_act_fwd(x, ldx, 64, ldw, type, None, M, N, K, act, None, 0, 0, None, 0, 64, ldy, 1, tile, ws, wsb, None)
     falla(fwd(type=3), 'type 3')
     falla(fwd(K=0), 'K=0')
     falla(fwd(act=5), 'act=5')
@@ -46,6 +46,7 @@ def test_entries_refuse():
     falla(fwd(ldx=7), 'leading')
     falla(fwd(ldy=4), 'leading')
     falla(fwd(ldw=1 << 21), '2^21')
+    falla(fwd(tile=7), 'unknown tile 7')
     falla(fwd(K=6, ldx=6, ldw=6), 'multiples of 4')
     falla(fwd(x=68), '16-byte')
     falla(fwd(M=64, N=64, K=4096, ldx=4096, ldw=4096, ldy=64), 'workspace')
