@@ -46,8 +46,8 @@ struct Selective {
 };
 
 // softplus(x) = max(x, 0) + log1p(exp(-|x|)); log1p(e) = 2 atanh(e / (2 + e)), whose series ends at s^15 / 15 of s <= 1/3
-__device__ __forceinline__ float softplus(float x) {
-  const float e = exp_fast(-fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+__device__ __forceinline__ float softplus_of(float x, float e) {
+  const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
   float p = fmaf(q, 1.f / 15, 1.f / 13);
   p = fmaf(q, p, 1.f / 11);
   p = fmaf(q, p, 1.f / 9);
@@ -56,6 +56,13 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(q, p, 1.f / 3);
   p = fmaf(q * s, p, s);
   return fmaxf(x, 0.f) + 2.f * p;
+}
+__device__ __forceinline__ float softplus(float x) { return softplus_of(x, exp_fast(-fabsf(x))); }
+// and its derivative, 1 / (1 + exp(-x))
+__device__ __forceinline__ float softplus(float x, float* slope) {
+  const float e = exp_fast(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.f + e);
+  *slope = x < 0.f ? e * r : r;
+  return softplus_of(x, e);
 }
 
 // DPP within a quad: lane ^ 1 and lane ^ 2
@@ -75,6 +82,9 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+
+// x is formed here: the compiler would put a sum that only the loop's next turn reads off to its end, its terms in registers
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
 
 // x[0 .. NPL) of LDS, NPL in {2, 4, 8}
 template <int NPL>
@@ -201,18 +211,20 @@ template <typename T>
 struct Rows {
   __amdgpu_buffer_rsrc_t rsrc;
   unsigned at, step;
-  __device__ __forceinline__ Rows(const T* row, int64_t st, const Place& p)
+  __device__ __forceinline__ Rows(const T* row, int64_t st, const Place& p, bool on = true)
       : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, kBufferBytes, 0x00027000)),
-        at(p.live ? p.c * (unsigned)sizeof(T) : kBufferBytes),
+        at(p.live && on ? p.c * (unsigned)sizeof(T) : kBufferBytes),
         // opaque: its multiples are formed where they are used, not kept over the tiles
         step(__builtin_amdgcn_readfirstlane((unsigned)st * (unsigned)sizeof(T))) {}
   __device__ __forceinline__ T load(unsigned row) const {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, row, 0));
     else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rsrc, at, row, 0));
   }
-  __device__ __forceinline__ void store(T v, unsigned row) const {
-    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, at, row, 0);
-    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, at, row, 0);
+  // without a branch: one between a tile's tokens would let the compiler put their sums off to its end
+  __device__ __forceinline__ void store(T v, unsigned row, bool in) const {
+    const unsigned to = in ? at : kBufferBytes;
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, to, row, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, to, row, 0);
   }
 };
 
@@ -322,7 +334,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective(Selective s) {
       }
       if (!LOCAL) {
         const float v = (quad_scatter(y, p.lane) + du[r]) * g[r];
-        if (r < left) out.store((T)v, r * out.step);
+        out.store((T)v, r * out.step, r < left);
       }
     };
 #pragma unroll
@@ -432,14 +444,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective_local_bwd(Selectiv
   if (p.live) s.total[(b * s.chunks + chunk) * s.d + p.c] = sum;
 }
 
-// The backward over one chunk, kCheck tokens at a time from its end: the states of those tokens again from the kept one, then
-// with G_t, the gradient of h_t, from the last to the first:
+// The backward over one chunk, a tile of kCheck tokens at a time from its end. A tile's values go to LDS, the next one's loads
+// are on their way meanwhile. Its states are formed again from the kept one, half a tile at a time (the registers hold no more),
+// then with G_t, the gradient of h_t, from the half's last token to its first:
 //   G_t += gy_t C_t;  dC_t += gy_t h_t;  dB_t += G_t delta_t u_t;  d(delta u) = sum G_t B_t;
 //   w = G_t exp(delta_t A) h_{t-1};  dA += w delta_t;  d delta += sum w A;  G_{t-1} = G_t exp(delta_t A)
 // dB and dC are summed over the lane's 4 channels, then over a row of 16 lanes; the rows' and waves' sums through LDS.
 template <typename T, int NPL>
-__global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s) {
-  constexpr int NP = 4 * NPL, TT = kCheck;
+__global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_bwd(Selective s) {
+  constexpr int NP = 4 * NPL, TT = kCheck, HALF = TT / 2;
   constexpr int NJ = (NPL + 3) / 4;               // values of dB (and of dC) that a lane leaves of its row's sums
   __shared__ float lds[kMaxWaves][TT * (384 + 2 * NP)];
   __shared__ float red[TT][2][kMaxWaves * 4][NP];
@@ -462,122 +475,149 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void k_selective_bwd(Selective s
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
   float dD = 0.f, dbias = 0.f;
   const int row = p.lane >> 4, cq = (p.lane >> 2) & 3;
-  for (int64_t t = t0 + (t1 - t0 - 1) / TT * TT; t >= t0; t -= TT) {
+  T u[TT], dl[TT], z[TT], gy[TT];
+  Shared<T, NPL, TT> mb, mc;
+  auto load = [&](int64_t t) {
+    load_channel<T, TT>(pu, s.ut, t, t1, p, u);
+    load_channel<T, TT>(pd, s.dlt, t, t1, p, dl);
+    load_channel<T, TT>(pg, s.gt, t, t1, p, gy);
+    if (gate) load_channel<T, TT>(pz, s.zt, t, t1, p, z);
+    mb.load(pB, s.Bt, t, t1, s.N, p.lane);
+    mc.load(pC, s.Ct, t, t1, s.N, p.lane);
+  };
+  int64_t t = t0 + (t1 - t0 - 1) / TT * TT;
+  load(t);
+  for (; t >= t0; t -= TT) {
     const int left = tokens_of<TT>(t, t1);
-    float h[TT + 1][4][NPL];
-    Own<NPL>::load(s.check + (b * checks + t / kCheck) * s.own, p, h[0]);
+    const float* check = s.check + (b * checks + t / kCheck) * s.own;
+    wave_lds_fence();
     {
-      T u[TT], dl[TT], z[TT], gy[TT];
-      Shared<T, NPL, TT> mb, mc;
-      load_channel<T, TT>(pu, s.ut, t, t1, p, u);
-      load_channel<T, TT>(pd, s.dlt, t, t1, p, dl);
-      load_channel<T, TT>(pg, s.gt, t, t1, p, gy);
-      if (gate) load_channel<T, TT>(pz, s.zt, t, t1, p, z);
-      mb.load(pB, s.Bt, t, t1, s.N, p.lane);
-      mc.load(pC, s.Ct, t, t1, s.N, p.lane);
-      wave_lds_fence();
-      float delta[TT];
-      step_sizes<T, TT>(dl, bias, s.softplus != 0, delta);
+      float delta[TT], sig[TT];
+      if (s.softplus) {
 #pragma unroll
-      for (int r = 0; r < TT; ++r) ls[r * 64] = s.softplus ? sigmoid((float)dl[r] + bias) : 1.f;
+        for (int r = 0; r < TT; ++r) delta[r] = softplus((float)dl[r] + bias, &sig[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < TT; ++r) {
+          delta[r] = (float)dl[r] + bias;
+          sig[r] = 1.f;
+        }
+      }
       if (left < TT)                  // past the text's end: a delta of 0 leaves the state as it is, and no gradient enters a sum
 #pragma unroll
         for (int r = 0; r < TT; ++r)
           if (r >= left) {
-            delta[r] = ls[r * 64] = 0.f;
+            delta[r] = sig[r] = 0.f;
             u[r] = gy[r] = z[r] = (T)0.f;
           }
 #pragma unroll
       for (int r = 0; r < TT; ++r) {
-        const float gf = (float)gy[r];
         sd[r * 64 + p.lane] = delta[r];
         su[r * 64 + p.lane] = delta[r] * (float)u[r];
         lu[r * 64] = (float)u[r];
-        sg[r * 64 + p.lane] = gf;
-        if (gate) {
-          const float zf = (float)z[r], q = sigmoid(zf);
-          sg[r * 64 + p.lane] = gf * (zf * q);
-          lz[r * 64] = gf * (q * (1.f + zf * (1.f - q)));
+        ls[r * 64] = sig[r];
+      }
+      if (gate) {
+#pragma unroll
+        for (int r = 0; r < TT; ++r) {
+          const float zf = (float)z[r], q = sigmoid(zf), gq = (float)gy[r] * q;
+          sg[r * 64 + p.lane] = gq * zf;
+          lz[r * 64] = gq * (1.f + zf * (1.f - q));
         }
+      } else {
+#pragma unroll
+        for (int r = 0; r < TT; ++r) sg[r * 64 + p.lane] = (float)gy[r];
       }
       mb.store(sB, p.lane);
       mc.store(sC, p.lane);
-      wave_lds_fence();
     }
-#pragma unroll
-    for (int r = 0; r < TT; ++r) {
-      float dt[4], x[4], B[NPL];
-      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
-      lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
-      lds_vec<NPL>(sB + r * NP + p.n0, B);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) h[r + 1][i][j] = fmaf(decay(dt[i], A2[i][j]), h[r][i][j], x[i] * B[j]);
-    }
-    wave_lds_fence();   // the values are read, and the decays formed, again: kept from above they would fill the registers
+    wave_lds_fence();
+    if (t > t0) load(t - TT);
     const int64_t o = (b * s.L + t) * s.d;
-    const Rows<T> odu(static_cast<T*>(s.du) + o, s.d, p), odl(static_cast<T*>(s.ddl) + o, s.d, p), odz(static_cast<T*>(s.dz) + o, s.d, p);
-    auto step = [&](int r) {
-      float dt[4], x[4], g[4], B[NPL], C[NPL], y[4], dx[4], dd[4], dB[NPL], dC[NPL];
-      lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
-      lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
-      lds_vec<4>(sg + r * 64 + (p.lane & ~3), g);
-      lds_vec<NPL>(sB + r * NP + p.n0, B);
-      lds_vec<NPL>(sC + r * NP + p.n0, C);
+    const Rows<T> odu(static_cast<T*>(s.du) + o, s.d, p), odl(static_cast<T*>(s.ddl) + o, s.d, p), odz(static_cast<T*>(s.dz) + o, s.d, p, gate);
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) dB[j] = dC[j] = 0.f;
+    for (int half = 1; half >= 0; --half) {
+      float h[HALF + 1][4][NPL];
+      Own<NPL>::load(check, p, h[0]);
+      // the state after token r, from `from`
+      auto again = [&](int r, const float (&from)[4][NPL], float (&to)[4][NPL]) __attribute__((always_inline)) {
+        float dt[4], x[4], B[NPL];
+        lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+        lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
+        lds_vec<NPL>(sB + r * NP + p.n0, B);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] = dx[i] = dd[i] = 0.f;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-          const float G1 = fmaf(g[i], C[j], G[i][j]);
-          y[i] = fmaf(h[r + 1][i][j], C[j], y[i]);
-          dC[j] = fmaf(g[i], h[r + 1][i][j], dC[j]);
-          dB[j] = fmaf(G1, x[i], dB[j]);
-          dx[i] = fmaf(G1, B[j], dx[i]);
-          G[i][j] = G1 * decay(dt[i], A2[i][j]);
-          const float w = G[i][j] * h[r][i][j];
-          dd[i] = fmaf(w, A2[i][j], dd[i]);
-          dA[i][j] = fmaf(w, dt[i], dA[i][j]);
-        }
-      }
-      const float ys = quad_scatter(y, p.lane), ds = quad_scatter(dx, p.lane), dds = quad_scatter(dd, p.lane);
-      const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane], uf = lu[r * 64];
-      const float ddl = fmaf(dds, kLn2, ds * uf) * ls[r * 64];
-      dbias += ddl;
-      dD = fmaf(gg, uf, dD);
-      if (r < left) {
-        odu.store((T)fmaf(ds, delta, gg * D), r * odu.step);
-        odl.store((T)ddl, r * odl.step);
-        if (gate) odz.store((T)(fmaf(D, uf, ys) * lz[r * 64]), r * odz.step);
+          for (int j = 0; j < NPL; ++j) to[i][j] = fmaf(decay(dt[i], A2[i][j]), from[i][j], x[i] * B[j]);
+        __builtin_amdgcn_sched_barrier(0);          // a step's LDS reads stay in it: the states leave few registers
+      };
+      if (half) {
+#pragma unroll
+        for (int r = 0; r < HALF; ++r) again(r, h[0], h[0]);
       }
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) {             // over the row's quads
-        dB[j] += dpp<0x128>(dB[j]);
-        dC[j] += dpp<0x128>(dC[j]);
-        dB[j] += dpp<0x124>(dB[j]);
-        dC[j] += dpp<0x124>(dC[j]);
-      }
+      for (int r = 0; r < HALF; ++r) again(half * HALF + r, h[r], h[r + 1]);
+      wave_lds_fence();   // the values are read, and the decays formed, again: kept from above they would fill the registers
 #pragma unroll
-      for (int k = 0; k < NJ; ++k) {              // quad cq of the row leaves values 4 k + cq
-        float vb = dB[4 * k], vc = dC[4 * k];
+      for (int k = HALF - 1; k >= 0; --k) {
+        const int r = half * HALF + k;
+        float dt[4], x[4], g[4], B[NPL], C[NPL], y[4], dx[4], dd[4], dB[NPL], dC[NPL];
+        lds_vec<4>(sd + r * 64 + (p.lane & ~3), dt);
+        lds_vec<4>(su + r * 64 + (p.lane & ~3), x);
+        lds_vec<4>(sg + r * 64 + (p.lane & ~3), g);
+        lds_vec<NPL>(sB + r * NP + p.n0, B);
+        lds_vec<NPL>(sC + r * NP + p.n0, C);
 #pragma unroll
-        for (int j = 1; j < 4; ++j)
-          if (4 * k + j < NPL) {
-            vb = cq == j ? dB[4 * k + j] : vb;
-            vc = cq == j ? dC[4 * k + j] : vc;
+        for (int j = 0; j < NPL; ++j) dB[j] = dC[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[i] = dx[i] = dd[i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < NPL; ++j) {
+            const float G1 = fmaf(g[i], C[j], G[i][j]);
+            y[i] = fmaf(h[k + 1][i][j], C[j], y[i]);
+            dC[j] = fmaf(g[i], h[k + 1][i][j], dC[j]);
+            dB[j] = fmaf(G1, x[i], dB[j]);
+            dx[i] = fmaf(G1, B[j], dx[i]);
+            G[i][j] = G1 * decay(dt[i], A2[i][j]);
+            const float w = G[i][j] * h[k][i][j];
+            dd[i] = fmaf(w, A2[i][j], dd[i]);
+            dA[i][j] = fmaf(w, dt[i], dA[i][j]);
+            pin(dA[i][j]);
           }
-        if (4 * k + cq < NPL) {
-          red[r][0][p.wave * 4 + row][p.n0 + 4 * k + cq] = vb;
-          red[r][1][p.wave * 4 + row][p.n0 + 4 * k + cq] = vc;
         }
-      }
-      __builtin_amdgcn_sched_barrier(0);          // a step's LDS reads stay in it: the states leave few registers
-    };
+        const float ys = quad_scatter(y, p.lane), ds = quad_scatter(dx, p.lane), dds = quad_scatter(dd, p.lane);
+        const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane], uf = lu[r * 64];
+        const float ddl = fmaf(dds, kLn2, ds * uf) * ls[r * 64];
+        dbias += ddl;
+        dD = fmaf(gg, uf, dD);
+        odu.store((T)fmaf(ds, delta, gg * D), r * odu.step, r < left);
+        odl.store((T)ddl, r * odl.step, r < left);
+        odz.store((T)(fmaf(D, uf, ys) * lz[r * 64]), r * odz.step, r < left);
 #pragma unroll
-    for (int r = TT - 1; r >= 0; --r) step(r);
+        for (int j = 0; j < NPL; ++j) {             // over the row's quads
+          dB[j] += dpp<0x128>(dB[j]);
+          dC[j] += dpp<0x128>(dC[j]);
+          dB[j] += dpp<0x124>(dB[j]);
+          dC[j] += dpp<0x124>(dC[j]);
+        }
+#pragma unroll
+        for (int q = 0; q < NJ; ++q) {              // quad cq of the row leaves values 4 q + cq
+          float vb = dB[4 * q], vc = dC[4 * q];
+#pragma unroll
+          for (int j = 1; j < 4; ++j)
+            if (4 * q + j < NPL) {
+              vb = cq == j ? dB[4 * q + j] : vb;
+              vc = cq == j ? dC[4 * q + j] : vc;
+            }
+          if (4 * q + cq < NPL) {
+            red[r][0][p.wave * 4 + row][p.n0 + 4 * q + cq] = vb;
+            red[r][1][p.wave * 4 + row][p.n0 + 4 * q + cq] = vc;
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < TT * 2 * s.N; e += blockDim.x) {
       const int r = e / (2 * s.N), k = e / s.N % 2, n = e % s.N;
