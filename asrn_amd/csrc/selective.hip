@@ -24,6 +24,7 @@ namespace asrn {
 constexpr int kCheck = 8;         // tokens between two kept states; also the tile of the backward
 constexpr int kTile = 16;         // tokens that the forward stages at once
 constexpr int kMaxWaves = 4;      // of a workgroup, 64 channels each
+constexpr int kMinChunk = 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Selective {
@@ -364,12 +365,24 @@ __global__ __launch_bounds__(256) void k_selective_carry(Selective s) {
   float h = x0 ? x0[(b * s.d + c) * s.N + n] : 0.f;
   float* x = s.carry + b * (s.chunks - 1) * s.own + e;
   const float* w = s.total + b * s.chunks * s.d + c;
+  constexpr int R = 16;               // loads under way at once
   const int m = s.chunks - 1;
-#pragma unroll 8
-  for (int k = 0; k < m; ++k) {
-    const int64_t j = BACK ? m - 1 - k : k;
-    h = fmaf(decay(w[(BACK ? j + 1 : j) * s.d], A2), h, x[j * s.own]);
-    x[j * s.own] = h;
+  for (int k0 = 0; k0 < m; k0 += R) {
+    float v[R], t[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = k0 + r < m ? k0 + r : m - 1;
+      const int64_t j = BACK ? m - 1 - k : k;
+      v[r] = x[j * s.own];
+      t[r] = w[(BACK ? j + 1 : j) * s.d];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (k0 + r < m) {
+        const int64_t j = BACK ? m - 1 - (k0 + r) : k0 + r;
+        h = fmaf(decay(t[r], A2), h, v[r]);
+        x[j * s.own] = h;
+      }
   }
 }
 
@@ -689,17 +702,34 @@ static void grid_of(int d, int& waves, int& blocks) {
   blocks = (n + waves - 1) / waves;
 }
 
-constexpr int kWantWaves = 2048;    // 2 a SIMD
-// Chunks of a text: as many as fill the card, of at least kMinChunk tokens (a chunk's tokens are walked twice when there
-// are several).
-constexpr int kMinChunk = 64;
+// Tokens of a chunk. A CU takes the workgroups in rounds of as many as fill its 4 SIMDs with one wave each, and walks a chunk's
+// tokens twice when there are several (the local pass takes 3/4 of the other's time); the chunks' states are joined one
+// after the other, about 0.4 tokens' time each. One wave a SIMD leaves about 2/5 of its time unused, two 1/5, three 1/10. Of the
+// chunks that make 1 to 8 rounds, the one of the least time: 8 texts of 2048 tokens x 768 channels in chunks of 112 (1.8
+// rounds) 445 us forward and backward, of 64 (3 rounds) 410; 2 prompts of 32768 in 208 (3.7) 453, in 256 (3.0) 424.
 static int64_t chunk_of(int64_t B, int64_t L, int d) {
-  const int64_t waves = B * ((d + 63) / 64);
-  int64_t n = kWantWaves / waves;
-  if (n < 2) return (L + kTile - 1) / kTile * kTile;
-  int64_t c = (L + n - 1) / n;
-  if (c < kMinChunk) c = kMinChunk;
-  return (c + kTile - 1) / kTile * kTile;
+  int waves, blocks;
+  grid_of(d, waves, blocks);
+  static const float used[] = {0.f, 0.6f, 0.8f, 0.9f};
+  const int64_t slots = 256 * 4 / waves, whole = (L + kTile - 1) / kTile * kTile;
+  int64_t best = 0;
+  float least = 0.f;
+  auto rate = [&](int64_t c) {
+    const int64_t n = (L + c - 1) / c, rounds = (B * blocks * n + slots - 1) / slots;
+    const float t = rounds * (c + 6.f) / used[rounds < 3 ? rounds : 3] * (n > 1 ? 1.75f : 1.f) + 0.4f * n;
+    if (best == 0 || t < least) {
+      least = t;
+      best = c;
+    }
+  };
+  rate(whole);
+  for (int r = 1; r <= 8; ++r) {
+    const int64_t n = r * slots / (B * blocks);
+    if (n < 2) continue;
+    const int64_t c = ((L + n - 1) / n + kTile - 1) / kTile * kTile;
+    rate(c < kMinChunk ? kMinChunk : c);
+  }
+  return best;
 }
 static int chunks_of(int64_t B, int64_t L, int d) {
   const int64_t c = chunk_of(B, L, d);
