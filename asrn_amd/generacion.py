@@ -2,8 +2,8 @@
 reference's _Escritor (model part) and escribir (asrn/nucleo.py:1717-1854, 1965-2043).
 
 EscritorModelo keeps, besides each ASRN layer's EscritorCapa state, each local block's last k - 1 LayerNorm rows (the
-causal convolution's window) and, for mezcla='memoria', its per-channel memory, so one new token costs the same work
-whatever the text length. A 'conv' block's step in fp32 is three fused kernels (asrn_block_step) that stream its
+causal convolution's window) and, for mezcla='memoria', its per-channel memory, for mezcla='selectiva' its scan's state, so
+one new token costs the same work whatever the text length. A 'conv' block's step in fp32 is three fused kernels (asrn_block_step) that stream its
 three weight matrices once for all rows, its window a ring indexed by the position. (The reference's step leaves the
 'memoria' blocks' memory out, nucleo:1811-1814; here the step equals the whole-text model for both block kinds.)
 
@@ -18,7 +18,7 @@ sampled ones follow the same distribution, not the same random stream.
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import ops, selectiva
 from .escritura import EscritorCapa
 from .modelo import _base, revisar_precision
 
@@ -50,10 +50,20 @@ class EscritorModelo:
         E = m.emb(x0)
         h = E
         self.ventanas, self.memorias, self.anillos, self.fusion = [], [], [], []
+        self.selectivas = {}                # a 'selectiva' block's scan state, and its decays, by the block's number
         if hasattr(self, 'espacio'):
             del self.espacio
         capas = iter(self.capas)
         for i, blq in enumerate(m.bloques):
+            if blq.mezcla == 'selectiva':
+                h, (z, estado) = blq.adelante_selectiva(h, devolver_estado=True)
+                self.selectivas[i] = (estado, blq.decaimientos())
+                self.ventanas.append(_ventana_inicial(z, blq.k))
+                self.anillos.append(None)
+                self.fusion.append(False)
+                if i in m.pos_largo:
+                    h = next(capas).inicio(E, h, x0, capacidad=self.cap)
+                continue
             z = blq.ln1(h)
             ventana = _ventana_inicial(z, blq.k)
             # the fused step keeps the window as a ring: position t at slot t mod (k - 1)
@@ -95,14 +105,19 @@ class EscritorModelo:
                 raise ValueError('EscritorModelo: the prompt ran the fused block step (fp32, no autocast); every step '
                                  'must run the same way')
             return ops.paso_bloque(blq, h, self.anillos[i], pos, self.espacio, previo=previo, terminar=terminar)
+        if blq.mezcla == 'selectiva':
+            return blq.paso_selectiva(h, self.ventanas[i], *self.selectivas[i])
         z = blq.ln1(h)
-        ventana = torch.cat([self.ventanas[i], z.unsqueeze(-1)], dim=-1)            # (B, d, k)
-        if blq.mezcla == 'conv':
-            c = F.linear(ventana.flatten(1), blq.conv.weight.flatten(1), blq.conv.bias)
+        if blq.mezcla == 'memoria' and blq.k <= selectiva.K_MAX and z.dtype in selectiva.TIPOS:
+            c, _ = selectiva.paso_conv_canal(z, self.ventanas[i], blq.conv.weight, blq.conv.bias, 'gelu')
         else:
-            c = (ventana * blq.conv.weight[:, 0, :]).sum(-1) + blq.conv.bias
-        self.ventanas[i].copy_(ventana[..., 1:])
-        c = F.gelu(c)
+            ventana = torch.cat([self.ventanas[i], z.unsqueeze(-1)], dim=-1)            # (B, d, k)
+            if blq.mezcla == 'conv':
+                c = F.linear(ventana.flatten(1), blq.conv.weight.flatten(1), blq.conv.bias)
+            else:
+                c = (ventana * blq.conv.weight[:, 0, :]).sum(-1) + blq.conv.bias
+            self.ventanas[i].copy_(ventana[..., 1:])
+            c = F.gelu(c)
         if blq.mezcla == 'memoria':
             u, f = blq.mem(z).float().chunk(2, dim=-1)
             f = torch.sigmoid(f) * blq.f_max

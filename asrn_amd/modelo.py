@@ -16,11 +16,12 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .capa import CapaASRNEstable, ngramas
-from . import ajuste, ops
+from . import ajuste, ops, selectiva
 from .ops import escaneo
-from .lineal import lineal, lineal8
+from .lineal import lineal, lineal8, lineal_activa
 
-MEZCLAS = ('conv', 'memoria')
+MEZCLAS = ('conv', 'memoria', 'selectiva')
+ESTADOS = 16               # states a channel of a 'selectiva' block
 OPCIONES_CAPA = ('n_tablas', 'n_bits', 'afin_oculto', 'chunk', 'tablas_contexto', 'confirmar', 'sufijo', 'vistos',
                  'nodos_racha', 'racha_max')
 MODOS_CHECKPOINT = ('no', 'asrn', 'todo', 'ocho')
@@ -70,8 +71,15 @@ def conv_causal(z, peso, sesgo):
     return lineal(cols, peso.reshape(peso.shape[0], -1), sesgo)
 
 
+def _conv_canal_ok(z, peso):
+    return z.is_cuda and z.dtype in selectiva.TIPOS and peso.dtype in selectiva.TIPOS and 1 <= peso.shape[-1] <= selectiva.K_MAX
+
+
 def conv_canal_causal(z, peso, sesgo):
-    """The per-channel (depthwise) version: peso (d, 1, k). k fused multiply-adds over shifted views."""
+    """The per-channel (depthwise) version: peso (d, 1, k). On the GPU one kernel (selectiva.conv_canal), else k multiply-adds
+    over shifted views."""
+    if _conv_canal_ok(z, peso):
+        return selectiva.conv_canal(z, peso, sesgo)
     k = peso.shape[-1]
     w = peso[:, 0, :].to(z.dtype)
     zp = F.pad(z, (0, 0, k - 1, 0))
@@ -92,21 +100,38 @@ class BloqueLocal(nn.Module):
     """Causal local context (asrn/nucleo.py:969-1014): h += GELU(causal conv of LayerNorm(h) over the current and
     k - 1 previous tokens); h += FF(LayerNorm(h)). mezcla='memoria': the convolution is per channel, plus a forgetting
     memory per channel m_t = f_t m_{t-1} + (1 - f_t) u_t, f < f_max = 1 - 1/memoria_max, computed by the library's
-    affine scan; channel c starts with a time scale of 10**(c log10(memoria_max) / (d - 1)) tokens."""
+    affine scan; channel c starts with a time scale of 10**(c log10(memoria_max) / (d - 1)) tokens.
+
+    mezcla='selectiva' (no counterpart in the reference): a selective state space of ESTADOS states a channel in place of the
+    memory. With z = LayerNorm(h): c = SiLU(per-channel conv of z); step sizes (through a rank of d / 16), Bm and C are linear
+    in c; h += W_o y, y the scan's output gated by SiLU(W_g z + b_g) (selectiva.escaneo_selectivo). The step sizes start at the
+    time scales above, the decays at -1 .. -ESTADOS. Its products run with their bias, activation and residual in their
+    epilogue (lineal_activa). GPU only."""
 
     def __init__(self, d, k=4, ff=128, dropout=0.0, mezcla='conv', memoria_max=1024):
         super().__init__()
         if mezcla not in MEZCLAS or memoria_max < 2:
             raise ValueError(f'mezcla={mezcla!r} (one of {MEZCLAS}), memoria_max={memoria_max} (>= 2)')
+        if mezcla == 'selectiva' and k > selectiva.K_MAX:
+            raise ValueError(f"k={k}: a 'selectiva' block's convolution has at most {selectiva.K_MAX} taps")
         self.k, self.mezcla = k, mezcla
         self.f_max = 1.0 - 1.0 / memoria_max
         # creation order fixes what a seed produces: ln1, conv, [mem, mem_o], ln2, ff
         self.ln1 = nn.LayerNorm(d)
-        self.conv = nn.Conv1d(d, d, k, groups=d if mezcla == 'memoria' else 1)
+        self.conv = nn.Conv1d(d, d, k, groups=1 if mezcla == 'conv' else d)
         if mezcla == 'memoria':
             self.mem = nn.Linear(d, 2 * d)
             self.mem_o = nn.Linear(d, d, bias=False)
             self._olvido_inicial(d, memoria_max)
+        elif mezcla == 'selectiva':
+            self.rango = -(-d // 16)
+            self.sel_x = nn.Linear(d, self.rango + 2 * ESTADOS, bias=False)
+            self.sel_dt = nn.Linear(self.rango, d)
+            self.sel_log_a = nn.Parameter(torch.arange(1.0, ESTADOS + 1).log().repeat(d))     # flat: no weight decay
+            self.sel_d = nn.Parameter(torch.ones(d))
+            self.sel_g = nn.Linear(d, d)
+            self.sel_o = nn.Linear(d, d, bias=False)
+            self._pasos_iniciales(d, memoria_max)
         self.ln2 = nn.LayerNorm(d)
         self.ff = nn.Sequential(nn.Linear(d, ff), nn.GELU(), nn.Linear(ff, d))
         self.drop = nn.Dropout(dropout)
@@ -118,6 +143,11 @@ class BloqueLocal(nn.Module):
         q = ((1 - 1 / tau) / self.f_max).clamp(1e-3, 1 - 1e-3)
         self.mem.bias[d:] = torch.log(q / (1 - q))
 
+    @torch.no_grad()
+    def _pasos_iniciales(self, d, memoria_max):
+        """Step-size biases such that softplus(b_c) = 1/tau_c, tau geometric from 1 to memoria_max."""
+        self.sel_dt.bias.copy_(torch.log(torch.expm1(1 / torch.logspace(0, math.log10(memoria_max), d))))
+
     def _memoria(self, z):
         u, f = self.mem(z).float().chunk(2, dim=-1)
         f = torch.sigmoid(f) * self.f_max
@@ -126,7 +156,10 @@ class BloqueLocal(nn.Module):
 
     def forward(self, h, ocho=False):
         """ocho: what the backward needs is kept in 8 bits (_en_ocho) where the block's products run in fp32 or bf16 on
-        the GPU and its feed-forward is this class's; the output is the same."""
+        the GPU and its feed-forward is this class's; the output is the same. A 'selectiva' block keeps what it keeps
+        otherwise."""
+        if self.mezcla == 'selectiva':
+            return self.adelante_selectiva(h)[0]
         if ocho and h.is_cuda and h.dtype == torch.float32 and _dtype_producto(h) in (torch.float32, torch.bfloat16) and \
                 type(self)._ff is BloqueLocal._ff and '_ff' not in vars(self):
             return self._en_ocho(h)
@@ -135,17 +168,66 @@ class BloqueLocal(nn.Module):
         z, h = ops.norma_residual(self.ln1, h, torch.float32)
         if self.mezcla == 'conv':
             c = conv_causal(z, self.conv.weight, self.conv.bias)
+            if self._sin_drop():
+                y, h = ops.suma_gelu_norma(self.ln2, h, c, _dtype_producto(h))
+                return h + self._ff(y)
+            c = F.gelu(c)
+        elif _conv_canal_ok(z, self.conv.weight):
+            c = selectiva.conv_canal(z, self.conv.weight, self.conv.bias, 'gelu')
         else:
-            c = conv_canal_causal(z, self.conv.weight, self.conv.bias)
-        if self.mezcla == 'conv' and self._sin_drop():
-            y, h = ops.suma_gelu_norma(self.ln2, h, c, _dtype_producto(h))
-            return h + self._ff(y)
-        c = F.gelu(c)
+            c = F.gelu(conv_canal_causal(z, self.conv.weight, self.conv.bias))
         if self.mezcla == 'memoria':
             c = c + self._memoria(z)
         h = h + self.drop(c)
         y, h = ops.norma_residual(self.ln2, h, _dtype_producto(h))
         return h + self.drop(self._ff(y))
+
+    def decaimientos(self):
+        """The scan's A (d, ESTADOS) of a 'selectiva' block."""
+        return -self.sel_log_a.exp().view(-1, ESTADOS)
+
+    def _entradas_selectivas(self, c):
+        """The step sizes before their bias, Bm and C of the convolution's output c (..., d)."""
+        dt, Bm, C = lineal_activa(c, self.sel_x.weight).split((self.rango, ESTADOS, ESTADOS), -1)
+        return lineal_activa(dt, self.sel_dt.weight), Bm, C
+
+    def _sumar(self, h, y, w, b=None):
+        """h + drop(y w^T + b), the sum in the product's epilogue where no dropout stands between."""
+        if self._sin_drop():
+            return lineal_activa(y, w, b, residuo=h)
+        return h + self.drop(lineal_activa(y, w, b))
+
+    def _ff_selectiva(self, h):
+        y, h = ops.norma_residual(self.ln2, h, _dtype_producto(h))
+        f0, act, f2 = self.ff
+        if type(act) is nn.GELU and act.approximate == 'none' and ops.sin_ganchos(act):
+            u = lineal_activa(y, f0.weight, f0.bias, 'gelu')
+        else:                       # an activation put in the GELU's place, or one with hooks or the tanh form, runs as it is
+            u = act(lineal_activa(y, f0.weight, f0.bias))
+        return self._sumar(h, u, f2.weight, f2.bias)
+
+    def adelante_selectiva(self, h, devolver_estado=False):
+        """forward of a 'selectiva' block -> (its output, None), or with devolver_estado (its output, (the convolution's inputs
+        z, the scan's last state)), what paso_selectiva goes on from."""
+        z, h = ops.norma_residual(self.ln1, h, _dtype_producto(h))
+        c = selectiva.conv_canal(z, self.conv.weight, self.conv.bias, 'silu')
+        delta, Bm, C = self._entradas_selectivas(c)
+        y = selectiva.escaneo_selectivo(c, delta, self.decaimientos(), Bm, C, D=self.sel_d,
+                                        puerta=lineal_activa(z, self.sel_g.weight, self.sel_g.bias),
+                                        sesgo_delta=self.sel_dt.bias, devolver_estado=devolver_estado)
+        y, fin = y if devolver_estado else (y, None)
+        h = self._ff_selectiva(self._sumar(h, y, self.sel_o.weight))
+        return h, (z, fin) if devolver_estado else None
+
+    def paso_selectiva(self, h, ventana, estado, A):
+        """The next token's state h (B, d) through a 'selectiva' block; ventana (B, d, k - 1) and estado are updated in place. A:
+        decaimientos()."""
+        z, h = ops.norma_residual(self.ln1, h, _dtype_producto(h))
+        c, _ = selectiva.paso_conv_canal(z, ventana, self.conv.weight, self.conv.bias, 'silu')
+        delta, Bm, C = self._entradas_selectivas(c)
+        y, _ = selectiva.paso_selectivo(c, delta, A, Bm, C, estado, D=self.sel_d,
+                                        puerta=lineal_activa(z, self.sel_g.weight, self.sel_g.bias), sesgo_delta=self.sel_dt.bias)
+        return self._ff_selectiva(self._sumar(h, y, self.sel_o.weight))
 
     def _en_ocho(self, h):
         """forward with the inputs of the LayerNorms and the GELUs kept in 8 bits (ops.norma8, ops.gelu8) and the products'
@@ -193,7 +275,8 @@ def _escalar_profundo(bloques, largos, n_capas):
     1/sqrt(2 n_capas)."""
     f = 1.0 / (2 * n_capas) ** 0.5
     for b in bloques:
-        salidas = [b.conv.weight, b.ff[2].weight] + ([b.mem_o.weight] if b.mezcla == 'memoria' else [])
+        salidas = [b.sel_o.weight if b.mezcla == 'selectiva' else b.conv.weight, b.ff[2].weight]
+        salidas += [b.mem_o.weight] if b.mezcla == 'memoria' else []
         for w in salidas:
             w.mul_(f)
     for c in largos:
@@ -373,6 +456,7 @@ class ConfigASRN:
         reglas += [
             (self.nodos_racha >= 2, 'nodos_racha must be >= 2'),
             (self.mezcla in MEZCLAS, f"mezcla={self.mezcla!r}: one of {', '.join(MEZCLAS)}"),
+            (self.mezcla != 'selectiva' or self.k <= selectiva.K_MAX, f"k={self.k}: at most {selectiva.K_MAX} with mezcla='selectiva'"),
             (_entero(self.memoria_max) and self.memoria_max >= 2, f'memoria_max={self.memoria_max!r}: an integer >= 2'),
         ]
         return [msg for ok, msg in reglas if not ok]

@@ -108,3 +108,30 @@ def test_entries_refuse(lib):
     assert lib.asrn_selective_fwd_workspace(0, 5, 8, 4) == 0 and lib.asrn_selective_fwd_workspace(2, 5, 0, 4) == -1
     # 12 waves fill 1/170 of the card: a long text is cut, and its chunks' states need room
     assert lib.asrn_selective_fwd_workspace(1, 1 << 15, 768, 16) > 0
+
+
+def test_blocks_and_configurations():
+    from asrn_amd.modelo import ESTADOS, BloqueLocal
+    b = BloqueLocal(40, 4, 80, mezcla='selectiva', memoria_max=64)
+    assert b.conv.weight.shape == (40, 1, 4) and b.rango == 3 and b.decaimientos().shape == (40, ESTADOS)
+    assert torch.allclose(b.decaimientos()[7], -torch.arange(1.0, ESTADOS + 1))
+    pasos = torch.nn.functional.softplus(b.sel_dt.bias)
+    assert torch.allclose(pasos[[0, -1]], torch.tensor([1.0, 1 / 64]), rtol=1e-4)
+    with pytest.raises(ValueError, match='taps'):
+        BloqueLocal(40, 17, 80, mezcla='selectiva')
+    with pytest.raises(ValueError, match='k=17'):
+        asrn_amd.ConfigASRN(V=10, k=17, mezcla='selectiva')
+    c = asrn_amd.ConfigASRN(V=48, d=32, n_capas=10, mezcla='selectiva')
+    m = asrn_amd.crear_desde_config(c, semilla=1)
+    assert c.contar_parametros() == m.num_parametros() and asrn_amd.ConfigASRN.desde_modelo(m) == c.con(init_profundo=True)
+    # the deep start shrinks what writes into the residual stream, and weight decay leaves the decays alone
+    recto = asrn_amd.crear_desde_config(c.con(init_profundo=False), semilla=1)
+    f = 20 ** -0.5
+    for a, r in zip(m.bloques, recto.bloques):
+        assert torch.allclose(a.sel_o.weight, f * r.sel_o.weight) and torch.equal(a.conv.weight, r.conv.weight)
+    from asrn_amd.entrenamiento import grupos_optimizador
+    for nombres, _, decae, _ in grupos_optimizador(m):
+        assert not decae or not any(n.endswith(('sel_log_a', 'sel_d')) for n in nombres)
+    # the other blocks' weights for a seed are what they were
+    assert list(BloqueLocal(8, 4, 16).state_dict()) == ['ln1.weight', 'ln1.bias', 'conv.weight', 'conv.bias', 'ln2.weight', 'ln2.bias',
+                                                        'ff.0.weight', 'ff.0.bias', 'ff.2.weight', 'ff.2.bias']
