@@ -157,7 +157,9 @@ def test_memory_modes_give_the_same_step(checkpoint):
         assert (a - b).norm() <= 1e-5 * b.norm() + 1e-9, n
 
 
-def test_training_runs_and_its_weights_move():
+def test_training_runs_and_its_weights_move(monkeypatch):
+    for b in (torch.backends.cuda.matmul, torch.backends.cudnn):      # entrenar allows what other tests' products must not have
+        monkeypatch.setattr(b, 'allow_tf32', b.allow_tf32)
     m, lotes = _modelo(2, 64)
     antes = {n: p.detach().clone() for n, p in m.named_parameters()}
     piezas = torch.randint(0, 97, (3000,))
