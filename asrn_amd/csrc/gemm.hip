@@ -79,7 +79,8 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
 
 // One operand's share of a K step: R rows (of op(A), or columns of op(B)) by BK. T: stored with the rows contiguous
 // (element (k, r) at k * ld + r), else with k contiguous. A thread holds U units of 8 consecutive k.
-template <int R, bool T, bool F32, int BK, int THR = kGemmThr>
+// ANY (F32, k-contiguous): rows on any 4-byte boundary, of any length.
+template <int R, bool T, bool F32, int BK, int THR = kGemmThr, bool ANY = false>
 struct Operand {
   static constexpr int CH = BK / 8;                          // units per row
   static constexpr int U = R * CH / THR;                     // units per thread
@@ -119,6 +120,15 @@ struct Operand {
         const int row = r0 + r < rows ? r0 + r : rows - 1, k = k0 + 8 * c;
         const float* p = x + (int64_t)row * ld + k;
         float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+        if constexpr (ANY) {
+          if (FULL) {
+            __builtin_memcpy(f[i], p, 32);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[i][j] = k + j < k1 ? p[j] : 0.f;
+          }
+          continue;
+        }
         if (FULL || k < k1) lo = *reinterpret_cast<const float4*>(p);
         if (FULL || k + 4 < k1) hi = *reinterpret_cast<const float4*>(p + 4);
         f[i][0] = lo.x; f[i][1] = lo.y; f[i][2] = lo.z; f[i][3] = lo.w;
@@ -216,8 +226,8 @@ constexpr int step_k() { return !F32 || BM + BN == 128 ? 64 : 32; }
 template <int BM, int BN, bool TA, bool TB, bool F32, bool EPI = false>
 __global__ __launch_bounds__(kGemmThr, 2) void k_gemm(Gemm g, Epilogue ep) {
   constexpr int BK = step_k<BM, BN, F32>();
-  using OA = Operand<BM, TA, F32, BK>;
-  using OB = Operand<BN, TB, F32, BK>;
+  using OA = Operand<BM, TA, F32, BK, kGemmThr, EPI>;
+  using OB = Operand<BN, TB, F32, BK, kGemmThr, EPI>;
   constexpr int MI = BM / 64, NI = BN / 64, PL = OA::PL;
   // the waves' blocks alternate down a tile: 4 waves of BLOCK rows, then the next unit's
   constexpr bool kSigned = F32 && !TA;
@@ -732,9 +742,6 @@ int64_t gemm_epilogue_workspace(int64_t M, int64_t N, int64_t K) {
 int gemm_epilogue(const float* x, int64_t ldx, const float* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e,
                   void* workspace, int64_t workspace_bytes, hipStream_t st) {
   const char* what = "asrn_linear_act_fwd";
-  ASRN_REQUIRE(K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0,
-               "%s: fp32 operands of more than a few rows must be 16-byte aligned, K and their leading dimensions multiples of 4 "
-               "(K=%lld ldx=%lld ldw=%lld)", what, (long long)K, (long long)ldx, (long long)ldw);
   const Plan p = plan_of(M, N, K, true, 0, 0);
   Gemm g = {x, ldx, w, ldw, nullptr, 0, (int)M, (int)N, (int)K, nullptr, 0, nullptr, (float*)workspace, (M * N + 3) / 4 * 4,
             p.splits, p.kper, (int)((M + p.bm - 1) / p.bm), (int)((N + p.bn - 1) / p.bn), p.tail, p.tsplits, p.tkper};

@@ -4,15 +4,25 @@
 
 namespace asrn {
 
-// GELU for products of 16-bit operands: Phi(-|x|) = t p(t) exp(-x^2 / 2) with Abramowitz and Stegun's 7.1.26, erfc within 1.5e-7 and
-// so GELU within 8e-8 |x|: one exponential and one reciprocal (erff costs about twice the instructions, and the epilogue counts
-// beside the product)
-__device__ __forceinline__ float gelu16(float x) {
+// For products of 16-bit operands: Phi(-|x|) = t p(t) exp(-x^2 / 2) with Abramowitz and Stegun's 7.1.26, erfc within 1.5e-7, so
+// GELU within 8e-8 |x| and its derivative within 8e-8: one exponential and one reciprocal (erff costs about twice the
+// instructions, and the epilogue counts beside the product). -> t p(t), *e = exp(-x^2 / 2)
+__device__ __forceinline__ float normal_tail(float x, float* e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
   const float z = x * 0.84932180028801904f;                        // sqrt(log2(e) / 2)
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
-                                   0.5f * -0.284496736f), 0.5f * 0.254829592f);
-  return fmaf(-fabsf(fminf(x, 64.f)), p * __builtin_amdgcn_exp2f(-z * z), fmaxf(x, 0.f));     // infinity stays itself
+  *e = __builtin_amdgcn_exp2f(-z * z);
+  return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                          0.5f * -0.284496736f), 0.5f * 0.254829592f);
+}
+__device__ __forceinline__ float gelu16(float x) {
+  float e;
+  const float p = normal_tail(x, &e);
+  return fmaf(-fabsf(fminf(x, 64.f)), p * e, fmaxf(x, 0.f));       // infinity stays itself
+}
+__device__ __forceinline__ float gelu16_grad(float x) {
+  float e;
+  const float p = normal_tail(x, &e), m = e * fmaf(-0.39894228040143268f, fabsf(x), p);
+  return x < 0.f ? m : 1.f - m;
 }
 
 struct Epilogue {

@@ -315,6 +315,59 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_direct(Linear g) {
   finish_all<T, MI, NI, THR>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(lds0));
 }
 
+// The sums over a wave's lanes of V values each (V = 16, 32 or 64), one a lane: at every distance a lane gives half of its
+// values away and adds the other half's; lane l ends with value sum_of_lane(l). The halves and the rows of 16 change places
+// by one instruction a pair; distances 8 to 1 by DPP (half a row mirrored stands for distance 4: its bit differs too).
+template <int V>
+__device__ __forceinline__ int sum_of_lane(int lane) {
+  const int b5 = lane >> 5 & 1, b4 = lane >> 4 & 1, low = (lane >> 3 & 1) * 8 + (lane >> 2 & 1) * 4 + (lane & 3);
+  if (V == 64) return b5 * 32 + b4 * 16 + low;
+  if (V == 32) return b4 ? -1 : b5 * 16 + low;
+  return b5 || b4 ? -1 : low;
+}
+template <int CTRL>
+__device__ __forceinline__ float give(float keep, float away) { return keep + dpp<CTRL>(away); }
+template <int V>
+__device__ __forceinline__ float lane_sums(float* v, int lane) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (V == 64) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 32]), false, false);
+      v[i] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 16]), false, false);
+      v[i] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+    }
+  } else if constexpr (V == 32) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 16]), false, false);
+      v[i] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += __shfl_xor(v[i], 16, 64);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] += __shfl_xor(v[i], 32, 64);
+      v[i] += __shfl_xor(v[i], 16, 64);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = give<0x128>(lane & 8 ? v[i + 8] : v[i], lane & 8 ? v[i] : v[i + 8]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = give<0x141>(lane & 4 ? v[i + 4] : v[i], lane & 4 ? v[i] : v[i + 4]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = give<0x4E>(lane & 2 ? v[i + 2] : v[i], lane & 2 ? v[i] : v[i + 2]);
+  return give<0xB1>(lane & 1 ? v[1] : v[0], lane & 1 ? v[0] : v[1]);
+#else
+  return 0.f;
+#endif
+}
+
 // Few rows (M <= 16): W is read once and each of its values meets every row, so the weights' bytes bound it. A wave takes 4
 // rows of W (columns of y) and all rows of x; its lanes run along k in units of 4, each with 4 x MR sums, which then
 // meet by a transposing exchange. x comes from the caches.
@@ -359,19 +412,12 @@ __global__ __launch_bounds__(256) void k_linear_rows(Linear g) {
         for (int j = 0; j < UN; ++j) acc[n][m] = fmaf(a[n][j], b[j], acc[n][m]);
     }
   }
-  // sums over the lanes, one value at a time; lane n MR + m keeps its own
-  float mine = 0.f;
-#pragma unroll
-  for (int n = 0; n < NR; ++n)
-#pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      const float v = wave_sum(acc[n][m]);
-      if (lane == n * MR + m) mine = v;
-    }
+  const float mine = lane_sums<NR * MR>(&acc[0][0], lane);
   red[wave][lane] = mine;
   __syncthreads();
-  if (wave == 0 && lane < NR * MR) {
-    const int n = n0 + lane / MR, m = m0 + lane % MR;
+  const int mine_is = sum_of_lane<NR * MR>(lane);
+  if (wave == 0 && mine_is >= 0) {
+    const int n = n0 + mine_is / MR, m = m0 + mine_is % MR;
     if (n < g.N && m < g.M) {
       const float v = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
       g.e.template one<T>(m, n, v);
@@ -398,7 +444,8 @@ __global__ __launch_bounds__(256) void k_act_grad(const G* gy, int64_t ldg, cons
       if (act != kActNone) load_v<V>(pre + r * ldp + c, p);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (act != kActNone) g[v] *= activate_grad(p[v], act);
+        if (act == kActGelu) g[v] *= sizeof(T) == 2 ? gelu16_grad(p[v]) : activate_grad(p[v], kActGelu);
+        else if (act == kActSilu) g[v] *= activate_grad(p[v], kActSilu);
         s[v] += g[v];
       }
       if (gp) store_v<V>(gp + r * N + c, g);

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -63,6 +64,14 @@ struct Biblioteca {
   decltype(&asrn_selective_bwd_workspace) sel_bwd_ws;
   decltype(&asrn_selective_bwd) sel_bwd;
   decltype(&asrn_selective_step) sel_paso;
+  decltype(&asrn_linear_act_workspace) act_ws;
+  decltype(&asrn_linear_act_fwd) act_fwd;
+  decltype(&asrn_act_grad_workspace) actg_ws;
+  decltype(&asrn_act_grad) act_grad;
+  decltype(&asrn_gemm_workspace) gemm_ws;
+  decltype(&asrn_gemm) gemm;
+  decltype(&asrn_column_sums_workspace) cols_ws;
+  decltype(&asrn_column_sums) cols;
 } lib;
 
 void vale(int rc, const char* que) {
@@ -526,6 +535,147 @@ std::pair<Tensor, Tensor> paso_selectivo(const Tensor& u, const Tensor& dl, cons
   return {y, sig};
 }
 
+// ---- the product with its epilogue ----------------------------------------------------------------------------------------
+// (M, k) rows of (..., k): adjacent values, a row stride that holds a row (an expanded tensor's does not) and fits the
+// kernels' 32-bit offsets
+Tensor filas(const Tensor& t) {
+  const int64_t k = t.size(-1);
+  Tensor r = (t.dim() == 2 ? t : t.reshape({k ? t.numel() / k : 0, k}));
+  return r.size(0) > 1 && (r.stride(0) < k || r.stride(0) >= (1 << 21)) ? r.contiguous()
+         : k > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+int64_t paso_fila(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
+
+// How the gradients' products run, by the rules in lineal.py: x's and w's on asrn_gemm, or the weight gradient as one product
+// (slabs 1) or a batch of slabs of the rows
+struct PlanLineal {
+  int64_t gx_gemm, gw_gemm, slabs;
+};
+
+Tensor producto_act(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res, int64_t act, at::ScalarType tipo_y,
+                    const Tensor& pre, const En& en) {
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0), wsb = lib.act_ws(M, N, K, tipo_de(x));
+  Tensor y = vacio({M, N}, x, tipo_y), ws = wsb > 0 ? espacio(wsb, x) : Tensor();
+  vale(lib.act_fwd(ptr(x), paso_fila(x), ptr(w), paso_fila(w), tipo_de(x), ptr(b), M, N, K, (int32_t)act, ptr(res),
+                   res.defined() ? paso_fila(res) : N, res.defined() && res.scalar_type() == at::kFloat, ptr(pre), N, ptr(y), N,
+                   tipo_y == at::kFloat, 0, ptr(ws), wsb, en.st), "asrn_linear_act_fwd");
+  return y;
+}
+
+// the operands are cast here, and only here
+struct SinAutocast {
+  c10::impl::ExcludeDispatchKeyGuard guarda{c10::autocast_dispatch_keyset};
+};
+
+struct LinealActiva : Function<LinealActiva> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opcional& b_, const Opcional& res_,
+                               int64_t act, int64_t dt_, const PlanLineal& plan) {
+    En en(x);
+    const SinAutocast sin;
+    const auto dt = (at::ScalarType)dt_;
+    const Tensor b = o_nada(b_), res = o_nada(res_);
+    const Tensor x2 = filas(x.to(dt)), wc = filas(w.to(dt)), bc = b.defined() ? b.to(dt).contiguous() : b;
+    Tensor pre = act ? vacio({x2.size(0), wc.size(0)}, x2, dt) : Tensor();
+    Tensor y = producto_act(x2, wc, bc, res.defined() ? filas(res) : res, act, res.defined() ? res.scalar_type() : dt, pre, en);
+    auto forma = x.sizes().vec();
+    ctx->save_for_backward({x2, wc, pre});
+    ctx->saved_data["n"] = std::vector<int64_t>{act, dt_, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
+                                                b.defined() ? (int64_t)b.scalar_type() : -1, res.defined(), plan.gx_gemm, plan.gw_gemm,
+                                                plan.slabs};
+    ctx->saved_data["f"] = forma;
+    forma.back() = wc.size(0);
+    return {y.view(forma)};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    una_vez("lineal_activa");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], &pre = s[2];
+    const auto n = ctx->saved_data["n"].toIntVector();
+    const auto dt = (at::ScalarType)n[1];
+    const bool con_b = n[4] >= 0, con_res = n[5] != 0;
+    En en(x);
+    const SinAutocast sin;
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+    const bool qx = ctx->needs_input_grad(0), qw = ctx->needs_input_grad(1), qb = con_b && ctx->needs_input_grad(2);
+    Tensor gx, gw, gb, cols;
+    if (qx || qw || qb) {
+      Tensor g2 = filas(g[0]), gp = g2;
+      const bool propio = n[0] != 0 || g2.scalar_type() != dt;
+      const bool suma = qb && (propio || !(qw && n[7]));          // else the weight gradient's product sums the columns too
+      if (M && N && (propio || suma)) {
+        const int64_t wsb = suma ? lib.actg_ws(M, N) : 0;
+        Tensor ws = suma ? espacio(wsb, x) : Tensor();
+        if (propio) gp = vacio({M, N}, x, dt);
+        if (suma) cols = vacio({N}, x);
+        vale(lib.act_grad(ptr(g2), paso_fila(g2), g2.scalar_type() == at::kFloat, ptr(pre), N, tipo_de(x), M, N, (int32_t)n[0],
+                          propio ? ptr(gp) : nullptr, f32(cols), ptr(ws), wsb, en.st), "asrn_act_grad");
+      } else {
+        if (suma) cols = at::zeros({N}, x.options().dtype(at::kFloat));
+        if (propio) gp = g2.to(dt);
+      }
+      if (qx) {
+        if (n[6]) {
+          const Tensor gc = alineado(gp.contiguous());
+          gx = vacio({M, K}, x);
+          const int64_t wsb = lib.gemm_ws(M, K, N, 0, 0, 0, 0);
+          Tensor ws = espacio(wsb, x);
+          vale(lib.gemm(ptr(gc), N, 0, ptr(w), w.stride(0), 0, 0, f32(gx), K, M, K, N, nullptr, 0, nullptr, 0, 0, ptr(ws), wsb, en.st),
+               "asrn_gemm");
+        } else {
+          gx = at::mm(gp, w);
+        }
+        gx = gx.to((at::ScalarType)n[2]).view(ctx->saved_data["f"].toIntVector());
+      }
+      if (qw) {
+        if (n[7]) {
+          const Tensor gc = alineado(gp.contiguous());
+          gw = vacio({N, K}, x);
+          const bool columnas = qb && !cols.defined();
+          if (columnas) cols = vacio({N}, x);
+          const int32_t bf = es16(x);
+          const int64_t wsb = lib.gemm_ws(N, K, M, bf, columnas, 0, 0);
+          Tensor ws = espacio(wsb, x);
+          vale(lib.gemm(ptr(gc), N, 1, ptr(x), x.stride(0), 0, bf, f32(gw), K, N, K, M, nullptr, 0, columnas ? f32(cols) : nullptr, 0, 0,
+                        ptr(ws), wsb, en.st), "asrn_gemm");
+        } else if (n[8] <= 1) {
+          gw = at::mm(gp.t(), x);
+        } else {
+          // left operand: the transposed slab of gp; right operand: x's slab as stored (never a transposed view)
+          const int64_t S = n[8];
+          const Tensor partes = at::bmm(gp.contiguous().view({S, M / S, N}).transpose(1, 2),
+                                        x.contiguous().view({S, M / S, K}));
+          if (dt == at::kHalf) {
+            gw = partes.sum(0, false, at::kFloat);
+          } else {
+            gw = vacio({N, K}, x);
+            const int64_t wsb = lib.cols_ws(S, N * K);
+            Tensor ws = espacio(wsb, x);
+            vale(lib.cols(ptr(partes), es16(x), S, N * K, N * K, f32(gw), ptr(ws), wsb, en.st), "asrn_column_sums");
+          }
+        }
+        gw = gw.to((at::ScalarType)n[3]);
+      }
+      if (qb) gb = cols.to((at::ScalarType)n[4]);
+    }
+    return {gx, gw, gb, con_res && ctx->needs_input_grad(con_b ? 3 : 2) ? g[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor lineal_activa(const Tensor& x, const Tensor& w, const Opcional& b, const Opcional& res, int64_t act, at::ScalarType dt,
+                     int64_t gx_gemm, int64_t gw_gemm, int64_t slabs) {
+  const Tensor bt = o_nada(b), rt = o_nada(res);
+  if (con_gradiente({&x, &w, &bt, &rt}))
+    return LinealActiva::apply(x, w, b, res, act, (int64_t)dt, PlanLineal{gx_gemm, gw_gemm, slabs})[0];
+  En en(x);
+  const SinAutocast sin;
+  const Tensor y = producto_act(filas(x.to(dt)), filas(w.to(dt)), bt.defined() ? bt.to(dt).contiguous() : bt,
+                                rt.defined() ? filas(rt) : rt, act, rt.defined() ? rt.scalar_type() : dt, Tensor(), en);
+  auto forma = x.sizes().vec();
+  forma.back() = w.size(0);
+  return y.view(forma);
+}
+
 // Whether a graph recorded on the default stream still holds one of these leaves' accumulators. A backward inside a
 // capture would run it on that stream, which no capture may wait for.
 bool hojas_en_uso(const std::vector<Tensor>& hojas) {
@@ -566,6 +716,14 @@ void iniciar(const py::function& direccion, py::object error) {
   de(lib.sel_bwd_ws, "asrn_selective_bwd_workspace");
   de(lib.sel_bwd, "asrn_selective_bwd");
   de(lib.sel_paso, "asrn_selective_step");
+  de(lib.act_ws, "asrn_linear_act_workspace");
+  de(lib.act_fwd, "asrn_linear_act_fwd");
+  de(lib.actg_ws, "asrn_act_grad_workspace");
+  de(lib.act_grad, "asrn_act_grad");
+  de(lib.gemm_ws, "asrn_gemm_workspace");
+  de(lib.gemm, "asrn_gemm");
+  de(lib.cols_ws, "asrn_column_sums_workspace");
+  de(lib.cols, "asrn_column_sums");
   static PyObject* clase;                     // held to the process's end
   clase = error.release().ptr();
   py::register_exception_translator([](std::exception_ptr p) {
@@ -592,4 +750,5 @@ PYBIND11_MODULE(_nodos, m) {
   m.def("paso_conv_canal", &paso_conv_canal, Libre());
   m.def("selectivo", &selectivo, Libre());
   m.def("paso_selectivo", &paso_selectivo, Libre());
+  m.def("lineal_activa", &lineal_activa, Libre());
 }

@@ -275,101 +275,23 @@ TIPOS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVACIONES = {None: 0, 'gelu': 1, 'silu': 2}
 
 
-def _en(t, nombre, *args):
-    """_lib.call on t's device's current stream, with that device as the current one."""
-    i = t.device.index
-    if torch.cuda.current_device() == i:
-        return _lib.call(nombre, *args, torch._C._cuda_getCurrentRawStream(i))
-    with torch.cuda.device(i):
-        return _lib.call(nombre, *args, torch._C._cuda_getCurrentRawStream(i))
-
-
-def _dir(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _filas(t):
-    """_rows whose row stride holds a row (an expanded tensor's does not) and fits the kernels' 32-bit offsets."""
-    t = _rows(t)
-    return t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) < 1 << 21 else t.contiguous()
-
-
-def _cuatro(t):
-    """An fp32 operand of asrn_gemm's form: rows of a multiple of 4, 16-byte aligned; else a copy padded with zeros."""
-    if t.shape[1] % 4 == 0 and _apto(t):
-        return t
-    return F.pad(t, (0, -t.shape[1] % 4)) if t.shape[1] % 4 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _activada(x2, w, b, act, res, tipo_y, con_pre):
-    """(y, the activation's input or None) of rows x2 (M, K), w (N, K), b and res (M, N)."""
-    (M, K), N = x2.shape, w.shape[0]
-    y = torch.empty((M, N), dtype=tipo_y, device=x2.device)
-    pre = torch.empty((M, N), dtype=x2.dtype, device=x2.device) if con_pre else None
-    if M == 0 or N == 0:
-        return y, pre
-    if x2.dtype == torch.float32 and M > 16:
-        x2, w = _cuatro(x2), _cuatro(w)
-        K = x2.shape[1]
-    wsb = _lib.query('asrn_linear_act_workspace', M, N, K, TIPOS[x2.dtype])
-    ws = torch.empty((wsb,), dtype=torch.uint8, device=x2.device) if wsb > 0 else None
-    _en(x2, 'asrn_linear_act_fwd', x2.data_ptr(), max(x2.stride(0), K), w.data_ptr(), max(w.stride(0), K), TIPOS[x2.dtype], _dir(b), M,
-        N, K, act, _dir(res), N if res is None else max(res.stride(0), N), int(res is not None and res.dtype == torch.float32),
-        _dir(pre), N, y.data_ptr(), N, int(tipo_y == torch.float32), 0, _dir(ws), wsb)
-    return y, pre
-
-
-def _antes(g2, pre, act, dt, columnas):
-    """(gy act'(pre) in dt, its fp32 column sums or None): g2 (M, N) fp32 or dt."""
-    M, N = g2.shape
-    gp = torch.empty((M, N), dtype=dt, device=g2.device)
-    cols = torch.zeros((N,), dtype=torch.float32, device=g2.device) if columnas and M == 0 else \
-        torch.empty((N,), dtype=torch.float32, device=g2.device) if columnas else None
-    if M and N:
-        wsb = _lib.query('asrn_act_grad_workspace', M, N) if columnas else 0
-        ws = torch.empty((wsb,), dtype=torch.uint8, device=g2.device) if wsb > 0 else None
-        _en(g2, 'asrn_act_grad', g2.data_ptr(), max(g2.stride(0), N), int(g2.dtype == torch.float32), _dir(pre), N, TIPOS[dt], M, N, act,
-            gp.data_ptr(), _dir(cols), _dir(ws), wsb)
-    return gp, cols
-
-
-class _LinealActiva(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, x, w, b, res, act, dt):
-        xc, wc = x.to(dt), w.to(dt)
-        x2, wc = _filas(xc), _filas(wc)
-        res2 = None if res is None else _filas(res)
-        y, pre = _activada(x2, wc, None if b is None else b.to(dt).contiguous(), act, res2, dt if res is None else res.dtype, act != 0)
-        ctx.save_for_backward(x2, wc, pre)
-        ctx.meta = (x.shape, x.dtype, w.dtype, None if b is None else b.dtype, act, dt)
-        return y.view(*x.shape[:-1], w.shape[0])
-
-    @staticmethod
-    def backward(ctx, g):
-        if torch.is_grad_enabled():
-            raise RuntimeError('lineal_activa: its gradient cannot be recorded (create_graph=True), the kernels have no second '
-                               'derivative')
-        x2, wc, pre = ctx.saved_tensors
-        forma, xdt, wdt, bdt, act, dt = ctx.meta
-        quiere = ctx.needs_input_grad
-        g2 = _filas(g)
-        gx = gw = gb = None
-        con_sesgo = bdt is not None and quiere[2]
-        if quiere[0] or quiere[1] or con_sesgo:
-            with torch.autocast(device_type=g.device.type, enabled=False):
-                gp, cols = (g2, None) if act == 0 and g2.dtype == dt else _antes(g2, pre, act, dt, con_sesgo)
-                if quiere[0]:
-                    gx = (gemm(gp, False, wc, False) if gemm_ok(gp, wc, False) else gp.mm(wc)).view(forma).to(xdt)
-                if quiere[1]:
-                    gw = weight_grad(gp, x2, con_sesgo and cols is None)
-                    if con_sesgo and cols is None:
-                        gw, cols = gw
-                    gw = gw.to(wdt)
-                elif con_sesgo and cols is None:
-                    cols = column_sums(gp)
-                gb = cols.to(bdt) if con_sesgo else None
-        return gx, gw, gb, g if quiere[3] else None, None, None
+def _plan_gradientes(x, w, M, N, K, dt):
+    """How the backward of lineal_activa forms x's gradient (on asrn_gemm or not) and w's (on asrn_gemm, or in so many slabs),
+    by the rules above for rows of a dense gradient (M, N), x (M, K) and w (N, K) in dt."""
+    f32 = dt == torch.float32
+    # _apto for both operands: dense rows of a multiple of 4 (fresh tensors and contiguous inputs are aligned)
+    cuatro = N % 4 == 0 and K % 4 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0
+    gx = f32 and cuatro and M * N * K >= MIN_PRODUCTO and K >= 64 and w.is_contiguous() and w.data_ptr() % 16 == 0
+    peso = N * K
+    if not cuatro or dt == torch.float16 or M == 0:
+        gw = False
+    elif f32:
+        gw = True
+    elif peso >= MAX_SLAB_WEIGHT:
+        gw = M * FICHAS_PESO[True] >= peso
+    else:
+        gw = peso <= MAX_PESO_16 or slabs_for(M, peso) == 1
+    return int(gx), int(gw), slabs_for(M, peso)
 
 
 def lineal_activa(x, w, b=None, activacion=None, residuo=None):
@@ -397,12 +319,10 @@ def lineal_activa(x, w, b=None, activacion=None, residuo=None):
             raise ValueError(f'{quien}: {nombre} is on {t.device}, x on {x.device}')
     if not x.is_cuda:
         raise RuntimeError('asrn_amd runs on the GPU only: got a CPU tensor (move the model and inputs to cuda)')
-    act = ACTIVACIONES[activacion]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b, residuo)):
-        return _LinealActiva.apply(x, w, b, residuo, act, dt)
-    y, _ = _activada(_filas(x.to(dt)), _filas(w.to(dt)), None if b is None else b.to(dt).contiguous(), act,
-                     None if residuo is None else _filas(residuo), dt if residuo is None else residuo.dtype, False)
-    return y.view(forma)
+    N, K = w.shape
+    M = x.numel() // K
+    plan = _plan_gradientes(x, w, M, N, K, dt) if torch.is_grad_enabled() else (0, 0, 1)
+    return _lib.nodos().lineal_activa(x, w, b, residuo, ACTIVACIONES[activacion], dt, *plan)
 
 
 linear_act = lineal_activa

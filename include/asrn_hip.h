@@ -778,9 +778,8 @@ int asrn_selective_step(const void* u, const void* delta, const void* B_, const 
  * The dense products of a local block (asrn/nucleo.py:969-1014) with what follows them: y = [res +] act(x W^T + bias).
  * x (M, K), W (N, K), bias (N, or null) in fp32, bf16 or fp16 (type 0, 1, 2), leading dimensions in elements (below 2^21 for x
  * and W); act 0 none, 1 GELU (erf), 2 SiLU; res (M, N, or null) and y in fp32 or in `type`; pre (or null) gets x W^T + bias in
- * `type`, for the backward. fp32 sums, results rounded once. 16-bit operands: any sizes and addresses (8 dividing K, the leading
- * dimensions and 16 bytes the addresses is the fast form); fp32 with M > 16: K and the leading dimensions multiples of 4, x
- * and W 16-byte aligned. workspace: asrn_linear_act_workspace bytes, 16-byte aligned (-1: bad sizes).
+ * `type`, for the backward. fp32 sums, results rounded once. Any sizes and addresses (for 16-bit operands, 8 dividing K, the leading
+ * dimensions and 16 bytes the addresses is the fast form). workspace: asrn_linear_act_workspace bytes, 16-byte aligned (-1: bad sizes).
  * act_grad: gp = gy act'(pre) in `type` (or null), gy in fp32 or in `type`; colsum (or null): the fp32 sums of its columns
  * before that rounding, in a fixed order; workspace (for colsum): asrn_act_grad_workspace bytes, 16-byte aligned.
  * tile (16-bit operands): 0 by the sizes, or a tile's rows << 8 | columns (256 << 8: 256 x 256).

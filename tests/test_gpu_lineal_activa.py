@@ -151,6 +151,13 @@ def test_under_autocast():
     assert all(g.dtype == F32 for g in gs)
     xb, wb, bb = (t.detach().to(BF16) for t in (x, w, b))
     assert torch.equal(y, asrn_amd.lineal_activa(xb, wb, bb, 'gelu', res))
+    # a backward inside an autocast region is the one outside: the operands were cast, or not, by the call
+    x, w = r(300, 40).requires_grad_(), r(24, 40).requires_grad_()
+    y, gy = asrn_amd.lineal_activa(x, w, activacion='silu'), r(300, 24)
+    fuera = torch.autograd.grad(y, (x, w), gy, retain_graph=True)
+    with torch.autocast('cuda', dtype=BF16):
+        dentro = torch.autograd.grad(y, (x, w), gy)
+    assert all(torch.equal(a, b) for a, b in zip(fuera, dentro))
 
 
 def test_empty():

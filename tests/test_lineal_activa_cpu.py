@@ -47,8 +47,6 @@ def test_entries_refuse():
     falla(fwd(ldy=4), 'leading')
     falla(fwd(ldw=1 << 21), '2^21')
     falla(fwd(tile=7), 'unknown tile 7')
-    falla(fwd(K=6, ldx=6, ldw=6), 'multiples of 4')
-    falla(fwd(x=68), '16-byte')
     falla(fwd(M=64, N=64, K=4096, ldx=4096, ldw=4096, ldy=64), 'workspace')
     assert fwd(M=0) == 0 and fwd(N=0) == 0
     assert lib.asrn_linear_act_workspace(64, 64, 4096, 0) > 0 and lib.asrn_linear_act_workspace(64, 64, 4096, 1) == 0
