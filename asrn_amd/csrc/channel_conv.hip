@@ -5,7 +5,8 @@
 // z is read once, y written once. The backward walks the same way: it forms the pre-activation again from z, with it the
 // gradient before the activation, g[t], keeps the last k - 1 of those too, and writes dz[t - (k - 1)] = sum_j w[c, j]
 // g[t - j] while it gathers dw and dbias of its piece; it reads k - 1 rows past the piece's end. One partial row a piece,
-// added in order (group_sums): no atomics. Both are bound by memory.
+// added in order (group_sums): no atomics. Both are bound by memory: 8 x 2048 x 768 bf16 with k = 4 and SiLU takes 15 us (3.4
+// TB/s) and 27 (2.8 TB/s, and 5 for the pieces' sums).
 #include "types.h"
 
 namespace asrn {
@@ -24,29 +25,62 @@ struct ChannelConv {
   int d, k, act, piece, pieces, groups;   // a piece's tokens, pieces a text, groups of V channels
 };
 
-// K: the taps that the registers hold, k <= K (the taps past k are skipped by a uniform branch)
-template <typename T, int V, int K>
+// The taps of a lane's V channels, w[j][v]: channel v's tap j, j < K. EXACT (k = K, V = 4): its 4 K floats are 16-byte vectors
+// next to each other; else tap by tap, 0 past k.
+template <int V, int K, bool EXACT>
+__device__ __forceinline__ void load_taps(const float* w, int k, float (&t)[K][V]) {
+  if constexpr (EXACT) {
+    float f[V * K];
+#pragma unroll
+    for (int i = 0; i < V * K / 4; ++i) {
+      const float4 q = reinterpret_cast<const float4*>(w)[i];
+      f[4 * i] = q.x; f[4 * i + 1] = q.y; f[4 * i + 2] = q.z; f[4 * i + 3] = q.w;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < K; ++j) t[j][v] = f[v * K + j];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < K; ++j) t[j][v] = j < k ? w[v * k + j] : 0.f;
+  }
+}
+
+// K: the taps that the registers hold, k <= K (EXACT: k = K). The taps past k are skipped by a uniform branch. The register of
+// the tap j tokens back is w[k - 1 - j]: w is read reversed, so that its number does not depend on k.
+template <typename T, int V, int K, bool EXACT>
 __global__ __launch_bounds__(kConvThreads) void k_channel_conv(ChannelConv a) {
   constexpr int R = 8;
   const int64_t i = (int64_t)blockIdx.x * kConvThreads + threadIdx.x;
   const int64_t row = i / a.groups;
   const int64_t b = row / a.pieces;
   if (b >= a.B) return;
-  const int c = (int)(i % a.groups) * V;
+  const int c = (int)(i % a.groups) * V, k = EXACT ? K : a.k;
   const int64_t t0 = (row % a.pieces) * a.piece, t1 = t0 + a.piece < a.L ? t0 + a.piece : a.L;
   const T* z = static_cast<const T*>(a.z) + b * a.zb + c;
   T* y = static_cast<T*>(a.out) + b * a.L * a.d + c;
   float w[K][V], bias[V], x[K - 1 + R][V];          // w[j]: the tap j tokens back
+  if constexpr (EXACT) {
+    float t[K][V];
+    load_taps<V, K, true>(a.w + (int64_t)c * K, K, t);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    bias[v] = a.bias ? a.bias[c + v] : 0.f;
+    for (int j = 0; j < K; ++j)
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j][v] = j < a.k ? a.w[(int64_t)(c + v) * a.k + a.k - 1 - j] : 0.f;
+      for (int v = 0; v < V; ++v) w[j][v] = t[K - 1 - j][v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][v] = j < k ? a.w[(int64_t)(c + v) * k + k - 1 - j] : 0.f;
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[c + v] : 0.f;
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {                 // x[j]: token t0 - (K - 1) + j
     const int64_t t = t0 - (K - 1) + j;
-    if (t >= 0 && K - 1 - j < a.k) load_v<V>(z + t * a.zt, x[j]);
+    if (t >= 0 && K - 1 - j < k) load_v<V>(z + t * a.zt, x[j]);
     else
 #pragma unroll
       for (int v = 0; v < V; ++v) x[j][v] = 0.f;
@@ -62,7 +96,7 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv(ChannelConv a) {
       for (int v = 0; v < V; ++v) s[v] = bias[v];
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (j < a.k)
+        if (j < k)
 #pragma unroll
           for (int v = 0; v < V; ++v) s[v] = fmaf(w[j][v], x[K - 1 + r - j][v], s[v]);
 #pragma unroll
@@ -76,35 +110,35 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv(ChannelConv a) {
   }
 }
 
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool EXACT>
 __global__ __launch_bounds__(kConvThreads) void k_channel_conv_bwd(ChannelConv a) {
   constexpr int R = 4;
   const int64_t i = (int64_t)blockIdx.x * kConvThreads + threadIdx.x;
   const int64_t row = i / a.groups;
   const int64_t b = row / a.pieces;
   if (b >= a.B) return;
-  const int c = (int)(i % a.groups) * V;
+  const int c = (int)(i % a.groups) * V, k = EXACT ? K : a.k;
   const int64_t t0 = (row % a.pieces) * a.piece, t1 = t0 + a.piece < a.L ? t0 + a.piece : a.L;
-  const int64_t end = t1 + a.k - 1 < a.L ? t1 + a.k - 1 : a.L;       // the tokens whose g this piece's dz needs
+  const int64_t end = t1 + k - 1 < a.L ? t1 + k - 1 : a.L;       // the tokens whose g this piece's dz needs
   const T* z = static_cast<const T*>(a.z) + b * a.zb + c;
   const T* gy = static_cast<const T*>(a.g) + b * a.L * a.d + c;
   T* dz = static_cast<T*>(a.out) + b * a.L * a.d + c;
-  float w[K][V], u[K][V], bias[V], dw[K][V], db[V], x[K - 1 + R][V], g[K - 1 + R][V];
+  float u[K][V], w[K][V], bias[V], dw[K][V], db[V], x[K - 1 + R][V], g[K - 1 + R][V];
+  load_taps<V, K, EXACT>(a.w + (int64_t)c * k, k, u);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     bias[v] = a.bias ? a.bias[c + v] : 0.f;
     db[v] = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      w[j][v] = j < a.k ? a.w[(int64_t)(c + v) * a.k + a.k - 1 - j] : 0.f;     // the tap j tokens back
-      u[j][v] = j < a.k ? a.w[(int64_t)(c + v) * a.k + j] : 0.f;
+      w[j][v] = EXACT ? u[K - 1 - j][v] : j < k ? a.w[(int64_t)(c + v) * k + k - 1 - j] : 0.f;     // the tap j tokens back
       dw[j][v] = 0.f;
     }
   }
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     const int64_t t = t0 - (K - 1) + j;
-    if (t >= 0 && K - 1 - j < a.k) load_v<V>(z + t * a.zt, x[j]);
+    if (t >= 0 && K - 1 - j < k) load_v<V>(z + t * a.zt, x[j]);
     else
 #pragma unroll
       for (int v = 0; v < V; ++v) x[j][v] = 0.f;
@@ -112,7 +146,7 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv_bwd(ChannelConv a
     for (int v = 0; v < V; ++v) g[j][v] = 0.f;
   }
   // tokens t0 .. t1 + k - 2; from the text's end on g is 0
-  for (int64_t t = t0; t < t1 + a.k - 1; t += R) {
+  for (int64_t t = t0; t < t1 + k - 1; t += R) {
     float e[R][V];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -127,29 +161,27 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv_bwd(ChannelConv a
       for (int v = 0; v < V; ++v) s[v] = bias[v];
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (j < a.k)
+        if (j < k)
 #pragma unroll
           for (int v = 0; v < V; ++v) s[v] = fmaf(w[j][v], x[K - 1 + r - j][v], s[v]);
       const bool here = t + r < end, mine = t + r < t1;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float q = here ? e[r][v] * activate_grad(s[v], a.act) : 0.f;
+        const float q = here ? e[r][v] * activate_grad(s[v], a.act) : 0.f, m = mine ? q : 0.f;
         g[K - 1 + r][v] = q;
-        if (mine) {
-          db[v] += q;
+        db[v] += m;
 #pragma unroll
-          for (int j = 0; j < K; ++j)
-            if (j < a.k) dw[j][v] = fmaf(q, x[K - 1 + r - j][v], dw[j][v]);
-        }
+        for (int j = 0; j < K; ++j)
+          if (j < k) dw[j][v] = mine ? fmaf(m, x[K - 1 + r - j][v], dw[j][v]) : dw[j][v];
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) s[v] = 0.f;
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (j < a.k)
+        if (j < k)
 #pragma unroll
           for (int v = 0; v < V; ++v) s[v] = fmaf(u[j][v], g[K - 1 + r - j][v], s[v]);
-      const int64_t o = t + r - (a.k - 1);
+      const int64_t o = t + r - (k - 1);
       if (o >= t0 && o < t1) store_v<V>(dz + o * a.d, s);
     }
 #pragma unroll
@@ -160,11 +192,11 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv_bwd(ChannelConv a
         g[j][v] = g[R + j][v];
       }
   }
-  float* p = a.part + row * (int64_t)(a.k + 1) * a.d + c;
+  float* p = a.part + row * (int64_t)(k + 1) * a.d + c;
 #pragma unroll
   for (int j = 0; j < K; ++j)
-    if (j < a.k) store_v<V>(p + (int64_t)(a.k - 1 - j) * a.d, dw[j]);
-  store_v<V>(p + (int64_t)a.k * a.d, db);
+    if (j < k) store_v<V>(p + (int64_t)(k - 1 - j) * a.d, dw[j]);
+  store_v<V>(p + (int64_t)k * a.d, db);
 }
 
 // One token: a lane takes a channel, its window of k - 1 values shifts by one.
@@ -189,9 +221,10 @@ __global__ __launch_bounds__(kConvThreads) void k_channel_conv_step(const T* z, 
   y[i] = (T)activate(fmaf(wc[k - 1], (float)x, s), act);
 }
 
-// A piece's tokens: enough lanes to fill the card (2 waves a SIMD), 16 at least for the k - 1 rows that a piece reads again.
+// A piece's tokens: enough lanes for 3 waves a SIMD, 16 at least for the k - 1 rows that a piece reads again. 8 x 2048 x 768 bf16,
+// k = 4, forward / backward in us: pieces of 8 16.9 / 31.6, 16 15.0 / 27.4, 32 18.2 / 31.2, 64 26.8 / 44.4.
 static int piece_of(int64_t B, int64_t L, int groups) {
-  const int64_t want = (int64_t)2 * 1024 * kWave;
+  const int64_t want = (int64_t)3 * 1024 * kWave;
   int64_t p = (B * L * groups + want - 1) / want;
   p = (p + 7) / 8 * 8;
   return (int)(p < 16 ? 16 : p > 128 ? 128 : p);
@@ -240,13 +273,13 @@ extern "C" int asrn_channel_conv_fwd(const void* z, int32_t type, int64_t stride
   return with_type(type, [&](auto t) {
     using T = decltype(t);
     if (V == 4) {
-      if (k <= 2) hipLaunchKernelGGL((k_channel_conv<T, 4, 2>), grid, thr, 0, st, a);
-      else if (k <= 4) hipLaunchKernelGGL((k_channel_conv<T, 4, 4>), grid, thr, 0, st, a);
-      else hipLaunchKernelGGL((k_channel_conv<T, 4, 8>), grid, thr, 0, st, a);
+      if (k == 4 && !((uintptr_t)w & 15)) hipLaunchKernelGGL((k_channel_conv<T, 4, 4, true>), grid, thr, 0, st, a);
+      else if (k <= 4) hipLaunchKernelGGL((k_channel_conv<T, 4, 4, false>), grid, thr, 0, st, a);
+      else hipLaunchKernelGGL((k_channel_conv<T, 4, 8, false>), grid, thr, 0, st, a);
     } else {
-      if (k <= 4) hipLaunchKernelGGL((k_channel_conv<T, 1, 4>), grid, thr, 0, st, a);
-      else if (k <= 8) hipLaunchKernelGGL((k_channel_conv<T, 1, 8>), grid, thr, 0, st, a);
-      else hipLaunchKernelGGL((k_channel_conv<T, 1, 16>), grid, thr, 0, st, a);
+      if (k <= 4) hipLaunchKernelGGL((k_channel_conv<T, 1, 4, false>), grid, thr, 0, st, a);
+      else if (k <= 8) hipLaunchKernelGGL((k_channel_conv<T, 1, 8, false>), grid, thr, 0, st, a);
+      else hipLaunchKernelGGL((k_channel_conv<T, 1, 16, false>), grid, thr, 0, st, a);
     }
     return check_launch("asrn_channel_conv_fwd");
   });
@@ -291,12 +324,12 @@ extern "C" int asrn_channel_conv_bwd(const void* z, int32_t type, int64_t stride
   const int rc = with_type(type, [&](auto t) {
     using T = decltype(t);
     if (V == 4) {
-      if (k <= 2) hipLaunchKernelGGL((k_channel_conv_bwd<T, 4, 2>), grid, thr, 0, st, a);
-      else hipLaunchKernelGGL((k_channel_conv_bwd<T, 4, 4>), grid, thr, 0, st, a);
+      if (k == 4 && !((uintptr_t)w & 15)) hipLaunchKernelGGL((k_channel_conv_bwd<T, 4, 4, true>), grid, thr, 0, st, a);
+      else hipLaunchKernelGGL((k_channel_conv_bwd<T, 4, 4, false>), grid, thr, 0, st, a);
     } else {
-      if (k <= 4) hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 4>), grid, thr, 0, st, a);
-      else if (k <= 8) hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 8>), grid, thr, 0, st, a);
-      else hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 16>), grid, thr, 0, st, a);
+      if (k <= 4) hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 4, false>), grid, thr, 0, st, a);
+      else if (k <= 8) hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 8, false>), grid, thr, 0, st, a);
+      else hipLaunchKernelGGL((k_channel_conv_bwd<T, 1, 16, false>), grid, thr, 0, st, a);
     }
     return check_launch("asrn_channel_conv_bwd");
   });
