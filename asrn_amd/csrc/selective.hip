@@ -78,6 +78,18 @@ __device__ __forceinline__ float quad_scatter(const float (&v)[4], int lane) {
   return (b1 ? r1 : r0) + quad_xor2(b1 ? r0 : r1);
 }
 
+// a's sums over the wave's four rows of 16 lanes in lanes 0 .. 15 (and 16 .. 31), b's in lanes 32 .. 47 (and 48 .. 63)
+__device__ __forceinline__ float rows_sum(float a, float b) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  const unsigned h = __float_as_uint(__uint_as_float(q[0]) + __uint_as_float(q[1]));
+  const auto r = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+#else
+  return a + b;
+#endif
+}
+
 // What one wave's lanes write to LDS is read by its other lanes: in order in the hardware, and for the compiler here.
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -468,7 +480,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_b
   constexpr int NP = 4 * NPL, TT = kCheck, HALF = TT / 2;
   constexpr int NJ = (NPL + 3) / 4;               // values of dB (and of dC) that a lane leaves of its row's sums
   __shared__ float lds[kMaxWaves][TT * (384 + 2 * NP)];
-  __shared__ float red[TT][2][kMaxWaves * 4][NP];
+  __shared__ float red[2][TT][2][kMaxWaves][NP];  // in turns, so that a tile has one barrier
   const Place p = place_of<NPL>(s);
   const int waves = blockDim.x >> 6;
   const int64_t b = blockIdx.z, chunk = blockIdx.y, t0 = chunk * s.chunk, t1 = t0 + s.chunk < s.L ? t0 + s.chunk : s.L;
@@ -487,7 +499,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_b
   else load_state<NPL>(s.ghend ? s.ghend + b * dN : nullptr, s, p, G);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
   float dD = 0.f, dbias = 0.f;
-  const int row = p.lane >> 4, cq = (p.lane >> 2) & 3;
+  const int cq = (p.lane >> 2) & 3;
+  int turn = 0;
   T u[TT], dl[TT], z[TT], gy[TT];
   Shared<T, NPL, TT> mb, mc;
   auto load = [&](int64_t t) {
@@ -623,24 +636,21 @@ __global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_b
               vb = cq == j ? dB[4 * q + j] : vb;
               vc = cq == j ? dC[4 * q + j] : vc;
             }
-          if (4 * q + cq < NPL) {
-            red[r][0][p.wave * 4 + row][p.n0 + 4 * q + cq] = vb;
-            red[r][1][p.wave * 4 + row][p.n0 + 4 * q + cq] = vc;
-          }
+          // over the rows: dB's sum stays in the lower 32 lanes, dC's in the upper
+          const float v = rows_sum(vb, vc);
+          if (4 * q + cq < NPL && (p.lane & 16) == 0) red[turn][r][p.lane >> 5][p.wave][p.n0 + 4 * q + cq] = v;
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < TT * 2 * s.N; e += blockDim.x) {
-      const int r = e / (2 * s.N), k = e / s.N % 2, n = e % s.N;
-      if (r < left) {
-        float v = 0.f;
-        for (int w = 0; w < 4 * waves; ++w) v += red[r][k][w][n];
-        s.bc[((blockIdx.x * s.B + b) * s.L + t + r) * 2 * s.N + k * s.N + n] = v;
-      }
+    for (int e = threadIdx.x; e < TT * 2 * NP; e += blockDim.x) {
+      const int r = e / (2 * NP), k = e / NP % 2, n = e % NP;
+      float v = red[turn][r][k][0][n];
+      for (int w = 1; w < waves; ++w) v += red[turn][r][k][w][n];
+      if (r < left && n < s.N) s.bc[((blockIdx.x * s.B + b) * s.L + t + r) * 2 * s.N + k * s.N + n] = v;
     }
-    __syncthreads();
+    turn ^= 1;                                    // the next tile's sums are written elsewhere, those after it past its barrier
   }
   float* part = s.part + (b * s.chunks + chunk) * (dN + 2 * s.d);
   store_state<NPL>(part, s, p, dA);
