@@ -215,6 +215,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(Linear g) {
   finish_all<T, MI, NI, THR>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(lds));
 }
 
+// Tiles in order: 4 rows of them at a time, column after column, so that the tiles which an XCD forms at once are as many
+// down as across and read as little as they can (8192 x 2048 x 4096 in tiles of 256 x 256: row by row 130 us, so 124)
+__device__ __forceinline__ void place_tile(int t, int tm, int tn, int& m, int& n) {
+  constexpr int G = 4;
+  const int group = t / (G * tn), first = group * G, rows = tm - first < G ? tm - first : G, r = t - group * G * tn;
+  m = first + r % rows;
+  n = r / rows;
+}
+
 // 16 bytes a lane from memory to LDS, lane i's to l[i] (l: the same in every lane)
 __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rsrc, uint4* l, unsigned at, unsigned off) {
 #ifdef __HIP_DEVICE_COMPILE__                     // the host's pass does not know the 16-byte form
@@ -235,7 +244,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_direct(Linear g) {
   const int total = g.tm * g.tn, per = (total + kXcdCount - 1) / kXcdCount;
   const int tile = (int)(blockIdx.x % kXcdCount) * per + (int)(blockIdx.x / kXcdCount);
   if (tile >= total || (int)(blockIdx.x / kXcdCount) >= per) return;
-  const int m0 = tile / g.tn * BM, n0 = tile % g.tn * BN;
+  int m0, n0;
+  place_tile(tile, g.tm, g.tn, m0, n0);
+  m0 *= BM;
+  n0 *= BN;
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lc = lane >> 5;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN), wr = w_row(lr);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
@@ -425,41 +437,51 @@ __global__ __launch_bounds__(256) void k_linear_rows(Linear g) {
   }
 }
 
-// The gradient before the activation, gp = gy act'(pre), and its column sums (the bias gradient) from the unrounded values:
-// 64 lanes of V columns by 4 rows a workgroup, a slab of rows each.
-template <typename T, typename G, int V>
+// The gradient before the activation, gp = gy act'(pre), and its column sums (the bias gradient) from the unrounded values: CW
+// lanes of V columns by 256 / CW rows a workgroup, a slab of rows each, 4 rows of a lane under way at once.
+template <typename T, typename G, int V, int CW>
 __global__ __launch_bounds__(256) void k_act_grad(const G* gy, int64_t ldg, const T* pre, int64_t ldp, int act, int64_t M, int N,
                                                   int64_t slab, T* gp, float* part) {
-  __shared__ float red[4][64 * V];
-  const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6;
-  const int c = (blockIdx.x * 64 + cl) * V;
+  constexpr int RL = 256 / CW, R = 4;
+  __shared__ float red[RL][CW * V];
+  const int cl = threadIdx.x % CW, rl = threadIdx.x / CW;
+  const int c = (blockIdx.x * CW + cl) * V;
   const int64_t r0 = blockIdx.y * slab, r1 = r0 + slab < M ? r0 + slab : M;
   float s[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) s[v] = 0.f;
   if (c < N) {
-    for (int64_t r = r0 + rl; r < r1; r += 4) {
-      float g[V], p[V];
-      load_v<V>(gy + r * ldg + c, g);
-      if (act != kActNone) load_v<V>(pre + r * ldp + c, p);
+    for (int64_t r = r0 + rl; r < r1; r += R * RL) {
+      float g[R][V], p[R][V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (act == kActGelu) g[v] *= sizeof(T) == 2 ? gelu16_grad(p[v]) : activate_grad(p[v], kActGelu);
-        else if (act == kActSilu) g[v] *= activate_grad(p[v], kActSilu);
-        s[v] += g[v];
+      for (int k = 0; k < R; ++k) {
+        const int64_t q = r + k * RL < r1 ? r + k * RL : r1 - 1;       // past the slab: its last row, neither stored nor added
+        load_v<V>(gy + q * ldg + c, g[k]);
+        if (act != kActNone) load_v<V>(pre + q * ldp + c, p[k]);
       }
-      if (gp) store_v<V>(gp + r * N + c, g);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (r + k * RL >= r1) break;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (act == kActGelu) g[k][v] *= sizeof(T) == 2 ? gelu16_grad(p[k][v]) : activate_grad(p[k][v], kActGelu);
+          else if (act == kActSilu) g[k][v] *= activate_grad(p[k][v], kActSilu);
+          s[v] += g[k][v];
+        }
+        if (gp) store_v<V>(gp + (r + k * RL) * N + c, g[k]);
+      }
     }
   }
+  if (!part) return;
 #pragma unroll
   for (int v = 0; v < V; ++v) red[rl][cl * V + v] = s[v];
   __syncthreads();
-  if (rl == 0 && c < N && part) {
+  for (int i = threadIdx.x; i < CW * V; i += 256) {
+    const int64_t n = (int64_t)blockIdx.x * CW * V + i;
+    float v = red[0][i];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = cl * V + v;
-      part[blockIdx.y * (int64_t)N + c + v] = ((red[0][i] + red[1][i]) + red[2][i]) + red[3][i];
-    }
+    for (int k = 1; k < RL; ++k) v += red[k][i];
+    if (n < N) part[blockIdx.y * (int64_t)N + n] = v;
   }
 }
 
@@ -567,20 +589,30 @@ extern "C" int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, in
   return type == 1 ? run(bf16_t{}) : run(fp16_t{});
 }
 
-// rows of a slab: enough slabs to fill the card, 16 rows a lane at least
+// column lanes of a workgroup, 64 or fewer where those leave fewer of them idle (768 columns by 8: 3 times 32)
+static int lanes_of(int64_t N, int V) {
+  const int64_t groups = (N + V - 1) / V;
+  int best = 64;
+  for (int cw : {32, 16})
+    if ((groups + cw - 1) / cw * cw < (groups + best - 1) / best * best) best = cw;
+  return best;
+}
+// rows of a slab: enough slabs to fill the card, 4 rows a lane at least
 static int64_t slab_of(int64_t M, int64_t N, int V) {
-  const int64_t cols = (N + 64 * V - 1) / (64 * V);
-  int64_t n = 1024 / cols;
+  const int cw = lanes_of(N, V);
+  const int64_t cols = (N + (int64_t)cw * V - 1) / ((int64_t)cw * V), least = 4 * (256 / cw);
+  int64_t n = 2048 / cols;
   if (n < 1) n = 1;
-  int64_t s = (M + n - 1) / n;
-  if (s < 64) s = 64;
-  return s;
+  const int64_t s = (M + n - 1) / n;
+  return s < least ? least : (s + least - 1) / least * least;
 }
 
 extern "C" int64_t asrn_act_grad_workspace(int64_t M, int64_t N) {
   if (M < 0 || N < 0) return -1;
   if (M == 0 || N == 0) return 0;
-  const int64_t a = slab_of(M, N, 1), b = slab_of(M, N, 8), s = a < b ? a : b;
+  int64_t s = slab_of(M, N, 1);                   // the width is chosen by the addresses: the smallest slab of the three
+  for (int V : {4, 8})
+    if (slab_of(M, N, V) < s) s = slab_of(M, N, V);
   return (M + s - 1) / s * N * 4;
 }
 
@@ -607,17 +639,27 @@ extern "C" int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const
                  (long long)workspace_bytes);
     part = (float*)workspace;
   }
-  const dim3 grid((unsigned)((N + 64 * V - 1) / (64 * V)), (unsigned)slabs);
+  const int cw = lanes_of(N, V);
+  const dim3 grid((unsigned)((N + (int64_t)cw * V - 1) / ((int64_t)cw * V)), (unsigned)slabs);
   hipStream_t st = (hipStream_t)stream;
   const int rc = with_type(type, [&](auto t) {
     using T = decltype(t);
     constexpr int WT = sizeof(T) == 4 ? 4 : 8;
     auto go = [&](auto g) {
       using G = decltype(g);
-      if (vec) hipLaunchKernelGGL((k_act_grad<T, G, WT>), grid, dim3(256), 0, st, (const G*)gy, ldg, (const T*)pre, ldp, act, M,
-                                  (int)N, slab, (T*)gp, part);
-      else hipLaunchKernelGGL((k_act_grad<T, G, 1>), grid, dim3(256), 0, st, (const G*)gy, ldg, (const T*)pre, ldp, act, M, (int)N,
-                              slab, (T*)gp, part);
+#define ASRN_ACT_GRAD(V, CW)                                                                                              \
+  hipLaunchKernelGGL((k_act_grad<T, G, V, CW>), grid, dim3(256), 0, st, (const G*)gy, ldg, (const T*)pre, ldp, act, M, (int)N, \
+                     slab, (T*)gp, part)
+      if (vec) {
+        if (cw == 64) ASRN_ACT_GRAD(WT, 64);
+        else if (cw == 32) ASRN_ACT_GRAD(WT, 32);
+        else ASRN_ACT_GRAD(WT, 16);
+      } else {
+        if (cw == 64) ASRN_ACT_GRAD(1, 64);
+        else if (cw == 32) ASRN_ACT_GRAD(1, 32);
+        else ASRN_ACT_GRAD(1, 16);
+      }
+#undef ASRN_ACT_GRAD
       return check_launch("asrn_act_grad");
     };
     return gy_fp32 ? go(float{}) : go(T{});
