@@ -99,12 +99,15 @@ __device__ __forceinline__ void wave_lds_fence() {
 // x is formed here: the compiler would put a sum that only the loop's next turn reads off to its end, its terms in registers
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
 
-// x[0 .. NPL) of LDS, NPL in {2, 4, 8}
+// x[0 .. NPL) of LDS, NPL in {2, 4, 6, 8}
 template <int NPL>
 __device__ __forceinline__ void lds_vec(const float* p, float (&x)[NPL]) {
-  if constexpr (NPL == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x; x[1] = v.y;
+  if constexpr (NPL % 4 != 0) {
+#pragma unroll
+    for (int i = 0; i < NPL / 2; ++i) {
+      const float2 v = reinterpret_cast<const float2*>(p)[i];
+      x[2 * i] = v.x; x[2 * i + 1] = v.y;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < NPL / 4; ++i) {
@@ -156,7 +159,7 @@ __device__ __forceinline__ void store_state(float* x, const Selective& s, const 
 // V of a lane, padded channels and states among them (0).
 template <int NPL>
 struct Own {
-  static constexpr int V = NPL < 4 ? NPL : 4, G = 4 * NPL / V;
+  static constexpr int V = NPL % 4 ? 2 : 4, G = 4 * NPL / V;
   typedef float FV __attribute__((ext_vector_type(V)));
   static __device__ __forceinline__ void load(const float* x, const Place& p, float (&h)[4][NPL]) {
     const FV* v = reinterpret_cast<const FV*>(x) + (int64_t)p.group * 64 * G;
@@ -761,6 +764,7 @@ template <typename F>
 static int with_states(int N, F&& f) {
   if (N <= 8) return f(std::integral_constant<int, 2>{});
   if (N <= 16) return f(std::integral_constant<int, 4>{});
+  if (N <= 24) return f(std::integral_constant<int, 6>{});
   return f(std::integral_constant<int, 8>{});
 }
 
@@ -768,7 +772,7 @@ static int with_states(int N, F&& f) {
 static int64_t own_floats(int d, int N) {
   int waves, blocks;
   grid_of(d, waves, blocks);
-  return (int64_t)blocks * waves * 64 * (N <= 8 ? 8 : N <= 16 ? 16 : 32);
+  return (int64_t)blocks * waves * 64 * (N <= 8 ? 8 : N <= 16 ? 16 : N <= 24 ? 24 : 32);
 }
 static int64_t carry_bytes(int64_t B, int chunks, int d, int N) {
   return chunks > 1 ? (B * ((chunks - 1) * own_floats(d, N) + (int64_t)chunks * d) * 4 + 255) / 256 * 256 : 0;

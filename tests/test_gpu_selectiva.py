@@ -251,7 +251,7 @@ def revisar(e, gy, gh, sp=True, con_fin=True, transformar=lambda t: t):
 @pytest.mark.parametrize('B,L,d,N,dt', [
     (1, 1, 1, 1, F32), (2, 1, 64, 16, BF16), (3, 7, 5, 3, F32), (2, 8, 65, 16, F32), (1, 9, 130, 8, F16), (2, 63, 20, 11, F32),
     (2, 64, 64, 16, BF16), (1, 65, 300, 17, F32), (3, 200, 70, 16, F32), (2, 333, 33, 32, BF16), (1, 1000, 12, 5, F32),
-    (1, 129, 520, 9, F32), (9, 40, 257, 2, BF16)])
+    (1, 129, 520, 9, F32), (9, 40, 257, 2, BF16), (2, 170, 100, 24, F32), (1, 90, 64, 25, BF16), (2, 77, 130, 20, F16)])
 def test_escaneo_selectivo(B, L, d, N, dt):
     e = entradas(B, L, d, N, dt)
     revisar(e, r(B, L, d, dt=dt), r(B, d, N))
