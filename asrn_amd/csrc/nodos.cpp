@@ -16,7 +16,6 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
-#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -544,7 +543,8 @@ Tensor filas(const Tensor& t) {
   return r.size(0) > 1 && (r.stride(0) < k || r.stride(0) >= (1 << 21)) ? r.contiguous()
          : k > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
-int64_t paso_fila(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
+// a single row's stride may be anything
+int64_t paso_fila(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 // How the gradients' products run, by the rules in lineal.py: x's and w's on asrn_gemm, or the weight gradient as one product
 // (slabs 1) or a batch of slabs of the rows
@@ -599,20 +599,21 @@ struct LinealActiva : Function<LinealActiva> {
     const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
     const bool qx = ctx->needs_input_grad(0), qw = ctx->needs_input_grad(1), qb = con_b && ctx->needs_input_grad(2);
     Tensor gx, gw, gb, cols;
-    if (qx || qw || qb) {
+    if (M == 0 || N == 0) {
+      if (qx) gx = at::zeros(ctx->saved_data["f"].toIntVector(), x.options().dtype((at::ScalarType)n[2]));
+      if (qw) gw = at::zeros({N, K}, x.options().dtype((at::ScalarType)n[3]));
+      if (qb) gb = at::zeros({N}, x.options().dtype((at::ScalarType)n[4]));
+    } else if (qx || qw || qb) {
       Tensor g2 = filas(g[0]), gp = g2;
       const bool propio = n[0] != 0 || g2.scalar_type() != dt;
       const bool suma = qb && (propio || !(qw && n[7]));          // else the weight gradient's product sums the columns too
-      if (M && N && (propio || suma)) {
+      if (propio || suma) {
         const int64_t wsb = suma ? lib.actg_ws(M, N) : 0;
         Tensor ws = suma ? espacio(wsb, x) : Tensor();
         if (propio) gp = vacio({M, N}, x, dt);
         if (suma) cols = vacio({N}, x);
         vale(lib.act_grad(ptr(g2), paso_fila(g2), g2.scalar_type() == at::kFloat, ptr(pre), N, tipo_de(x), M, N, (int32_t)n[0],
                           propio ? ptr(gp) : nullptr, f32(cols), ptr(ws), wsb, en.st), "asrn_act_grad");
-      } else {
-        if (suma) cols = at::zeros({N}, x.options().dtype(at::kFloat));
-        if (propio) gp = g2.to(dt);
       }
       if (qx) {
         if (n[6]) {
@@ -620,7 +621,7 @@ struct LinealActiva : Function<LinealActiva> {
           gx = vacio({M, K}, x);
           const int64_t wsb = lib.gemm_ws(M, K, N, 0, 0, 0, 0);
           Tensor ws = espacio(wsb, x);
-          vale(lib.gemm(ptr(gc), N, 0, ptr(w), w.stride(0), 0, 0, f32(gx), K, M, K, N, nullptr, 0, nullptr, 0, 0, ptr(ws), wsb, en.st),
+          vale(lib.gemm(ptr(gc), N, 0, ptr(w), paso_fila(w), 0, 0, f32(gx), K, M, K, N, nullptr, 0, nullptr, 0, 0, ptr(ws), wsb, en.st),
                "asrn_gemm");
         } else {
           gx = at::mm(gp, w);
@@ -636,7 +637,7 @@ struct LinealActiva : Function<LinealActiva> {
           const int32_t bf = es16(x);
           const int64_t wsb = lib.gemm_ws(N, K, M, bf, columnas, 0, 0);
           Tensor ws = espacio(wsb, x);
-          vale(lib.gemm(ptr(gc), N, 1, ptr(x), x.stride(0), 0, bf, f32(gw), K, N, K, M, nullptr, 0, columnas ? f32(cols) : nullptr, 0, 0,
+          vale(lib.gemm(ptr(gc), N, 1, ptr(x), paso_fila(x), 0, bf, f32(gw), K, N, K, M, nullptr, 0, columnas ? f32(cols) : nullptr, 0, 0,
                         ptr(ws), wsb, en.st), "asrn_gemm");
         } else if (n[8] <= 1) {
           gw = at::mm(gp.t(), x);

@@ -170,6 +170,30 @@ def test_empty():
         assert gx.shape == x.shape and not gw.any() and not gb.any()
 
 
+@pytest.mark.parametrize('dt', [F32, BF16])
+@pytest.mark.parametrize('act', [None, 'gelu'])
+def test_no_columns(act, dt):
+    for forma in ((3, 8), (2, 3, 8), (2, 0, 8)):
+        x, w, b = r(*forma, dt=dt).requires_grad_(), r(0, 8, dt=dt).requires_grad_(), r(0, dt=dt).requires_grad_()
+        y = asrn_amd.lineal_activa(x, w, b, act)
+        assert y.shape == (*forma[:-1], 0)
+        gs = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+        assert [g.shape for g in gs] == [x.shape, w.shape, b.shape] and not gs[0].any()
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+@pytest.mark.parametrize('M,N', [(1, 8), (1, 1), (40, 1)])
+def test_one_row_of_any_stride(M, N, dt):
+    """A matrix of one row is contiguous with whatever stride its row has."""
+    def fila(n, K):
+        t = r(K, n, dt=dt).t()
+        assert n > 1 or (t.is_contiguous() and t.stride(0) == 1)
+        return t.requires_grad_()
+    x, w, b, res, gy = fila(M, 8), fila(N, 8), r(N, dt=dt).requires_grad_(), r(M, N, dt=dt).requires_grad_(), r(M, N, dt=dt)
+    y = asrn_amd.lineal_activa(x, w, b, 'silu', res)
+    revisar(x.detach(), w.detach(), b.detach(), 'silu', res.detach(), gy, y.detach(), torch.autograd.grad(y, (x, w, b, res), gy))
+
+
 @pytest.mark.parametrize('M', [5, 100])
 @pytest.mark.parametrize('dt', [F32, BF16])
 def test_nonfinite(M, dt):
