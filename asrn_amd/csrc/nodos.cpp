@@ -396,6 +396,11 @@ void sin_gradiente(const char* que, std::initializer_list<const Tensor*> ts) {
   if (con_gradiente(ts)) throw Fallo(std::string(que) + ": a token's step has no gradient: call it under torch.no_grad()");
 }
 
+// t was written in place: a graph that kept it for its backward finds out
+void escrito(const Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 // z (B, L, d), w (d, k) or (d, 1, k), b (d) or undefined
 struct ConvCanal : Function<ConvCanal> {
   static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& w, const Opcional& sesgo, int64_t act) {
@@ -432,12 +437,14 @@ Tensor conv_canal(const Tensor& z, const Tensor& w, const Opcional& b, int64_t a
 // z (B, d), ventana (B, d, k - 1) dense -> y and the next window, the same tensor or a new one
 std::pair<Tensor, Tensor> paso_conv_canal(const Tensor& z, const Tensor& ventana, const Tensor& w, const Opcional& b, int64_t act,
                                           bool en_sitio) {
-  sin_gradiente("paso_conv_canal", {&z, &ventana, &w});
+  const Tensor bt = o_nada(b);
+  sin_gradiente("paso_conv_canal", {&z, &ventana, &w, &bt});
   En en(z);
-  const Tensor zc = por_canal(z), wc = denso(w), bc = f32_o_nada(o_nada(b));
+  const Tensor zc = por_canal(z), wc = denso(w), bc = f32_o_nada(bt);
   Tensor y = vacio(z.sizes(), z, z.scalar_type()), sig = en_sitio ? ventana : at::empty_like(ventana);
   vale(lib.conv_paso(ptr(zc), tipo_de(z), zc.stride(0), ptr(ventana), ptr(sig), f32(wc), f32(bc), z.size(0), (int32_t)z.size(1),
                      (int32_t)w.size(-1), (int32_t)act, ptr(y), en.st), "asrn_channel_conv_step");
+  if (en_sitio) escrito(ventana);
   return {y, sig};
 }
 
@@ -522,15 +529,16 @@ std::pair<Tensor, Opcional> selectivo(const Tensor& u, const Tensor& dl, const T
 std::pair<Tensor, Tensor> paso_selectivo(const Tensor& u, const Tensor& dl, const Tensor& A, const Tensor& Bm, const Tensor& C,
                                          const Tensor& h, const Opcional& D, const Opcional& z, const Opcional& sesgo,
                                          bool softplus, bool en_sitio) {
-  const Tensor zt = o_nada(z);
-  sin_gradiente("paso_selectivo", {&u, &dl, &A, &Bm, &C, &h, &zt});
+  const Tensor zt = o_nada(z), Dt = o_nada(D), st_ = o_nada(sesgo);
+  sin_gradiente("paso_selectivo", {&u, &dl, &A, &Bm, &C, &h, &zt, &Dt, &st_});
   En en(u);
   const Tensor uc = por_canal(u), dc = por_canal(dl), Bc = por_canal(Bm), Cc = por_canal(C), zc = por_canal(zt);
-  const Tensor Ac = denso(A), Dc = f32_o_nada(o_nada(D)), sc = f32_o_nada(o_nada(sesgo));
+  const Tensor Ac = denso(A), Dc = f32_o_nada(Dt), sc = f32_o_nada(st_);
   Tensor y = vacio(u.sizes(), u, u.scalar_type()), sig = en_sitio ? h : at::empty_like(h);
   const int64_t st[5] = {uc.stride(0), dc.stride(0), Bc.stride(0), Cc.stride(0), zc.defined() ? zc.stride(0) : 0};
   vale(lib.sel_paso(ptr(uc), ptr(dc), ptr(Bc), ptr(Cc), ptr(zc), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(h), f32(sig),
                     u.size(0), (int32_t)u.size(1), (int32_t)A.size(1), softplus, ptr(y), en.st), "asrn_selective_step");
+  if (en_sitio) escrito(h);
   return {y, sig};
 }
 

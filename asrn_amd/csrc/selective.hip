@@ -25,6 +25,7 @@ constexpr int kCheck = 8;         // tokens between two kept states; also the ti
 constexpr int kTile = 16;         // tokens that the forward stages at once
 constexpr int kMaxWaves = 4;      // of a workgroup, 64 channels each
 constexpr int kMinChunk = 32;
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;         // of a grid
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Selective {
@@ -136,15 +137,22 @@ __device__ __forceinline__ Place place_of(const Selective& s) {
   return p;
 }
 
-// the lane's 4 x NPL values of a (d, N) array, 0 outside it
-template <int NPL>
-__device__ __forceinline__ void load_state(const float* x, const Selective& s, const Place& p, float (&h)[4][NPL],
-                                           float scale = 1.f) {
+// A in units of the binary exponent, finite: times a delta of 0 (past a chunk's end) an infinite one would not be 0
+__device__ __forceinline__ float rate_of(float A) {
+  const float x = A * kLog2e;
+  return fabsf(x) == INFINITY ? copysignf(3.4e38f, x) : x;
+}
+
+// the lane's 4 x NPL values of a (d, N) array, 0 outside it; RATE: of A
+template <int NPL, bool RATE = false>
+__device__ __forceinline__ void load_state(const float* x, const Selective& s, const Place& p, float (&h)[4][NPL]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      h[i][j] = x && p.q + i < s.d && p.n0 + j < s.N ? scale * x[(int64_t)(p.q + i) * s.N + p.n0 + j] : 0.f;
+    for (int j = 0; j < NPL; ++j) {
+      const float v = x && p.q + i < s.d && p.n0 + j < s.N ? x[(int64_t)(p.q + i) * s.N + p.n0 + j] : 0.f;
+      h[i][j] = RATE ? rate_of(v) : v;
+    }
 }
 template <int NPL>
 __device__ __forceinline__ void store_state(float* x, const Selective& s, const Place& p, const float (&h)[4][NPL]) {
@@ -287,7 +295,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective(Selective s) {
   T* py = static_cast<T*>(s.y) + b * s.L * s.d;
   const bool gate = s.z != nullptr;
   float A2[4][NPL], h[4][NPL];
-  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL, true>(s.A, s, p, A2);
   if (!LOCAL && chunk) Own<NPL>::load(s.carry + (b * (s.chunks - 1) + chunk - 1) * s.own, p, h);
   else load_state<NPL>(!LOCAL && s.h0 ? s.h0 + b * dN : nullptr, s, p, h);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f, D = s.D && p.live ? s.D[p.c] : 0.f;
@@ -376,7 +384,7 @@ __global__ __launch_bounds__(256) void k_selective_carry(Selective s) {
   int n;
   Own<NPL>::where(e, c, n);
   if (c >= s.d || n >= s.N) return;               // stay 0
-  const float A2 = s.A[c * s.N + n] * kLog2e, *x0 = BACK ? s.ghend : s.h0;
+  const float A2 = rate_of(s.A[c * s.N + n]), *x0 = BACK ? s.ghend : s.h0;
   float h = x0 ? x0[(b * s.d + c) * s.N + n] : 0.f;
   float* x = s.carry + b * (s.chunks - 1) * s.own + e;
   const float* w = s.total + b * s.chunks * s.d + c;
@@ -414,7 +422,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_selective_local_bwd(Selectiv
           *pC = static_cast<const T*>(s.Cm) + b * s.Cb, *pg = static_cast<const T*>(s.gy) + b * s.gb;
   const bool gate = s.z != nullptr;
   float A2[4][NPL], g[4][NPL];
-  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL, true>(s.A, s, p, A2);
   load_state<NPL>(nullptr, s, p, g);
   const float bias = s.bias && p.live ? s.bias[p.c] : 0.f;
   float sum = 0.f;
@@ -496,7 +504,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_b
           *pC = static_cast<const T*>(s.Cm) + b * s.Cb, *pg = static_cast<const T*>(s.gy) + b * s.gb;
   const bool gate = s.z != nullptr;
   float A2[4][NPL], dA[4][NPL], G[4][NPL];
-  load_state<NPL>(s.A, s, p, A2, kLog2e);
+  load_state<NPL, true>(s.A, s, p, A2);
   load_state<NPL>(nullptr, s, p, dA);
   if (chunk + 1 < s.chunks) Own<NPL>::load(s.carry + (b * (s.chunks - 1) + chunk) * s.own, p, G);
   else load_state<NPL>(s.ghend ? s.ghend + b * dN : nullptr, s, p, G);
@@ -691,7 +699,7 @@ __global__ __launch_bounds__(256) void k_selective_step(Selective s, const float
   float* hw = next + (bb * s.d + c) * s.N;
   float y = 0.f;
   for (int n = ng; n < s.N; n += 4) {
-    const float x = fmaf(decay(delta, s.A[(int64_t)c * s.N + n] * kLog2e), hr[n], delta * u * (float)Bm[n]);
+    const float x = fmaf(decay(delta, rate_of(s.A[(int64_t)c * s.N + n])), hr[n], delta * u * (float)Bm[n]);
     if (live) hw[n] = x;
     y = fmaf(x, (float)Cm[n], y);
   }
@@ -811,6 +819,7 @@ extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* 
   s.chunks = chunks_of(B, L, d);
   s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_fwd: too many chunks");
+  ASRN_REQUIRE(!checks || B * L * 2 * N < kMaxThreads, "asrn_selective_fwd: too many tokens for a backward");
   const int64_t need = carry_bytes(B, s.chunks, d, N);
   if (need) {
     ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
@@ -871,6 +880,7 @@ extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* 
   s.chunks = chunks_of(B, L, d);
   s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_bwd: too many chunks");
+  ASRN_REQUIRE(B * L * 2 * N < kMaxThreads, "asrn_selective_bwd: too many tokens");
   const int64_t need = asrn_selective_bwd_workspace(B, L, d, N), groups = B * s.chunks, cols = (int64_t)d * N + 2 * d;
   ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
                "asrn_selective_bwd: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
@@ -911,6 +921,7 @@ extern "C" int asrn_selective_step(const void* u, const void* delta, const void*
   if (check(s, type, "asrn_selective_step")) return 1;
   if (B == 0) return 0;
   ASRN_REQUIRE(u && delta && B_ && C_ && A && y && h && next && strides, "asrn_selective_step: null pointer");
+  ASRN_REQUIRE(B * d * 4 < kMaxThreads, "asrn_selective_step: too many channels");
   s.ub = strides[0]; s.dlb = strides[1]; s.Bb = strides[2]; s.Cb = strides[3]; s.zb = strides[4];
   return with_type(type, [&](auto t) {
     hipLaunchKernelGGL((k_selective_step<decltype(t)>), dim3((unsigned)((B * d * 4 + 255) / 256)), dim3(256), 0,

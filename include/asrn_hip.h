@@ -757,7 +757,8 @@ int asrn_channel_conv_step(const void* z, int32_t type, int64_t stride_b, const 
  * gradient; du, ddelta, dz (with z), dB, dC dense in the inputs' type; dparams = dA (d, N), then dD (d), then dbias (d); dh0
  * (or null). Sums in a fixed order. workspaces 16-byte aligned, of the stated sizes (-1: bad sizes). B L = 0 writes nothing.
  * step: one token; strides (host) = the rows' of u, delta, B_, C_, z; next (the same buffer, or another) gets the state.
- * Requires 1 <= N <= 32, d < 2^22, B < 2^16, L < 2^30, B L < 2^36, token strides below 2^24. */
+ * Requires 1 <= N <= 32, d < 2^22, B < 2^16, L < 2^30, B L < 2^36, token strides below 2^24; with checks and in bwd B L N <
+ * 2^31, in step B d < 2^30. */
 int64_t asrn_selective_checks(int64_t B, int64_t L, int32_t d, int32_t N);
 int64_t asrn_selective_fwd_workspace(int64_t B, int64_t L, int32_t d, int32_t N);
 int asrn_selective_fwd(const void* u, const void* delta, const void* B_, const void* C_, const void* z, int32_t type,

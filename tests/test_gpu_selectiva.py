@@ -388,6 +388,46 @@ def test_steps_refuse_gradients():
         asrn_amd.paso_selectivo(u[:, 0], dl[:, 0], A.requires_grad_(), Bm[:, 0], C[:, 0], h)
 
 
+def test_steps_refuse_their_parameters_gradients():
+    with pytest.raises(_lib.ASRNHipError, match='no_grad'):
+        asrn_amd.paso_conv_canal(r(2, 4), r(2, 4, 2), r(4, 3), r(4).requires_grad_())
+    u, dl, A, Bm, C, D, z, s, h = entradas(2, 1, 4, 3, F32)
+    for de, con in ((D.detach().requires_grad_(), s), (D, s.detach().requires_grad_())):
+        with pytest.raises(_lib.ASRNHipError, match='no_grad'):
+            asrn_amd.paso_selectivo(u[:, 0], dl[:, 0], A, Bm[:, 0], C[:, 0], h, D=de, sesgo_delta=con)
+
+
+def test_a_step_in_place_is_seen_by_a_graph_that_kept_its_state():
+    p = r(2, 4, 3).requires_grad_()
+    u, dl, A, Bm, C, D, z, s, h = entradas(2, 1, 4, 3, F32)
+    for estado, paso in ((r(2, 4, 3), lambda v: asrn_amd.paso_conv_canal(u[:, 0], v, r(4, 4))),
+                         (h, lambda v: asrn_amd.paso_selectivo(u[:, 0], dl[:, 0], A, Bm[:, 0], C[:, 0], v))):
+        q = (p * estado).sum()
+        with torch.no_grad():
+            paso(estado)
+        with pytest.raises(RuntimeError, match='inplace'):
+            q.backward()
+        with torch.inference_mode():
+            paso(estado.clone())
+
+
+def test_infinite_decay():
+    """A state of A = -inf forgets all but the newest token, also where the last tile and chunk are not whole."""
+    for L in (5, 16, 37, 300):
+        e = [t.detach() for t in entradas(1, L, 70, 3, F32)]
+        e[2][:, 1] = -torch.inf
+        e[2][3, 0] = -3e38              # beyond fp32 in units of the binary exponent
+        hojas = [t.requires_grad_() for t in e]
+        y, fin = llamar(hojas, devolver_estado=True)
+        ult = [t[:, -1].detach().double() for t in (e[0], e[1], e[3])]
+        dt = torch.nn.functional.softplus(ult[1] + e[7].detach().double())
+        espera = dt * ult[0] * ult[2][:, 1:2]
+        # 20 roundings of softplus from its exponential on, 10 of the exponential's argument (|x| < 10), the two products'
+        cerca(fin[..., 1].detach(), espera, espera.abs(), 32, 'fin')
+        gs = torch.autograd.grad(y.sum() + fin.sum(), hojas)
+        assert y.isfinite().all() and all(g.isfinite().all() for i, g in enumerate(gs) if i != 2)
+
+
 def test_captured_and_replayed():
     """A training call of both in a graph, replayed on new values with eager work between, on another stream than theirs."""
     B, L, d, N, k = 2, 200, 70, 16, 4
