@@ -291,3 +291,25 @@ def test_every_tile(tile, M, K, N, dt):
     p = x.double() @ w.double().t() + b.double()
     cerca(pre, p, (K + 24) * U * (x.double().abs() @ w.double().abs().t() + b.double().abs()), 'pre')
     assert torch.equal(y, asrn_amd.lineal_activa(x, w, b, 'silu', res))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values of x, y and its gradient: the last rows are those of the same rows alone, up to the sums' order."""
+    M, K, N = 2 ** 20 + 70, 2056, 2072
+    x = torch.empty(M, K, device=DEV, dtype=BF16).normal_().requires_grad_()
+    w, b = (r(N, K, dt=BF16) / 64).requires_grad_(), r(N, dt=BF16).requires_grad_()
+    y = asrn_amd.lineal_activa(x, w, b, 'gelu')
+    fin = x.detach()[-300:].clone().requires_grad_()
+    z = asrn_amd.lineal_activa(fin, w, b, 'gelu')
+    gz = r(300, N, dt=BF16)
+    gy = torch.zeros_like(y)
+    gy[-300:] = gz
+    cota = 4 * medio(BF16)
+    a, c = y.detach()[-300:].double(), z.detach().double()
+    assert ((a - c).abs() <= cota * c.abs() + 2 ** -12).all()
+    largo, corto = torch.autograd.grad(y, (x, w, b), gy), torch.autograd.grad(z, (fin, w, b), gz)
+    for g, h in ((largo[0][-300:], corto[0]), *zip(largo[1:], corto[1:])):
+        g, h = g.double(), h.double()
+        assert ((g - h).abs() <= cota * h.abs() + 2 ** -7 * h.abs().max()).all()
+    assert not largo[0][:-300].any()
+    torch.cuda.empty_cache()

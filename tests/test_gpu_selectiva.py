@@ -476,3 +476,34 @@ def test_same_bits_again_and_on_another_stream():
     torch.cuda.synchronize()
     for a, b, c in zip(uno, dos, tres):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_offsets_past_32_bits():
+    """Texts of more than 2^31 values: the end of the last one against the same tokens alone. Steps of 5 and more forget what lies
+    100 tokens back (exp(-500)); both round once to bf16 from fp32 values some 2^-18 apart."""
+    B, L, d, N, m = 2, 2 ** 20 + 19, 1024, 4, 128
+    u, dl = (torch.empty(B, L, d, device=DEV, dtype=BF16).normal_() for _ in range(2))
+    dl += 9
+    Bm, C, A = r(B, L, N, dt=BF16), r(B, L, N, dt=BF16), -1 - torch.rand(d, N, device=DEV)
+    fin = [t[1:, -m:].clone() for t in (u, dl, Bm, C)]
+    with torch.no_grad():
+        w, b = r(d, 4), r(d)
+        c = asrn_amd.conv_canal(u, w, b, 'silu')
+        assert torch.equal(c[1, -m + 3:], asrn_amd.conv_canal(fin[0], w, b, 'silu')[0, 3:])
+        del c
+        y = asrn_amd.escaneo_selectivo(u, dl, A, Bm, C)[1, -20:].double()
+    torch.cuda.empty_cache()
+    hojas = [t.requires_grad_() for t in fin]
+    ref = asrn_amd.escaneo_selectivo(hojas[0], hojas[1], A, hojas[2], hojas[3])[0, -20:].detach().double()
+    assert ((y - ref).abs() <= 2 ** -7 * ref.abs() + 2 ** -14 * ref.abs().max()).all()
+    # the gradients of the last tokens from a gradient of theirs alone
+    for t in (u, dl, Bm, C):
+        t.requires_grad_()
+    gy = r(20, d, dt=BF16)
+    largo = torch.autograd.grad(asrn_amd.escaneo_selectivo(u, dl, A, Bm, C)[1, -20:], (u, dl, Bm, C), gy)
+    corto = torch.autograd.grad(asrn_amd.escaneo_selectivo(hojas[0], hojas[1], A, hojas[2], hojas[3])[0, -20:], hojas, gy)
+    for a, b in zip(largo, corto):
+        a, b = a[1, -20:].double(), b[0, -20:].double()
+        assert ((a - b).abs() <= 2 ** -7 * b.abs() + 2 ** -14 * b.abs().max()).all()
+        assert not largo[0][0].any()
+    torch.cuda.empty_cache()
