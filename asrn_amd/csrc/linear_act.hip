@@ -382,7 +382,8 @@ __device__ __forceinline__ float lane_sums(float* v, int lane) {
 
 // Few rows (M <= 16): W is read once and each of its values meets every row, so the weights' bytes bound it. A wave takes 4
 // rows of W (columns of y) and all rows of x; its lanes run along k in units of 4, each with 4 x MR sums, which then
-// meet by a transposing exchange. x comes from the caches.
+// meet by a transposing exchange. x comes from the caches. 16 rows, 768 x 1536 fp32: 6.7 us, where 4.7 MB of weights from the
+// caches and a launch are the rest of a call's 7.2.
 template <typename T, int MR, bool VEC>
 __global__ __launch_bounds__(256) void k_linear_rows(Linear g) {
   constexpr int NR = 4, UN = sizeof(T) == 4 ? 4 : 8;
@@ -514,8 +515,8 @@ constexpr int kFewRows = 16;
 // The tile by an estimate of the time: a start of 3 us and 4 a 768 of k (the steps wait for their loads), and for each tile that a
 // CU takes its products at 2.5 PFLOP/s times what the tile needs over that. Measured (us; 64 x 64, 128 x 128, 256 x 192,
 // 256 x 256, without an epilogue): 1024 x 768 x 768 8.2 / 12.2 / 18.5 / 23.4, 2048 x 768 x 1536 (M, K, N) 11.5 / 16.1 / 24.3 /
-// 31.3, 4096 x 1024 x 1024 16.1 / 17.9 / 28.3 / 36.0, 16384 x 768 x 1536 58 / 49 / 43 / 51, 4096 x 4096 x 4096 280 / 155 / 156 /
-// 116, 8192 x 2048 x 4096 276 / 172 / 141 / 125 (hipBLASLt's product alone: 45 at the fourth, 108 and 106 at the last two).
+// 31.3, 4096 x 1024 x 1024 16.1 / 17.9 / 28.3 / 36.0, 16384 x 768 x 1536 64 / 53 / 47 / 54, 4096 x 4096 x 4096 203 / 136 / 166 /
+// 116, 8192 x 2048 x 4096 211 / 146 / 149 / 124 (the library's product alone: 46 at the fourth, 108 and 106 at the last two).
 static int tile_of(int64_t M, int64_t N, int64_t K) {
   struct Tile { int bm, bn; float over; };
   static const Tile all[] = {{64, 64, 2.5f}, {128, 128, 2.3f}, {256, 192, 1.9f}, {256, 256, 1.75f}};

@@ -8,7 +8,7 @@ namespace asrn {
 typedef __bf16 bf16_t;
 typedef _Float16 fp16_t;
 
-// f(the C++ type of `type`), for types that check_type has passed
+// f(the C++ type of `type`), for types that type_ok has passed
 template <typename F>
 inline int with_type(int32_t type, F&& f) {
   if (type == 1) return f(bf16_t{});
