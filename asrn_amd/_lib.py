@@ -150,6 +150,8 @@ SIGNATURES = {
                                            _I32, _I32, _P, _I64, _P]),
     'asrn_act_grad_workspace': (_I64, [_I64, _I64]),
     'asrn_act_grad': (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _I64, _I64, _I32, _P, _P, _P, _I64, _P]),
+    'asrn_weight_grad_workspace': (_I64, [_I64, _I64, _I64, _I32, _I32]),
+    'asrn_weight_grad': (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _I64, _P, _I32, _I32, _I32, _P, _I64, _P]),
     'asrn_selective_step': (ctypes.c_int, [_P] * 5 + [_I32] + [_P] * 6 + [_I64, _I32, _I32, _I32, _P, _P]),
 }
 

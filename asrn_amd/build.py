@@ -21,7 +21,7 @@ SOURCES = ['errors.hip', 'graph.hip', 'bucket_sort.hip', 'ngram.hip', 'scan.hip'
            'phi.hip', 'sampling.hip', 'block_step.hip', 'cross_entropy.hip', 'conv_window.hip',
            'layernorm.hip', 'clip.hip', 'embedding.hip', 'key_rows.hip',
            'token_logp.hip', 'preference.hip', 'policy.hip', 'eight_bits.hip', 'channel_conv.hip', 'selective.hip',
-           'linear_act.hip']
+           'linear_act.hip', 'weight_grad.hip']
 ARCH = os.environ.get('ASRN_OFFLOAD_ARCH', 'gfx950')
 INCLUDE = os.path.join(os.path.dirname(HERE), 'include')
 COMMON = ['-O3', '-fPIC', '-std=c++17', f'--offload-arch={ARCH}', '-Xclang', '-target-feature', '-Xclang',

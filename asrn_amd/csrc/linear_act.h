@@ -1,8 +1,25 @@
-// The epilogue of a product: bias, activation, residual, and the activation's input kept for the backward.
+// What the 16-bit products share, and the epilogue of a product: bias, activation, residual, and the activation's input kept for
+// the backward.
 #pragma once
 #include "types.h"
 
 namespace asrn {
+
+typedef float fx16 __attribute__((ext_vector_type(16)));
+typedef bf16_t bfx8 __attribute__((ext_vector_type(8)));
+typedef fp16_t hx8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ fx16 mfma32(bfx8 a, bfx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ fx16 mfma32(hx8 a, hx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+constexpr unsigned kPast = 1u << 31;              // past the end of a buffer of this many bytes: reads 0
+
+// 16 bytes a lane from memory to LDS, lane i's to l[i] (l: the same in every lane)
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rsrc, uint4* l, unsigned at, unsigned off) {
+#ifdef __HIP_DEVICE_COMPILE__                     // the host's pass does not know the 16-byte form
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)l, 16, at, off, 0, 0);
+#endif
+}
 
 // For products of 16-bit operands: Phi(-|x|) = t p(t) exp(-x^2 / 2) with Abramowitz and Stegun's 7.1.26, erfc within 1.5e-7, so
 // GELU within 8e-8 |x| and its derivative within 8e-8: one exponential and one reciprocal (erff costs about twice the

@@ -12,13 +12,6 @@
 
 namespace asrn {
 
-typedef float fx16 __attribute__((ext_vector_type(16)));
-typedef bf16_t bfx8 __attribute__((ext_vector_type(8)));
-typedef fp16_t hx8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ fx16 mfma32(bfx8 a, bfx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ fx16 mfma32(hx8 a, hx8 b, fx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
 struct Linear {
   const void* x; int64_t ldx; const void* w; int64_t ldw;
   int M, N, K;
@@ -99,7 +92,6 @@ __device__ __forceinline__ void finish_all(const Linear& g, fx16 (&acc)[MI][NI],
 // An operand's share of a step: R rows by 64 k, units of 8 k; a thread loads U units, 8 neighbouring threads a row's 128 bytes.
 // VEC: the units are 16 bytes on their boundary (8 divides K and the row stride); else they are read wherever they lie, those
 // of the last step element by element.
-constexpr unsigned kPast = 1u << 31;
 template <typename T, int R, int THR, bool VEC>
 struct Units {
   static constexpr int U = R * 8 / THR;
@@ -222,13 +214,6 @@ __device__ __forceinline__ void place_tile(int t, int tm, int tn, int& m, int& n
   const int group = t / (G * tn), first = group * G, rows = tm - first < G ? tm - first : G, r = t - group * G * tn;
   m = first + r % rows;
   n = r / rows;
-}
-
-// 16 bytes a lane from memory to LDS, lane i's to l[i] (l: the same in every lane)
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t rsrc, uint4* l, unsigned at, unsigned off) {
-#ifdef __HIP_DEVICE_COMPILE__                     // the host's pass does not know the 16-byte form
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)l, 16, at, off, 0, 0);
-#endif
 }
 
 // The same with the operands straight from memory to LDS, without registers in between (whole steps; a last part of one goes

@@ -67,6 +67,8 @@ struct Biblioteca {
   decltype(&asrn_linear_act_fwd) act_fwd;
   decltype(&asrn_act_grad_workspace) actg_ws;
   decltype(&asrn_act_grad) act_grad;
+  decltype(&asrn_weight_grad_workspace) wg_ws;
+  decltype(&asrn_weight_grad) wg;
   decltype(&asrn_gemm_workspace) gemm_ws;
   decltype(&asrn_gemm) gemm;
   decltype(&asrn_column_sums_workspace) cols_ws;
@@ -551,11 +553,15 @@ Tensor filas(const Tensor& t) {
   return r.size(0) > 1 && (r.stride(0) < k || r.stride(0) >= (1 << 21)) ? r.contiguous()
          : k > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
+bool en_unidades(const Tensor& t) {    // 16-bit rows in whole units of 16 bytes
+  return t.scalar_type() != at::kFloat && t.size(1) % 8 == 0 && (t.size(0) < 2 || t.stride(0) % 8 == 0) &&
+         reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+}
 // a single row's stride may be anything
 int64_t paso_fila(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 // How the gradients' products run, by the rules in lineal.py: x's and w's on asrn_gemm, or the weight gradient as one product
-// (slabs 1) or a batch of slabs of the rows
+// (slabs 1) or a batch of slabs of the rows; w's from 16-bit rows on 16-byte boundaries on asrn_weight_grad instead
 struct PlanLineal {
   int64_t gx_gemm, gw_gemm, slabs;
 };
@@ -614,7 +620,8 @@ struct LinealActiva : Function<LinealActiva> {
     } else if (qx || qw || qb) {
       Tensor g2 = filas(g[0]), gp = g2;
       const bool propio = n[0] != 0 || g2.scalar_type() != dt;
-      const bool suma = qb && (propio || !(qw && n[7]));          // else the weight gradient's product sums the columns too
+      const bool unidades = en_unidades(x) && N % 8 == 0 && N < (1 << 21);
+      const bool suma = qb && (propio || !(qw && n[7] && !unidades));          // else the weight gradient's product sums the columns too
       if (propio || suma) {
         const int64_t wsb = suma ? lib.actg_ws(M, N) : 0;
         Tensor ws = suma ? espacio(wsb, x) : Tensor();
@@ -637,7 +644,14 @@ struct LinealActiva : Function<LinealActiva> {
         gx = gx.to((at::ScalarType)n[2]).view(ctx->saved_data["f"].toIntVector());
       }
       if (qw) {
-        if (n[7]) {
+        if (unidades) {
+          const Tensor gc = en_unidades(gp) ? gp : alineado(gp.contiguous());
+          gw = vacio({N, K}, x, (at::ScalarType)n[3] == dt ? dt : at::kFloat);
+          const int64_t wsb = lib.wg_ws(M, N, K, 0, 0);
+          Tensor ws = wsb > 0 ? espacio(wsb, x) : Tensor();
+          vale(lib.wg(ptr(gc), paso_fila(gc), ptr(x), paso_fila(x), tipo_de(x), M, N, K, ptr(gw), gw.scalar_type() == at::kFloat, 0, 0,
+                      ptr(ws), wsb, en.st), "asrn_weight_grad");
+        } else if (n[7]) {
           const Tensor gc = alineado(gp.contiguous());
           gw = vacio({N, K}, x);
           const bool columnas = qb && !cols.defined();
@@ -729,6 +743,8 @@ void iniciar(const py::function& direccion, py::object error) {
   de(lib.act_fwd, "asrn_linear_act_fwd");
   de(lib.actg_ws, "asrn_act_grad_workspace");
   de(lib.act_grad, "asrn_act_grad");
+  de(lib.wg_ws, "asrn_weight_grad_workspace");
+  de(lib.wg, "asrn_weight_grad");
   de(lib.gemm_ws, "asrn_gemm_workspace");
   de(lib.gemm, "asrn_gemm");
   de(lib.cols_ws, "asrn_column_sums_workspace");

@@ -792,6 +792,13 @@ int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
 int64_t asrn_act_grad_workspace(int64_t M, int64_t N);
 int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const void* pre, int64_t ldp, int32_t type, int64_t M, int64_t N,
                   int32_t act, void* gp, float* colsum, void* workspace, int64_t workspace_bytes, void* stream);
+/* weight_grad: out (N, K) dense, in fp32 or in `type`, = g^T x of g (M, N) and x (M, K) in bf16 or fp16 (type 1, 2); N, K and the
+ * leading dimensions multiples of 8 below 2^21, 16-byte aligned. fp32 sums in a fixed order, rounded once. tile: 0 by the sizes,
+ * or 128 or 256 rows and columns; slabs of the rows: 0 by the sizes. workspace: asrn_weight_grad_workspace bytes, 16-byte aligned (-1: bad sizes). M N K = 0 writes
+ * nothing. */
+int64_t asrn_weight_grad_workspace(int64_t M, int64_t N, int64_t K, int32_t tile, int32_t slabs);
+int asrn_weight_grad(const void* g, int64_t ldg, const void* x, int64_t ldx, int32_t type, int64_t M, int64_t N, int64_t K, void* out,
+                     int32_t out_fp32, int32_t tile, int32_t slabs, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -293,6 +293,33 @@ def test_every_tile(tile, M, K, N, dt):
     assert torch.equal(y, asrn_amd.lineal_activa(x, w, b, 'silu', res))
 
 
+@pytest.mark.parametrize('tile', [0, 128, 256])
+@pytest.mark.parametrize('M,N,K,slabs', [(1, 8, 8, 0), (64, 128, 128, 1), (63, 136, 8, 1), (65, 8, 264, 2), (130, 256, 256, 3),
+                                         (1000, 264, 520, 0), (2049, 768, 72, 5), (5000, 40, 1032, 0), (700, 520, 392, 100)])
+@pytest.mark.parametrize('dt', [BF16, F16])
+def test_weight_gradient(tile, M, N, K, slabs, dt):
+    """The entry itself: every tile, slabs that leave steps and rows over, rows with other values between them, both results."""
+    g, x = r(M, N + 24, dt=dt)[:, 8:8 + N], r(M, K + 8, dt=dt)[:, :K]
+    ref, mag = g.double().t() @ x.double(), g.double().abs().t() @ x.double().abs()
+    lib = _lib.load()
+    ws = torch.empty(lib.asrn_weight_grad_workspace(M, N, K, tile, slabs), device=DEV, dtype=torch.uint8)
+    for tipo in (F32, dt):
+        out = torch.full((N + 1, K), 7.0, device=DEV, dtype=tipo)
+        _lib.call('asrn_weight_grad', g.data_ptr(), N + 24, x.data_ptr(), K + 8, {BF16: 1, F16: 2}[dt], M, N, K, out.data_ptr(),
+                  int(tipo == F32), tile, slabs, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        cerca(out[:N], ref, M * U * mag, 'dw')
+        assert (out[N] == 7).all()
+
+
+def test_weight_gradient_keeps_infinities_in_their_rows():
+    """Rows past the last and columns past the edge enter nothing: an infinite g reaches its own row of dW alone."""
+    g, x = r(70, 40, dt=BF16), r(70, 48, dt=BF16)
+    g[69, 39], x[3, 47] = torch.inf, torch.nan
+    w = r(40, 48, dt=BF16).requires_grad_()
+    dw, = torch.autograd.grad(asrn_amd.lineal_activa(x, w), w, g)
+    assert dw[:39, :47].isfinite().all() and not dw[39, :47].isfinite().any() and dw[:, 47].isnan().all()
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 values of x, y and its gradient: the last rows are those of the same rows alone, up to the sums' order."""
     M, K, N = 2 ** 20 + 70, 2056, 2072

@@ -54,3 +54,26 @@ def test_entries_refuse():
     falla(lib.asrn_act_grad(64, 8, 1, None, 0, 1, 4, 8, 1, 64, None, None, 0, None), 'null')
     falla(lib.asrn_act_grad(64, 8, 1, 64, 8, 1, 4, 8, 1, 64, 64, None, 0, None), 'workspace')
     falla(lib.asrn_act_grad(64, 4, 1, 64, 8, 1, 4, 8, 1, 64, None, None, 0, None), 'leading')
+
+
+def test_weight_gradient_refuses():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip('libasrn_hip.so not built (run `python -m asrn_amd.build`)')
+    lib = _lib.load()
+
+    def falla(que, g=64, ldg=16, x=64, ldx=16, type=1, M=64, N=16, K=16, out=64, tile=0, slabs=0, ws=None, wsb=0):
+        rc = lib.asrn_weight_grad(g, ldg, x, ldx, type, M, N, K, out, 1, tile, slabs, ws, wsb, None)
+        assert rc != 0 and que in lib.asrn_hip_last_error().decode(), lib.asrn_hip_last_error().decode()
+    falla('type 0', type=0)
+    falla('multiples of 8', N=12)
+    falla('multiples of 8', K=1 << 21, ldx=1 << 21)
+    falla('unknown tile', tile=64)
+    falla('unknown tile', slabs=-1)
+    falla('null', x=None)
+    falla('leading', ldg=8)
+    falla('leading', ldx=20)
+    falla('misaligned', g=72)
+    falla('workspace', M=4096, slabs=4)
+    assert lib.asrn_weight_grad(64, 16, 64, 16, 1, 0, 16, 16, 64, 1, 0, 0, None, 0, None) == 0
+    assert lib.asrn_weight_grad_workspace(4096, 16, 16, 0, 4) == 4 * 16 * 16 * 4
+    assert lib.asrn_weight_grad_workspace(64, 12, 16, 0, 0) == -1 and lib.asrn_weight_grad_workspace(64, 16, 16, 3, 0) == -1
