@@ -32,7 +32,16 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, floa
       for (int i = 0; i < 4; ++i) v[k + i] += b[i];
     }
   }
-  if (e.pre) store_v<V>(static_cast<T*>(e.pre) + m * e.ldp + n, v);
+  if (e.pre) {                    // past the caches: the backward reads it much later (16384 x 768 x 1536 with GELU 69 -> 67 us)
+    typedef T TV __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int k = 0; k < V; k += 8) {
+      TV q;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = (T)v[k + i];
+      __builtin_nontemporal_store(q, reinterpret_cast<TV*>(static_cast<T*>(e.pre) + m * e.ldp + n + k));
+    }
+  }
   if (e.act == kActGelu) {
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = gelu16(v[k]);
