@@ -277,7 +277,8 @@ ACTIVACIONES = {None: 0, 'gelu': 1, 'silu': 2}
 
 def _plan_gradientes(x, w, M, N, K, dt):
     """How the backward of lineal_activa forms x's gradient (on asrn_gemm or not) and w's (on asrn_gemm, or in so many slabs),
-    by the rules above for rows of a dense gradient (M, N), x (M, K) and w (N, K) in dt."""
+    by the rules above for rows of a dense gradient (M, N), x (M, K) and w (N, K) in dt. w's from 16-bit rows of whole 16-byte
+    units is asrn_weight_grad's, which is faster at most sizes (its figures: csrc/weight_grad.hip)."""
     f32 = dt == torch.float32
     # _apto for both operands: dense rows of a multiple of 4 (fresh tensors and contiguous inputs are aligned)
     cuatro = N % 4 == 0 and K % 4 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0
