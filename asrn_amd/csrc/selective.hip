@@ -630,7 +630,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, NPL > 4 ? 1 : 2) void k_selective_b
         const float ys = quad_scatter(y, p.lane), ds = quad_scatter(dx, p.lane), dds = quad_scatter(dd, p.lane);
         const float delta = sd[r * 64 + p.lane], gg = sg[r * 64 + p.lane], uf = lu[r * 64];
         const float ddl = fmaf(dds, kLn2, ds * uf) * ls[r * 64];
-        dbias += ddl;
+        // past the text's end the state stays and w = G h: times an infinite decay's rate its sum may overflow, and 0 of it be NaN
+        dbias += r < left ? ddl : 0.f;
         dD = fmaf(gg, uf, dD);
         odu.store((T)fmaf(ds, delta, gg * D), r * odu.step, r < left);
         odl.store((T)ddl, r * odl.step, r < left);

@@ -507,3 +507,20 @@ def test_offsets_past_32_bits():
         assert ((a - b).abs() <= 2 ** -7 * b.abs() + 2 ** -14 * b.abs().max()).all()
         assert not largo[0][0].any()
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('L', [5, 37, 64, 301])
+def test_tokens_past_a_texts_end_enter_no_gradient(L):
+    """States that forget at once, by a decay of -inf, one beyond fp32 in units of the binary exponent and one of -1e7 (step sizes
+    of 2^-16 and more: exp(-150) is 0), and a gradient of the last state in the hundreds: the same bits from each, also where
+    the last tile is not whole."""
+    e = [t.detach() for t in entradas(1, L, 70, 3, F32)]
+    gy, gh = r(1, L, 70), 300 * r(1, 70, 3)
+
+    def todo(uno, otro):
+        e[2][:, 1], e[2][3, 0] = uno, otro
+        hojas = [t.clone().requires_grad_() for t in e]
+        y, fin = llamar(hojas, devolver_estado=True)
+        return y.detach(), fin.detach(), *torch.autograd.grad((y, fin), hojas, (gy, gh))
+    for nombre, a, b in zip(NOMBRES, todo(-1e7, -1e7), todo(-torch.inf, -3e38)):
+        assert b.isfinite().all() and torch.equal(a, b), nombre
