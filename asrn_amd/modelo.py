@@ -161,7 +161,7 @@ class BloqueLocal(nn.Module):
         if self.mezcla == 'selectiva':
             return self.adelante_selectiva(h)[0]
         if ocho and h.is_cuda and h.dtype == torch.float32 and _dtype_producto(h) in (torch.float32, torch.bfloat16) and \
-                type(self)._ff is BloqueLocal._ff and '_ff' not in vars(self):
+                self._ff_de_clase():
             return self._en_ocho(h)
         # the LayerNorms run fused (ops.norma_residual): ln2's output comes out in the feed-forward's dtype, and the
         # residual path's gradient joins each LayerNorm's backward
@@ -199,6 +199,8 @@ class BloqueLocal(nn.Module):
 
     def _ff_selectiva(self, h):
         y, h = ops.norma_residual(self.ln2, h, _dtype_producto(h))
+        if not self._ff_de_clase():
+            return h + self.drop(self._ff(y))
         f0, act, f2 = self.ff
         if type(act) is nn.GELU and act.approximate == 'none' and ops.sin_ganchos(act):
             u = lineal_activa(y, f0.weight, f0.bias, 'gelu')
@@ -262,6 +264,10 @@ class BloqueLocal(nn.Module):
         in its place has its own forward, and need not have p), inactive, without hooks."""
         d = self.drop
         return type(d) is nn.Dropout and not (d.training and d.p > 0) and ops.sin_ganchos(d)
+
+    def _ff_de_clase(self):
+        """Whether the feed-forward is this class's: a subclass's or an instance's own _ff runs in its place."""
+        return type(self)._ff is BloqueLocal._ff and '_ff' not in vars(self)
 
     def _ff(self, y):
         """self.ff on the library's Linear (lineal: the bias gradients as the library's fixed-order column sums)."""

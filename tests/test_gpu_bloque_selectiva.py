@@ -206,3 +206,29 @@ def test_per_channel_convolution_of_memoria_blocks(k, dt):
     ref, m = (v * w.double()[:, 0]).sum(-1) + b.double(), (v * w.double()[:, 0]).abs().sum(-1) + b.double().abs()
     assert y.dtype == dt
     assert ((y.double() - ref).abs() <= (k + 2) * min(U, torch.finfo(dt).eps) * m + torch.finfo(dt).eps / 2 * (ref.abs() + 1e-6)).all()
+
+
+@pytest.mark.parametrize('como', ['subclase', 'ejemplar'])
+def test_block_with_its_own_feed_forward(como):
+    """A block whose feed-forward was replaced runs it, over a text and for a token."""
+    b, vistas = bloque(32), []
+
+    def propia(y):
+        vistas.append(y.shape)
+        return torch.tanh(y) / 2
+    h = torch.randn(2, 9, 32, device=DEV)
+    sin = copy.deepcopy(b)                          # the same block without a feed-forward
+    with torch.no_grad():
+        sin.ff[2].weight.zero_()
+        sin.ff[2].bias.zero_()
+        medio = sin(h)
+        if como == 'subclase':
+            b.__class__ = type('Otro', (BloqueLocal,), {'_ff': lambda s, y: propia(y)})
+        else:
+            b._ff = propia
+        y = b(h)
+        assert (y - medio - torch.tanh(b.ln2(medio)) / 2).abs().max() <= 1e-5 and vistas == [h.shape]
+        z, s = b.adelante_selectiva(h[:, :-1], devolver_estado=True)[1]
+        ventana = F.pad(z, (0, 0, b.k - 1, 0))[:, z.shape[1]:].transpose(1, 2).contiguous()
+        paso = b.paso_selectiva(h[:, -1].contiguous(), ventana, s, b.decaimientos())
+    assert (paso - y[:, -1]).abs().max() <= 1e-4 and vistas[-1] == (2, 32)
