@@ -394,8 +394,15 @@ bool con_gradiente(std::initializer_list<const Tensor*> ts) {
       if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// whether one carries a tangent of forward mode, which only the nodes refuse
+bool con_tangente(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
 void sin_gradiente(const char* que, std::initializer_list<const Tensor*> ts) {
   if (con_gradiente(ts)) throw Fallo(std::string(que) + ": a token's step has no gradient: call it under torch.no_grad()");
+  if (con_tangente(ts)) throw Fallo(std::string(que) + ": a token's step has no derivative in forward mode");
 }
 
 // t was written in place: a graph that kept it for its backward finds out
@@ -688,7 +695,7 @@ struct LinealActiva : Function<LinealActiva> {
 Tensor lineal_activa(const Tensor& x, const Tensor& w, const Opcional& b, const Opcional& res, int64_t act, at::ScalarType dt,
                      int64_t gx_gemm, int64_t gw_gemm, int64_t slabs) {
   const Tensor bt = o_nada(b), rt = o_nada(res);
-  if (con_gradiente({&x, &w, &bt, &rt}))
+  if (con_gradiente({&x, &w, &bt, &rt}) || con_tangente({&x, &w, &bt, &rt}))
     return LinealActiva::apply(x, w, b, res, act, (int64_t)dt, PlanLineal{gx_gemm, gw_gemm, slabs})[0];
   En en(x);
   const SinAutocast sin;

@@ -340,3 +340,14 @@ def test_offsets_past_32_bits():
         assert ((g - h).abs() <= cota * h.abs() + 2 ** -7 * h.abs().max()).all()
     assert not largo[0][:-300].any()
     torch.cuda.empty_cache()
+
+
+def test_forward_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    args = [r(20, 8), r(6, 8), r(6), r(20, 6)]
+    for i in range(4):
+        for grad in (True, False):
+            with fwd.dual_level(), torch.set_grad_enabled(grad):
+                x, w, b, res = [fwd.make_dual(t.clone(), torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match='jvp|forward'):
+                    asrn_amd.lineal_activa(x, w, b, 'gelu', res)

@@ -524,3 +524,21 @@ def test_tokens_past_a_texts_end_enter_no_gradient(L):
         return y.detach(), fin.detach(), *torch.autograd.grad((y, fin), hojas, (gy, gh))
     for nombre, a, b in zip(NOMBRES, todo(-1e7, -1e7), todo(-torch.inf, -3e38)):
         assert b.isfinite().all() and torch.equal(a, b), nombre
+
+
+def test_forward_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    z, w, b = r(2, 5, 4), r(4, 3), r(4)
+    e = [t.detach() for t in entradas(2, 5, 4, 3, F32)]
+    u, dl, A, Bm, C, D, p, s, h = e
+    casos = [(lambda *a: asrn_amd.conv_canal(*a, 'silu'), (z, w, b)), (lambda *a: llamar(a), e),
+             (lambda *a: asrn_amd.paso_conv_canal(a[0], a[1], a[2], a[3]), (z[:, 0], r(2, 4, 2), w, b)),
+             (lambda *a: asrn_amd.paso_selectivo(a[0], a[1], a[2], a[3], a[4], a[5], D=a[6], puerta=a[7], sesgo_delta=a[8]),
+              (u[:, 0], dl[:, 0], A, Bm[:, 0], C[:, 0], h, D, p[:, 0], s))]
+    for f, args in casos:
+        for i in range(len(args)):
+            for grad in (True, False):
+                with fwd.dual_level(), torch.set_grad_enabled(grad):
+                    dual = [fwd.make_dual(t.clone(), torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                    with pytest.raises(RuntimeError, match='jvp|forward'):
+                        f(*dual)
