@@ -573,10 +573,11 @@ struct PlanLineal {
   int64_t gx_gemm, gw_gemm, slabs;
 };
 
+// x's rows (M, K) -> y in its own shape (..., N): no view, which a caller under autograd could not change in place
 Tensor producto_act(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res, int64_t act, at::ScalarType tipo_y,
-                    const Tensor& pre, const En& en) {
+                    const Tensor& pre, at::IntArrayRef forma, const En& en) {
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0), wsb = lib.act_ws(M, N, K, tipo_de(x));
-  Tensor y = vacio({M, N}, x, tipo_y), ws = wsb > 0 ? espacio(wsb, x) : Tensor();
+  Tensor y = vacio(forma, x, tipo_y), ws = wsb > 0 ? espacio(wsb, x) : Tensor();
   vale(lib.act_fwd(ptr(x), paso_fila(x), ptr(w), paso_fila(w), tipo_de(x), ptr(b), M, N, K, (int32_t)act, ptr(res),
                    res.defined() ? paso_fila(res) : N, res.defined() && res.scalar_type() == at::kFloat, ptr(pre), N, ptr(y), N,
                    tipo_y == at::kFloat, 0, ptr(ws), wsb, en.st), "asrn_linear_act_fwd");
@@ -597,15 +598,15 @@ struct LinealActiva : Function<LinealActiva> {
     const Tensor b = o_nada(b_), res = o_nada(res_);
     const Tensor x2 = filas(x.to(dt)), wc = filas(w.to(dt)), bc = b.defined() ? b.to(dt).contiguous() : b;
     Tensor pre = act ? vacio({x2.size(0), wc.size(0)}, x2, dt) : Tensor();
-    Tensor y = producto_act(x2, wc, bc, res.defined() ? filas(res) : res, act, res.defined() ? res.scalar_type() : dt, pre, en);
     auto forma = x.sizes().vec();
+    forma.back() = wc.size(0);
+    Tensor y = producto_act(x2, wc, bc, res.defined() ? filas(res) : res, act, res.defined() ? res.scalar_type() : dt, pre, forma, en);
     ctx->save_for_backward({x2, wc, pre});
     ctx->saved_data["n"] = std::vector<int64_t>{act, dt_, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
                                                 b.defined() ? (int64_t)b.scalar_type() : -1, res.defined(), plan.gx_gemm, plan.gw_gemm,
                                                 plan.slabs};
-    ctx->saved_data["f"] = forma;
-    forma.back() = wc.size(0);
-    return {y.view(forma)};
+    ctx->saved_data["f"] = x.sizes().vec();
+    return {y};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -699,11 +700,10 @@ Tensor lineal_activa(const Tensor& x, const Tensor& w, const Opcional& b, const 
     return LinealActiva::apply(x, w, b, res, act, (int64_t)dt, PlanLineal{gx_gemm, gw_gemm, slabs})[0];
   En en(x);
   const SinAutocast sin;
-  const Tensor y = producto_act(filas(x.to(dt)), filas(w.to(dt)), bt.defined() ? bt.to(dt).contiguous() : bt,
-                                rt.defined() ? filas(rt) : rt, act, rt.defined() ? rt.scalar_type() : dt, Tensor(), en);
   auto forma = x.sizes().vec();
   forma.back() = w.size(0);
-  return y.view(forma);
+  return producto_act(filas(x.to(dt)), filas(w.to(dt)), bt.defined() ? bt.to(dt).contiguous() : bt,
+                      rt.defined() ? filas(rt) : rt, act, rt.defined() ? rt.scalar_type() : dt, Tensor(), forma, en);
 }
 
 // Whether a graph recorded on the default stream still holds one of these leaves' accumulators. A backward inside a

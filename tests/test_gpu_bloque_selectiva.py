@@ -232,3 +232,13 @@ def test_block_with_its_own_feed_forward(como):
         ventana = F.pad(z, (0, 0, b.k - 1, 0))[:, z.shape[1]:].transpose(1, 2).contiguous()
         paso = b.paso_selectiva(h[:, -1].contiguous(), ventana, s, b.decaimientos())
     assert (paso - y[:, -1]).abs().max() <= 1e-4 and vistas[-1] == (2, 32)
+
+
+def test_block_with_an_activation_in_place():
+    """An activation that changes what it is given, in the GELU's place, trains as the one that does not."""
+    b, h, gy = bloque(32), torch.randn(2, 20, 32, device=DEV), torch.randn(2, 20, 32, device=DEV)
+    gs = []
+    for en_sitio in (False, True):
+        b.ff[1] = torch.nn.ReLU(inplace=en_sitio)
+        gs.append(torch.autograd.grad(b(h), list(b.parameters()), gy))
+    assert all(torch.equal(x, y) for x, y in zip(*gs))

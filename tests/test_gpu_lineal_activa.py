@@ -351,3 +351,23 @@ def test_forward_tangents_are_refused():
                 x, w, b, res = [fwd.make_dual(t.clone(), torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
                 with pytest.raises(RuntimeError, match='jvp|forward'):
                     asrn_amd.lineal_activa(x, w, b, 'gelu', res)
+
+
+@pytest.mark.parametrize('forma', [(5, 8), (100, 8), (2, 60, 8), (8,)])
+def test_result_changed_in_place(forma):
+    """As F.linear's result, this one may be changed in place, under autograd and when it was made without."""
+    x, w, b = r(*forma).requires_grad_(), r(6, 8).requires_grad_(), r(6).requires_grad_()
+    y = asrn_amd.lineal_activa(x, w, b, 'silu')
+    gy = torch.randn_like(y)
+    ref = torch.autograd.grad(torch.relu(2 * y), (x, w, b), gy)
+    y = asrn_amd.lineal_activa(x, w, b, 'silu')
+    y *= 2
+    y.relu_()
+    for a, v in zip(torch.autograd.grad(y, (x, w, b), gy), ref):
+        assert torch.equal(a, v)
+    p = r(6).requires_grad_()
+    with torch.no_grad():
+        y = asrn_amd.lineal_activa(x, w, b)
+    antes = y.clone()
+    y *= p
+    assert torch.equal(torch.autograd.grad(y, p, gy)[0], (antes * gy).reshape(-1, 6).sum(0))
