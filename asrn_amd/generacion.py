@@ -108,7 +108,7 @@ class EscritorModelo:
         if blq.mezcla == 'selectiva':
             return blq.paso_selectiva(h, self.ventanas[i], *self.selectivas[i])
         z = blq.ln1(h)
-        if blq.mezcla == 'memoria' and blq.k <= selectiva.K_MAX and z.dtype in selectiva.TIPOS:
+        if blq.mezcla == 'memoria' and selectiva.disponible(z.dtype, blq.k):
             c, _ = selectiva.paso_conv_canal(z, self.ventanas[i], blq.conv.weight, blq.conv.bias, 'gelu')
         else:
             ventana = torch.cat([self.ventanas[i], z.unsqueeze(-1)], dim=-1)            # (B, d, k)

@@ -72,12 +72,12 @@ def conv_causal(z, peso, sesgo):
 
 
 def _conv_canal_ok(z, peso):
-    return z.is_cuda and z.dtype in selectiva.TIPOS and peso.dtype in selectiva.TIPOS and 1 <= peso.shape[-1] <= selectiva.K_MAX
+    return z.is_cuda and peso.dtype in selectiva.TIPOS and selectiva.disponible(z.dtype, peso.shape[-1])
 
 
 def conv_canal_causal(z, peso, sesgo):
-    """The per-channel (depthwise) version: peso (d, 1, k). On the GPU one kernel (selectiva.conv_canal), else k multiply-adds
-    over shifted views."""
+    """The per-channel (depthwise) version: peso (d, 1, k). On the GPU one kernel (selectiva.conv_canal) where it
+    takes the call, else k multiply-adds over shifted views."""
     if _conv_canal_ok(z, peso):
         return selectiva.conv_canal(z, peso, sesgo)
     k = peso.shape[-1]

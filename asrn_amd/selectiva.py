@@ -12,13 +12,25 @@ GPU only. Nothing waits on the host, so a step over them can be captured in a HI
 """
 import torch
 
-from ._lib import nodos
+from ._lib import ASRNHipError, nodos
 from .ops import _dev
 
 TIPOS = (torch.float32, torch.bfloat16, torch.float16)       # what the kernels read and write
 ACTIVACIONES = (None, 'gelu', 'silu')
 K_MAX = 16                        # taps of a channel's convolution
 ESTADOS_MAX = 32                  # states a channel
+
+
+def disponible(tipo, k):
+    """Whether the convolution of each channel runs here on values of dtype `tipo` with k taps: a library that was built without
+    the nodes has none of this module's operators."""
+    if tipo not in TIPOS or not 1 <= k <= K_MAX:
+        return False
+    try:
+        nodos()
+    except ASRNHipError:
+        return False
+    return True
 
 
 def _activacion(quien, a):

@@ -242,3 +242,29 @@ def test_block_with_an_activation_in_place():
         b.ff[1] = torch.nn.ReLU(inplace=en_sitio)
         gs.append(torch.autograd.grad(b(h), list(b.parameters()), gy))
     assert all(torch.equal(x, y) for x, y in zip(*gs))
+
+
+def test_memoria_without_the_nodes(monkeypatch):
+    """A library that was built alone runs 'memoria' models on torch's operators: trained and written as with the nodes."""
+    from asrn_amd import _lib
+    m = asrn_amd.crear_modelo(60, d=32, n_capas=2, semilla=1, mezcla='memoria', memoria_max=64, **REDUCIDA).to(DEV)
+    x = synth.tokens(2, 41, 60, seed=0).to(DEV)
+
+    def todo():
+        m.train()
+        gs = torch.autograd.grad(m.perdida(x[:, :-1], x[:, 1:]), list(m.parameters()))
+        m.eval()
+        return gs, asrn_amd.escribir(m, x, n_nuevos=20, top_k=1)[1]
+    gs, escrito = todo()
+
+    def faltan():
+        raise _lib.ASRNHipError('_nodos.so is missing')
+    for sitio in ('selectiva', 'ops', 'entrenamiento', '_lib'):
+        monkeypatch.setattr(f'asrn_amd.{sitio}.nodos', faltan)
+    gs2, escrito2 = todo()
+    for a, b in zip(gs, gs2):
+        assert (a - b).norm() <= 1e-4 * a.norm() + 1e-7
+    assert (escrito - escrito2).abs().max() <= 1e-3
+    b = m.bloques[0]
+    with pytest.raises(_lib.ASRNHipError, match='missing'):
+        asrn_amd.conv_canal(torch.randn(1, 3, 32, device=DEV), b.conv.weight)
