@@ -380,8 +380,14 @@ std::tuple<Tensor, Tensor, Tensor> norma8(const Tensor& x, const Tensor& gamma, 
 int32_t tipo_de(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
 // the channels next to each other: the kernels read the other axes through their strides
 Tensor por_canal(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-// a scan's (B, L, .): its tokens within the kernels' 32-bit offsets too
-Tensor cercanas(const Tensor& t) { return t.defined() && t.stride(1) >= (1 << 24) ? t.contiguous() : por_canal(t); }
+// a scan's (B, L, .): its tokens within the kernels' 32-bit offsets too. The stride of a single token, or of none, may be
+// anything (such a tensor is contiguous with it) and is not used: 0 stands for it.
+int64_t paso_token(const Tensor& t) { return t.numel() && t.size(1) > 1 ? t.stride(1) : 0; }
+Tensor cercanas(const Tensor& t) { return t.defined() && paso_token(t) >= (1 << 24) ? t.contiguous() : por_canal(t); }
+void pasos_texto(const Tensor& t, int64_t* s) {
+  s[0] = t.defined() ? t.stride(0) : 0;
+  s[1] = t.defined() ? paso_token(t) : 0;
+}
 Tensor como(const Tensor& g, const Tensor& x) {       // a gradient in x's type, dense
   return g.scalar_type() == x.scalar_type() && g.is_contiguous() ? g : g.to(x.scalar_type()).contiguous();
 }
@@ -472,11 +478,11 @@ struct Selectivo : Function<Selectivo> {
       fin = B * L ? vacio({B, d, N}, u) : hc.defined() ? hc.clone() : at::zeros({B, d, N}, u.options().dtype(at::kFloat));
     if (guarda) marcas = vacio({lib.sel_marcas(B, L, (int32_t)d, (int32_t)N)}, u);
     int64_t st[10];
-    pasos(uc, st);
-    pasos(dc, st + 2);
-    pasos(Bc, st + 4);
-    pasos(Cc, st + 6);
-    pasos(zc.defined() ? Opcional(zc) : std::nullopt, st + 8);
+    pasos_texto(uc, st);
+    pasos_texto(dc, st + 2);
+    pasos_texto(Bc, st + 4);
+    pasos_texto(Cc, st + 6);
+    pasos_texto(zc, st + 8);
     vale(lib.sel_fwd(ptr(uc), ptr(dc), ptr(Bc), ptr(Cc), ptr(zc), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(hc), B, L,
                      (int32_t)d, (int32_t)N, softplus, ptr(y), f32(fin), f32(marcas), ptr(ws), wsb, en.st), "asrn_selective_fwd");
     ctx->save_for_backward({uc, dc, A, Bc, Cc, D, zc, sesgo, marcas});
@@ -503,12 +509,12 @@ struct Selectivo : Function<Selectivo> {
     if (n[1] >= 0)
       dh = B * L ? vacio({B, d, N}, u) : gfin.defined() ? gfin.clone() : at::zeros({B, d, N}, u.options().dtype(at::kFloat));
     int64_t st[12];
-    pasos(u, st);
-    pasos(dl, st + 2);
-    pasos(Bm, st + 4);
-    pasos(C, st + 6);
-    pasos(z.defined() ? Opcional(z) : std::nullopt, st + 8);
-    pasos(gy, st + 10);
+    pasos_texto(u, st);
+    pasos_texto(dl, st + 2);
+    pasos_texto(Bm, st + 4);
+    pasos_texto(C, st + 6);
+    pasos_texto(z, st + 8);
+    pasos_texto(gy, st + 10);
     vale(lib.sel_bwd(ptr(u), ptr(dl), ptr(Bm), ptr(C), ptr(z), ptr(gy), tipo_de(u), st, f32(Ac), f32(Dc), f32(sc), f32(marcas),
                      f32(gfin), B, L, (int32_t)d, (int32_t)N, (int32_t)n[0], ptr(du), ptr(ddl), ptr(dB), ptr(dC), ptr(dz), f32(dp),
                      f32(dh), ptr(ws), wsb, en.st), "asrn_selective_bwd");

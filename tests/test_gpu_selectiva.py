@@ -542,3 +542,29 @@ def test_forward_tangents_are_refused():
                     dual = [fwd.make_dual(t.clone(), torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
                     with pytest.raises(RuntimeError, match='jvp|forward'):
                         f(*dual)
+
+
+def lejos(t):
+    """t (B, 1, .) as a token-major text of that many values has it: the stride of its one token is 2^24 and more."""
+    return torch.as_strided(t.contiguous(), t.shape, (t.stride(0), 2 ** 24 + 8, 1))
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_one_token_of_any_stride(dt):
+    B, d, N = 3, 24, 5
+    e = entradas(B, 1, d, N, dt)
+    gy, gh = r(B, 1, d, dt=dt), r(B, d, N)
+
+    def todo(f):
+        hojas = [f(t.detach()).requires_grad_() if n in (0, 1, 3, 4, 6) else t.detach().requires_grad_() for n, t in enumerate(e)]
+        y, fin = llamar(hojas, devolver_estado=True)
+        return y.detach(), fin.detach(), *torch.autograd.grad((y, fin), hojas, (f(gy), gh))
+    for nombre, a, b in zip(NOMBRES, todo(lambda t: t.clone()), todo(lejos)):
+        assert torch.equal(a, b), nombre
+    # no text of such strides
+    hojas = [t.detach()[:0].requires_grad_() if n in (8,) else lejos(t.detach())[:0].requires_grad_() if n in (0, 1, 3, 4, 6)
+             else t for n, t in enumerate(e)]
+    y, fin = llamar(hojas, devolver_estado=True)
+    assert y.shape == (0, 1, d) and torch.autograd.grad(y.sum() + fin.sum(), hojas[0])[0].shape == (0, 1, d)
+    z, w = e[0], r(d, 4)
+    assert torch.equal(asrn_amd.conv_canal(lejos(z), w), asrn_amd.conv_canal(z, w))
