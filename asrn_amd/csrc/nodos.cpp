@@ -678,18 +678,16 @@ struct LinealActiva : Function<LinealActiva> {
         } else if (n[8] <= 1) {
           gw = at::mm(gp.t(), x);
         } else {
-          // left operand: the transposed slab of gp; right operand: x's slab as stored (never a transposed view)
+          // left operand: the transposed slab of gp; right operand: x's slab as stored (never a transposed view). The slabs'
+          // products stay in fp32: rounded to 16 bits, sums that cancel would keep their roundings (16 slabs of 1,024 rows of
+          // ones and minus ones: 56 for a sum of 44), and the time is the same (1001 x 775 over 16384 rows 56 us)
           const int64_t S = n[8];
-          const Tensor partes = at::bmm(gp.contiguous().view({S, M / S, N}).transpose(1, 2),
-                                        x.contiguous().view({S, M / S, K}));
-          if (dt == at::kHalf) {
-            gw = partes.sum(0, false, at::kFloat);
-          } else {
-            gw = vacio({N, K}, x);
-            const int64_t wsb = lib.cols_ws(S, N * K);
-            Tensor ws = espacio(wsb, x);
-            vale(lib.cols(ptr(partes), es16(x), S, N * K, N * K, f32(gw), ptr(ws), wsb, en.st), "asrn_column_sums");
-          }
+          const Tensor gs = gp.contiguous().view({S, M / S, N}).transpose(1, 2), xs = x.contiguous().view({S, M / S, K});
+          const Tensor partes = dt == at::kFloat ? at::bmm(gs, xs) : at::bmm(gs, xs, at::kFloat);
+          gw = vacio({N, K}, x);
+          const int64_t wsb = lib.cols_ws(S, N * K);
+          Tensor ws = espacio(wsb, x);
+          vale(lib.cols(ptr(partes), 0, S, N * K, N * K, f32(gw), ptr(ws), wsb, en.st), "asrn_column_sums");
         }
         gw = gw.to((at::ScalarType)n[3]);
       }

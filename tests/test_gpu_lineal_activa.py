@@ -371,3 +371,47 @@ def test_result_changed_in_place(forma):
     antes = y.clone()
     y *= p
     assert torch.equal(torch.autograd.grad(y, p, gy)[0], (antes * gy).reshape(-1, 6).sum(0))
+
+
+@pytest.mark.parametrize('dt', [BF16, F16])
+def test_weight_gradient_of_odd_widths_keeps_its_sums(dt):
+    """16-bit rows that no vector divides: the sums over the rows stay in fp32 to their end, as those of whole units do. Values
+    in sixteenths whose sums fp32 holds exactly, in 16 blocks of rows that nearly cancel: only the result is rounded."""
+    M, N, K = 16384, 9, 7
+    x = 1 + torch.randint(0, 16, (M, K), device=DEV) / 16
+    x = x * (1 - 2 * (torch.arange(M, device=DEV) // 1024 % 2))[:, None]
+    g = torch.randint(-2, 3, (M, N), device=DEV).float()
+    g[:, 0] = 1
+    ref = g.double().t() @ x.double()
+    w, x, g = r(N, K, dt=dt).requires_grad_(), x.to(dt), g.to(dt)
+    dw, = torch.autograd.grad(asrn_amd.lineal_activa(x, w), w, g)
+    assert torch.equal(dw, ref.to(dt))
+    w = r(N, K).requires_grad_()
+    with torch.autocast('cuda', dtype=dt):
+        y = asrn_amd.lineal_activa(x, w)
+    assert torch.equal(torch.autograd.grad(y, w, g)[0].double(), ref)
+
+
+@pytest.mark.parametrize('dt', [BF16, F16])
+def test_odd_widths_captured_and_replayed(dt):
+    """The weight gradient in slabs in a graph, on new values each time, with eager work between."""
+    x, w, b, gy = r(4096, 33, dt=dt), r(41, 33, dt=dt).requires_grad_(), r(41, dt=dt).requires_grad_(), r(4096, 41, dt=dt)
+
+    def paso():
+        return torch.autograd.grad(asrn_amd.lineal_activa(x, w, b, 'silu'), (w, b), gy)
+    lado = torch.cuda.Stream()
+    lado.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(lado):
+        paso()
+    torch.cuda.current_stream().wait_stream(lado)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fijos = paso()
+    for i in range(4):
+        x.copy_(r(4096, 33))
+        gy.copy_(r(4096, 41))
+        eager = [t.clone() for t in paso()]
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, v) for a, v in zip(fijos, eager)), i
