@@ -268,6 +268,7 @@ extern "C" int asrn_channel_conv_fwd(const void* z, int32_t type, int64_t stride
   if (V == 4) plan<4>(a);
   else plan<1>(a);
   const int64_t n = a.B * a.pieces * a.groups;
+  ASRN_REQUIRE(grid_ok(n, kConvThreads), "asrn_channel_conv_fwd: too many texts and channels");
   const dim3 grid((unsigned)((n + kConvThreads - 1) / kConvThreads)), thr(kConvThreads);
   hipStream_t st = (hipStream_t)stream;
   return with_type(type, [&](auto t) {
@@ -319,6 +320,7 @@ extern "C" int asrn_channel_conv_bwd(const void* z, int32_t type, int64_t stride
                (long long)(rows * cols * 4), (long long)workspace_bytes);
   ASRN_REQUIRE(rows < (1 << 30) && cols < (1 << 30), "asrn_channel_conv_bwd: too many pieces");
   const int64_t n = rows * a.groups;
+  ASRN_REQUIRE(grid_ok(n, kConvThreads), "asrn_channel_conv_bwd: too many texts and channels");
   const dim3 grid((unsigned)((n + kConvThreads - 1) / kConvThreads)), thr(kConvThreads);
   hipStream_t st = (hipStream_t)stream;
   const int rc = with_type(type, [&](auto t) {
@@ -344,6 +346,7 @@ extern "C" int asrn_channel_conv_step(const void* z, int32_t type, int64_t strid
   if (B == 0) return 0;
   ASRN_REQUIRE(z && w && y && (k == 1 || (window && next)), "asrn_channel_conv_step: null pointer");
   const int64_t n = B * d;
+  ASRN_REQUIRE(grid_ok(n, kConvThreads), "asrn_channel_conv_step: too many texts and channels");
   const dim3 grid((unsigned)((n + kConvThreads - 1) / kConvThreads)), thr(kConvThreads);
   return with_type(type, [&](auto t) {
     using T = decltype(t);

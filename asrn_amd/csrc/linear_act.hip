@@ -483,6 +483,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const G* gy, int64_t ldg, cons
 template <typename T, bool VEC>
 static int launch_rows(const Linear& g, hipStream_t st) {
   const unsigned gx = (unsigned)((g.N + 3) / 4);
+  ASRN_REQUIRE(grid_ok((int64_t)gx * 256, 256), "asrn_linear_act_fwd: too many columns");
   if (g.M <= 4)
     hipLaunchKernelGGL((k_linear_rows<T, 4, VEC>), dim3(gx, (g.M + 3) / 4), dim3(256), 0, st, g);
   else if (g.M <= 8)
@@ -497,7 +498,7 @@ static int launch_tiles(Linear g, bool vec, hipStream_t st) {
   g.tm = (g.M + BM - 1) / BM;
   g.tn = (g.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)g.tm * g.tn;
-  ASRN_REQUIRE(tiles < (1 << 30), "asrn_linear_act_fwd: too many tiles");
+  ASRN_REQUIRE(grid_ok((tiles + kXcdCount) * (64 * WM * WN), 64 * WM * WN), "asrn_linear_act_fwd: too many tiles");
   const unsigned grid = (unsigned)((tiles + kXcdCount - 1) / kXcdCount * kXcdCount);
   if (vec) hipLaunchKernelGGL((k_linear_direct<T, BM, BN, WM, WN>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
   else hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, false>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
@@ -636,6 +637,7 @@ extern "C" int asrn_act_grad(const void* gy, int64_t ldg, int32_t gy_fp32, const
   }
   const int cw = lanes_of(N, V);
   const dim3 grid((unsigned)((N + (int64_t)cw * V - 1) / ((int64_t)cw * V)), (unsigned)slabs);
+  ASRN_REQUIRE(grid_ok((int64_t)grid.x * 256, 256), "%s: too many columns", what);
   hipStream_t st = (hipStream_t)stream;
   const int rc = with_type(type, [&](auto t) {
     using T = decltype(t);

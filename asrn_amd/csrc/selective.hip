@@ -29,7 +29,6 @@ constexpr int kCheck = 8;         // tokens between two kept states; also the ti
 constexpr int kTile = 16;         // tokens that the forward stages at once
 constexpr int kMaxWaves = 4;      // of a workgroup, 64 channels each
 constexpr int kMinChunk = 32;
-constexpr int64_t kMaxThreads = (int64_t)1 << 32;         // of a grid
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Selective {
@@ -824,7 +823,7 @@ extern "C" int asrn_selective_fwd(const void* u, const void* delta, const void* 
   s.chunks = chunks_of(B, L, d);
   s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_fwd: too many chunks");
-  ASRN_REQUIRE(!checks || B * L * 2 * N < kMaxThreads, "asrn_selective_fwd: too many tokens for a backward");
+  ASRN_REQUIRE(!checks || grid_ok(B * L * 2 * N, 256), "asrn_selective_fwd: too many tokens for a backward");
   const int64_t need = carry_bytes(B, s.chunks, d, N);
   if (need) {
     ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
@@ -885,7 +884,7 @@ extern "C" int asrn_selective_bwd(const void* u, const void* delta, const void* 
   s.chunks = chunks_of(B, L, d);
   s.own = own_floats(d, N);
   ASRN_REQUIRE(s.chunks < 65536, "asrn_selective_bwd: too many chunks");
-  ASRN_REQUIRE(B * L * 2 * N < kMaxThreads, "asrn_selective_bwd: too many tokens");
+  ASRN_REQUIRE(grid_ok(B * L * 2 * N, 256), "asrn_selective_bwd: too many tokens");
   const int64_t need = asrn_selective_bwd_workspace(B, L, d, N), groups = B * s.chunks, cols = (int64_t)d * N + 2 * d;
   ASRN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
                "asrn_selective_bwd: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
@@ -926,7 +925,7 @@ extern "C" int asrn_selective_step(const void* u, const void* delta, const void*
   if (check(s, type, "asrn_selective_step")) return 1;
   if (B == 0) return 0;
   ASRN_REQUIRE(u && delta && B_ && C_ && A && y && h && next && strides, "asrn_selective_step: null pointer");
-  ASRN_REQUIRE(B * d * 4 < kMaxThreads, "asrn_selective_step: too many channels");
+  ASRN_REQUIRE(grid_ok(B * d * 4, 256), "asrn_selective_step: too many channels");
   s.ub = strides[0]; s.dlb = strides[1]; s.Bb = strides[2]; s.Cb = strides[3]; s.zb = strides[4];
   return with_type(type, [&](auto t) {
     hipLaunchKernelGGL((k_selective_step<decltype(t)>), dim3((unsigned)((B * d * 4 + 255) / 256)), dim3(256), 0,

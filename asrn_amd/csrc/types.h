@@ -16,6 +16,8 @@ inline int with_type(int32_t type, F&& f) {
   return f(float{});
 }
 inline bool type_ok(int32_t type) { return type >= 0 && type <= 2; }
+// whether n threads in workgroups of `group` are a launch: fewer than 2^32
+inline bool grid_ok(int64_t n, int group) { return (n + group - 1) / group * group < ((int64_t)1 << 32); }
 inline int type_bytes(int32_t type) { return type == 0 ? 4 : 2; }
 
 // V adjacent values, one access of V elements (V = 1: no alignment beyond the element's)

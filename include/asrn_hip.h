@@ -736,7 +736,8 @@ int asrn_norm8_read(const int8_t* q, const uint8_t* e, const float* gamma, const
  * bwd: dy dense; dz (B, L, d) dense; dparams (k + 1, d): dw[c, j] at (j, c), then dbias; summed in a fixed order.
  * workspace: asrn_channel_conv_bwd_workspace bytes (-1: bad sizes), 16-byte aligned. B L = 0 writes nothing.
  * step: one token, z (B, d), rows stride_b apart; window (B, d, k - 1) dense, the values before it, oldest first; next (the
- * same buffer, or another) gets the window after it. */
+ * same buffer, or another) gets the window after it.
+ * Lanes (a channel, or 4, of a piece of 16 tokens and more; of a token in step) below 2^32. */
 int asrn_channel_conv_fwd(const void* z, int32_t type, int64_t stride_b, int64_t stride_t, const float* w, const float* bias,
                           int64_t B, int64_t L, int32_t d, int32_t k, int32_t act, void* y, void* stream);
 int64_t asrn_channel_conv_bwd_workspace(int64_t B, int64_t L, int32_t d, int32_t k);
@@ -784,7 +785,7 @@ int asrn_selective_step(const void* u, const void* delta, const void* B_, const 
  * act_grad: gp = gy act'(pre) in `type` (or null), gy in fp32 or in `type`; colsum (or null): the fp32 sums of its columns
  * before that rounding, in a fixed order; workspace (for colsum): asrn_act_grad_workspace bytes, 16-byte aligned.
  * tile (16-bit operands): 0 by the sizes, or a tile's rows << 8 | columns (256 << 8: 256 x 256).
- * M N = 0 writes nothing. */
+ * N below 2^26 for M <= 16, and below 2^28 in act_grad. M N = 0 writes nothing. */
 int64_t asrn_linear_act_workspace(int64_t M, int64_t N, int64_t K, int32_t type);
 int asrn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t type, const void* bias, int64_t M,
                         int64_t N, int64_t K, int32_t act, const void* res, int64_t ldr, int32_t res_fp32, void* pre, int64_t ldp,

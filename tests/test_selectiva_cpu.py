@@ -135,3 +135,16 @@ def test_blocks_and_configurations():
     # the other blocks' weights for a seed are what they were
     assert list(BloqueLocal(8, 4, 16).state_dict()) == ['ln1.weight', 'ln1.bias', 'conv.weight', 'conv.bias', 'ln2.weight', 'ln2.bias',
                                                         'ff.0.weight', 'ff.0.bias', 'ff.2.weight', 'ff.2.bias']
+
+
+def test_entries_refuse_grids_past_the_launches(lib):
+    """A launch has fewer than 2^32 threads."""
+    def falla(rc):
+        assert rc != 0 and 'too many' in lib.asrn_hip_last_error().decode(), lib.asrn_hip_last_error().decode()
+    grande = (1 << 22, 1, 1025)                    # a lane a channel and text
+    falla(lib.asrn_channel_conv_fwd(64, 0, 1025, 1025, 64, N, *grande, 4, 0, 64, N))
+    wsb = lib.asrn_channel_conv_bwd_workspace(*grande, 4)
+    falla(lib.asrn_channel_conv_bwd(64, 0, 1025, 1025, 64, N, 64, *grande, 4, 0, 64, 64, 64, wsb, N))
+    falla(lib.asrn_channel_conv_step(64, 0, 1024, 64, 64, 64, N, 1 << 22, 1024, 4, 0, 64, N))
+    falla(lib.asrn_linear_act_fwd(64, 1, 64, 1, 0, N, 1, 1 << 26, 1, 0, N, 0, 0, N, 0, 64, 1 << 26, 1, 0, N, 0, N))
+    falla(lib.asrn_act_grad(64, (1 << 28) + 1, 1, 64, (1 << 28) + 1, 0, 1, (1 << 28) + 1, 1, 64, N, N, 0, N))     # 16 lanes of one column
