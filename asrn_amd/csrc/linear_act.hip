@@ -1,8 +1,9 @@
 // A product with its epilogue: y = [res +] act(x W^T + bias), x (M, K), W (N, K), and the gradient before the activation.
 //
-// 16-bit operands run on the matrix cores (k_linear): a workgroup forms a BM x BN tile in steps of 64 k. The operands come in
-// 16-byte units of 8 k, go through registers one step ahead and lie in LDS as units whose column is exchanged by the
-// row's number, so that 8 lanes that read neighbouring rows use all banks. The matrix instruction's rows are W's, in an order
+// 16-bit operands run on the matrix cores: a workgroup forms a BM x BN tile in steps of 64 k. The operands come in 16-byte
+// units of 8 k and lie in LDS as units whose column is exchanged by the row's number, so that 8 lanes that read neighbouring
+// rows use all banks. Rows of whole units on 16-byte boundaries go from memory straight to LDS (k_linear_direct), others
+// through registers one step ahead (k_linear). The matrix instruction's rows are W's, in an order
 // that leaves a lane with 16 neighbouring columns of one row of y: the epilogue reads and writes whole vectors from the
 // accumulators, with no pass through LDS. Sums are fp32; the activation's input (kept in the operands' type for the backward)
 // and y are rounded once each.
@@ -99,20 +100,17 @@ __device__ __forceinline__ void finish_all(const Linear& g, fx16 (&acc)[MI][NI],
 }
 
 // An operand's share of a step: R rows by 64 k, units of 8 k; a thread loads U units, 8 neighbouring threads a row's 128 bytes.
-// VEC: the units are 16 bytes on their boundary (8 divides K and the row stride); else they are read wherever they lie, those
-// of the last step element by element.
-template <typename T, int R, int THR, bool VEC>
+// The units are read wherever they lie, those of the last step element by element.
+template <typename T, int R, int THR>
 struct Units {
   static constexpr int U = R * 8 / THR;
   static_assert(R * 8 % THR == 0 && THR % 8 == 0, "whole units");
-  __amdgpu_buffer_rsrc_t rsrc;
   const T* base;
   unsigned at[U], c;              // byte offsets of the rows; the thread's column of units
   uint4 v[U];
   // rows past the matrix repeat its last one: their results are not stored
   __device__ __forceinline__ void start(const void* X, int64_t ld, int r0, int rows, int tid) {
     base = static_cast<const T*>(X) + r0 * ld;
-    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, kPast, 0x00027000);
     c = tid % 8;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -122,24 +120,16 @@ struct Units {
   }
   // k past K reads as 0
   __device__ __forceinline__ void load(int k0, int K) {
-    const unsigned off = (unsigned)k0 * (unsigned)sizeof(T);
-    if constexpr (VEC) {
-      const bool in = k0 + 8 * (int)c < K;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? at[i] : kPast, off, 0));
-    } else {
+    for (int i = 0; i < U; ++i) {
+      const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at[i]) + k0;
+      if (k0 + 64 <= K) {                         // uniform
+        __builtin_memcpy(&v[i], p, 16);
+      } else {
+        unsigned q[8];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + at[i]) + k0;
-        if (k0 + 64 <= K) {                       // uniform
-          __builtin_memcpy(&v[i], p, 16);
-        } else {
-          unsigned q[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) q[j] = k0 + 8 * (int)c + j < K ? __builtin_bit_cast(unsigned short, p[j]) : 0u;
-          v[i] = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
-        }
+        for (int j = 0; j < 8; ++j) q[j] = k0 + 8 * (int)c + j < K ? __builtin_bit_cast(unsigned short, p[j]) : 0u;
+        v[i] = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
       }
     }
   }
@@ -159,7 +149,8 @@ __device__ __forceinline__ int x_key(int r) { return r & 7; }
 __device__ __forceinline__ int w_key(int r) { return (r & 3) | (r >> 2 & 4); }
 __device__ __forceinline__ int w_row(int i) { return (i >> 2 & 1) * 16 + (i >> 3) * 4 + (i & 3); }
 
-template <typename T, int BM, int BN, int WM, int WN, bool VEC>
+// Operands on any boundary, of any width
+template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear(Linear g) {
   constexpr int THR = 64 * WM * WN, BK = 64, MI = BM / WM / 32, NI = BN / WN / 32;
   typedef T TX8 __attribute__((ext_vector_type(8)));
@@ -171,8 +162,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(Linear g) {
   const int m0 = tile / g.tn * BM, n0 = tile % g.tn * BN;
   const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, lr = lane & 31, lc = lane >> 5;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN), wr = w_row(lr);
-  Units<T, BM, THR, VEC> ux;
-  Units<T, BN, THR, VEC> uw;
+  Units<T, BM, THR> ux;
+  Units<T, BN, THR> uw;
   ux.start(g.x, g.ldx, m0, g.M, tid);
   uw.start(g.w, g.ldw, n0, g.N, tid);
   fx16 acc[MI][NI];
@@ -501,7 +492,7 @@ static int launch_tiles(Linear g, bool vec, hipStream_t st) {
   ASRN_REQUIRE(grid_ok((tiles + kXcdCount) * (64 * WM * WN), 64 * WM * WN), "asrn_linear_act_fwd: too many tiles");
   const unsigned grid = (unsigned)((tiles + kXcdCount - 1) / kXcdCount * kXcdCount);
   if (vec) hipLaunchKernelGGL((k_linear_direct<T, BM, BN, WM, WN>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
-  else hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN, false>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
+  else hipLaunchKernelGGL((k_linear<T, BM, BN, WM, WN>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
   return check_launch("asrn_linear_act_fwd");
 }
 
