@@ -415,3 +415,22 @@ def test_odd_widths_captured_and_replayed(dt):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, v) for a, v in zip(fijos, eager)), i
+
+
+@pytest.mark.parametrize('dt', [BF16, F16])
+def test_gelu_of_16_bit_products(dt):
+    """GELU alone (the product with the unit matrix, results in fp32) and its derivative. Phi of erfc's approximation is within
+    0.75e-7, and fp32 adds at most: the reciprocal's 2^-23 and its argument's 2^-24 by the slope of t p(t), up to 1.72, 3.1e-7;
+    three coefficients and two sums below 1, 2^-25 each, two coefficients below 1/4, two sums and a product below 1/2, 2.1e-7;
+    of the exponential, whose square's 5 roundings count x^2 / 2 times, and the last product, Phi (2^-23 + 5 x^2 2^-25) and
+    2^-26, 1.0e-7: together below 7e-7 (2.7e-7 found)."""
+    x = torch.linspace(-9, 9, 64 * 4000, device=DEV).to(dt).view(-1, 64).requires_grad_()
+    uno, cero = torch.eye(64, device=DEV, dtype=dt), torch.zeros(x.shape, device=DEV)
+    y = asrn_amd.lineal_activa(x, uno, activacion='gelu', residuo=cero)
+    x64 = x.detach().double()
+    ref, der = act64(x64, 'gelu')
+    assert ((y.double() - ref).abs() <= 7e-7 * x64.abs() + 2 * U * ref.abs()).all()
+    # its derivative, rounded to dt: Phi as above and x phi(x), whose roundings are 6 U and the exponential's
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    cota = 7e-7 + 12 * U * x64.abs()
+    assert ((g.double() - der).abs() <= cota + medio(dt) * (der.abs() + cota) + menor(dt)).all()
