@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -416,37 +417,69 @@ void escrito(const Tensor& t) {
   if (!t.is_inference()) torch::autograd::impl::bump_version(t);
 }
 
+// The gradients of a convolution of each channel in torch's operators, which record them: of z, w, b where they ask for one
+variable_list conv_registrada(const Tensor& z, const Tensor& w, const Tensor& b, const Tensor& gy, int64_t act) {
+  const int64_t L = z.size(1), d = z.size(2), k = w.size(-1);
+  const Tensor zp = at::constant_pad_nd(z.to(at::kFloat), {0, 0, k - 1, 0}), wf = w.reshape({d, k}).to(at::kFloat);
+  Tensor s = zp.narrow(1, 0, L) * wf.select(1, 0);
+  for (int64_t j = 1; j < k; ++j) s = s + zp.narrow(1, j, L) * wf.select(1, j);
+  if (b.defined()) s = s + b.to(at::kFloat);
+  variable_list r(4), de;
+  std::vector<int> sitio;
+  for (int i = 0; i < 3; ++i) {
+    const Tensor& t = i == 0 ? z : i == 1 ? w : b;
+    if (!t.defined() || !t.requires_grad()) continue;
+    de.push_back(t);
+    sitio.push_back(i);
+  }
+  const variable_list g = torch::autograd::grad({act == 1 ? at::gelu(s) : act == 2 ? at::silu(s) : s}, de, {gy.to(at::kFloat)},
+                                                /*retain_graph=*/true, /*create_graph=*/true);
+  for (size_t i = 0; i < g.size(); ++i) r[sitio[i]] = g[i];
+  return r;
+}
+
 // z (B, L, d), w (d, k) or (d, 1, k), b (d) or undefined
 struct ConvCanal : Function<ConvCanal> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& w, const Opcional& sesgo, int64_t act) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& w, const Opcional& sesgo, int64_t act,
+                               bool registrable) {
     En en(z);
     const Tensor b = o_nada(sesgo);
     const Tensor zc = por_canal(z), wc = denso(w), bc = f32_o_nada(b);
     Tensor y = vacio(z.sizes(), z, z.scalar_type());
     vale(lib.conv_fwd(ptr(zc), tipo_de(z), zc.stride(0), zc.stride(1), f32(wc), f32(bc), z.size(0), z.size(1), (int32_t)z.size(2),
                       (int32_t)w.size(-1), (int32_t)act, ptr(y), en.st), "asrn_channel_conv_fwd");
-    ctx->save_for_backward({zc, w, b});
+    // a recorded backward needs z itself, not a copy
+    ctx->save_for_backward({registrable ? z : zc, w, b});
     ctx->saved_data["a"] = act;
+    ctx->saved_data["r"] = registrable;
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    una_vez("conv_canal");
+    const bool registrada = at::GradMode::is_enabled() && ctx->saved_data["r"].toBool();
+    if (!registrada) una_vez("conv_canal");
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &z = s[0], &w = s[1], &b = s[2];
-    En en(z);
+    const Tensor &w = s[1], &b = s[2];
+    const int64_t act = ctx->saved_data["a"].toInt();
+    En en(s[0]);
+    if (registrada) {
+      variable_list r = conv_registrada(s[0], w, b, g[0], act);
+      r.emplace_back();
+      return r;
+    }
+    const Tensor z = por_canal(s[0]);
     const int64_t B = z.size(0), L = z.size(1), d = z.size(2), k = w.size(-1), wsb = lib.conv_ws(B, L, (int32_t)d, (int32_t)k);
     const Tensor gy = como(g[0], z), wc = denso(w), bc = f32_o_nada(b);
     Tensor dz = vacio(z.sizes(), z, z.scalar_type()), ws = espacio(wsb, z);
     Tensor dp = B * L ? vacio({k + 1, d}, z) : at::zeros({k + 1, d}, z.options().dtype(at::kFloat));
     vale(lib.conv_bwd(ptr(z), tipo_de(z), z.stride(0), z.stride(1), f32(wc), f32(bc), ptr(gy), B, L, (int32_t)d, (int32_t)k,
-                      (int32_t)ctx->saved_data["a"].toInt(), ptr(dz), f32(dp), ptr(ws), wsb, en.st), "asrn_channel_conv_bwd");
+                      (int32_t)act, ptr(dz), f32(dp), ptr(ws), wsb, en.st), "asrn_channel_conv_bwd");
     return {dz, dp.narrow(0, 0, k).t().view_as(w).to(w.scalar_type()),
-            b.defined() ? dp.select(0, k).to(b.scalar_type()) : Tensor(), Tensor()};
+            b.defined() ? dp.select(0, k).to(b.scalar_type()) : Tensor(), Tensor(), Tensor()};
   }
 };
 
-Tensor conv_canal(const Tensor& z, const Tensor& w, const Opcional& b, int64_t act) {
-  return ConvCanal::apply(z, w, b, act)[0];
+Tensor conv_canal(const Tensor& z, const Tensor& w, const Opcional& b, int64_t act, bool registrable) {
+  return ConvCanal::apply(z, w, b, act, registrable)[0];
 }
 
 // z (B, d), ventana (B, d, k - 1) dense -> y and the next window, the same tensor or a new one

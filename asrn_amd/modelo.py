@@ -79,7 +79,7 @@ def conv_canal_causal(z, peso, sesgo):
     """The per-channel (depthwise) version: peso (d, 1, k). On the GPU one kernel (selectiva.conv_canal) where it
     takes the call, else k multiply-adds over shifted views."""
     if _conv_canal_ok(z, peso):
-        return selectiva.conv_canal(z, peso, sesgo)
+        return selectiva.conv_canal(z, peso, sesgo, registrable=True)
     k = peso.shape[-1]
     w = peso[:, 0, :].to(z.dtype)
     zp = F.pad(z, (0, 0, k - 1, 0))
@@ -173,7 +173,7 @@ class BloqueLocal(nn.Module):
                 return h + self._ff(y)
             c = F.gelu(c)
         elif _conv_canal_ok(z, self.conv.weight):
-            c = selectiva.conv_canal(z, self.conv.weight, self.conv.bias, 'gelu')
+            c = selectiva.conv_canal(z, self.conv.weight, self.conv.bias, 'gelu', registrable=True)
         else:
             c = F.gelu(conv_canal_causal(z, self.conv.weight, self.conv.bias))
         if self.mezcla == 'memoria':

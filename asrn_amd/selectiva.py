@@ -77,16 +77,17 @@ def _conv(quien, z, peso, sesgo, ejes):
     return k
 
 
-def conv_canal(z, peso, sesgo=None, activacion=None):
+def conv_canal(z, peso, sesgo=None, activacion=None, registrable=False):
     """act(sesgo + sum_j peso[:, j] z[:, t - (k - 1) + j]) of each channel, zeros before a text's start: z (B, L, d) fp32,
     bf16 or fp16, read through its strides; peso (d, k) or nn.Conv1d's depthwise (d, 1, k), k <= 16; activacion None, 'gelu'
     (erf's) or 'silu'. The result is dense in z's dtype; products, sums and the activation are in fp32, rounded once.
-    The backward forms the activation's input again: nothing but z is kept."""
+    The backward forms the activation's input again: nothing but z is kept. A backward that is itself recorded
+    (create_graph=True) is refused, or with registrable=True runs in torch's operators, which have a second derivative."""
     quien = 'conv_canal'
     _conv(quien, z, peso, sesgo, 3)
     a = _activacion(quien, activacion)
     _dev(z)
-    return nodos().conv_canal(z, peso, sesgo, a)
+    return nodos().conv_canal(z, peso, sesgo, a, bool(registrable))
 
 
 def paso_conv_canal(z, ventana, peso, sesgo=None, activacion=None, en_sitio=True):

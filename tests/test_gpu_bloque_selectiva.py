@@ -268,3 +268,45 @@ def test_memoria_without_the_nodes(monkeypatch):
     b = m.bloques[0]
     with pytest.raises(_lib.ASRNHipError, match='missing'):
         asrn_amd.conv_canal(torch.randn(1, 3, 32, device=DEV), b.conv.weight)
+
+
+@pytest.mark.parametrize('act', [None, 'gelu', 'silu'])
+@pytest.mark.parametrize('forma', ['densa', 'traspuesta'])
+def test_second_gradient_of_the_convolution_where_it_is_recorded(act, forma):
+    """registrable: the gradients that are recorded are the formula's, and so are theirs (fp32 sums of some 20 terms around 1: 64
+    roundings of the largest value)."""
+    z, w, b = torch.randn(2, 9, 8, device=DEV), torch.randn(8, 1, 4, device=DEV), torch.randn(8, device=DEV)
+    if forma == 'traspuesta':
+        z = z.transpose(1, 2).contiguous().transpose(1, 2)
+    g1, g2 = torch.randn(2, 9, 8, device=DEV), [torch.randn_like(t) for t in (z, w, b)]
+
+    def formula(z, w, b):
+        v = F.pad(z, (0, 0, 3, 0)).unfold(1, 4, 1)
+        pre = (v * w[:, 0]).sum(-1) + b
+        return pre if act is None else F.gelu(pre) if act == 'gelu' else F.silu(pre)
+
+    def dos(f, dt):
+        hojas = [t.to(dt).requires_grad_() for t in (z.detach(), w, b)]
+        gs = torch.autograd.grad(f(*hojas), hojas, g1.to(dt).requires_grad_(), create_graph=True)
+        total = sum((a * c.to(dt)).sum() for a, c in zip(gs, g2))
+        return [*gs, *torch.autograd.grad(total, hojas, allow_unused=True, materialize_grads=True)]    # without act b enters none
+    propia = dos(lambda *a: asrn_amd.conv_canal(*a, act, registrable=True), torch.float32)
+    for a, v in zip(propia, dos(formula, torch.float64)):
+        assert (a - v).abs().max() <= 64 * U * 20 * max(1, v.abs().max())
+    solo = torch.randn(2, 5, 8, device=DEV).requires_grad_()         # one argument alone asks for a gradient
+    g, = torch.autograd.grad(asrn_amd.conv_canal(solo, w, b, act, registrable=True).sum(), solo, create_graph=True)
+    ref, = torch.autograd.grad(asrn_amd.conv_canal(solo, w, b, act).sum(), solo)
+    assert (g - ref).abs().max() <= 64 * U * 20
+
+
+def test_memoria_model_with_a_recorded_gradient():
+    """Gradients with create_graph=True are those without."""
+    m = asrn_amd.crear_modelo(60, d=32, n_capas=2, semilla=1, mezcla='memoria', memoria_max=64, **REDUCIDA).to(DEV)
+    x = synth.tokens(2, 41, 60, seed=0).to(DEV)
+    ps = list(m.parameters())
+    ref, got = (torch.autograd.grad(m.perdida(x[:, :-1], x[:, 1:]), ps, create_graph=c) for c in (False, True))
+    for a, b in zip(ref, got):
+        assert (a - b).norm() <= 2e-3 * a.norm() + 1e-7
+    z, w = torch.randn(2, 9, 8, device=DEV).requires_grad_(), torch.randn(8, 1, 4, device=DEV).requires_grad_()
+    g, = torch.autograd.grad(conv_canal_causal(z, w, torch.randn(8, device=DEV)).square().sum(), z, create_graph=True)
+    assert torch.autograd.grad(g.square().sum(), w)[0].abs().sum() > 0
