@@ -568,3 +568,10 @@ def test_one_token_of_any_stride(dt):
     assert y.shape == (0, 1, d) and torch.autograd.grad(y.sum() + fin.sum(), hojas[0])[0].shape == (0, 1, d)
     z, w = e[0], r(d, 4)
     assert torch.equal(asrn_amd.conv_canal(lejos(z), w), asrn_amd.conv_canal(z, w))
+
+
+@pytest.mark.parametrize('B,L,d,k,act,dt', [(2, 9001, 768, 4, 'silu', BF16), (2, 9001, 768, 3, 'gelu', F32),
+                                            (1, 3301, 1021, 7, None, F32), (3, 1501, 801, 4, 'silu', F16)])
+def test_conv_canal_in_long_pieces(B, L, d, k, act, dt):
+    """So many values that a piece has more than the 16 tokens of the smallest ones (12.6 M of four channels a lane, 3.1 M of one)."""
+    test_conv_canal(B, L, d, k, act, dt, True)
