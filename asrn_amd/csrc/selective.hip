@@ -9,10 +9,11 @@
 // leaves channel l in lane l again, and the sums over the channels that the backward needs (dB, dC) begin inside a lane.
 // A wave's LDS is its own: no barriers in the forward.
 // Every channel and state has its own decay, so there is no matrix product in it: what bounds it is the vector units' issue.
-// A wave's token of 16 states a channel takes about 130 instructions forward (16 of them exponentials, of two slots each; at the
-// least 3 multiply-adds and an exponential a value, 80 slots) and 404 backward; 65 to 80% of the issue slots are used.
+// A wave's token of 16 states a channel takes about 130 instructions forward (16 of them exponentials, of two slots each: 146
+// slots; at the least the exponent's product, x B, two multiply-adds and an exponential a value, 96) and 404 backward; 65 to
+// 80% of the issue slots are used.
 // Measured, 16 states, bf16: 2 texts of 32768 tokens x 768 channels forward 398 us (a trace has 164 for the chunks' ends, 15 for
-// their starts and 240 for all chunks), 8 texts of 2048 traced forward 127 and backward 279 (the tokens' kernel 209); the bytes
+// their starts and 240 for all chunks), 8 texts of 2048 traced forward 124 and backward 276 (the tokens' kernel 207); the bytes
 // at a copy's rate take 80, 20 and 36.
 // Texts too few to fill the card are cut into chunks: each chunk's end state from a zero state and its sum of delta
 // first, then the chunks' start states one after the other (exp(A sum delta) carries a state over a chunk), then all chunks

@@ -300,7 +300,7 @@ def lineal_activa(x, w, b=None, activacion=None, residuo=None):
     activacion None, 'gelu' (erf's) or 'silu'. fp32, bf16 or fp16; under autocast the product's operands are cast as F.linear's
     are. The result is in the residual's dtype (fp32 or the product's), else in the product's; sums, the activation and the
     residual's addition are in fp32, rounded once. Gradients go to all four tensors; the activation's input is kept in the
-    product's dtype. Second gradients are refused."""
+    product's dtype. Second gradients and tangents of forward mode are refused, and rows of 2^21 values and more."""
     quien = 'lineal_activa'
     if activacion not in ACTIVACIONES:
         raise ValueError(f'{quien}: activacion={activacion!r}: one of {tuple(ACTIVACIONES)}')
