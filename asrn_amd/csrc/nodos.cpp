@@ -417,8 +417,10 @@ void escrito(const Tensor& t) {
   if (!t.is_inference()) torch::autograd::impl::bump_version(t);
 }
 
-// The gradients of a convolution of each channel in torch's operators, which record them: of z, w, b where they ask for one
-variable_list conv_registrada(const Tensor& z, const Tensor& w, const Tensor& b, const Tensor& gy, int64_t act) {
+// The gradients of a convolution of each channel in torch's operators, which record them: of z, w, b where they ask for one.
+// Taken of aliases: the tensors' own hooks see the gradient once, when this backward has returned it.
+variable_list conv_registrada(const Tensor& z0, const Tensor& w0, const Tensor& b0, const Tensor& gy, int64_t act) {
+  const Tensor z = z0.alias(), w = w0.alias(), b = b0.defined() ? b0.alias() : b0;
   const int64_t L = z.size(1), d = z.size(2), k = w.size(-1);
   const Tensor zp = at::constant_pad_nd(z.to(at::kFloat), {0, 0, k - 1, 0}), wf = w.reshape({d, k}).to(at::kFloat);
   Tensor s = zp.narrow(1, 0, L) * wf.select(1, 0);

@@ -310,3 +310,16 @@ def test_memoria_model_with_a_recorded_gradient():
     z, w = torch.randn(2, 9, 8, device=DEV).requires_grad_(), torch.randn(8, 1, 4, device=DEV).requires_grad_()
     g, = torch.autograd.grad(conv_canal_causal(z, w, torch.randn(8, device=DEV)).square().sum(), z, create_graph=True)
     assert torch.autograd.grad(g.square().sum(), w)[0].abs().sum() > 0
+
+
+def test_hooks_see_a_recorded_gradient_once():
+    hojas = [torch.randn(2, 9, 8, device=DEV).requires_grad_(), torch.randn(8, 1, 4, device=DEV).requires_grad_(),
+             torch.randn(8, device=DEV).requires_grad_()]
+    vistas = []
+    for t in hojas:
+        t.register_hook(lambda g: vistas.append(g.shape) or 2 * g)
+    ref, got = (torch.autograd.grad(asrn_amd.conv_canal(1 * hojas[0], *hojas[1:], 'gelu', registrable=True).sum(), hojas, create_graph=c)
+                for c in (False, True))
+    assert len(vistas) == 6
+    for a, b in zip(ref, got):
+        assert (a - b).abs().max() <= 64 * U * 20
